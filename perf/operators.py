@@ -71,7 +71,9 @@ def listed():
 def draw(rng):
     """1 to 16384 tokens (1 to 32768 rows of a single projection); half of the cases at the benchmark's sizes, the others
     with 8 to 160 experts, hidden 256 to 4096 and intermediate 128 to 1536 in steps of 32, or, with up to 2048 rows, of
-    any size from 32 to 1024; some with skewed routing."""
+    any size from 32 to 1024; some with skewed routing.  float32 activations only where it is the inputs that are
+    quantised: what is quantised in the middle (the gated unit's result, its gradients) comes out of 32-bit sums, whose last
+    bits put a value next to a border of the 8-bit grid on either side."""
 
     def log_between(a, b):
         return int(round(math.exp(rng.uniform(math.log(a), math.log(b)))))
@@ -82,6 +84,8 @@ def draw(rng):
         single = kind.startswith("linear")
         c = {"kind": kind, "tokens": log_between(1, 32768 if single else 16384), "experts": 128, "top_k": 1 if single else 8,
              "hidden": 2048, "inter": 768, "dtype": rng.choice(("bf16", "bf16", "bf16", "fp16", "fp32")), "zipf": 0.0}
+        if c["dtype"] == "fp32" and kind in ("glu_backward", "mlp"):
+            c["dtype"] = "bf16"
         sizes = rng.choice(("benchmark", "benchmark", "other", "odd"))
         if sizes != "benchmark":
             c["experts"] = rng.choice((8, 16, 60, 64, 96, 128, 160))
