@@ -479,6 +479,62 @@ MFL_API int mfl_moe_block_bwd(const mfl_moe_block *b, const void *dout, const vo
                       void *d_logits, void *d_gate, void *d_up, void *d_down, void *workspace,
                       size_t ws_bytes, void *stream);
 
+/* ---- expert products in 8-bit floating point ----------------------------------------- */
+
+/* Values are e4m3 (OCP).  Weights (E,N,K) carry one fp32 scale per 128 x 128 block, (E, ceil(N/128), ceil(K/128)), any
+ * finite value.  The left operand comes in bf16 / fp16 / fp32 and is quantised by the call: one scale per row and 128
+ * elements of the reduction, the smallest power of two, 2^-117 at least, that brings the largest finite magnitude of the
+ * block to 448 or below; every element is rounded once (nearest, ties to even); elements that are infinite or no number
+ * become NaN and leave the scale to the others.  Sums are fp32, rounded once to out_dtype.  The reference has no
+ * counterpart.
+ *
+ * workspace: mfl_fp8_workspace(...) bytes, 256-byte aligned (NULL where that is 0); it is scratch: nothing is kept in it
+ * from one call to the next, and calls that can overlap in time need one each. */
+typedef struct mfl_fp8_weight {
+    const void *q;      /* e4m3 bytes */
+    const float *scale; /* NaN scales make their block's products NaN */
+} mfl_fp8_weight;
+
+#define MFL_FP8_FWD 0 /* mfl_gemm_fwd_fp8: (src_rows, K) quantised; R, N, K, E of the product */
+#define MFL_FP8_DX 1  /* mfl_gemm_dx_fp8 (src_rows is not used) */
+#define MFL_FP8_GLU 2 /* mfl_glu_fwd_fp8 */
+#define MFL_FP8_GLU_BWD 3 /* mfl_glu_bwd_fp8 (src_rows is not used) */
+#define MFL_FP8_MLP 4 /* mfl_mlp_fwd_fp8, N the intermediate and K the hidden size */
+MFL_API size_t mfl_fp8_workspace(int op, int64_t src_rows, int64_t R, int N, int K, int E);
+
+/* y[r,n] = sum_k w[e(r),n,k] x[s(r),k], e(r) from m_sizes as in mfl_gemm_fwd, s(r) = row_idx[r] / idx_div of src_rows rows
+ * (row_idx NULL: r).  Rows past sum(m_sizes) are not written. */
+MFL_API int mfl_gemm_fwd_fp8(const void *x, int64_t src_rows, const int32_t *row_idx, int idx_div, const mfl_fp8_weight *w,
+                     const void *m_sizes, int m_sizes_dtype, void *y, int64_t R, int N, int K, int E, int in_dtype,
+                     int out_dtype, void *workspace, size_t ws_bytes, void *stream);
+/* dx[r,k] = sum_n w[e(r),n,k] dy[r,n], dy quantised along n. */
+MFL_API int mfl_gemm_dx_fp8(const void *dy, const mfl_fp8_weight *w, const void *m_sizes, int m_sizes_dtype, void *dx,
+                     int64_t R, int N, int K, int E, int in_dtype, int out_dtype, void *workspace, size_t ws_bytes,
+                     void *stream);
+/* h = silu(e) * g with e = x gate^T, g = x up^T in fp32; e_out / g_out (R,N), where not NULL, receive the two products.
+ * All tensors of `dtype`. */
+MFL_API int mfl_glu_fwd_fp8(const void *x, int64_t src_rows, const int32_t *row_idx, int idx_div, const mfl_fp8_weight *gate,
+                    const mfl_fp8_weight *up, const void *m_sizes, int m_sizes_dtype, void *h, void *e_out, void *g_out,
+                    int64_t R, int N, int K, int E, int dtype, void *workspace, size_t ws_bytes, void *stream);
+/* dx = de gate + dg up, de and dg the gradients of h = silu(e) * g in fp32, quantised along n. */
+MFL_API int mfl_glu_bwd_fp8(const void *dh, const void *e, const void *g, const mfl_fp8_weight *gate, const mfl_fp8_weight *up,
+                    const void *m_sizes, int m_sizes_dtype, void *dx, int64_t R, int N, int K, int E, int dtype,
+                    void *workspace, size_t ws_bytes, void *stream);
+/* y = h down^T with h as in mfl_glu_fwd_fp8 (N = I, K = H), quantised along its columns from the fp32 values; down (E,H,I),
+ * y (R,H). */
+MFL_API int mfl_mlp_fwd_fp8(const void *x, int64_t src_rows, const int32_t *row_idx, int idx_div, const mfl_fp8_weight *gate,
+                    const mfl_fp8_weight *up, const mfl_fp8_weight *down, const void *m_sizes, int m_sizes_dtype, void *y,
+                    void *e_out, void *g_out, int64_t R, int I, int H, int E, int dtype, void *workspace,
+                    size_t ws_bytes, void *stream);
+
+/* Quantised rows by themselves: q (R, 128 ceil(K/128)) bytes, zeros behind column K, and scale (R, 4 ceil(ceil(K/128)/4))
+ * biased exponent bytes (the scale is 2^(byte - 127)), of which the first ceil(K/128) of a row are written. */
+MFL_API int mfl_fp8_quant_rows(const void *x, int dtype, int64_t R, int K, void *q, uint8_t *scale, void *stream);
+MFL_API int mfl_fp8_dequant_rows(const void *q, const uint8_t *scale, int64_t R, int K, void *out, int out_dtype, void *stream);
+/* Weights: q (E,N,K) and scales by the rule of the rows, over 128 x 128 blocks. */
+MFL_API int mfl_fp8_quant_blocks(const void *w, int dtype, int E, int N, int K, void *q, float *scale, void *stream);
+MFL_API int mfl_fp8_dequant_blocks(const void *q, const float *scale, int E, int N, int K, void *out, int out_dtype, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

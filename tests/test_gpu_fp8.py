@@ -1,0 +1,554 @@
+"""Expert products in 8-bit floating point against their definition in 64 bits: quantisation bit for bit, the grouped product
+and its input gradient, the gated unit and its backward pass, the expert MLP, the module and the block."""
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from fp8_reference import (GAMMA, assert_within, blocks_of, dense, gated, gated_backward, grouped, product, quantize,
+                           scale_exponent)
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+FP8 = torch.float8_e4m3fn
+
+
+def cut_in(out):
+    return out.dtype != torch.float32
+
+
+def make_rows(rows, k, dtype, seed, spread=True):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn((rows, k), generator=g)
+    if spread:  # blocks of very different size
+        x *= torch.exp2(torch.randint(-6, 7, (rows, 1), generator=g).float())
+    return x.to(dtype).to(DEV)
+
+
+def make_weight(experts, n, k, seed):
+    """Any bytes but NaN, any fp32 scales."""
+    g = torch.Generator().manual_seed(seed)
+    w = (torch.randn((experts, n, k), generator=g) * 40).clamp_(-448, 448).to(FP8)
+    scale = torch.rand((experts, blocks_of(n), blocks_of(k)), generator=g) * 1e-3 + 1e-4
+    return w.to(DEV), scale.to(DEV)
+
+
+def counts_of(rows, experts, kind, seed=0):
+    if kind == "one":  # all rows with the last expert
+        return [0] * (experts - 1) + [rows]
+    if kind == "few":  # fewer rows than the operand has
+        c = [0] * experts
+        c[experts // 2] = rows // 2
+        return c
+    g = torch.Generator().manual_seed(seed)
+    return torch.bincount(torch.randint(0, experts, (rows,), generator=g), minlength=experts).tolist()
+
+
+def sizes(counts, dtype=torch.int32):
+    return torch.tensor(counts, dtype=dtype, device=DEV)
+
+
+def routed(tokens, k, experts, seed):
+    from qwen3_moe_fused.kernels.indexing import get_expert_counts_and_idx
+
+    g = torch.Generator().manual_seed(seed)
+    sel = torch.rand((tokens, experts), generator=g).topk(k, dim=1).indices.reshape(-1).to(DEV)
+    m_sizes, sort_idx, inv = get_expert_counts_and_idx(sel, experts)
+    return m_sizes, sort_idx, inv, m_sizes.tolist()
+
+
+# ---- quantisation ------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,k", [(1, 1), (3, 127), (5, 128), (2, 129), (67, 640), (33, 1001), (1, 5000), (300, 264)])
+def test_rows_are_quantised_bit_for_bit(dtype, rows, k):
+    from qwen3_moe_fused.quantize.fp8 import dequantize_fp8_rows, quantize_fp8_rows
+
+    x = make_rows(rows, k, dtype, rows + k)
+    x[0] = 0
+    if rows > 2:
+        x[1] *= 2.0 ** -14
+        x[2, k // 2] = torch.finfo(dtype).max
+    q, s = quantize_fp8_rows(x)
+    ref, e, _ = quantize(x.double())
+    assert q.shape == (rows, k) and q.dtype == FP8 and s.shape == (rows, blocks_of(k)) and s.dtype == torch.float8_e8m0fnu
+    assert torch.equal(s.view(torch.uint8).double() - 127, e)
+    values = q.double() * torch.exp2(e).repeat_interleave(128, 1)[:, :k]
+    assert torch.equal(values, ref)
+    for out in (torch.float32, torch.bfloat16):
+        assert torch.equal(dequantize_fp8_rows(q, s, out), ref.to(out))
+
+
+def test_rows_with_infinities_nan_and_the_borders_of_the_scale():
+    from qwen3_moe_fused.quantize.fp8 import quantize_fp8_rows
+
+    x = torch.zeros((9, 128), device=DEV)
+    x[0, 5], x[0, 6] = float("inf"), 3.0
+    x[1, 0], x[1, 1] = float("nan"), -448.0
+    x[2, :] = float("-inf")
+    x[3, 0] = 448.0
+    x[4, 0] = 448.0 * (1 + 2.0 ** -23)  # the next scale
+    x[5, 0] = 2.0 ** -140  # subnormal: the least scale
+    x[6, 0] = torch.finfo(torch.float32).max
+    x[7, 0], x[7, 1] = 448.0, 2.0 ** -9 * 1.5  # a tie between the grid's two smallest values
+    x[8, 0], x[8, 1] = 448.0, -17.0  # a tie: to the even neighbour
+    q, s = quantize_fp8_rows(x)
+    ref, e, _ = quantize(x.double())
+    assert torch.equal(s.view(torch.uint8).double() - 127, e)
+    values = q.double() * torch.exp2(e).repeat_interleave(128, 1)
+    assert torch.equal(values.isnan(), ref.isnan()) and torch.equal(values.nan_to_num(), ref.nan_to_num())
+    assert q[0, 5].isnan() and not q[0, 6].isnan() and q[2].isnan().all()
+    assert q[7, 1].float() == 2.0 ** -8 and q[8, 1].float() == -16.0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("shape", [(1, 1, 1), (2, 128, 256), (3, 130, 257), (2, 31, 5)])
+def test_blocks_are_quantised_bit_for_bit(dtype, shape):
+    from qwen3_moe_fused.quantize.fp8 import dequantize_fp8_blocks, quantize_fp8_blocks
+
+    experts, n, k = shape
+    w = make_rows(experts * n, k, dtype, sum(shape)).view(shape)
+    q, s = quantize_fp8_blocks(w)
+    assert q.shape == w.shape and s.shape == (experts, blocks_of(n), blocks_of(k))
+    pad = torch.zeros((experts, blocks_of(n) * 128, blocks_of(k) * 128), dtype=torch.float64, device=DEV)
+    pad[:, :n, :k] = w.double()
+    amax = pad.abs().view(experts, blocks_of(n), 128, blocks_of(k), 128).amax(dim=(2, 4))
+    e = scale_exponent(amax)
+    assert torch.equal(s.double(), torch.exp2(e))
+    v = w.double() / torch.exp2(e).repeat_interleave(128, 1)[:, :n].repeat_interleave(128, 2)[:, :, :k]
+    step = torch.exp2((torch.frexp(v).exponent - 1).clamp(min=-6).double() - 3)
+    assert torch.equal(q.double(), torch.round(v / step) * step)
+    # any scales on the way back, rounded once
+    s = s * 0.7
+    for out in (torch.float32, torch.bfloat16):
+        back = dequantize_fp8_blocks(q, s, out)
+        assert torch.equal(back, dense(q, s).to(out))
+
+
+# ---- the product and its input gradient -----------------------------------------------------------------------------------
+
+# rows, experts, out, in, how the rows are dealt out
+SHAPES = [
+    (8, 128, 96, 256, "spread"),      # less than a row per expert
+    (1, 3, 128, 128, "one"),
+    (37, 5, 200, 328, "spread"),      # partial blocks both ways, 16-byte rows on neither side
+    (70, 4, 33, 1001, "spread"),      # rows of odd length
+    (300, 7, 256, 384, "spread"),
+    (515, 2, 130, 64, "spread"),      # several row tiles per expert
+    (129, 600, 64, 160, "spread"),    # more experts than a table of 512 holds
+    (1000, 8, 768, 2048, "spread"),
+    (700, 3, 384, 512, "one"),
+    (90, 6, 272, 144, "few"),         # rows behind the last sequence
+]
+
+
+@pytest.mark.parametrize("rows,experts,n,k,kind", SHAPES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_product_and_input_gradient(rows, experts, n, k, kind, dtype):
+    from qwen3_moe_fused.quantize.layer_fp8 import moe_fused_linear_fp8
+
+    counts = counts_of(rows, experts, kind)
+    x, dy = make_rows(rows, k, dtype, 1, spread=False).requires_grad_(), make_rows(rows, n, dtype, 2, spread=False)
+    w, s = make_weight(experts, n, k, 3)
+    y = moe_fused_linear_fp8(x, w, s, sizes(counts))
+    y.backward(dy)
+    used, full = sum(counts), dense(w, s)
+    for out, given, transposed in ((y.detach(), x.detach(), False), (x.grad, dy, True)):
+        q, _, slack = quantize(given.double())
+        ref, bound = product(q, slack, full, counts, transposed, cut_in(out))
+        assert out.dtype == dtype
+        assert_within(out[:used], ref[:used], bound[:used], "input gradient" if transposed else "forward")
+
+
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("index", [torch.int64, torch.int32, torch.uint8])
+def test_output_types_and_row_count_types(out_dtype, index):
+    from qwen3_moe_fused.grouped_gemm.forward_fp8 import grouped_gemm_forward_fp8, grouped_gemm_forward_transposed_fp8
+
+    counts = [3, 0, 41, 20]
+    x, dy = make_rows(64, 256, torch.bfloat16, 4, spread=False), make_rows(64, 128, torch.bfloat16, 5, spread=False)
+    w, s = make_weight(4, 128, 256, 6)
+    y = grouped_gemm_forward_fp8(x, w, s, sizes(counts, index), out_dtype)
+    dx = grouped_gemm_forward_transposed_fp8(dy, w, s, sizes(counts, index), out_dtype)
+    for out, given, transposed in ((y, x, False), (dx, dy, True)):
+        q, _, slack = quantize(given.double())
+        assert out.dtype == out_dtype
+        assert_within(out, *product(q, slack, dense(w, s), counts, transposed, cut_in(out)))
+
+
+@pytest.mark.parametrize("rows", [24, 400, 3000])
+def test_rows_outside_the_experts_are_left_as_they_were(rows):
+    """Row counts that sum to less than the rows leave the others unwritten; more are cut at the last row, and negative ones
+    count as none."""
+    from qwen3_moe_fused import _lib
+    from qwen3_moe_fused.grouped_gemm.forward_fp8 import DX, FWD, fp8_weight, fp8_workspace
+
+    n = k = 256
+    x, dy = make_rows(rows, k, torch.bfloat16, 7, spread=False), make_rows(rows, n, torch.bfloat16, 8, spread=False)
+    w, s = make_weight(3, n, k, 9)
+    for counts in ([rows // 3, -5, rows // 4], [0, 0, 0], [rows // 2, rows, rows]):
+        ms = sizes(counts)
+        seen = [max(c, 0) for c in counts]
+        used = min(sum(seen), rows)
+        for transposed, given in ((False, x), (True, dy)):
+            out = torch.full((rows + 8, 256), 7.0, device=DEV, dtype=torch.bfloat16)
+            keep, ws, size = fp8_workspace(DX if transposed else FWD, x, rows, rows, n, k, 3)
+            args = (ms.data_ptr(), _lib.I32, out.data_ptr(), rows, n, k, 3, _lib.BF16, _lib.BF16, ws, size, _lib.stream())
+            if transposed:
+                rc = _lib.lib().mfl_gemm_dx_fp8(given.data_ptr(), fp8_weight(w, s), *args)
+            else:
+                rc = _lib.lib().mfl_gemm_fwd_fp8(given.data_ptr(), rows, None, 1, fp8_weight(w, s), *args)
+            assert rc == 0
+            q, _, slack = quantize(given.double())
+            ref, bound = product(q, slack, dense(w, s), seen, transposed, True)
+            assert_within(out[:used], ref[:used], bound[:used])
+            assert (out[used:] == 7.0).all()
+
+
+def test_nan_and_infinity_stay_in_their_row_and_block():
+    from qwen3_moe_fused.grouped_gemm.forward_fp8 import grouped_gemm_forward_fp8
+
+    for rows in (6, 200):
+        x = make_rows(rows, 384, torch.bfloat16, 10, spread=False)
+        w, s = make_weight(2, 256, 384, 11)
+        clean = grouped_gemm_forward_fp8(x, w, s, sizes([rows - 2, 2]))
+        x[1, 200], x[2, 3] = float("nan"), float("inf")
+        s[1, 1, 2] = float("nan")  # the second expert's columns from 128 on
+        y = grouped_gemm_forward_fp8(x, w, s, sizes([rows - 2, 2]))
+        bad = torch.zeros_like(y, dtype=torch.bool)
+        bad[1], bad[2], bad[-2:, 128:] = True, True, True
+        assert torch.equal(y.isnan(), bad) and torch.equal(y[~bad], clean[~bad])
+
+
+def test_partial_blocks_read_nothing_behind_them():
+    """NaN weights of the next row, column or expert do not reach sums whose block ends before them."""
+    from qwen3_moe_fused.grouped_gemm.forward_fp8 import grouped_gemm_forward_fp8, grouped_gemm_forward_transposed_fp8
+
+    for n, k in ((48, 208), (48, 77)):
+        for rows in (5, 170):
+            w, s = make_weight(3, n, k, 12)
+            w[1] = torch.full_like(w[1].float(), float("nan")).to(FP8)
+            counts = [rows, 0, 2]
+            x, dy = make_rows(rows + 2, k, torch.float32, 13, False), make_rows(rows + 2, n, torch.float32, 14, False)
+            full = dense(w, s)
+            full[1] = 0
+            for out, given, transposed in ((grouped_gemm_forward_fp8(x, w, s, sizes(counts)), x, False),
+                                           (grouped_gemm_forward_transposed_fp8(dy, w, s, sizes(counts)), dy, True)):
+                q, _, slack = quantize(given.double())
+                assert_within(out, *product(q, slack, full, counts, transposed, cut_in(out)))
+
+
+def test_gradient_against_differences():
+    """The product is linear between points of the grid: rows and directions of small whole numbers, whose blocks share one
+    scale, are on it, and so are the output gradients."""
+    from qwen3_moe_fused.quantize.layer_fp8 import moe_fused_linear_fp8
+
+    g = torch.Generator().manual_seed(15)
+    rows, n, k, counts = 40, 160, 192, [13, 0, 27]
+    x = torch.randint(-4, 5, (rows, k), generator=g).float()
+    d = torch.randint(-2, 3, (rows, k), generator=g).float()
+    dy = torch.randint(-7, 8, (rows, n), generator=g).float()
+    w, s = make_weight(3, n, k, 16)
+    x, d, dy = x.to(DEV).requires_grad_(), d.to(DEV), dy.to(DEV)
+    y0 = moe_fused_linear_fp8(x, w, s, sizes(counts))
+    y0.backward(dy)
+    y1 = moe_fused_linear_fp8(x.detach() + d, w, s, sizes(counts))
+    diff = ((y1 - y0.detach()).double() * dy.double()).sum()
+    full = dense(w, s)
+    size = (grouped(x.detach().double().abs() + d.double().abs(), full.abs(), counts) * dy.double().abs()).sum()
+    assert abs(float(diff - (x.grad.double() * d.double()).sum())) <= 4 * (k + n) * GAMMA * float(size)
+
+
+# ---- the gated unit -------------------------------------------------------------------------------------------------------
+
+GATED = [
+    # tokens, selected, experts, hidden, intermediate
+    (1, 8, 128, 256, 96),
+    (1, 1, 2, 128, 128),
+    (5, 3, 7, 200, 72),
+    (60, 4, 9, 1001, 33),
+    (96, 4, 4, 512, 384),
+    (700, 2, 6, 320, 272),
+    (33, 2, 600, 128, 64),
+]
+
+
+def gated_reference(tokens, w, sort_idx, k, counts):
+    q, _, slack = quantize(tokens.double())
+    q = q[sort_idx.long() // k]
+    slack = torch.zeros_like(q)
+    e, de = product(q, slack, dense(*w[0]), counts, cut=cut_in(tokens))
+    g, dg = product(q, slack, dense(*w[1]), counts, cut=cut_in(tokens))
+    return e, de, g, dg
+
+
+@pytest.mark.parametrize("tokens,k,experts,hidden,inter", GATED)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_gated_unit_and_its_backward(tokens, k, experts, hidden, inter, dtype):
+    from qwen3_moe_fused.grouped_gemm.fused import grouped_glu_backward_fp8, grouped_glu_forward_fp8
+
+    m_sizes, sort_idx, _, counts = routed(tokens, k, experts, 20)
+    x = make_rows(tokens, hidden, dtype, 21, spread=False)
+    w = [make_weight(experts, inter, hidden, 22 + i) for i in range(2)]
+    w = [(q, s / s.mean() * (40.0 * hidden ** 0.5) ** -1) for q, s in w]  # projections of about unit variance
+    h, e, g = grouped_glu_forward_fp8(x, *w[0], *w[1], m_sizes, sort_idx, k, return_products=True)
+    re, de, rg, dg = gated_reference(x, w, sort_idx, k, counts)
+    assert_within(e, re, de, "gate projection")
+    assert_within(g, rg, dg, "up projection")
+    assert_within(h, *gated(re, de, rg, dg), "gated unit")
+    only = grouped_glu_forward_fp8(x, *w[0], *w[1], m_sizes, sort_idx, k)
+    assert torch.equal(only, h)
+
+    dh = make_rows(tokens * k, inter, dtype, 24, spread=False)
+    dx = grouped_glu_backward_fp8(dh, e, g, *w[0], *w[1], m_sizes)
+    a, ea, b, eb = gated_backward(dh.double(), e.double(), g.double())
+    total, bound = 0, 0
+    for v, err, (q, s) in ((a, ea, w[0]), (b, eb, w[1])):
+        qv, _, slack = quantize(v, err)
+        t, bd = product(qv, slack, dense(q, s), counts, True, cut_in(dx))
+        total, bound = total + t, bound + 2 * bd  # (one sum over both terms: twice as many additions)
+    assert_within(dx, total, bound, "gradient of the rows")
+
+
+def test_gated_unit_without_gathered_rows():
+    from qwen3_moe_fused.grouped_gemm.fused import grouped_glu_forward_fp8
+
+    counts = [0, 17, 3]
+    x = make_rows(20, 256, torch.bfloat16, 25, spread=False)
+    w = [make_weight(3, 128, 256, 26 + i) for i in range(2)]
+    idx = torch.arange(20, device=DEV, dtype=torch.int32)
+    a = grouped_glu_forward_fp8(x, *w[0], *w[1], sizes(counts))
+    assert torch.equal(a, grouped_glu_forward_fp8(x, *w[0], *w[1], sizes(counts), idx, 1))
+
+
+def test_gated_unit_under_autograd_sums_each_tokens_rows():
+    from qwen3_moe_fused.fused_mlp import moe_fused_glu_fp8
+    from qwen3_moe_fused.grouped_gemm.fused import grouped_glu_backward_fp8, grouped_glu_forward_fp8
+    from qwen3_moe_fused.kernels.routing import _combine
+
+    m_sizes, sort_idx, inv, _ = routed(50, 3, 8, 28)
+    x = make_rows(50, 256, torch.bfloat16, 29, spread=False).requires_grad_()
+    w = [t for i in range(2) for t in make_weight(8, 128, 256, 30 + i)]
+    h = moe_fused_glu_fp8(x, *w, m_sizes, sort_idx, inv, 3)
+    dh = make_rows(150, 128, torch.bfloat16, 32, spread=False)
+    h.backward(dh)
+    h2, e, g = grouped_glu_forward_fp8(x.detach(), *w, m_sizes, sort_idx, 3, return_products=True)
+    assert torch.equal(h, h2)
+    rows = grouped_glu_backward_fp8(dh, e, g, *w, m_sizes)
+    assert torch.equal(x.grad, _combine(rows, inv, None, 50, 3))
+
+
+# ---- the expert MLP -------------------------------------------------------------------------------------------------------
+
+def mlp_weights(experts, hidden, inter, seed):
+    out = []
+    for i, (n, k) in enumerate(((inter, hidden), (inter, hidden), (hidden, inter))):
+        q, s = make_weight(experts, n, k, seed + i)
+        out += [q, s / s.mean() * (40.0 * k ** 0.5) ** -1]
+    return out
+
+
+@pytest.mark.parametrize("tokens,k,experts,hidden,inter", GATED + [(1200, 4, 8, 256, 256)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_expert_mlp(tokens, k, experts, hidden, inter, dtype):
+    from qwen3_moe_fused.fused_mlp import moe_fused_mlp_fp8
+
+    m_sizes, sort_idx, inv, counts = routed(tokens, k, experts, 33)
+    x = make_rows(tokens, hidden, dtype, 34, spread=False)
+    w = mlp_weights(experts, hidden, inter, 35)
+    y = moe_fused_mlp_fp8(x, *w, m_sizes, sort_idx, inv, k)
+    h, dh = gated(*gated_reference(x, ((w[0], w[1]), (w[2], w[3])), sort_idx, k, counts))
+    q, _, slack = quantize(h, dh)
+    assert_within(y, *product(q, slack, dense(w[4], w[5]), counts, cut=cut_in(y)), "expert MLP")
+
+
+def test_expert_mlp_backward_is_its_parts():
+    from qwen3_moe_fused.fused_mlp import moe_fused_mlp_fp8
+    from qwen3_moe_fused.grouped_gemm.forward_fp8 import grouped_gemm_forward_transposed_fp8
+    from qwen3_moe_fused.grouped_gemm.fused import grouped_glu_backward_fp8, grouped_glu_forward_fp8
+    from qwen3_moe_fused.kernels.routing import _combine
+
+    m_sizes, sort_idx, inv, _ = routed(70, 4, 8, 36)
+    x = make_rows(70, 256, torch.bfloat16, 37, spread=False).requires_grad_()
+    w = mlp_weights(8, 256, 128, 38)
+    y = moe_fused_mlp_fp8(x, *w, m_sizes, sort_idx, inv, 4)
+    dy = make_rows(280, 256, torch.bfloat16, 39, spread=False)
+    y.backward(dy)
+    _, e, g = grouped_glu_forward_fp8(x.detach(), *w[:4], m_sizes, sort_idx, 4, return_products=True)
+    dh = grouped_gemm_forward_transposed_fp8(dy, w[4], w[5], m_sizes)
+    assert torch.equal(x.grad, _combine(grouped_glu_backward_fp8(dh, e, g, *w[:4], m_sizes), inv, None, 70, 4))
+    with torch.no_grad():
+        assert torch.equal(moe_fused_mlp_fp8(x, *w, m_sizes, sort_idx, inv, 4), y)
+
+
+# ---- empty calls, streams, graphs -----------------------------------------------------------------------------------------
+
+def test_no_rows_and_no_tokens():
+    from qwen3_moe_fused.fused_mlp import moe_fused_glu_fp8, moe_fused_mlp_fp8
+    from qwen3_moe_fused.quantize.fp8 import dequantize_fp8_rows, quantize_fp8_rows
+    from qwen3_moe_fused.quantize.layer_fp8 import moe_fused_linear_fp8
+
+    w = mlp_weights(4, 128, 96, 40)
+    none = torch.zeros(4, dtype=torch.int32, device=DEV)
+    x = torch.empty((0, 128), device=DEV, dtype=torch.bfloat16, requires_grad=True)
+    y = moe_fused_linear_fp8(x, w[0], w[1], none)
+    y.sum().backward()
+    assert y.shape == (0, 96) and x.grad.shape == (0, 128)
+    idx = torch.empty(0, dtype=torch.int32, device=DEV)
+    assert moe_fused_glu_fp8(x.detach(), *w[:4], none, idx, idx, 2).shape == (0, 96)
+    assert moe_fused_mlp_fp8(x.detach(), *w, none, idx, idx, 2).shape == (0, 128)
+    q, s = quantize_fp8_rows(x.detach())
+    assert dequantize_fp8_rows(q, s).shape == (0, 128)
+
+
+def test_another_stream_and_replayed_graphs():
+    """Two graphs of one pool, replayed in turn with eager calls between them, and a call on a stream of its own."""
+    from qwen3_moe_fused.fused_mlp import moe_fused_mlp_fp8
+
+    w = mlp_weights(8, 256, 128, 41)
+    cases = []
+    for tokens, seed in ((3, 42), (300, 43)):
+        m_sizes, sort_idx, inv, _ = routed(tokens, 2, 8, seed)
+        cases.append((make_rows(tokens, 256, torch.bfloat16, seed, spread=False), m_sizes, sort_idx, inv))
+
+    def run(c):
+        return moe_fused_mlp_fp8(c[0], *w, *c[1:], 2)
+
+    expect = [run(c).clone() for c in cases]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        others = [run(c) for c in cases]
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(others, expect))
+    graphs, outs, pool = [], [], None
+    for c in cases:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool):
+            outs.append(run(c))
+        pool = graph.pool()
+        graphs.append(graph)
+    for turn in range(4):
+        for i in (0, 1):
+            cases[i][0].mul_(-1)  # new inputs in place
+            graphs[i].replay()
+            torch.cuda.synchronize()
+            assert torch.equal(outs[i], run(cases[i])), (turn, i)
+
+
+# ---- the module and the block ---------------------------------------------------------------------------------------------
+
+def make_block(dtype, hidden=256, inter=128, experts=8, k=2, seed=50):
+    from qwen3_moe_fused.modular_qwen3_moe_fused import Qwen3MoeFusedSparseMoeBlock
+    from qwen3_moe_fused.quantize.layer_fp8 import MoeFusedLinearFp8
+
+    torch.manual_seed(seed)
+    block = Qwen3MoeFusedSparseMoeBlock(SimpleNamespace(num_experts=experts, num_experts_per_tok=k, norm_topk_prob=True,
+                                                        hidden_size=hidden, moe_intermediate_size=inter, hidden_act="silu"))
+    block = block.to(DEV).to(dtype)
+    for name in ("gate_proj", "up_proj", "down_proj"):
+        setattr(block, name, MoeFusedLinearFp8.from_linear(getattr(block, name)))
+    return block
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("tokens", [1, 130])
+def test_block_runs_on_the_8_bit_projections(dtype, tokens):
+    """The block against its parts called one by one, forward and backward."""
+    from qwen3_moe_fused.fused_mlp import moe_fused_mlp_fp8
+    from qwen3_moe_fused.kernels.routing import combine_rows
+    from qwen3_moe_fused.modular_qwen3_moe_fused import route_tokens
+
+    block = make_block(dtype)
+    x = make_rows(tokens, 256, dtype, 51, spread=False).view(1, tokens, 256)
+    dout = make_rows(tokens, 256, dtype, 52, spread=False).view(1, tokens, 256)
+    results = []
+    for parts in (False, True):
+        block.zero_grad(set_to_none=True)
+        xi = x.clone().requires_grad_()
+        if parts:
+            t = xi.view(tokens, 256)
+            logits, weights, m_sizes, sort_idx, inv = route_tokens(block, t)
+            w = [p for m in (block.gate_proj, block.up_proj, block.down_proj) for p in (m.weight, m.weight_scale_inv)]
+            out = combine_rows(moe_fused_mlp_fp8(t, *w, m_sizes, sort_idx, inv, 2), inv, weights, sort_idx).view(x.shape)
+        else:
+            out, logits = block(xi)
+        out.backward(dout)
+        results.append((out.detach(), logits.detach(), xi.grad, block.gate.weight.grad))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+    with torch.no_grad():
+        assert torch.equal(block(x)[0], results[0][0])
+
+
+def test_block_with_a_hook_or_separate_steps_calls_the_modules():
+    block = make_block(torch.bfloat16)
+    x = make_rows(40, 256, torch.bfloat16, 53, spread=False).view(1, 40, 256)
+    calls = []
+    with torch.no_grad():
+        expect = block(x)[0]
+        handle = block.down_proj.register_forward_hook(lambda *a: calls.append(1))
+        hooked = block(x)[0]
+        handle.remove()
+        block.fuse_front = False
+        separate = block(x)[0]
+    assert calls == [1]
+    # h rounded to bf16 before it is quantised: a rounding of a step in places
+    for other in (hooked, separate):
+        assert (other.float() - expect.float()).norm() <= 0.05 * expect.float().norm()
+
+
+def test_module_keeps_its_types_and_its_state(tmp_path):
+    from qwen3_moe_fused.modular_qwen3_moe_fused import MoeFusedLinear
+    from qwen3_moe_fused.quantize.fp8 import quantize_fp8_blocks
+    from qwen3_moe_fused.quantize.layer_fp8 import MoeFusedLinearFp8
+
+    torch.manual_seed(54)
+    plain = MoeFusedLinear(200, 136, 3).to(DEV)
+    q, s = quantize_fp8_blocks(plain.weight.detach())
+    module = MoeFusedLinearFp8.from_linear(plain)
+    assert torch.equal(module.weight.view(torch.uint8), q.view(torch.uint8)) and torch.equal(module.weight_scale_inv, s)
+    for moved in (module.to(torch.bfloat16), module.half(), module.cpu().to(DEV)):
+        assert moved.weight.dtype == FP8 and moved.weight_scale_inv.dtype == torch.float32 and not moved.weight.requires_grad
+        assert torch.equal(moved.weight.view(torch.uint8), q.view(torch.uint8)) and torch.equal(moved.weight_scale_inv, s)
+    torch.save(module.state_dict(), tmp_path / "state.pt")
+    state = torch.load(tmp_path / "state.pt", weights_only=True)
+    assert set(state) == {"weight", "weight_scale_inv"}
+    for other in (MoeFusedLinearFp8(200, 136, 3, device=DEV), MoeFusedLinearFp8(200, 136, 3).to(DEV)):
+        other.load_state_dict(state)
+        x = make_rows(10, 200, torch.bfloat16, 55)
+        assert torch.equal(other(x, sizes([4, 0, 6])), module(x, sizes([4, 0, 6])))
+    other = MoeFusedLinearFp8(200, 136, 3, device=DEV)
+    other.load_state_dict(plain.state_dict())  # a floating-point weight is quantised
+    assert torch.equal(other.weight.view(torch.uint8), q.view(torch.uint8))
+
+
+def test_lora_over_8_bit_weights():
+    """An adapter over a frozen 8-bit projection: the base product's gradient plus the adapter's; the joined LoRA path, which
+    does not know the scales, refuses."""
+    from qwen3_moe_fused.fast_lora import get_lora_parameters
+    from qwen3_moe_fused.functional import moe_fused_linear
+    from qwen3_moe_fused.lora import HAVE_PEFT, LoraMoeFusedLinear
+    from qwen3_moe_fused.modular_qwen3_moe_fused import MoeFusedLinear
+    from qwen3_moe_fused.quantize.layer_fp8 import MoeFusedLinearFp8, moe_fused_linear_fp8
+
+    if HAVE_PEFT:
+        pytest.skip("written against the stand-in base class")
+    torch.manual_seed(56)
+    base = MoeFusedLinearFp8.from_linear(MoeFusedLinear(128, 96, 4).to(DEV))
+    lora = LoraMoeFusedLinear(base, "default", r=8, lora_alpha=16).to(DEV)
+    a, b = lora.lora_A["default"].weight, lora.lora_B["default"].weight
+    assert a.dtype == torch.float32
+    with torch.no_grad():
+        b.normal_(0, 0.1)
+    x = make_rows(30, 128, torch.float32, 57, spread=False).requires_grad_()
+    ms, dy = sizes([10, 0, 15, 5]), make_rows(30, 96, torch.float32, 58, spread=False)
+    lora(x, ms).backward(dy)
+    got = (x.grad, a.grad, b.grad)
+    x2, a2, b2 = x.detach().clone().requires_grad_(), a.detach().clone().requires_grad_(), b.detach().clone().requires_grad_()
+    (moe_fused_linear_fp8(x2, base.weight, base.weight_scale_inv, ms)
+     + moe_fused_linear(moe_fused_linear(x2, a2, ms), b2, ms) * 2.0).backward(dy)
+    for u, v in zip(got, (x2.grad, a2.grad, b2.grad)):
+        assert torch.equal(u, v)
+    with pytest.raises(NotImplementedError):
+        get_lora_parameters(lora)

@@ -1,0 +1,237 @@
+// extern "C" surface of the expert products in 8-bit floating point: argument validation and dispatch only.
+#include "fp8.h"
+
+using namespace mfl;
+
+namespace {
+
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+
+// Room for quantised rows in a workspace, and where they lie.
+size_t rows_bytes(int64_t rows, int K) { return up256((size_t)rows * fp8_ld(K)) + up256((size_t)rows * fp8_ld_scale(K)); }
+struct RowsRoom {
+    uint8_t *q, *scale;
+    RowsRoom(uint8_t *at, int64_t rows, int K) : q(at), scale(at + up256((size_t)rows * fp8_ld(K))) {}
+    Fp8Rows rows() const { return {q, scale}; }
+};
+
+bool sizes_ok(int64_t R, int N, int K, int E) { return R >= 0 && R <= 0x7fffffff && N > 0 && K > 0 && E > 0; }
+
+int check_call(const void *m_sizes, int ms_dtype, int64_t R, int N, int K, int E, int in_dtype, int out_dtype) {
+    if (!sizes_ok(R, N, K, E)) return MFL_ERR_SHAPE;
+    if (!dtype_ok(in_dtype) || !dtype_ok(out_dtype) || !itype_ok(ms_dtype)) return MFL_ERR_DTYPE;
+    if (!m_sizes) return MFL_ERR_NULL;
+    if (!aligned(m_sizes, ms_dtype == MFL_I64 ? 8 : 4)) return MFL_ERR_ALIGN;
+    return MFL_OK;
+}
+int check_source(int64_t src_rows, const int32_t *row_idx, int idx_div, int64_t R) {
+    if (row_idx != nullptr && (idx_div <= 0 || src_rows <= 0)) return MFL_ERR_SHAPE;
+    if (row_idx == nullptr && src_rows < R) return MFL_ERR_SHAPE;
+    if (!aligned(row_idx, 4)) return MFL_ERR_ALIGN;
+    return MFL_OK;
+}
+int check_weight(const mfl_fp8_weight *w) {
+    if (!w || !w->q || !w->scale) return MFL_ERR_NULL;
+    return aligned(w->scale, 4) ? MFL_OK : MFL_ERR_ALIGN;
+}
+int check_workspace(int op, int64_t src_rows, int64_t R, int N, int K, int E, const void *ws, size_t ws_bytes) {
+    const size_t need = mfl_fp8_workspace(op, src_rows, R, N, K, E);
+    if (need == 0) return MFL_OK;
+    if (!ws || ws_bytes < need) return MFL_ERR_WORKSPACE;
+    return aligned(ws, 256) ? MFL_OK : MFL_ERR_ALIGN;
+}
+Fp8Matrix matrix(const mfl_fp8_weight *w) { return {(const uint8_t *)w->q, w->scale}; }
+
+// the rows of the left operand that a product reads
+int64_t source_rows(int64_t src_rows, const int32_t *row_idx, int64_t R) { return row_idx != nullptr ? src_rows : R; }
+
+}  // namespace
+
+extern "C" {
+
+size_t mfl_fp8_workspace(int op, int64_t src_rows, int64_t R, int N, int K, int E) {
+    if (!sizes_ok(R, N, K, E) || src_rows < 0 || R == 0) return 0;
+    switch (op) {
+        case MFL_FP8_FWD:
+        case MFL_FP8_GLU:
+            return rows_bytes(src_rows, K);
+        case MFL_FP8_DX:
+            return rows_bytes(R, N);
+        case MFL_FP8_GLU_BWD:
+            return 2 * rows_bytes(R, N);
+        case MFL_FP8_MLP:
+            return rows_bytes(src_rows, K) + rows_bytes(R, N) + up256((size_t)R * N * 4);
+        default:
+            return 0;
+    }
+}
+
+int mfl_gemm_fwd_fp8(const void *x, int64_t src_rows, const int32_t *row_idx, int idx_div, const mfl_fp8_weight *w,
+                     const void *m_sizes, int m_sizes_dtype, void *y, int64_t R, int N, int K, int E, int in_dtype,
+                     int out_dtype, void *workspace, size_t ws_bytes, void *stream) {
+    int rc = check_call(m_sizes, m_sizes_dtype, R, N, K, E, in_dtype, out_dtype);
+    if (!rc) rc = check_source(src_rows, row_idx, idx_div, R);
+    if (rc) return rc;
+    if (R == 0) return MFL_OK;
+    if (!x || !y) return MFL_ERR_NULL;
+    rc = check_weight(w);
+    if (rc) return rc;
+    if (!aligned(x, dtype_size(in_dtype)) || !aligned(y, dtype_size(out_dtype))) return MFL_ERR_ALIGN;
+    rc = check_workspace(MFL_FP8_FWD, src_rows, R, N, K, E, workspace, ws_bytes);
+    if (rc) return rc;
+    const int64_t used = source_rows(src_rows, row_idx, R);
+    const RowsRoom room((uint8_t *)workspace, used, K);
+    rc = fp8_quant_rows(x, in_dtype, used, K, room.q, room.scale, (hipStream_t)stream);
+    if (rc) return rc;
+    Fp8Product p = {};
+    p.terms = 1, p.a[0] = room.rows(), p.w[0] = matrix(w);
+    p.row_idx = row_idx, p.idx_div = idx_div, p.src_rows = used;
+    p.m_sizes = m_sizes, p.ms_i64 = m_sizes_dtype == MFL_I64;
+    p.out = y, p.out_dtype = out_dtype, p.R = R, p.N = N, p.K = K, p.E = E;
+    return gemm_fp8_generic(p, (hipStream_t)stream);
+}
+
+int mfl_gemm_dx_fp8(const void *dy, const mfl_fp8_weight *w, const void *m_sizes, int m_sizes_dtype, void *dx, int64_t R, int N,
+                    int K, int E, int in_dtype, int out_dtype, void *workspace, size_t ws_bytes, void *stream) {
+    int rc = check_call(m_sizes, m_sizes_dtype, R, N, K, E, in_dtype, out_dtype);
+    if (rc) return rc;
+    if (R == 0) return MFL_OK;
+    if (!dy || !dx) return MFL_ERR_NULL;
+    rc = check_weight(w);
+    if (rc) return rc;
+    if (!aligned(dy, dtype_size(in_dtype)) || !aligned(dx, dtype_size(out_dtype))) return MFL_ERR_ALIGN;
+    rc = check_workspace(MFL_FP8_DX, 0, R, N, K, E, workspace, ws_bytes);
+    if (rc) return rc;
+    const RowsRoom room((uint8_t *)workspace, R, N);
+    rc = fp8_quant_rows(dy, in_dtype, R, N, room.q, room.scale, (hipStream_t)stream);
+    if (rc) return rc;
+    Fp8Product p = {};
+    p.dx = true, p.terms = 1, p.a[0] = room.rows(), p.w[0] = matrix(w);
+    p.m_sizes = m_sizes, p.ms_i64 = m_sizes_dtype == MFL_I64;
+    p.out = dx, p.out_dtype = out_dtype, p.R = R, p.N = N, p.K = K, p.E = E;
+    return gemm_fp8_generic(p, (hipStream_t)stream);
+}
+
+int mfl_glu_fwd_fp8(const void *x, int64_t src_rows, const int32_t *row_idx, int idx_div, const mfl_fp8_weight *gate,
+                    const mfl_fp8_weight *up, const void *m_sizes, int m_sizes_dtype, void *h, void *e_out, void *g_out,
+                    int64_t R, int N, int K, int E, int dtype, void *workspace, size_t ws_bytes, void *stream) {
+    int rc = check_call(m_sizes, m_sizes_dtype, R, N, K, E, dtype, dtype);
+    if (!rc) rc = check_source(src_rows, row_idx, idx_div, R);
+    if (rc) return rc;
+    if (R == 0) return MFL_OK;
+    if (!x || !h) return MFL_ERR_NULL;
+    rc = check_weight(gate);
+    if (!rc) rc = check_weight(up);
+    if (rc) return rc;
+    const size_t size = dtype_size(dtype);
+    if (!aligned(x, size) || !aligned(h, size) || !aligned(e_out, size) || !aligned(g_out, size)) return MFL_ERR_ALIGN;
+    rc = check_workspace(MFL_FP8_GLU, src_rows, R, N, K, E, workspace, ws_bytes);
+    if (rc) return rc;
+    const int64_t used = source_rows(src_rows, row_idx, R);
+    const RowsRoom room((uint8_t *)workspace, used, K);
+    rc = fp8_quant_rows(x, dtype, used, K, room.q, room.scale, (hipStream_t)stream);
+    if (rc) return rc;
+    Fp8Product p = {};
+    p.glu = true, p.terms = 1, p.a[0] = room.rows(), p.w[0] = matrix(gate), p.w[1] = matrix(up);
+    p.row_idx = row_idx, p.idx_div = idx_div, p.src_rows = used;
+    p.m_sizes = m_sizes, p.ms_i64 = m_sizes_dtype == MFL_I64;
+    p.out = h, p.e_out = e_out, p.g_out = g_out, p.out_dtype = p.prod_dtype = dtype, p.R = R, p.N = N, p.K = K, p.E = E;
+    return gemm_fp8_generic(p, (hipStream_t)stream);
+}
+
+int mfl_glu_bwd_fp8(const void *dh, const void *e, const void *g, const mfl_fp8_weight *gate, const mfl_fp8_weight *up,
+                    const void *m_sizes, int m_sizes_dtype, void *dx, int64_t R, int N, int K, int E, int dtype,
+                    void *workspace, size_t ws_bytes, void *stream) {
+    int rc = check_call(m_sizes, m_sizes_dtype, R, N, K, E, dtype, dtype);
+    if (rc) return rc;
+    if (R == 0) return MFL_OK;
+    if (!dh || !e || !g || !dx) return MFL_ERR_NULL;
+    rc = check_weight(gate);
+    if (!rc) rc = check_weight(up);
+    if (rc) return rc;
+    const size_t size = dtype_size(dtype);
+    if (!aligned(dh, size) || !aligned(e, size) || !aligned(g, size) || !aligned(dx, size)) return MFL_ERR_ALIGN;
+    rc = check_workspace(MFL_FP8_GLU_BWD, 0, R, N, K, E, workspace, ws_bytes);
+    if (rc) return rc;
+    const RowsRoom de((uint8_t *)workspace, R, N), dg((uint8_t *)workspace + rows_bytes(R, N), R, N);
+    rc = fp8_silu_bwd_quant(dh, e, g, dtype, R, N, de.q, de.scale, dg.q, dg.scale, (hipStream_t)stream);
+    if (rc) return rc;
+    Fp8Product p = {};
+    p.dx = true, p.terms = 2, p.a[0] = de.rows(), p.a[1] = dg.rows(), p.w[0] = matrix(gate), p.w[1] = matrix(up);
+    p.m_sizes = m_sizes, p.ms_i64 = m_sizes_dtype == MFL_I64;
+    p.out = dx, p.out_dtype = dtype, p.R = R, p.N = N, p.K = K, p.E = E;
+    return gemm_fp8_generic(p, (hipStream_t)stream);
+}
+
+int mfl_mlp_fwd_fp8(const void *x, int64_t src_rows, const int32_t *row_idx, int idx_div, const mfl_fp8_weight *gate,
+                    const mfl_fp8_weight *up, const mfl_fp8_weight *down, const void *m_sizes, int m_sizes_dtype, void *y,
+                    void *e_out, void *g_out, int64_t R, int I, int H, int E, int dtype, void *workspace, size_t ws_bytes,
+                    void *stream) {
+    int rc = check_call(m_sizes, m_sizes_dtype, R, I, H, E, dtype, dtype);
+    if (!rc) rc = check_source(src_rows, row_idx, idx_div, R);
+    if (rc) return rc;
+    if (R == 0) return MFL_OK;
+    if (!x || !y) return MFL_ERR_NULL;
+    rc = check_weight(gate);
+    if (!rc) rc = check_weight(up);
+    if (!rc) rc = check_weight(down);
+    if (rc) return rc;
+    const size_t size = dtype_size(dtype);
+    if (!aligned(x, size) || !aligned(y, size) || !aligned(e_out, size) || !aligned(g_out, size)) return MFL_ERR_ALIGN;
+    if ((e_out == nullptr) != (g_out == nullptr)) return MFL_ERR_NULL;
+    rc = check_workspace(MFL_FP8_MLP, src_rows, R, I, H, E, workspace, ws_bytes);
+    if (rc) return rc;
+    const int64_t used = source_rows(src_rows, row_idx, R);
+    const RowsRoom room((uint8_t *)workspace, used, H), hidden((uint8_t *)workspace + rows_bytes(src_rows, H), R, I);
+    void *const h = (uint8_t *)workspace + rows_bytes(src_rows, H) + rows_bytes(R, I);
+    rc = fp8_quant_rows(x, dtype, used, H, room.q, room.scale, (hipStream_t)stream);
+    if (rc) return rc;
+    Fp8Product p = {};
+    p.glu = true, p.terms = 1, p.a[0] = room.rows(), p.w[0] = matrix(gate), p.w[1] = matrix(up);
+    p.row_idx = row_idx, p.idx_div = idx_div, p.src_rows = used;
+    p.m_sizes = m_sizes, p.ms_i64 = m_sizes_dtype == MFL_I64;
+    p.out = h, p.e_out = e_out, p.g_out = g_out, p.out_dtype = MFL_F32, p.prod_dtype = dtype, p.R = R, p.N = I, p.K = H, p.E = E;
+    rc = gemm_fp8_generic(p, (hipStream_t)stream);
+    if (rc) return rc;
+    rc = fp8_quant_rows(h, MFL_F32, R, I, hidden.q, hidden.scale, (hipStream_t)stream);
+    if (rc) return rc;
+    p.glu = false, p.a[0] = hidden.rows(), p.w[0] = matrix(down), p.row_idx = nullptr, p.src_rows = R;
+    p.out = y, p.e_out = p.g_out = nullptr, p.out_dtype = dtype, p.N = H, p.K = I;
+    return gemm_fp8_generic(p, (hipStream_t)stream);
+}
+
+int mfl_fp8_quant_rows(const void *x, int dtype, int64_t R, int K, void *q, uint8_t *scale, void *stream) {
+    if (R < 0 || K <= 0) return MFL_ERR_SHAPE;
+    if (!dtype_ok(dtype)) return MFL_ERR_DTYPE;
+    if (R == 0) return MFL_OK;
+    if (!x || !q || !scale) return MFL_ERR_NULL;
+    if (!aligned(x, dtype_size(dtype)) || !aligned(q, 16)) return MFL_ERR_ALIGN;
+    return fp8_quant_rows(x, dtype, R, K, (uint8_t *)q, scale, (hipStream_t)stream);
+}
+
+int mfl_fp8_dequant_rows(const void *q, const uint8_t *scale, int64_t R, int K, void *out, int out_dtype, void *stream) {
+    if (R < 0 || K <= 0) return MFL_ERR_SHAPE;
+    if (!dtype_ok(out_dtype)) return MFL_ERR_DTYPE;
+    if (R == 0) return MFL_OK;
+    if (!q || !scale || !out) return MFL_ERR_NULL;
+    if (!aligned(out, dtype_size(out_dtype))) return MFL_ERR_ALIGN;
+    return fp8_dequant_rows((const uint8_t *)q, scale, R, K, out, out_dtype, (hipStream_t)stream);
+}
+
+int mfl_fp8_quant_blocks(const void *w, int dtype, int E, int N, int K, void *q, float *scale, void *stream) {
+    if (E <= 0 || N <= 0 || K <= 0) return MFL_ERR_SHAPE;
+    if (!dtype_ok(dtype)) return MFL_ERR_DTYPE;
+    if (!w || !q || !scale) return MFL_ERR_NULL;
+    if (!aligned(w, dtype_size(dtype)) || !aligned(scale, 4)) return MFL_ERR_ALIGN;
+    return fp8_quant_blocks(w, dtype, E, N, K, (uint8_t *)q, scale, (hipStream_t)stream);
+}
+
+int mfl_fp8_dequant_blocks(const void *q, const float *scale, int E, int N, int K, void *out, int out_dtype, void *stream) {
+    if (E <= 0 || N <= 0 || K <= 0) return MFL_ERR_SHAPE;
+    if (!dtype_ok(out_dtype)) return MFL_ERR_DTYPE;
+    if (!q || !scale || !out) return MFL_ERR_NULL;
+    if (!aligned(scale, 4) || !aligned(out, dtype_size(out_dtype))) return MFL_ERR_ALIGN;
+    return fp8_dequant_blocks((const uint8_t *)q, scale, E, N, K, out, out_dtype, (hipStream_t)stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,137 @@
+// Expert products in 8-bit floating point: internal interface between the C ABI (api_fp8.hip) and the kernel files, and
+// what the kernels share.
+//
+// Values are e4m3 (OCP: largest 448, no infinity, NaN 0x7f).  Rows (activations, gradients) carry one power-of-two scale per
+// row and 128 elements of the reduction, as a biased exponent byte; weights one fp32 scale per 128 x 128 block.  The scale
+// of a row block is the smallest power of two, at least 2^-117, that brings the block's largest finite magnitude to 448 or
+// below.  A power of two because then x / scale is exact: a value is rounded once, what it is rounded to does not depend on
+// how the division is done, and the matrix instruction applies the scale itself.  2^-117 because the smallest value of the
+// grid, 2^-9, is a normal float at that scale.  Elements that are no number or infinite become NaN and leave the block's
+// scale to the others.
+#pragma once
+#include "common.h"
+
+namespace mfl {
+
+constexpr int kFp8Block = 128;
+
+__host__ __device__ constexpr int fp8_blocks(int n) { return (n + kFp8Block - 1) / kFp8Block; }
+// Quantised rows lie `fp8_ld(K)` bytes apart, zeros behind the row's end, and their scales `fp8_ld_scale(K)` bytes apart (whole
+// dwords, which the kernels fetch four blocks at a time).
+__host__ __device__ constexpr int64_t fp8_ld(int K) { return (int64_t)fp8_blocks(K) * kFp8Block; }
+__host__ __device__ constexpr int64_t fp8_ld_scale(int K) { return (fp8_blocks(K) + 3) / 4 * 4; }
+
+struct Fp8Rows {
+    const uint8_t *q;
+    const uint8_t *scale;
+};
+struct Fp8Matrix {  // (E, out, in) with (E, ceil(out / 128), ceil(in / 128)) scales
+    const uint8_t *q;
+    const float *scale;
+};
+
+// One product over rows grouped by expert.  Forward: out (R, N) = a (., K) w^T, gathered rows where row_idx is given; gated
+// (glu): out = silu(a w[0]^T) * (a w[1]^T), the two products to e_out / g_out where given.  Input gradient (dx): out (R, K) =
+// a[0] (R, N) w[0], plus a[1] w[1] where terms is 2.
+struct Fp8Product {
+    bool dx, glu;
+    int terms;
+    Fp8Rows a[2];
+    Fp8Matrix w[2];
+    const int32_t *row_idx;
+    int idx_div;
+    int64_t src_rows;
+    const void *m_sizes;
+    int ms_i64;
+    void *out, *e_out, *g_out;
+    int out_dtype, prod_dtype;  // prod_dtype: of e_out and g_out
+    int64_t R;
+    int N, K, E;
+};
+
+// Any shape; MFL_OK or a launch error.
+int gemm_fp8_generic(const Fp8Product &p, hipStream_t stream);
+
+int fp8_quant_rows(const void *x, int dtype, int64_t R, int K, uint8_t *q, uint8_t *scale, hipStream_t stream);
+int fp8_dequant_rows(const uint8_t *q, const uint8_t *scale, int64_t R, int K, void *out, int out_dtype, hipStream_t stream);
+// The gated unit's backward, de and dg straight to quantised rows.
+int fp8_silu_bwd_quant(const void *dh, const void *e, const void *g, int dtype, int64_t R, int N, uint8_t *de_q,
+                       uint8_t *de_scale, uint8_t *dg_q, uint8_t *dg_scale, hipStream_t stream);
+int fp8_quant_blocks(const void *w, int dtype, int E, int N, int K, uint8_t *q, float *scale, hipStream_t stream);
+int fp8_dequant_blocks(const uint8_t *q, const float *scale, int E, int N, int K, void *out, int out_dtype, hipStream_t stream);
+
+typedef __attribute__((ext_vector_type(8))) int intx8;
+
+// Biased exponent byte of the scale for a block whose largest finite magnitude is amax: amax = f 2^p with 1 <= f < 2 fits
+// 448 2^e = 1.75 2^(8 + e) with e = p - 8 if f <= 1.75, else p - 7.  (amax 0 or subnormal: the least exponent.)
+__device__ __forceinline__ int fp8_scale_byte(float amax) {
+    const uint32_t b = __float_as_uint(amax);
+    const int byte = (int)(b >> 23) - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return byte < 10 ? 10 : byte;
+}
+__device__ __forceinline__ float fp8_scale_of(int byte) { return __uint_as_float((uint32_t)byte << 23); }
+__device__ __forceinline__ float fp8_inverse_of(int byte) { return __uint_as_float((uint32_t)(254 - byte) << 23); }
+
+// |v|, or 0 where v is infinite or no number
+__device__ __forceinline__ float fp8_finite_abs(float v) {
+    const float a = __builtin_fabsf(v);
+    return a <= 3.4028234663852886e38f ? a : 0.0f;
+}
+
+// Four values times a power of two, rounded to e4m3 (nearest, ties to even): one dword.
+__device__ __forceinline__ float fp8_ready(float v, float inverse) {
+    const float a = __builtin_fabsf(v);
+    return a <= 3.4028234663852886e38f ? v * inverse : __uint_as_float(0x7fc00000u);
+}
+__device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d, float inverse) {
+    int r = 0;
+    r = __builtin_amdgcn_cvt_pk_fp8_f32(fp8_ready(a, inverse), fp8_ready(b, inverse), r, false);
+    r = __builtin_amdgcn_cvt_pk_fp8_f32(fp8_ready(c, inverse), fp8_ready(d, inverse), r, true);
+    return (uint32_t)r;
+}
+
+// The largest of a row of 16 lanes, in all of them.
+template <int CTRL>
+__device__ __forceinline__ float fp8_dpp_max(float x) {
+    return __builtin_fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true)));
+}
+__device__ __forceinline__ float fp8_max16(float x) {
+    x = fp8_dpp_max<0x128>(x);  // row_ror 8, 4, 2, 1
+    x = fp8_dpp_max<0x124>(x);
+    x = fp8_dpp_max<0x122>(x);
+    return fp8_dpp_max<0x121>(x);
+}
+
+// Where tile `slot` of the row tiles of BM rows lies: every wave scans the row counts, 64 experts at a time.  Sizes that sum to
+// more than R rows are cut at R, negative ones count as none.  False past the last tile.
+template <int BM>
+__device__ __forceinline__ bool fp8_find_tile(const void *m_sizes, int ms_i64, int E, int64_t R, int slot, int lane, int &expert,
+                                              int64_t &row0, int &rows) {
+    int tiles_before = 0;
+    int64_t rows_before = 0;
+    for (int e0 = 0; e0 < E; e0 += 64) {
+        const int e = e0 + lane;
+        int m = e < E ? load_msize(m_sizes, ms_i64, e) : 0;
+        if (m < 0) m = 0;
+        const int t = ceil_div(m, BM);
+        const int mi = wave_inclusive_scan(m), ti = wave_inclusive_scan(t);
+        const uint64_t past = __ballot(tiles_before + ti > slot);
+        if (past) {
+            const int src = __ffsll((unsigned long long)past) - 1;
+            const int m_e = __builtin_amdgcn_readlane(m, src);
+            const int tile = slot - (tiles_before + __builtin_amdgcn_readlane(ti, src) - __builtin_amdgcn_readlane(t, src));
+            expert = e0 + src;
+            row0 = rows_before + __builtin_amdgcn_readlane(mi, src) - m_e + (int64_t)tile * BM;
+            rows = m_e - tile * BM < BM ? m_e - tile * BM : BM;
+            if (row0 + rows > R) rows = (int)(R - row0);
+            return rows > 0;
+        }
+        rows_before += wave_last(mi);
+        tiles_before += wave_last(ti);
+    }
+    return false;
+}
+// Row tiles that a launch has to provide for (the sizes are known on the device only).
+inline int64_t fp8_max_tiles(int64_t R, int E, int bm) { return R / bm + (R < E ? R : E); }
+
+}  // namespace mfl

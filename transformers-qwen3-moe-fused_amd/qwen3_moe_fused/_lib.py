@@ -6,6 +6,7 @@ the first call raises, it never silently computes on another path.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from typing import Optional
@@ -36,6 +37,15 @@ class Nf4Weight(ctypes.Structure):
 
 
 _nf4p = ctypes.POINTER(Nf4Weight)
+
+
+class Fp8Weight(ctypes.Structure):
+    """``mfl_fp8_weight``: e4m3 values and fp32 scales per 128 x 128 block, as device pointers."""
+
+    _fields_ = [("q", _vp), ("scale", _vp)]
+
+
+_fp8p = ctypes.POINTER(Fp8Weight)
 
 
 class MoeBlock(ctypes.Structure):
@@ -112,6 +122,17 @@ _SIGNATURES = {
     "mfl_rows_dot": (_i, [_vp, _vp, _vp, _vp, _i64, _i, _i, _i, _vp]),
     "mfl_silu_mul_fwd": (_i, [_vp, _vp, _vp, _i64, _i, _vp]),
     "mfl_silu_mul_bwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i, _vp]),
+    "mfl_fp8_workspace": (_sz, [_i, _i64, _i64, _i, _i, _i]),
+    "mfl_gemm_fwd_fp8": (_i, [_vp, _i64, _vp, _i, _fp8p, _vp, _i, _vp, _i64, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
+    "mfl_gemm_dx_fp8": (_i, [_vp, _fp8p, _vp, _i, _vp, _i64, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
+    "mfl_glu_fwd_fp8": (_i, [_vp, _i64, _vp, _i, _fp8p, _fp8p, _vp, _i, _vp, _vp, _vp, _i64, _i, _i, _i, _i, _vp, _sz, _vp]),
+    "mfl_glu_bwd_fp8": (_i, [_vp, _vp, _vp, _fp8p, _fp8p, _vp, _i, _vp, _i64, _i, _i, _i, _i, _vp, _sz, _vp]),
+    "mfl_mlp_fwd_fp8": (_i, [_vp, _i64, _vp, _i, _fp8p, _fp8p, _fp8p, _vp, _i, _vp, _vp, _vp, _i64, _i, _i, _i, _i, _vp, _sz,
+                             _vp]),
+    "mfl_fp8_quant_rows": (_i, [_vp, _i, _i64, _i, _vp, _vp, _vp]),
+    "mfl_fp8_dequant_rows": (_i, [_vp, _vp, _i64, _i, _vp, _i, _vp]),
+    "mfl_fp8_quant_blocks": (_i, [_vp, _i, _i, _i, _i, _vp, _vp, _vp]),
+    "mfl_fp8_dequant_blocks": (_i, [_vp, _vp, _i, _i, _i, _vp, _i, _vp]),
     "mfl_moe_block_workspace": (_sz, [_blockp]),
     "mfl_moe_block_fwd": (_i, [_blockp, _vp, _vp, _sz, _vp]),
     "mfl_moe_block_bwd_workspace": (_sz, [_blockp]),
@@ -180,6 +201,17 @@ def stream() -> int:
     if _raw_stream is None or _device is None:
         return torch.cuda.current_stream().cuda_stream
     return _raw_stream(_device())
+
+
+_here = contextlib.nullcontext()
+
+
+def on_device_of(t: torch.Tensor):
+    """A context in which ``t``'s device is the current one, whose current stream ``stream()`` then is."""
+    index = t.device.index
+    if index is None or (torch.cuda.current_device() if _device is None else _device()) == index:
+        return _here
+    return torch.cuda.device(index)
 
 
 # (bound once: the questions are asked in every call, and in a backward pass on another core than the forward's)

@@ -20,6 +20,8 @@ def get_lora_parameters(proj: nn.Module) -> tuple[torch.Tensor, Optional[Any], t
         raise NotImplementedError("fast LoRA needs the adapter enabled and unmerged")
     base = getattr(proj, "base_layer", proj)
     weight = base.weight
+    if weight.dtype == torch.float8_e4m3fn:
+        raise NotImplementedError("fast LoRA does not take 8-bit floating-point base weights: use the block's own forward")
     active = getattr(proj, "active_adapters", None)
     if active is None:
         name = getattr(proj, "active_adapter", "default")

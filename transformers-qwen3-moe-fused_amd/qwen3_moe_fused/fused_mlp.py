@@ -16,8 +16,10 @@ import torch
 from . import _lib
 from .grouped_gemm.backward_dw import grouped_gemm_backward_dw
 from .grouped_gemm.forward import grouped_gemm_forward
+from .grouped_gemm.forward_fp8 import grouped_gemm_forward_transposed_fp8
 from .grouped_gemm.fused import (grouped_gemm_forward_transposed_dual, grouped_gemm_forward_transposed_silu_bwd,
-                                 grouped_glu_forward, grouped_glu_forward_4bit)
+                                 grouped_glu_backward_fp8, grouped_glu_forward, grouped_glu_forward_4bit,
+                                 grouped_glu_forward_fp8, grouped_mlp_forward_fp8)
 from .kernels.routing import _combine, _gather, _scatter
 from .kernels.silu_mul import silu_mul_backward
 from .grouped_gemm.forward_4bit import UNSUPPORTED, check_packed, grouped_gemm_forward_transposed_4bit
@@ -144,6 +146,75 @@ def moe_fused_glu_4bit(tokens: torch.Tensor, gate_weight: torch.Tensor, up_weigh
     assert not gate_weight.requires_grad and not up_weight.requires_grad
     return _GluGathered4bit.apply(tokens, gate_weight.data, gate_weight.quant_state, up_weight.data,
                                   up_weight.quant_state, m_sizes, sort_idx, inv_sort_idx, num_selected)
+
+
+class _GluGatheredFp8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, tokens, w_gate, gate_scale, w_up, up_scale, m_sizes, sort_idx, inv_sort_idx, k):
+        h, e, g = grouped_glu_forward_fp8(tokens, w_gate, gate_scale, w_up, up_scale, m_sizes, sort_idx, k,
+                                          return_products=True)
+        ctx.save_for_backward(w_gate, gate_scale, w_up, up_scale, m_sizes, inv_sort_idx, e, g)
+        ctx.k, ctx.n_tokens = k, tokens.shape[0]
+        return h
+
+    @staticmethod
+    def backward(ctx, dh):
+        w_gate, gate_scale, w_up, up_scale, m_sizes, inv_sort_idx, e, g = ctx.saved_tensors
+        dx = grouped_glu_backward_fp8(dh.contiguous(), e, g, w_gate, gate_scale, w_up, up_scale, m_sizes)
+        with _lib.on_device_of(dx):
+            return _combine(dx, inv_sort_idx, None, ctx.n_tokens, ctx.k), *(None,) * 8
+
+
+def _check_routing(tokens, sort_idx, inv_sort_idx, k):
+    for idx in (sort_idx, inv_sort_idx):
+        assert idx.dtype == torch.int32 and idx.shape == (tokens.shape[0] * k,) and idx.is_contiguous()
+        assert idx.device == tokens.device
+
+
+def moe_fused_glu_fp8(tokens: torch.Tensor, w_gate: torch.Tensor, gate_scale: torch.Tensor, w_up: torch.Tensor,
+                      up_scale: torch.Tensor, m_sizes: torch.Tensor, sort_idx: torch.Tensor, inv_sort_idx: torch.Tensor,
+                      num_selected: int) -> torch.Tensor:
+    """``moe_fused_glu`` on weights in 8-bit floating point with their block scales (frozen), in bf16, fp16 or fp32.
+    Differentiable in ``tokens``; the gradients of the two products are quantised like the forward's rows."""
+    assert not any(t.requires_grad for t in (w_gate, gate_scale, w_up, up_scale)), "8-bit expert weights are frozen"
+    _check_routing(tokens, sort_idx, inv_sort_idx, num_selected)
+    if not (torch.is_grad_enabled() and tokens.requires_grad):
+        return grouped_glu_forward_fp8(tokens, w_gate, gate_scale, w_up, up_scale, m_sizes, sort_idx, num_selected)
+    return _GluGatheredFp8.apply(tokens, w_gate, gate_scale, w_up, up_scale, m_sizes, sort_idx, inv_sort_idx, num_selected)
+
+
+class _MlpGatheredFp8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, tokens, w_gate, gate_scale, w_up, up_scale, w_down, down_scale, m_sizes, sort_idx, inv_sort_idx, k):
+        y, e, g = grouped_mlp_forward_fp8(tokens, w_gate, gate_scale, w_up, up_scale, w_down, down_scale, m_sizes, sort_idx, k,
+                                          return_products=True)
+        ctx.save_for_backward(w_gate, gate_scale, w_up, up_scale, w_down, down_scale, m_sizes, inv_sort_idx, e, g)
+        ctx.k, ctx.n_tokens = k, tokens.shape[0]
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        w_gate, gate_scale, w_up, up_scale, w_down, down_scale, m_sizes, inv_sort_idx, e, g = ctx.saved_tensors
+        dh = grouped_gemm_forward_transposed_fp8(dy.contiguous(), w_down, down_scale, m_sizes)
+        dx = grouped_glu_backward_fp8(dh, e, g, w_gate, gate_scale, w_up, up_scale, m_sizes)
+        with _lib.on_device_of(dx):
+            return _combine(dx, inv_sort_idx, None, ctx.n_tokens, ctx.k), *(None,) * 10
+
+
+def moe_fused_mlp_fp8(tokens: torch.Tensor, w_gate: torch.Tensor, gate_scale: torch.Tensor, w_up: torch.Tensor,
+                      up_scale: torch.Tensor, w_down: torch.Tensor, down_scale: torch.Tensor, m_sizes: torch.Tensor,
+                      sort_idx: torch.Tensor, inv_sort_idx: torch.Tensor, num_selected: int) -> torch.Tensor:
+    """``moe_fused_mlp`` on weights in 8-bit floating point with their block scales (frozen), in bf16, fp16 or fp32: between
+    the gated unit and the down projection there are only quantised rows, made from the unit's fp32 values.  Differentiable
+    in ``tokens``."""
+    assert not any(t.requires_grad for t in (w_gate, gate_scale, w_up, up_scale, w_down, down_scale)), \
+        "8-bit expert weights are frozen"
+    _check_routing(tokens, sort_idx, inv_sort_idx, num_selected)
+    if not (torch.is_grad_enabled() and tokens.requires_grad):
+        return grouped_mlp_forward_fp8(tokens, w_gate, gate_scale, w_up, up_scale, w_down, down_scale, m_sizes, sort_idx,
+                                       num_selected)
+    return _MlpGatheredFp8.apply(tokens, w_gate, gate_scale, w_up, up_scale, w_down, down_scale, m_sizes, sort_idx,
+                                 inv_sort_idx, num_selected)
 
 
 class _MoeBlock(torch.autograd.Function):

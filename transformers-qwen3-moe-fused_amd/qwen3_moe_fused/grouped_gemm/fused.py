@@ -26,7 +26,9 @@ from ..kernels.silu_mul import silu_mul_forward
 from ..quantize.nf4 import packed_weight, resolve_absmax
 from ._common import check_operands, is_int_tensor
 from .forward import grouped_gemm_forward
+from ..quantize.fp8 import check_fp8_weight
 from .forward_4bit import UNSUPPORTED, check_packed, grouped_gemm_forward_4bit
+from .forward_fp8 import GLU, GLU_BWD, MLP, check_rows, fp8_weight, fp8_workspace
 
 
 def _gather(x_src: torch.Tensor, row_idx: torch.Tensor, idx_div: int) -> torch.Tensor:
@@ -411,3 +413,73 @@ def grouped_glu_forward_lora(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.
         return silu_mul_forward(e, g), e, g
     _lib.check(rc, "mfl_glu_fwd_lora")
     return h, e, g
+
+
+def grouped_glu_forward_fp8(x: torch.Tensor, w_gate: torch.Tensor, gate_scale: torch.Tensor, w_up: torch.Tensor,
+                            up_scale: torch.Tensor, m_sizes: torch.Tensor, row_idx: Optional[torch.Tensor] = None,
+                            idx_div: int = 1, return_products: bool = False):
+    """``grouped_glu_forward`` with gate and up weights in 8-bit floating point (``grouped_gemm_forward_fp8``'s form), in
+    bf16, fp16 or fp32: every row of ``x`` is quantised once, the gated unit takes the fp32 sums.  ``h``, or ``(h, e, g)``
+    with ``return_products``, each rounded once."""
+    check_rows(m_sizes, x)
+    rows = _check_gather(x, row_idx, idx_div)
+    experts, n, k = check_fp8_weight(x, w_gate, gate_scale)
+    assert check_fp8_weight(x, w_up, up_scale) == (experts, n, k) and x.shape[1] == k and m_sizes.numel() == experts
+    assert rows == 0 or x.shape[0] > 0
+    with _lib.on_device_of(x):
+        h = torch.empty((rows, n), device=x.device, dtype=x.dtype)
+        e = torch.empty_like(h) if return_products else None
+        g = torch.empty_like(h) if return_products else None
+        ms = _lib.as_index_tensor(m_sizes)
+        _keep, ws, ws_bytes = fp8_workspace(GLU, x, x.shape[0], rows, n, k, experts)
+        rc = _lib.lib().mfl_glu_fwd_fp8(x.data_ptr(), x.shape[0], _lib.ptr(row_idx), idx_div, fp8_weight(w_gate, gate_scale),
+                                        fp8_weight(w_up, up_scale), ms.data_ptr(), _lib.itype_code(ms.dtype), h.data_ptr(),
+                                        _lib.ptr(e), _lib.ptr(g), rows, n, k, experts, _lib.dtype_code(x.dtype), ws, ws_bytes,
+                                        _lib.stream())
+    _lib.check(rc, "mfl_glu_fwd_fp8")
+    return (h, e, g) if return_products else h
+
+
+def grouped_glu_backward_fp8(dh: torch.Tensor, e: torch.Tensor, g: torch.Tensor, w_gate: torch.Tensor,
+                             gate_scale: torch.Tensor, w_up: torch.Tensor, up_scale: torch.Tensor,
+                             m_sizes: torch.Tensor) -> torch.Tensor:
+    """Gradient of ``grouped_glu_forward_fp8`` with respect to its (gathered) rows, from the gradient of ``h`` and the two
+    products: ``de @ w_gate + dg @ w_up`` with ``de``, ``dg`` computed in fp32 and quantised along their columns."""
+    check_rows(m_sizes, dh, e, g)
+    rows, n = dh.shape
+    experts, n_w, k = check_fp8_weight(dh, w_gate, gate_scale)
+    assert check_fp8_weight(dh, w_up, up_scale) == (experts, n, k) and n_w == n and m_sizes.numel() == experts
+    with _lib.on_device_of(dh):
+        dx = torch.empty((rows, k), device=dh.device, dtype=dh.dtype)
+        ms = _lib.as_index_tensor(m_sizes)
+        _keep, ws, ws_bytes = fp8_workspace(GLU_BWD, dh, rows, rows, n, k, experts)
+        rc = _lib.lib().mfl_glu_bwd_fp8(dh.data_ptr(), e.data_ptr(), g.data_ptr(), fp8_weight(w_gate, gate_scale),
+                                        fp8_weight(w_up, up_scale), ms.data_ptr(), _lib.itype_code(ms.dtype), dx.data_ptr(),
+                                        rows, n, k, experts, _lib.dtype_code(dh.dtype), ws, ws_bytes, _lib.stream())
+    _lib.check(rc, "mfl_glu_bwd_fp8")
+    return dx
+
+
+def grouped_mlp_forward_fp8(x: torch.Tensor, w_gate: torch.Tensor, gate_scale: torch.Tensor, w_up: torch.Tensor,
+                            up_scale: torch.Tensor, w_down: torch.Tensor, down_scale: torch.Tensor, m_sizes: torch.Tensor,
+                            row_idx: Optional[torch.Tensor] = None, idx_div: int = 1, return_products: bool = False):
+    """The gated unit followed by the down projection (``w_down`` (E, hidden, intermediate)); the unit's result goes from its
+    fp32 values to quantised rows.  ``y``, or ``(y, e, g)`` with ``return_products``."""
+    check_rows(m_sizes, x)
+    rows = _check_gather(x, row_idx, idx_div)
+    experts, n, k = check_fp8_weight(x, w_gate, gate_scale)
+    assert check_fp8_weight(x, w_up, up_scale) == (experts, n, k) and check_fp8_weight(x, w_down, down_scale) == (experts, k, n)
+    assert x.shape[1] == k and m_sizes.numel() == experts
+    assert rows == 0 or x.shape[0] > 0
+    with _lib.on_device_of(x):
+        y = torch.empty((rows, k), device=x.device, dtype=x.dtype)
+        e = torch.empty((rows, n), device=x.device, dtype=x.dtype) if return_products else None
+        g = torch.empty_like(e) if return_products else None
+        ms = _lib.as_index_tensor(m_sizes)
+        _keep, ws, ws_bytes = fp8_workspace(MLP, x, x.shape[0], rows, n, k, experts)
+        rc = _lib.lib().mfl_mlp_fwd_fp8(x.data_ptr(), x.shape[0], _lib.ptr(row_idx), idx_div, fp8_weight(w_gate, gate_scale),
+                                        fp8_weight(w_up, up_scale), fp8_weight(w_down, down_scale), ms.data_ptr(),
+                                        _lib.itype_code(ms.dtype), y.data_ptr(), _lib.ptr(e), _lib.ptr(g), rows, n, k, experts,
+                                        _lib.dtype_code(x.dtype), ws, ws_bytes, _lib.stream())
+    _lib.check(rc, "mfl_mlp_fwd_fp8")
+    return (y, e, g) if return_products else y

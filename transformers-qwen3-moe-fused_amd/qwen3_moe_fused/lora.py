@@ -80,7 +80,8 @@ except ImportError:
 
         def _move_adapter_to_device_of_base_layer(self, adapter_name: str) -> None:
             weight = self.base_layer.weight
-            dtype = weight.dtype if weight.dtype.is_floating_point else None
+            # (packed and 8-bit floating-point base weights leave the adapter in its own type)
+            dtype = weight.dtype if weight.dtype.is_floating_point and weight.dtype.itemsize > 1 else None
             self.lora_A[adapter_name].to(device=weight.device, dtype=dtype)
             self.lora_B[adapter_name].to(device=weight.device, dtype=dtype)
 

@@ -109,10 +109,14 @@ class Qwen3MoeFusedSparseMoeBlock(nn.Module):
     keep_routing = False
 
     def _fused_front(self, tokens, m_sizes, sort_idx, inv_sort_idx) -> Optional[torch.Tensor]:
-        from .fused_mlp import moe_fused_glu, moe_fused_glu_4bit
+        from .fused_mlp import moe_fused_glu, moe_fused_glu_4bit, moe_fused_glu_fp8
         from .quantize.layer import MoeFusedLinear4bit
+        from .quantize.layer_fp8 import MoeFusedLinearFp8
 
         gate, up = self.gate_proj, self.up_proj
+        if type(gate) is MoeFusedLinearFp8 and type(up) is MoeFusedLinearFp8:
+            return moe_fused_glu_fp8(tokens, gate.weight, gate.weight_scale_inv, up.weight, up.weight_scale_inv, m_sizes,
+                                     sort_idx, inv_sort_idx, self.num_selected)
         if tokens.dtype != torch.bfloat16 or type(gate) is not type(up):
             return None
         if type(gate) is MoeFusedLinear:
@@ -131,9 +135,19 @@ class Qwen3MoeFusedSparseMoeBlock(nn.Module):
         """The three projections as one node of the graph when all are plain bf16 expert matrices and a gradient
         will be asked for: the backward then runs the gated unit's backward inside the down projection's input
         gradient.  Without gradients the front half and the down projection are the same two launches anyway."""
-        from .fused_mlp import moe_fused_mlp
+        from .fused_mlp import moe_fused_mlp, moe_fused_mlp_fp8
+        from .quantize.layer_fp8 import MoeFusedLinearFp8
 
         projs = (self.gate_proj, self.up_proj, self.down_proj)
+        if all(type(p) is MoeFusedLinearFp8 for p in projs):
+            # 8-bit floating point: with the down projection in the call the gated unit's result is written in 8 bits only
+            down = projs[2]
+            if (down._forward_hooks or down._forward_pre_hooks or down._backward_hooks or down._backward_pre_hooks
+                    or "forward" in down.__dict__ or MoeFusedLinearFp8.forward is not MoeFusedLinearFp8._own_forward
+                    or torch.nn.modules.module._has_any_global_hook()):
+                return None
+            weights = [t for p in projs for t in (p.weight, p.weight_scale_inv)]
+            return moe_fused_mlp_fp8(tokens, *weights, m_sizes, sort_idx, inv_sort_idx, self.num_selected)
         if not self.fuse_backward or tokens.dtype != torch.bfloat16 or not torch.is_grad_enabled():
             return None
         if any(type(p) is not MoeFusedLinear or p.weight.dtype != torch.bfloat16 for p in projs):

@@ -24,6 +24,7 @@ from torch import nn
 
 from ..modular_qwen3_moe_fused import MoeFusedLinear
 from .layer import MoeFusedLinear4bit
+from .layer_fp8 import MoeFusedLinearFp8
 
 try:  # pragma: no cover - depends on the environment
     from bitsandbytes.nn import Linear4bit
@@ -49,7 +50,7 @@ def _replace(model: nn.Module, modules_to_not_convert: list[str], path: list[str
     for name, module in model.named_children():
         path.append(name)
         is_linear = isinstance(module, nn.Linear) or (Conv1D != () and isinstance(module, Conv1D))
-        if isinstance(module, MoeFusedLinear) and not isinstance(module, MoeFusedLinear4bit):
+        if isinstance(module, MoeFusedLinear) and not isinstance(module, (MoeFusedLinear4bit, MoeFusedLinearFp8)):
             if not _skipped(name, ".".join(path), modules_to_not_convert):
                 new = MoeFusedLinear4bit(module.in_features, module.out_features, module.num_experts,
                                          compute_dtype=config.bnb_4bit_compute_dtype,
