@@ -45,6 +45,11 @@ Fp8Matrix matrix(const mfl_fp8_weight *w) { return {(const uint8_t *)w->q, w->sc
 // the rows of the left operand that a product reads
 int64_t source_rows(int64_t src_rows, const int32_t *row_idx, int64_t R) { return row_idx != nullptr ? src_rows : R; }
 
+int run_product(const Fp8Product &p, hipStream_t stream) {
+    const int rc = gemm_fp8_tile(p, stream);
+    return rc != MFL_ERR_UNSUPPORTED ? rc : gemm_fp8_generic(p, stream);
+}
+
 }  // namespace
 
 extern "C" {
@@ -88,7 +93,7 @@ int mfl_gemm_fwd_fp8(const void *x, int64_t src_rows, const int32_t *row_idx, in
     p.row_idx = row_idx, p.idx_div = idx_div, p.src_rows = used;
     p.m_sizes = m_sizes, p.ms_i64 = m_sizes_dtype == MFL_I64;
     p.out = y, p.out_dtype = out_dtype, p.R = R, p.N = N, p.K = K, p.E = E;
-    return gemm_fp8_generic(p, (hipStream_t)stream);
+    return run_product(p, (hipStream_t)stream);
 }
 
 int mfl_gemm_dx_fp8(const void *dy, const mfl_fp8_weight *w, const void *m_sizes, int m_sizes_dtype, void *dx, int64_t R, int N,
@@ -109,7 +114,7 @@ int mfl_gemm_dx_fp8(const void *dy, const mfl_fp8_weight *w, const void *m_sizes
     p.dx = true, p.terms = 1, p.a[0] = room.rows(), p.w[0] = matrix(w);
     p.m_sizes = m_sizes, p.ms_i64 = m_sizes_dtype == MFL_I64;
     p.out = dx, p.out_dtype = out_dtype, p.R = R, p.N = N, p.K = K, p.E = E;
-    return gemm_fp8_generic(p, (hipStream_t)stream);
+    return run_product(p, (hipStream_t)stream);
 }
 
 int mfl_glu_fwd_fp8(const void *x, int64_t src_rows, const int32_t *row_idx, int idx_div, const mfl_fp8_weight *gate,
@@ -135,8 +140,8 @@ int mfl_glu_fwd_fp8(const void *x, int64_t src_rows, const int32_t *row_idx, int
     p.glu = true, p.terms = 1, p.a[0] = room.rows(), p.w[0] = matrix(gate), p.w[1] = matrix(up);
     p.row_idx = row_idx, p.idx_div = idx_div, p.src_rows = used;
     p.m_sizes = m_sizes, p.ms_i64 = m_sizes_dtype == MFL_I64;
-    p.out = h, p.e_out = e_out, p.g_out = g_out, p.out_dtype = p.prod_dtype = dtype, p.R = R, p.N = N, p.K = K, p.E = E;
-    return gemm_fp8_generic(p, (hipStream_t)stream);
+    p.out = h, p.e_out = e_out, p.g_out = g_out, p.out_dtype = dtype, p.R = R, p.N = N, p.K = K, p.E = E;
+    return run_product(p, (hipStream_t)stream);
 }
 
 int mfl_glu_bwd_fp8(const void *dh, const void *e, const void *g, const mfl_fp8_weight *gate, const mfl_fp8_weight *up,
@@ -160,7 +165,7 @@ int mfl_glu_bwd_fp8(const void *dh, const void *e, const void *g, const mfl_fp8_
     p.dx = true, p.terms = 2, p.a[0] = de.rows(), p.a[1] = dg.rows(), p.w[0] = matrix(gate), p.w[1] = matrix(up);
     p.m_sizes = m_sizes, p.ms_i64 = m_sizes_dtype == MFL_I64;
     p.out = dx, p.out_dtype = dtype, p.R = R, p.N = N, p.K = K, p.E = E;
-    return gemm_fp8_generic(p, (hipStream_t)stream);
+    return run_product(p, (hipStream_t)stream);
 }
 
 int mfl_mlp_fwd_fp8(const void *x, int64_t src_rows, const int32_t *row_idx, int idx_div, const mfl_fp8_weight *gate,
@@ -190,14 +195,20 @@ int mfl_mlp_fwd_fp8(const void *x, int64_t src_rows, const int32_t *row_idx, int
     p.glu = true, p.terms = 1, p.a[0] = room.rows(), p.w[0] = matrix(gate), p.w[1] = matrix(up);
     p.row_idx = row_idx, p.idx_div = idx_div, p.src_rows = used;
     p.m_sizes = m_sizes, p.ms_i64 = m_sizes_dtype == MFL_I64;
-    p.out = h, p.e_out = e_out, p.g_out = g_out, p.out_dtype = MFL_F32, p.prod_dtype = dtype, p.R = R, p.N = I, p.K = H, p.E = E;
-    rc = gemm_fp8_generic(p, (hipStream_t)stream);
+    p.e_out = e_out, p.g_out = g_out, p.out_dtype = dtype, p.R = R, p.N = I, p.K = H, p.E = E;
+    p.hq = hidden.q, p.hq_scale = hidden.scale;
+    rc = gemm_fp8_tile(p, (hipStream_t)stream);
+    if (rc == MFL_ERR_UNSUPPORTED) {
+        // the kernel for any shape leaves fp32 values
+        p.hq = p.hq_scale = nullptr, p.h32 = (float *)h;
+        rc = gemm_fp8_generic(p, (hipStream_t)stream);
+        if (!rc) rc = fp8_quant_rows(h, MFL_F32, R, I, hidden.q, hidden.scale, (hipStream_t)stream);
+    }
     if (rc) return rc;
-    rc = fp8_quant_rows(h, MFL_F32, R, I, hidden.q, hidden.scale, (hipStream_t)stream);
-    if (rc) return rc;
+    p.hq = p.hq_scale = nullptr, p.h32 = nullptr;
     p.glu = false, p.a[0] = hidden.rows(), p.w[0] = matrix(down), p.row_idx = nullptr, p.src_rows = R;
     p.out = y, p.e_out = p.g_out = nullptr, p.out_dtype = dtype, p.N = H, p.K = I;
-    return gemm_fp8_generic(p, (hipStream_t)stream);
+    return run_product(p, (hipStream_t)stream);
 }
 
 int mfl_fp8_quant_rows(const void *x, int dtype, int64_t R, int K, void *q, uint8_t *scale, void *stream) {

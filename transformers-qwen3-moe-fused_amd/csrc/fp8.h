@@ -44,11 +44,15 @@ struct Fp8Product {
     const void *m_sizes;
     int ms_i64;
     void *out, *e_out, *g_out;
-    int out_dtype, prod_dtype;  // prod_dtype: of e_out and g_out
+    int out_dtype;
+    uint8_t *hq, *hq_scale;  // (glu) where given, `out` is not written but quantised rows, made from the fp32 values
+    float *h32;              // (glu, any-shape kernel) where given, `out` is not written but these fp32 values
     int64_t R;
     int N, K, E;
 };
 
+// Tiles in LDS, 16-bit outputs, K % 16 == 0; MFL_ERR_UNSUPPORTED for the rest.
+int gemm_fp8_tile(const Fp8Product &p, hipStream_t stream);
 // Any shape; MFL_OK or a launch error.
 int gemm_fp8_generic(const Fp8Product &p, hipStream_t stream);
 

@@ -38,15 +38,6 @@ __device__ __forceinline__ void store16(uint8_t *dst, const uint4_t v) {
     *(bf16x8 *)dst = out[0], *(bf16x8 *)(dst + 16) = out[1];
 }
 
-__device__ __forceinline__ void store_as(void *out, int dtype, int64_t at, float v) {
-    if (dtype == MFL_F32)
-        ((float *)out)[at] = v;
-    else if (dtype == MFL_BF16)
-        ((bf16_t *)out)[at] = from_f32<bf16_t>(v);
-    else
-        ((f16_t *)out)[at] = from_f32<f16_t>(v);
-}
-
 template <bool DX, bool GLU, typename TO>
 __global__ __launch_bounds__(256) void fp8_generic_kernel(Fp8Product p) {
     constexpr int CB = GLU ? 2 : 1;
@@ -164,9 +155,13 @@ __global__ __launch_bounds__(256) void fp8_generic_kernel(Fp8Product p) {
         if (n >= cols) continue;
         if (GLU) {
             const float ev = acc[0][i], gv = acc[CB - 1][i];
-            ((TO *)p.out)[at + n] = from_f32<TO>(ev * sigmoid_f32(ev) * gv);
-            if (p.e_out != nullptr) store_as(p.e_out, p.prod_dtype, at + n, ev);
-            if (p.g_out != nullptr) store_as(p.g_out, p.prod_dtype, at + n, gv);
+            const float h = ev * sigmoid_f32(ev) * gv;
+            if (p.h32 != nullptr)
+                p.h32[at + n] = h;
+            else
+                ((TO *)p.out)[at + n] = from_f32<TO>(h);
+            if (p.e_out != nullptr) ((TO *)p.e_out)[at + n] = from_f32<TO>(ev);
+            if (p.g_out != nullptr) ((TO *)p.g_out)[at + n] = from_f32<TO>(gv);
         } else {
             ((TO *)p.out)[at + n] = from_f32<TO>(acc[0][i]);
         }
