@@ -23,6 +23,8 @@
 // instruction does not matter as long as both operands agree.  Input gradient: the weights lie as in memory, 128 rows of the
 // reduction by BN columns, chunk c of row n at c ^ ((n & 7) << 1), and are read with ds_read_b64_tr_b8 (a group of 16 lanes
 // reads 8 rows of 16 bytes and gets 8 rows of one column each), four of them for the same 32 elements.
+#include <type_traits>
+
 #include "fp8.h"
 
 namespace mfl {
@@ -32,6 +34,9 @@ namespace {
 typedef __attribute__((address_space(3))) void *lds_void_ptr;
 typedef __attribute__((ext_vector_type(2))) int intx2;
 typedef __attribute__((address_space(3))) intx2 *lds_intx2_ptr;
+typedef const __attribute__((address_space(3))) uint4_t *lds_uint4_ptr;
+typedef const __attribute__((address_space(3))) uint32_t *lds_uint32_ptr;
+typedef const __attribute__((address_space(3))) float *lds_float_ptr;
 
 constexpr int kXcd = 8;
 constexpr int kMaxExperts = 512;  // prefix tables in LDS
@@ -258,26 +263,42 @@ __global__ __launch_bounds__(kThreads) void fp8_tile_kernel(Fp8Product p) {
     // ---- the consumer's side
     // (a wave's row blocks are dealt in turn, so that a tile of few blocks keeps all rows of waves at work)
     const int acol0 = GLU ? wn * 32 : wn * NI * 32;
+    static_assert(32 % S::kSLanes == 0 || S::kSLanes % 32 == 0, "a row block's scales: whole regions, or one part");
+    // Where the lane's fragments lie in a stage; sub-steps and pieces are an exclusive or of the address's chunk bits away,
+    // blocks of rows and columns a constant.
+    const uint32_t swizzled = (half ^ ((l >> 1) & 7)) * 16;
+    const uint32_t xoff = (wm * 32 + l) * 128 + swizzled;
+    const int first_row = wm * 32 + l;
+    const uint32_t soff = S::kA + S::kB + first_row / S::kSLanes * S::kSWave + first_row % S::kSLanes * 4;
+    uint32_t woff;
+    if (!DX) {
+        woff = S::kA + (acol0 + l) * 128 + swizzled;
+    } else {
+        const int g = lane >> 4, il = lane & 15;
+        woff = S::kA + ((g >> 1) * 16 + (il >> 1)) * BN + (((acol0 >> 4) + (g & 1)) ^ ((il >> 1) << 1)) * 16 + (il & 1) * 8;
+    }
     int cstage = 0;
     while (true) {
         floatx16 acc[MI][NI];
+        const int blocks = (cur.rows + 31) / 32;
+        // the steps of a tile whose waves have `rb` row blocks each (the last wave row one less)
+        auto steps = [&](auto rb) {
+        constexpr int RB = decltype(rb)::value;
 #pragma unroll
-        for (int i = 0; i < MI; ++i)
+        for (int i = 0; i < RB; ++i)
 #pragma unroll
             for (int j = 0; j < NI; ++j)
 #pragma unroll
                 for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.0f;
-        const int blocks = (cur.rows + 31) / 32;
         for (int step = 0; step < KT; ++step) {
             const int b = DX && step >= steps_of_term ? step - steps_of_term : step;
             if (more || step + STAGES - 2 < KT - 1) publish<(STAGES - 2) * S::kOps>();
             else publish<0>();
             if (more) issue();
-            const unsigned char *st = smem + cstage * S::kStage;
-            const unsigned char *scales = st + S::kA + S::kB;
+            const uint32_t st = lds0 + cstage * S::kStage;
             float wscale[2];
 #pragma unroll
-            for (int j = 0; j < (GLU ? 2 : 1); ++j) wscale[j] = *(const float *)(scales + wave * S::kSWave + (S::kSLanes + j) * 4);
+            for (int j = 0; j < (GLU ? 2 : 1); ++j) wscale[j] = *(lds_float_ptr)(uintptr_t)(st + S::kA + S::kB + wave * S::kSWave + (S::kSLanes + j) * 4);
             union Frag {
                 uint4_t v[2];
                 intx2 t[4];
@@ -285,57 +306,83 @@ __global__ __launch_bounds__(kThreads) void fp8_tile_kernel(Fp8Product p) {
             };
             Frag fw[NI][2];
 #pragma unroll
-            for (int j = 0; j < NI; ++j) {
-                const int n0 = GLU ? j * BNC + acol0 : acol0 + j * 32;
+            for (int j = 0; j < NI; ++j)
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
                     if (!DX) {
-                        const int r = n0 + l;
-                        const unsigned char *row = st + S::kA + r * 128;
-                        fw[j][s].v[0] = *(const uint4_t *)(row + (((4 * s + half) ^ ((r >> 1) & 7)) * 16));
-                        fw[j][s].v[1] = *(const uint4_t *)(row + (((4 * s + 2 + half) ^ ((r >> 1) & 7)) * 16));
-                    } else {
-                        const int g = lane >> 4, il = lane & 15;
-                        const int c = (n0 >> 4) + (g & 1);
+                        constexpr int kNext = GLU ? BNC * 128 : 32 * 128;  // to the wave's next block of columns
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            const int n = s * 64 + (q >> 1) * 32 + (g >> 1) * 16 + (q & 1) * 8 + (il >> 1);
-                            unsigned char *at = (unsigned char *)st + S::kA + n * BN + ((c ^ ((n & 7) << 1)) * 16) + (il & 1) * 8;
-                            fw[j][s].t[q] = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_intx2_ptr)at);
+                        for (int u = 0; u < 2; ++u)
+                            fw[j][s].v[u] = *(lds_uint4_ptr)(uintptr_t)(((st + woff) ^ (64 * s + 32 * u)) + j * kNext);
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+                            fw[j][s].t[q] = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                                (lds_intx2_ptr)(uintptr_t)(((st + woff) ^ (32 * j)) + (s * 64 + (q >> 1) * 32 + (q & 1) * 8) * BN));
+                    }
+                }
+            // The matrix unit never waits for the additions: a block's partial sum is added to its running sum while the next
+            // block's second half, or the next row block's first, is multiplied.  A row block's fragments of a sub-step are
+            // asked for as soon as those of the row block before have gone into the unit.
+            Frag fa[2];
+            int xscale[2];
+            auto fetch = [&](int i, int s) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+                    fa[s].v[u] = *(lds_uint4_ptr)(uintptr_t)(((st + xoff) ^ (64 * s + 32 * u)) + i * WM * 32 * 128);
+            };
+            auto fetch_scale = [&](int i) {
+                xscale[i & 1] = (int)(*(lds_uint32_ptr)(uintptr_t)(st + soff + i * WM * 32 / S::kSLanes * S::kSWave) >> ((b & 3) * 8));
+            };
+            floatx16 part[NI];
+            auto multiply = [&](int i, int s, int j) {
+                if (s == 0) {
+#pragma unroll
+                    for (int q = 0; q < 16; ++q) part[j][q] = 0.0f;
+                }
+                part[j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fw[j][s].i, fa[s].i, part[j], 0, 0, 0, 127, 0, xscale[i & 1]);
+            };
+            auto add = [&](int i, int j) {
+#pragma unroll
+                for (int q = 0; q < 16; ++q) acc[i][j][q] = __builtin_fmaf(wscale[GLU ? j : 0], part[j][q], acc[i][j][q]);
+            };
+            fetch(0, 0);
+            fetch_scale(0);
+            fetch(0, 1);
+#pragma unroll
+            for (int i = 0; i < RB; ++i) {
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+#pragma unroll
+                    for (int j = 0; j < NI; ++j) {
+                        multiply(i, s, j);
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (s == 0 && j == 0 && i > 0) {
+                            add(i - 1, NI - 1);
+                            __builtin_amdgcn_sched_barrier(0);
                         }
                     }
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < MI; ++i) {
-                if (i * WM + wm < blocks) {
-                    const int r = (i * WM + wm) * 32 + l;
-                    const unsigned char *row = st + r * 128;
-                    Frag fa[2];
-#pragma unroll
-                    for (int s = 0; s < 2; ++s) {
-                        fa[s].v[0] = *(const uint4_t *)(row + (((4 * s + half) ^ ((r >> 1) & 7)) * 16));
-                        fa[s].v[1] = *(const uint4_t *)(row + (((4 * s + 2 + half) ^ ((r >> 1) & 7)) * 16));
+                    if (i + 1 < RB) {
+                        fetch(i + 1, s);
+                        if (s == 0) fetch_scale(i + 1);
                     }
-                    const int xscale = (int)(*(const uint32_t *)(scales + r / S::kSLanes * S::kSWave + r % S::kSLanes * 4) >> ((b & 3) * 8));
-                    floatx16 part[NI];
-#pragma unroll
-                    for (int j = 0; j < NI; ++j)
-#pragma unroll
-                        for (int q = 0; q < 16; ++q) part[j][q] = 0.0f;
-#pragma unroll
-                    for (int s = 0; s < 2; ++s)
-#pragma unroll
-                        for (int j = 0; j < NI; ++j)
-                            part[j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fw[j][s].i, fa[s].i, part[j], 0, 0, 0, 127, 0, xscale);
-#pragma unroll
-                    for (int j = 0; j < NI; ++j)
-#pragma unroll
-                        for (int q = 0; q < 16; ++q) acc[i][j][q] = __builtin_fmaf(wscale[GLU ? j : 0], part[j][q], acc[i][j][q]);
                 }
+#pragma unroll
+                for (int j = 0; j < NI - 1; ++j) add(i, j);
+                __builtin_amdgcn_sched_barrier(0);
             }
+            add(RB - 1, NI - 1);
             if (++cstage == STAGES) cstage = 0;
         }
+        };
+        const int mine = (blocks + WM - 1) / WM;
+        if constexpr (MI >= 4)
+            if (mine == 4) steps(std::integral_constant<int, 4>{});
+        if constexpr (MI >= 3)
+            if (mine == 3) steps(std::integral_constant<int, 3>{});
+        if constexpr (MI >= 2)
+            if (mine == 2) steps(std::integral_constant<int, 2>{});
+        if (mine == 1) steps(std::integral_constant<int, 1>{});
 
         // ---- output: a lane's runs of four columns, joined to eight with the other half of the wave
         auto store = [&](void *base, int64_t at, const float (&v)[16], int n0) {
