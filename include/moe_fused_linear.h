@@ -489,7 +489,8 @@ MFL_API int mfl_moe_block_bwd(const mfl_moe_block *b, const void *dout, const vo
  * counterpart.
  *
  * workspace: mfl_fp8_workspace(...) bytes, 256-byte aligned (NULL where that is 0); it is scratch: nothing is kept in it
- * from one call to the next, and calls that can overlap in time need one each. */
+ * from one call to the next, and calls that can overlap in time need one each.  The forward product and the gated unit do
+ * without at decode sizes; a call that needs one and has none answers MFL_ERR_WORKSPACE before it enqueues anything. */
 typedef struct mfl_fp8_weight {
     const void *q;      /* e4m3 bytes */
     const float *scale; /* NaN scales make their block's products NaN */

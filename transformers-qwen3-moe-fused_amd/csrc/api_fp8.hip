@@ -82,17 +82,19 @@ int mfl_gemm_fwd_fp8(const void *x, int64_t src_rows, const int32_t *row_idx, in
     rc = check_weight(w);
     if (rc) return rc;
     if (!aligned(x, dtype_size(in_dtype)) || !aligned(y, dtype_size(out_dtype))) return MFL_ERR_ALIGN;
-    rc = check_workspace(MFL_FP8_FWD, src_rows, R, N, K, E, workspace, ws_bytes);
-    if (rc) return rc;
     const int64_t used = source_rows(src_rows, row_idx, R);
     const RowsRoom room((uint8_t *)workspace, used, K);
-    rc = fp8_quant_rows(x, in_dtype, used, K, room.q, room.scale, (hipStream_t)stream);
-    if (rc) return rc;
     Fp8Product p = {};
     p.terms = 1, p.a[0] = room.rows(), p.w[0] = matrix(w);
     p.row_idx = row_idx, p.idx_div = idx_div, p.src_rows = used;
     p.m_sizes = m_sizes, p.ms_i64 = m_sizes_dtype == MFL_I64;
     p.out = y, p.out_dtype = out_dtype, p.R = R, p.N = N, p.K = K, p.E = E;
+    rc = gemm_fp8_decode(p, x, in_dtype, (hipStream_t)stream);
+    if (rc != MFL_ERR_UNSUPPORTED) return rc;
+    rc = check_workspace(MFL_FP8_FWD, src_rows, R, N, K, E, workspace, ws_bytes);
+    if (rc) return rc;
+    rc = fp8_quant_rows(x, in_dtype, used, K, room.q, room.scale, (hipStream_t)stream);
+    if (rc) return rc;
     return run_product(p, (hipStream_t)stream);
 }
 
@@ -130,17 +132,19 @@ int mfl_glu_fwd_fp8(const void *x, int64_t src_rows, const int32_t *row_idx, int
     if (rc) return rc;
     const size_t size = dtype_size(dtype);
     if (!aligned(x, size) || !aligned(h, size) || !aligned(e_out, size) || !aligned(g_out, size)) return MFL_ERR_ALIGN;
-    rc = check_workspace(MFL_FP8_GLU, src_rows, R, N, K, E, workspace, ws_bytes);
-    if (rc) return rc;
     const int64_t used = source_rows(src_rows, row_idx, R);
     const RowsRoom room((uint8_t *)workspace, used, K);
-    rc = fp8_quant_rows(x, dtype, used, K, room.q, room.scale, (hipStream_t)stream);
-    if (rc) return rc;
     Fp8Product p = {};
     p.glu = true, p.terms = 1, p.a[0] = room.rows(), p.w[0] = matrix(gate), p.w[1] = matrix(up);
     p.row_idx = row_idx, p.idx_div = idx_div, p.src_rows = used;
     p.m_sizes = m_sizes, p.ms_i64 = m_sizes_dtype == MFL_I64;
     p.out = h, p.e_out = e_out, p.g_out = g_out, p.out_dtype = dtype, p.R = R, p.N = N, p.K = K, p.E = E;
+    rc = gemm_fp8_decode(p, x, dtype, (hipStream_t)stream);
+    if (rc != MFL_ERR_UNSUPPORTED) return rc;
+    rc = check_workspace(MFL_FP8_GLU, src_rows, R, N, K, E, workspace, ws_bytes);
+    if (rc) return rc;
+    rc = fp8_quant_rows(x, dtype, used, K, room.q, room.scale, (hipStream_t)stream);
+    if (rc) return rc;
     return run_product(p, (hipStream_t)stream);
 }
 
@@ -189,13 +193,22 @@ int mfl_mlp_fwd_fp8(const void *x, int64_t src_rows, const int32_t *row_idx, int
     const int64_t used = source_rows(src_rows, row_idx, R);
     const RowsRoom room((uint8_t *)workspace, used, H), hidden((uint8_t *)workspace + rows_bytes(src_rows, H), R, I);
     void *const h = (uint8_t *)workspace + rows_bytes(src_rows, H) + rows_bytes(R, I);
-    rc = fp8_quant_rows(x, dtype, used, H, room.q, room.scale, (hipStream_t)stream);
-    if (rc) return rc;
     Fp8Product p = {};
     p.glu = true, p.terms = 1, p.a[0] = room.rows(), p.w[0] = matrix(gate), p.w[1] = matrix(up);
     p.row_idx = row_idx, p.idx_div = idx_div, p.src_rows = used;
     p.m_sizes = m_sizes, p.ms_i64 = m_sizes_dtype == MFL_I64;
     p.e_out = e_out, p.g_out = g_out, p.out_dtype = dtype, p.R = R, p.N = I, p.K = H, p.E = E;
+    Fp8Product d = p;  // the down projection
+    d.glu = false, d.a[0] = hidden.rows(), d.w[0] = matrix(down), d.row_idx = nullptr, d.src_rows = R;
+    d.out = y, d.e_out = d.g_out = nullptr, d.N = H, d.K = I;
+    if (gemm_fp8_decodes(p) && gemm_fp8_decodes(d) && aligned(x, 16)) {
+        // a few rows: both kernels quantise their rows themselves, from the fp32 values between them
+        p.h32 = (float *)h;
+        rc = gemm_fp8_decode(p, x, dtype, (hipStream_t)stream);
+        return rc ? rc : gemm_fp8_decode(d, h, MFL_F32, (hipStream_t)stream);
+    }
+    rc = fp8_quant_rows(x, dtype, used, H, room.q, room.scale, (hipStream_t)stream);
+    if (rc) return rc;
     p.hq = hidden.q, p.hq_scale = hidden.scale;
     rc = gemm_fp8_tile(p, (hipStream_t)stream);
     if (rc == MFL_ERR_UNSUPPORTED) {
@@ -204,11 +217,7 @@ int mfl_mlp_fwd_fp8(const void *x, int64_t src_rows, const int32_t *row_idx, int
         rc = gemm_fp8_generic(p, (hipStream_t)stream);
         if (!rc) rc = fp8_quant_rows(h, MFL_F32, R, I, hidden.q, hidden.scale, (hipStream_t)stream);
     }
-    if (rc) return rc;
-    p.hq = p.hq_scale = nullptr, p.h32 = nullptr;
-    p.glu = false, p.a[0] = hidden.rows(), p.w[0] = matrix(down), p.row_idx = nullptr, p.src_rows = R;
-    p.out = y, p.e_out = p.g_out = nullptr, p.out_dtype = dtype, p.N = H, p.K = I;
-    return run_product(p, (hipStream_t)stream);
+    return rc ? rc : run_product(d, (hipStream_t)stream);
 }
 
 int mfl_fp8_quant_rows(const void *x, int dtype, int64_t R, int K, void *q, uint8_t *scale, void *stream) {

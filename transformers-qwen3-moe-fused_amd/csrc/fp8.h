@@ -46,11 +46,17 @@ struct Fp8Product {
     void *out, *e_out, *g_out;
     int out_dtype;
     uint8_t *hq, *hq_scale;  // (glu) where given, `out` is not written but quantised rows, made from the fp32 values
-    float *h32;              // (glu, any-shape kernel) where given, `out` is not written but these fp32 values
+    float *h32;              // (glu; not on tiles) where given, `out` is not written but these fp32 values
     int64_t R;
     int N, K, E;
 };
 
+// A few rows per expert (kFp8DecodeRowsPerExpert on average), forward and gated, 16-bit outputs, K % 16 == 0: the rows come as
+// they are (x, of the output's type or fp32) and are quantised on the way; p.a is not read.  MFL_ERR_UNSUPPORTED for the rest;
+// gemm_fp8_decodes: whether it takes the product with an aligned x.
+constexpr int kFp8DecodeRowsPerExpert = 8;
+bool gemm_fp8_decodes(const Fp8Product &p);
+int gemm_fp8_decode(const Fp8Product &p, const void *x, int x_dtype, hipStream_t stream);
 // Tiles in LDS, 16-bit outputs, K % 16 == 0; MFL_ERR_UNSUPPORTED for the rest.
 int gemm_fp8_tile(const Fp8Product &p, hipStream_t stream);
 // Any shape; MFL_OK or a launch error.
@@ -66,40 +72,46 @@ int fp8_dequant_blocks(const uint8_t *q, const float *scale, int E, int N, int K
 
 typedef __attribute__((ext_vector_type(8))) int intx8;
 
-// Biased exponent byte of the scale for a block whose largest finite magnitude is amax: amax = f 2^p with 1 <= f < 2 fits
+// Biased exponent byte of the scale for a block whose largest finite magnitude has the bits b: amax = f 2^p with 1 <= f < 2 fits
 // 448 2^e = 1.75 2^(8 + e) with e = p - 8 if f <= 1.75, else p - 7.  (amax 0 or subnormal: the least exponent.)
-__device__ __forceinline__ int fp8_scale_byte(float amax) {
-    const uint32_t b = __float_as_uint(amax);
+__device__ __forceinline__ int fp8_scale_byte(uint32_t b) {
     const int byte = (int)(b >> 23) - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
     return byte < 10 ? 10 : byte;
 }
 __device__ __forceinline__ float fp8_scale_of(int byte) { return __uint_as_float((uint32_t)byte << 23); }
 __device__ __forceinline__ float fp8_inverse_of(int byte) { return __uint_as_float((uint32_t)(254 - byte) << 23); }
 
-// |v|, or 0 where v is infinite or no number
+// Largest magnitude of a block.  Magnitudes are compared as whole numbers (their order is that of the values, infinity and then
+// NaN above all): fp8_wider takes another value's bits in, fp8_unusual says whether there is one that is no finite number; only
+// then do the values have to be looked at one by one (fp8_finite_abs, fp8_finite).
+__device__ __forceinline__ uint32_t fp8_wider(uint32_t bits, float v) {
+    const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
+    return bits > b ? bits : b;
+}
+__device__ __forceinline__ bool fp8_unusual(uint32_t bits) { return bits >= 0x7f800000u; }
 __device__ __forceinline__ float fp8_finite_abs(float v) {
     const float a = __builtin_fabsf(v);
     return a <= 3.4028234663852886e38f ? a : 0.0f;
 }
-
-// Four values times a power of two, rounded to e4m3 (nearest, ties to even): one dword.
-__device__ __forceinline__ float fp8_ready(float v, float inverse) {
-    const float a = __builtin_fabsf(v);
-    return a <= 3.4028234663852886e38f ? v * inverse : __uint_as_float(0x7fc00000u);
+// v, or NaN where it is infinite
+__device__ __forceinline__ float fp8_finite(float v) {
+    return __builtin_fabsf(v) <= 3.4028234663852886e38f ? v : __uint_as_float(0x7fc00000u);
 }
+// Four values times a power of two, rounded to e4m3 (nearest, ties to even): one dword.  None of them infinite.
 __device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d, float inverse) {
     int r = 0;
-    r = __builtin_amdgcn_cvt_pk_fp8_f32(fp8_ready(a, inverse), fp8_ready(b, inverse), r, false);
-    r = __builtin_amdgcn_cvt_pk_fp8_f32(fp8_ready(c, inverse), fp8_ready(d, inverse), r, true);
+    r = __builtin_amdgcn_cvt_pk_fp8_f32(a * inverse, b * inverse, r, false);
+    r = __builtin_amdgcn_cvt_pk_fp8_f32(c * inverse, d * inverse, r, true);
     return (uint32_t)r;
 }
 
 // The largest of a row of 16 lanes, in all of them.
 template <int CTRL>
-__device__ __forceinline__ float fp8_dpp_max(float x) {
-    return __builtin_fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true)));
+__device__ __forceinline__ uint32_t fp8_dpp_max(uint32_t x) {
+    const uint32_t y = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true);
+    return x > y ? x : y;
 }
-__device__ __forceinline__ float fp8_max16(float x) {
+__device__ __forceinline__ uint32_t fp8_max16(uint32_t x) {
     x = fp8_dpp_max<0x128>(x);  // row_ror 8, 4, 2, 1
     x = fp8_dpp_max<0x124>(x);
     x = fp8_dpp_max<0x122>(x);

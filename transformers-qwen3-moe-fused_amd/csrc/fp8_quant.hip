@@ -28,16 +28,19 @@ __device__ __forceinline__ void load8(const T *row, int k, int K, float (&v)[8])
     }
 }
 
-__device__ __forceinline__ float amax8(const float (&v)[8]) {
-    float a = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) a = __builtin_fmaxf(a, fp8_finite_abs(v[i]));
-    return a;
-}
-
 // The lane's 8 values of a block (16 lanes) to q, the block's scale byte to scale.
-__device__ __forceinline__ void store_block(const float (&v)[8], uint8_t *q, uint8_t *scale, bool first) {
-    const int byte = fp8_scale_byte(fp8_max16(amax8(v)));
+__device__ __forceinline__ void store_block(float (&v)[8], uint8_t *q, uint8_t *scale, bool first) {
+    uint32_t a = 0u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a = fp8_wider(a, v[i]);
+    a = fp8_max16(a);
+    if (fp8_unusual(a)) {
+        a = 0u;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a = fp8_wider(a, fp8_finite_abs(v[i])), v[i] = fp8_finite(v[i]);
+        a = fp8_max16(a);
+    }
+    const int byte = fp8_scale_byte(a);
     const float inverse = fp8_inverse_of(byte);
     *(uint2_t *)q = uint2_t{fp8_pack4(v[0], v[1], v[2], v[3], inverse), fp8_pack4(v[4], v[5], v[6], v[7], inverse)};
     if (first) *scale = (uint8_t)byte;
@@ -129,12 +132,12 @@ __global__ __launch_bounds__(256) void quant_blocks_kernel(const T *__restrict__
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = a;
     __syncthreads();
     a = __builtin_fmaxf(__builtin_fmaxf(part[0], part[1]), __builtin_fmaxf(part[2], part[3]));
-    const int byte = fp8_scale_byte(a);
+    const int byte = fp8_scale_byte(__float_as_uint(a));
     const float inverse = fp8_inverse_of(byte);
     if (threadIdx.x == 0) scale[block] = fp8_scale_of(byte);
     if (k < K)
         for (int r = threadIdx.x >> 7; r < rows; r += 2) {
-            const float v = to_f32(w[base + (int64_t)r * K]);
+            const float v = fp8_finite(to_f32(w[base + (int64_t)r * K]));
             q[base + (int64_t)r * K] = (uint8_t)fp8_pack4(v, 0.0f, 0.0f, 0.0f, inverse);
         }
 }

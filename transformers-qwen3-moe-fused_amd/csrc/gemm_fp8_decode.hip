@@ -1,0 +1,278 @@
+// Expert products in 8-bit floating point for a few rows per expert: the forward product and the gated unit in one launch,
+// the rows quantised on the way.
+//
+// The weights are all the traffic.  A workgroup (four waves) owns 16 rows of an expert and PIECES blocks of 16 columns (gated:
+// half of them of either matrix); its waves share the reduction, wave w taking the blocks of 128 number w, w + 4, ...  A block
+// of 16 columns is one v_mfma_scale_f32_16x16x128_f8f6f4, whose operands come straight from memory into registers: nothing is
+// shared between waves, so nothing goes through LDS, and the next two pieces' weights are on their way while one is
+// multiplied.  A lane holds bytes 16 g .. 16 g + 15 and 64 + 16 g .. of a row of the block (g: its quarter of the wave), so that
+// four lanes read 64 bytes of a row together; the rows are loaded in the same order, their largest magnitude found over the
+// four lanes, and rounded to e4m3 in registers (the order within the block does not matter as long as both operands agree).
+// The waves' sums meet in LDS.  Bound by the weights' bytes, or by latency (row counts, row index, rows, weights one behind
+// the other) where there are few of them.
+#include "fp8.h"
+
+namespace mfl {
+
+namespace {
+
+constexpr int kRows = 16, kWaves = 4;
+constexpr int kBuffers = 3;  // pieces of weights in registers
+
+// 16 elements of a row, where they lie inside it
+template <typename T>
+struct Piece {
+    uint4_t q[sizeof(T)];
+    __device__ __forceinline__ void load(const T *p) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T); ++i) q[i] = ((const uint4_t *)p)[i];
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T); ++i) q[i] = uint4_t{0u, 0u, 0u, 0u};
+    }
+    __device__ __forceinline__ float at(int i) const {
+        union {
+            uint4_t v;
+            T e[16 / sizeof(T)];
+        } u;
+        u.v = q[i / (16 / (int)sizeof(T))];
+        return to_f32(u.e[i % (16 / (int)sizeof(T))]);
+    }
+};
+
+// The largest of the four lanes that hold a row's block, in all of them.
+__device__ __forceinline__ uint32_t over_block(uint32_t a) {
+    uint32_t b = (uint32_t)__shfl_xor((int)a, 16);
+    a = a > b ? a : b;
+    b = (uint32_t)__shfl_xor((int)a, 32);
+    return a > b ? a : b;
+}
+
+// The sizes of up to 256 experts at once (their loads in flight together), then 64 at a time.
+__device__ __forceinline__ bool find_rows(const Fp8Product &p, int slot, int lane, int &expert, int64_t &row0, int &rows) {
+    int tiles_before = 0;
+    int64_t rows_before = 0;
+    for (int e0 = 0; e0 < p.E; e0 += 256) {
+        int m[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int e = e0 + 64 * i + lane;
+            m[i] = e < p.E ? load_msize(p.m_sizes, p.ms_i64, e) : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (m[i] < 0) m[i] = 0;
+            const int t = ceil_div(m[i], kRows);
+            const int mi = wave_inclusive_scan(m[i]), ti = wave_inclusive_scan(t);
+            const uint64_t past = __ballot(tiles_before + ti > slot);
+            if (past) {
+                const int src = __ffsll((unsigned long long)past) - 1;
+                const int m_e = __builtin_amdgcn_readlane(m[i], src);
+                const int tile = slot - (tiles_before + __builtin_amdgcn_readlane(ti, src) - __builtin_amdgcn_readlane(t, src));
+                expert = e0 + 64 * i + src;
+                row0 = rows_before + __builtin_amdgcn_readlane(mi, src) - m_e + (int64_t)tile * kRows;
+                rows = m_e - tile * kRows < kRows ? m_e - tile * kRows : kRows;
+                if (row0 + rows > p.R) rows = (int)(p.R - row0);
+                return rows > 0;
+            }
+            rows_before += wave_last(mi);
+            tiles_before += wave_last(ti);
+        }
+    }
+    return false;
+}
+
+// AHEAD: blocks of the reduction that a wave holds of the rows, and of every piece, at a time.
+template <bool GLU, int PIECES, int AHEAD, typename TX, typename TO>
+__global__ __launch_bounds__(kWaves * 64, 2) void fp8_decode_kernel(Fp8Product p, const TX *__restrict__ x) {
+    static_assert(!GLU || PIECES % 2 == 0, "gated: blocks of columns of both matrices");
+    constexpr int TILES = GLU ? PIECES / 2 : PIECES;  // blocks of output columns
+    __shared__ floatx4 sums[kWaves][PIECES][64];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = lane & 15, g = lane >> 4;
+    int e, rows;
+    int64_t row0;
+    if (!find_rows(p, blockIdx.y, lane, e, row0, rows)) return;
+    const int n0 = blockIdx.x * 16 * TILES;
+    const int blocks = fp8_blocks(p.K), nbn = fp8_blocks(p.N);
+
+    int64_t src = row0 + (c < rows ? c : rows - 1);
+    int looked_up = 0;
+    if (p.row_idx != nullptr) looked_up = p.row_idx[src];
+
+    union Frag {
+        uint4_t v[2];
+        intx8 i;
+    };
+    // piece t: columns n0 + 16 (t / 2) of matrix t % 2 where gated, else n0 + 16 t.  Columns past the last are not stored.
+    Frag fw[kBuffers][AHEAD];
+    auto load = [&](int t, int b0) {
+        const Fp8Matrix &m = p.w[GLU ? t & 1 : 0];
+        int n = n0 + 16 * (GLU ? t / 2 : t) + c;
+        if (n >= p.N) n = p.N - 1;
+        const uint8_t *w = m.q + ((int64_t)e * p.N + n) * p.K + 16 * g;
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int b = b0 + kWaves * u;
+            if (b < blocks) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int k = b * kFp8Block + 64 * h;
+                    if (k + 16 * g < p.K) fw[t % kBuffers][u].v[h] = *(const uint4_t *)(w + k);  // (K is a multiple of 16)
+                    else fw[t % kBuffers][u].v[h] = uint4_t{0u, 0u, 0u, 0u};
+                }
+            }
+        }
+    };
+
+    floatx4 acc[PIECES];
+#pragma unroll
+    for (int t = 0; t < PIECES; ++t) acc[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int b0 = wave; b0 < blocks; b0 += kWaves * AHEAD) {
+#pragma unroll
+        for (int t = 0; t < kBuffers - 1 && t < PIECES; ++t) load(t, b0);
+        // the rows' blocks, quantised
+        intx8 q[AHEAD];
+        int byte[AHEAD];
+        {
+            int64_t row = src;
+            if (p.row_idx != nullptr) {
+                const int i = looked_up / p.idx_div;
+                row = i < 0 ? 0 : i >= p.src_rows ? p.src_rows - 1 : i;
+            }
+            const TX *const xr = x + row * p.K + 16 * g;
+            Piece<TX> fx[AHEAD][2];
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const int b = b0 + kWaves * u;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int k = b * kFp8Block + 64 * h;
+                    if (b < blocks && k + 16 * g < p.K) fx[u][h].load(xr + k);
+                    else fx[u][h].clear();
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                uint32_t a = 0u;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) a = fp8_wider(a, fx[u][h].at(i));
+                a = over_block(a);
+                const bool unusual = __any(fp8_unusual(a));
+                if (unusual) {
+                    a = 0u;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) a = fp8_wider(a, fp8_finite_abs(fx[u][h].at(i)));
+                    a = over_block(a);
+                }
+                byte[u] = fp8_scale_byte(a);
+                const float inverse = fp8_inverse_of(byte[u]);
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        q[u][4 * h + i] = (int)(unusual ? fp8_pack4(fp8_finite(fx[u][h].at(4 * i)), fp8_finite(fx[u][h].at(4 * i + 1)),
+                                                                    fp8_finite(fx[u][h].at(4 * i + 2)), fp8_finite(fx[u][h].at(4 * i + 3)), inverse)
+                                                        : fp8_pack4(fx[u][h].at(4 * i), fx[u][h].at(4 * i + 1), fx[u][h].at(4 * i + 2),
+                                                                    fx[u][h].at(4 * i + 3), inverse));
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < PIECES; ++t) {
+            if (t + kBuffers - 1 < PIECES) load(t + kBuffers - 1, b0);
+            int nb = (n0 + 16 * (GLU ? t / 2 : t)) / kFp8Block;
+            if (nb >= nbn) nb = nbn - 1;
+            const float *scale = p.w[GLU ? t & 1 : 0].scale + ((int64_t)e * nbn + nb) * blocks;
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const int b = b0 + kWaves * u;
+                if (b < blocks) {
+                    const floatx4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+                    const floatx4 part = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw[t % kBuffers][u].i, q[u], zero, 0, 0, 0, 127, 0, byte[u]);
+                    const float s = scale[b];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[t][i] = __builtin_fmaf(s, part[i], acc[t][i]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < PIECES; ++t) sums[wave][t][lane] = acc[t];
+    __syncthreads();
+    if (c >= rows) return;
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+        if (t % kWaves != wave) continue;
+        floatx4 v[GLU ? 2 : 1];
+#pragma unroll
+        for (int m = 0; m < (GLU ? 2 : 1); ++m) {
+            v[m] = sums[0][GLU ? 2 * t + m : t][lane];
+#pragma unroll
+            for (int s = 1; s < kWaves; ++s) v[m] += sums[s][GLU ? 2 * t + m : t][lane];
+        }
+        // four columns of row c
+        const int n = n0 + 16 * t + 4 * g;
+        const int64_t at = (row0 + c) * p.N + n;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (n + i >= p.N) continue;
+            if (!GLU) {
+                ((TO *)p.out)[at + i] = from_f32<TO>(v[0][i]);
+            } else {
+                const float ev = v[0][i], gv = v[GLU ? 1 : 0][i];
+                const float h = ev * sigmoid_f32(ev) * gv;
+                if (p.h32 != nullptr)
+                    p.h32[at + i] = h;
+                else
+                    ((TO *)p.out)[at + i] = from_f32<TO>(h);
+                if (p.e_out != nullptr) ((TO *)p.e_out)[at + i] = from_f32<TO>(ev);
+                if (p.g_out != nullptr) ((TO *)p.g_out)[at + i] = from_f32<TO>(gv);
+            }
+        }
+    }
+}
+
+template <int PIECES, int AHEAD, typename TX, typename TO>
+int launch_as(const Fp8Product &p, const TX *x, hipStream_t stream) {
+    const unsigned slots = (unsigned)fp8_max_tiles(p.R, p.E, kRows);
+    if (p.glu)
+        fp8_decode_kernel<true, PIECES, AHEAD, TX, TO><<<dim3(ceil_div(p.N, 8 * PIECES), slots), kWaves * 64, 0, stream>>>(p, x);
+    else
+        fp8_decode_kernel<false, PIECES, AHEAD, TX, TO><<<dim3(ceil_div(p.N, 16 * PIECES), slots), kWaves * 64, 0, stream>>>(p, x);
+    return launch_status();
+}
+
+template <typename TX, typename TO>
+int launch(const Fp8Product &p, const TX *x, hipStream_t stream) {
+    // Pieces of a workgroup: two where there are few (latency counts: as many workgroups as there can be), else eight, two
+    // workgroups a CU.
+    const int64_t row_tiles = p.R < p.E ? p.R : p.E;
+    const bool few = row_tiles * ceil_div(p.N, 16) * (p.glu ? 2 : 1) < (int64_t)8 * 2 * device_info().cu_count;
+    // (fp32 rows of four blocks and eight pieces do not fit the registers)
+    if (fp8_blocks(p.K) <= 2 * kWaves || sizeof(TX) == 4) return few ? launch_as<2, 2, TX, TO>(p, x, stream) : launch_as<8, 2, TX, TO>(p, x, stream);
+    return few ? launch_as<2, 4, TX, TO>(p, x, stream) : launch_as<8, 4, TX, TO>(p, x, stream);
+}
+
+}  // namespace
+
+bool gemm_fp8_decodes(const Fp8Product &p) {
+    if (p.dx || p.out_dtype == MFL_F32 || p.K % 16 != 0 || p.R > (int64_t)kFp8DecodeRowsPerExpert * p.E) return false;
+    if (fp8_max_tiles(p.R, p.E, kRows) > 65535) return false;
+    return aligned(p.w[0].q, 16) && (!p.glu || aligned(p.w[1].q, 16));
+}
+
+int gemm_fp8_decode(const Fp8Product &p, const void *x, int x_dtype, hipStream_t stream) {
+    if (!gemm_fp8_decodes(p) || !aligned(x, 16)) return MFL_ERR_UNSUPPORTED;
+    if (x_dtype == MFL_F32)
+        return p.out_dtype == MFL_BF16 ? launch<float, bf16_t>(p, (const float *)x, stream) : launch<float, f16_t>(p, (const float *)x, stream);
+    if (x_dtype != p.out_dtype) return MFL_ERR_UNSUPPORTED;
+    return p.out_dtype == MFL_BF16 ? launch<bf16_t, bf16_t>(p, (const bf16_t *)x, stream) : launch<f16_t, f16_t>(p, (const f16_t *)x, stream);
+}
+
+}  // namespace mfl

@@ -21,7 +21,7 @@
 // LDS layouts.  Rows of 128 bytes along the reduction: 16-byte chunk c of row r at c ^ ((r >> 1) & 7).  A lane's 32 bytes of a
 // 64-wide sub-step are chunks 4 s + h and 4 s + 2 + h (h: its half of the wave); which reduction element sits where in the
 // instruction does not matter as long as both operands agree.  Input gradient: the weights lie as in memory, 128 rows of the
-// reduction by BN columns, chunk c of row n at c ^ ((n & 7) << 1), and are read with ds_read_b64_tr_b8 (a group of 16 lanes
+// reduction by BN columns, chunk c of row n at c ^ ((n & 7) << 1) (BN 128: ^ ((n & 6)), and are read with ds_read_b64_tr_b8 (a group of 16 lanes
 // reads 8 rows of 16 bytes and gets 8 rows of one column each), four of them for the same 32 elements.
 #include <type_traits>
 
@@ -40,7 +40,6 @@ typedef const __attribute__((address_space(3))) float *lds_float_ptr;
 
 constexpr int kXcd = 8;
 constexpr int kMaxExperts = 512;  // prefix tables in LDS
-constexpr int kWaves = 8, kThreads = kWaves * 64;
 
 __device__ uint4_t g_fp8_zeros = {0u, 0u, 0u, 0u};
 
@@ -64,34 +63,53 @@ __device__ __forceinline__ void publish() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(N) : "memory");
 }
 
+// The same behind a tile's output: the `newer` stores that the wave has issued since the copies it waits for need not have
+// landed (the counter retires in order).
+template <int N>
+__device__ __forceinline__ void publish_past(int newer) {
+    static_assert(N >= 0 && N + 16 < 64, "vmcnt is a 6-bit counter");
+    asm volatile(
+        "s_cmp_ge_u32 %0, 16\n\ts_cbranch_scc1 1f\n\ts_cmp_ge_u32 %0, 8\n\ts_cbranch_scc1 2f\n\ts_cmp_ge_u32 %0, 4\n\ts_cbranch_scc1 3f\n\t"
+        "s_waitcnt vmcnt(%1) lgkmcnt(0)\n\ts_branch 4f\n"
+        "1:\n\ts_waitcnt vmcnt(%2) lgkmcnt(0)\n\ts_branch 4f\n"
+        "2:\n\ts_waitcnt vmcnt(%3) lgkmcnt(0)\n\ts_branch 4f\n"
+        "3:\n\ts_waitcnt vmcnt(%4) lgkmcnt(0)\n"
+        "4:\n\ts_barrier"
+        :
+        : "s"(__builtin_amdgcn_readfirstlane(newer)), "n"(N), "n"(N + 16), "n"(N + 8), "n"(N + 4)
+        : "memory", "scc");
+}
+
 // WM x WN waves of MI x NI blocks of 32 x 32.
 template <int WM, int WN, int MI, int NI, int STAGES>
 struct Shape {
-    static_assert(WM * WN == kWaves, "eight waves");
+    static constexpr int kWaves = WM * WN, kThreads = kWaves * 64;
     static constexpr int BM = WM * MI * 32, BN = WN * NI * 32;
     static constexpr int kSLanes = BM / kWaves;                    // rows whose scale dwords a wave copies,
-    static constexpr int kSWave = (kSLanes + 2) * 4;               // and behind them the weights' scales of its columns
+    static constexpr int kSWave = 64 * 4;                          // and behind them the weights' scales of its columns
     static constexpr int kA = BM * 128, kB = BN * 128, kS = kWaves * kSWave;
     static constexpr int kStage = (kA + kB + kS + 1023) / 1024 * 1024;
     static constexpr int kACopies = kA / 1024 / kWaves, kBCopies = kB / 1024 / kWaves;
     static constexpr int kOps = kACopies + kBCopies + 1;  // vector-memory operations a wave issues for a stage
-    static constexpr int kTables = 2 * (kMaxExperts + 1) * 4;
-    static constexpr int kLds = STAGES * kStage + kTables;
+    static constexpr int kTables = (2 * (kMaxExperts + 1) * 4 + 127) / 128 * 128;
+    static constexpr int kOut = 2048;  // a wave's place for turning its output
+    static constexpr int kLds = STAGES * kStage + kTables + kWaves * kOut;
     static_assert(kA % (1024 * kWaves) == 0 && kB % (1024 * kWaves) == 0 && kSLanes + 2 <= 64, "whole copies");
 };
 
-// HQ: the gated unit's result leaves as quantised rows.
-template <bool DX, bool GLU, bool HQ, int WM, int WN, int MI, int NI, int STAGES, typename TO>
-__global__ __launch_bounds__(kThreads) void fp8_tile_kernel(Fp8Product p) {
+// HQ: the gated unit's result leaves as quantised rows.  PARTIAL: the reduction ends inside a block of 128.
+template <bool DX, bool GLU, bool HQ, bool PARTIAL, int WM, int WN, int MI, int NI, int STAGES, typename TO>
+__global__ __launch_bounds__(WM * WN * 64, 2) void fp8_tile_kernel(Fp8Product p) {
     using S = Shape<WM, WN, MI, NI, STAGES>;
-    constexpr int BM = S::BM, BN = S::BN;
+    constexpr int BM = S::BM, BN = S::BN, kWaves = S::kWaves;
     constexpr int BNC = GLU ? BN / 2 : BN;  // output columns of a tile
     static_assert(!GLU || NI == 2, "gated: a wave holds one block of either matrix");
     static_assert(!HQ || (GLU && BNC == kFp8Block), "quantised output: a tile's columns are one scale block");
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
     int *const tab_rows = (int *)(smem + STAGES * S::kStage);
     int *const tab_tiles = tab_rows + kMaxExperts + 1;
-    float *const amax = (float *)(tab_tiles + kMaxExperts + 1);  // (HQ) per row and wave column
+    unsigned char *const turn = smem + STAGES * S::kStage + S::kTables;         // the waves' places
+    uint32_t *const amax = (uint32_t *)(smem + S::kLds);                            // (HQ) per row and wave column
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave % WM, wn = wave / WM;
@@ -102,6 +120,10 @@ __global__ __launch_bounds__(kThreads) void fp8_tile_kernel(Fp8Product p) {
     const int nbn = fp8_blocks(p.N), kbk = fp8_blocks(p.K);
     const int64_t lda = fp8_ld(red);
     const int lds_ = (int)fp8_ld_scale(red);
+
+    // (DX) which chunks of a row of the reduction are exchanged, by its number: eight rows' pieces of 32 bytes in all 64 banks
+    static_assert(!DX || BN == 128 || BN == 256, "rows of half or all of the banks");
+    auto spread = [](int n) { return BN == 128 ? ((n >> 1) & 3) << 1 : (n & 7) << 1; };
 
     // ---- rows and row tiles before every expert; an expert's rows are cut into tiles of equal height, a multiple of 32
     {
@@ -130,7 +152,14 @@ __global__ __launch_bounds__(kThreads) void fp8_tile_kernel(Fp8Product p) {
     struct Tile {
         int index, expert, row0, rows, col0;
     };
+    // The lane, for what is computed once a tile: taken from here, its terms are not kept in registers through the steps.
+    auto lane_now = [&]() {
+        int now = lane;
+        asm volatile("" : "+v"(now));
+        return now;
+    };
     auto decode = [&](Tile &t) {
+        const int lane = lane_now();
         const int v = t.index / col_tiles;
         int e = 0;
         for (int e0 = 0; e0 < p.E; e0 += 64) {
@@ -159,42 +188,40 @@ __global__ __launch_bounds__(kThreads) void fp8_tile_kernel(Fp8Product p) {
 
     // ---- the producer's side: per-lane sources of the copies of the tile whose steps it is issuing
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void_ptr)smem;
-    Tile pt = cur;
+    Tile pt = cur, nt = cur;  // the producer's tile, and the one it takes up next
     int pstep = 0, pstage = 0;
-    bool more = true;
     // (rows that are not gathered are addressed from the tile's first one; gathered ones from the first of all, within 32 bits)
     const bool gathered = !DX && p.row_idx != nullptr;
     uint32_t aoff[S::kACopies], boff[S::kBCopies];
     const uint8_t *sptr;  // the lane's scale dword: of a row, or of the weights
+    int src_row = 0;
     const uint8_t *abase, *bbase;
-    auto source = [&](int r) -> int {
-        const int i = r < pt.rows ? r : pt.rows - 1;
-        if (!gathered) return i;
-        const int at = p.row_idx[pt.row0 + i] / p.idx_div;
-        return at < 0 ? 0 : at >= (int)p.src_rows ? (int)p.src_rows - 1 : at;
+    // Lane i of a wave looks up the source of row i of the wave's BM / 8 rows when the tile is known, several steps before
+    // its first copies.
+    int looked_up = 0;
+    auto look_up = [&]() {
+        const int lane = lane_now();
+        const int r = wave * S::kSLanes + (S::kSLanes >= 64 ? lane : lane % S::kSLanes);
+        looked_up = r < nt.rows ? r : nt.rows - 1;
+        if (gathered) looked_up = p.row_idx[nt.row0 + looked_up];
     };
     // column block of the weights' scales of the wave's columns (which lie in one: 64 or 32 columns from a multiple of that)
     auto scale_block = [&](const Tile &t) {
         const int at = (t.col0 + (GLU ? wn * 32 : wn * NI * 32)) / kFp8Block, end = DX ? kbk : nbn;
         return at < end ? at : end - 1;
     };
-    auto start_term = [&](int term) {
-        const Fp8Rows a = term ? p.a[1] : p.a[0];
-        const uint8_t *w = (term ? p.w[1].q : p.w[0].q) + (int64_t)pt.expert * p.N * p.K;
-        const int64_t first = gathered ? 0 : pt.row0;
-        abase = a.q + first * lda;
-        bbase = DX ? w + pt.col0 : w + (int64_t)pt.col0 * p.K;
-        const int sl = lane < S::kSLanes ? lane : 0;
-        const uint8_t *row = a.scale + (first + source(wave * S::kSLanes + sl)) * lds_;
-        const float *ws = (term || (GLU && lane > S::kSLanes) ? p.w[1].scale : p.w[0].scale) + (int64_t)pt.expert * nbn * kbk;
-        ws += DX ? scale_block(pt) : (int64_t)scale_block(pt) * kbk;
-        sptr = lane < S::kSLanes ? row : (const uint8_t *)ws;
-    };
     auto start_tile = [&]() {
+        const int lane = lane_now();
+        pt = nt, pstep = 0;
+        src_row = looked_up;
+        if (gathered) {
+            src_row /= p.idx_div;
+            src_row = src_row < 0 ? 0 : src_row >= (int)p.src_rows ? (int)p.src_rows - 1 : src_row;
+        }
 #pragma unroll
         for (int c = 0; c < S::kACopies; ++c) {
             const int r = (wave * S::kACopies + c) * 8 + (lane >> 3);
-            aoff[c] = (uint32_t)source(r) * (uint32_t)lda + ((lane & 7) ^ ((r >> 1) & 7)) * 16;
+            aoff[c] = (uint32_t)__shfl(src_row, c * 8 + (lane >> 3)) * (uint32_t)lda + ((lane & 7) ^ ((r >> 1) & 7)) * 16;
         }
 #pragma unroll
         for (int c = 0; c < S::kBCopies; ++c) {
@@ -207,58 +234,61 @@ __global__ __launch_bounds__(kThreads) void fp8_tile_kernel(Fp8Product p) {
             } else {
                 constexpr int CPR = BN / 16;  // chunks of a row of the reduction
                 const int r = (load * 64 + lane) / CPR;
-                int k = ((lane % CPR) ^ ((r & 7) << 1)) * 16;
+                int k = ((lane % CPR) ^ spread(r)) * 16;
                 if (pt.col0 + k >= p.K) k = p.K - 16 - pt.col0;  // (columns that are not stored)
                 boff[c] = (uint32_t)r * (uint32_t)p.K + k;
             }
         }
-        start_term(0);
+        const Fp8Rows a = p.a[0];
+        const int64_t first = gathered ? 0 : pt.row0, mat = (int64_t)pt.expert * p.N * p.K;
+        abase = a.q + first * lda;
+        bbase = p.w[0].q + mat + (DX ? pt.col0 : (int64_t)pt.col0 * p.K);
+        const float *ws = (GLU && lane > S::kSLanes ? p.w[1].scale : p.w[0].scale) + (int64_t)pt.expert * nbn * kbk;
+        ws += DX ? scale_block(pt) : (int64_t)scale_block(pt) * kbk;
+        sptr = lane < S::kSLanes ? a.scale + (first + src_row) * lds_ : (const uint8_t *)ws;
     };
-    start_tile();
-
-    // The copies of one step.
+    // The copies of one step.  Without a branch, so that the compiler leaves the order of the steps' arithmetic alone.
     auto issue = [&]() {
-        if (DX && pstep == steps_of_term) start_term(1);
         const int b = DX && pstep >= steps_of_term ? pstep - steps_of_term : pstep;
         const uint32_t st = lds0 + pstage * S::kStage;
 #pragma unroll
         for (int c = 0; c < S::kACopies; ++c) copy16(abase, aoff[c], st + (wave * S::kACopies + c) * 1024);
-        abase += 128;
         // (gated: the upper half of the waves copies the second matrix)
         const uint8_t *bb = bbase;
-        if (GLU && wave >= kWaves / 2) bb += p.w[1].q - p.w[0].q;
-        const bool partial = red % kFp8Block != 0 && b == steps_of_term - 1;
-        if (!partial) {
+        if (GLU) bb += wave >= kWaves / 2 ? p.w[1].q - p.w[0].q : 0;
 #pragma unroll
-            for (int c = 0; c < S::kBCopies; ++c) copy16(bb, boff[c], st + S::kA + (wave * S::kBCopies + c) * 1024);
-        } else {
-            // the last, partial block of the reduction: zeros behind its end (the rows have zeros there, but 0 * NaN is NaN)
-#pragma unroll
-            for (int c = 0; c < S::kBCopies; ++c) {
-                const int load = wave * S::kBCopies + c;
+        for (int c = 0; c < S::kBCopies; ++c) {
+            const int load = wave * S::kBCopies + c;
+            if (!PARTIAL) {
+                copy16(bb, boff[c], st + S::kA + load * 1024);
+            } else {
+                // zeros behind the end of the reduction (the rows have zeros there, but 0 * NaN is NaN)
                 const int r = DX ? (load * 64 + lane) / (BN / 16) : load * 8 + (lane >> 3);
                 const int at = b * kFp8Block + (DX ? r : ((lane & 7) ^ ((r >> 1) & 7)) * 16);
                 copy16(at < red ? bb + boff[c] : (const uint8_t *)&g_fp8_zeros, st + S::kA + load * 1024);
             }
         }
-        bbase += DX ? (int64_t)128 * p.K : 128;
-        if (lane < S::kSLanes + (GLU ? 2 : 1)) copy4(sptr, st + S::kA + S::kB + wave * S::kSWave);
-        sptr += lane >= S::kSLanes ? (DX ? kbk * 4 : 4) : (b & 3) == 3 ? 4 : 0;
-        if (++pstage == STAGES) pstage = 0;
-        if (++pstep == KT) {
-            pstep = 0;
-            pt.index += stride;
-            if (pt.index < last) {
-                decode(pt);
-                start_tile();
-            } else {
-                more = false;
-            }
+        copy4(sptr, st + S::kA + S::kB + wave * S::kSWave);
+        int64_t a_step = 128, b_step = DX ? (int64_t)128 * p.K : 128, row_step = (b & 3) == 3 ? 4 : 0, w_step = DX ? kbk * 4 : 4;
+        if (DX) {
+            // to the second term's operands
+            const bool jump = pstep + 1 == steps_of_term && p.terms == 2;
+            a_step = jump ? p.a[1].q - p.a[0].q - (int64_t)(steps_of_term - 1) * 128 : a_step;
+            b_step = jump ? p.w[1].q - p.w[0].q - (int64_t)(steps_of_term - 1) * 128 * p.K : b_step;
+            row_step = jump ? p.a[1].scale - p.a[0].scale - (steps_of_term - 1) / 4 * 4 : row_step;
+            w_step = jump ? (const uint8_t *)p.w[1].scale - (const uint8_t *)p.w[0].scale - (int64_t)(steps_of_term - 1) * kbk * 4 : w_step;
         }
+        abase += a_step, bbase += b_step;
+        sptr += lane >= S::kSLanes ? w_step : row_step;
+        pstage = pstage + 1 == STAGES ? 0 : pstage + 1;
+        ++pstep;
     };
+    // (a tile has at least as many steps as there are stages)
+    look_up();
+    start_tile();
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i)
-        if (more) issue();
+    for (int i = 0; i < STAGES; ++i) issue();
+    publish<(STAGES - 1) * S::kOps>();
 
     // ---- the consumer's side
     // (a wave's row blocks are dealt in turn, so that a tile of few blocks keeps all rows of waves at work)
@@ -275,12 +305,17 @@ __global__ __launch_bounds__(kThreads) void fp8_tile_kernel(Fp8Product p) {
         woff = S::kA + (acol0 + l) * 128 + swizzled;
     } else {
         const int g = lane >> 4, il = lane & 15;
-        woff = S::kA + ((g >> 1) * 16 + (il >> 1)) * BN + (((acol0 >> 4) + (g & 1)) ^ ((il >> 1) << 1)) * 16 + (il & 1) * 8;
+        woff = S::kA + ((g >> 1) * 16 + (il >> 1)) * BN + (((acol0 >> 4) + (g & 1)) ^ spread(il >> 1)) * 16 + (il & 1) * 8;
     }
-    int cstage = 0;
+    int cstage = 0, newer = 0;
     while (true) {
         floatx16 acc[MI][NI];
         const int blocks = (cur.rows + 31) / 32;
+        nt.index = cur.index + stride;
+        const bool follows = nt.index < last;
+        if (follows) decode(nt);
+        else nt = cur;
+        look_up();
         // the steps of a tile whose waves have `rb` row blocks each (the last wave row one less)
         auto steps = [&](auto rb) {
         constexpr int RB = decltype(rb)::value;
@@ -290,90 +325,118 @@ __global__ __launch_bounds__(kThreads) void fp8_tile_kernel(Fp8Product p) {
             for (int j = 0; j < NI; ++j)
 #pragma unroll
                 for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.0f;
-        for (int step = 0; step < KT; ++step) {
+        union Frag {
+            uint4_t v[2];
+            intx2 t[4];
+            intx8 i;
+        };
+        Frag fw[NI][2], fa[2];
+        int xscale[2];
+        float wscale[2], wlast = 0.0f;  // the weights' scales of this step, and of the last one's last block
+        floatx16 part[NI];
+        uint32_t st = lds0 + cstage * S::kStage;
+        auto fetch_w = [&](int s) {
+#pragma unroll
+            for (int j = 0; j < NI; ++j) {
+                if (!DX) {
+                    constexpr int kNext = GLU ? BNC * 128 : 32 * 128;  // to the wave's next block of columns
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+                        fw[j][s].v[u] = *(lds_uint4_ptr)(uintptr_t)(((st + woff) ^ (64 * s + 32 * u)) + j * kNext);
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        fw[j][s].t[q] = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                            (lds_intx2_ptr)(uintptr_t)(((st + woff) ^ (32 * j)) + (s * 64 + (q >> 1) * 32 + (q & 1) * 8) * BN));
+                }
+            }
+        };
+        auto fetch_scales = [&]() {
+#pragma unroll
+            for (int j = 0; j < (GLU ? 2 : 1); ++j)
+                wscale[j] = *(lds_float_ptr)(uintptr_t)(st + S::kA + S::kB + wave * S::kSWave + (S::kSLanes + j) * 4);
+        };
+        auto fetch = [&](int i, int s) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+                fa[s].v[u] = *(lds_uint4_ptr)(uintptr_t)(((st + xoff) ^ (64 * s + 32 * u)) + i * WM * 32 * 128);
+        };
+        auto fetch_scale = [&](int i, int b) {
+            xscale[i & 1] = (int)(*(lds_uint32_ptr)(uintptr_t)(st + soff + i * WM * 32 / S::kSLanes * S::kSWave) >> ((b & 3) * 8));
+        };
+        auto multiply = [&](int i, int s, int j) {
+            if (s == 0) {
+#pragma unroll
+                for (int q = 0; q < 16; ++q) part[j][q] = 0.0f;
+            }
+            part[j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fw[j][s].i, fa[s].i, part[j], 0, 0, 0, 127, 0, xscale[i & 1]);
+        };
+        auto add = [&](int i, int j, float scale) {
+#pragma unroll
+            for (int q = 0; q < 16; ++q) acc[i][j][q] = __builtin_fmaf(scale, part[j][q], acc[i][j][q]);
+        };
+        // The matrix unit never waits for the additions: a block's partial sum is added to its running sum while the next block's
+        // second half, or the next row block's first, is multiplied.  A row block's fragments of a sub-step are asked for as soon
+        // as those of the row block before have gone into the unit, those of the next step behind the barrier, which lies before
+        // the step's last sub-step.
+#pragma unroll
+        for (int q = 0; q < 16; ++q) part[NI - 1][q] = 0.0f;
+        fetch_w(0);
+        fetch(0, 0);
+        fetch_scale(0, 0);
+        fetch_scales();
+        fetch_w(1);
+        fetch(0, 1);
+        // (the last steps' copies are the next tile's first; behind the last tile this one's again, which nobody reads)
+        int step = 0;
+        for (int end = KT - STAGES; step < KT; end = KT) {
+          if (step == KT - STAGES) start_tile();
+          for (; step < end; ++step) {
             const int b = DX && step >= steps_of_term ? step - steps_of_term : step;
-            if (more || step + STAGES - 2 < KT - 1) publish<(STAGES - 2) * S::kOps>();
-            else publish<0>();
-            if (more) issue();
-            const uint32_t st = lds0 + cstage * S::kStage;
-            float wscale[2];
-#pragma unroll
-            for (int j = 0; j < (GLU ? 2 : 1); ++j) wscale[j] = *(lds_float_ptr)(uintptr_t)(st + S::kA + S::kB + wave * S::kSWave + (S::kSLanes + j) * 4);
-            union Frag {
-                uint4_t v[2];
-                intx2 t[4];
-                intx8 i;
-            };
-            Frag fw[NI][2];
-#pragma unroll
-            for (int j = 0; j < NI; ++j)
-#pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    if (!DX) {
-                        constexpr int kNext = GLU ? BNC * 128 : 32 * 128;  // to the wave's next block of columns
-#pragma unroll
-                        for (int u = 0; u < 2; ++u)
-                            fw[j][s].v[u] = *(lds_uint4_ptr)(uintptr_t)(((st + woff) ^ (64 * s + 32 * u)) + j * kNext);
-                    } else {
-#pragma unroll
-                        for (int q = 0; q < 4; ++q)
-                            fw[j][s].t[q] = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                                (lds_intx2_ptr)(uintptr_t)(((st + woff) ^ (32 * j)) + (s * 64 + (q >> 1) * 32 + (q & 1) * 8) * BN));
-                    }
-                }
-            // The matrix unit never waits for the additions: a block's partial sum is added to its running sum while the next
-            // block's second half, or the next row block's first, is multiplied.  A row block's fragments of a sub-step are
-            // asked for as soon as those of the row block before have gone into the unit.
-            Frag fa[2];
-            int xscale[2];
-            auto fetch = [&](int i, int s) {
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-                    fa[s].v[u] = *(lds_uint4_ptr)(uintptr_t)(((st + xoff) ^ (64 * s + 32 * u)) + i * WM * 32 * 128);
-            };
-            auto fetch_scale = [&](int i) {
-                xscale[i & 1] = (int)(*(lds_uint32_ptr)(uintptr_t)(st + soff + i * WM * 32 / S::kSLanes * S::kSWave) >> ((b & 3) * 8));
-            };
-            floatx16 part[NI];
-            auto multiply = [&](int i, int s, int j) {
-                if (s == 0) {
-#pragma unroll
-                    for (int q = 0; q < 16; ++q) part[j][q] = 0.0f;
-                }
-                part[j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fw[j][s].i, fa[s].i, part[j], 0, 0, 0, 127, 0, xscale[i & 1]);
-            };
-            auto add = [&](int i, int j) {
-#pragma unroll
-                for (int q = 0; q < 16; ++q) acc[i][j][q] = __builtin_fmaf(wscale[GLU ? j : 0], part[j][q], acc[i][j][q]);
-            };
-            fetch(0, 0);
-            fetch_scale(0);
-            fetch(0, 1);
 #pragma unroll
             for (int i = 0; i < RB; ++i) {
+                multiply(i, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+                if (i == 0) add(RB - 1, NI - 1, wlast);
+                else add(i - 1, NI - 1, wscale[GLU ? NI - 1 : 0]);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int s = 0; s < 2; ++s) {
-#pragma unroll
-                    for (int j = 0; j < NI; ++j) {
-                        multiply(i, s, j);
-                        __builtin_amdgcn_sched_barrier(0);
-                        if (s == 0 && j == 0 && i > 0) {
-                            add(i - 1, NI - 1);
-                            __builtin_amdgcn_sched_barrier(0);
-                        }
-                    }
-                    if (i + 1 < RB) {
-                        fetch(i + 1, s);
-                        if (s == 0) fetch_scale(i + 1);
-                    }
+                for (int j = 1; j < NI; ++j) multiply(i, 0, j);
+                __builtin_amdgcn_sched_barrier(0);
+                const int bn = DX && step + 1 >= steps_of_term ? step + 1 - steps_of_term : step + 1;
+                if (i + 1 < RB) {
+                    fetch(i + 1, 0);
+                    fetch_scale(i + 1, b);
+                } else {
+                    wlast = wscale[GLU ? NI - 1 : 0];
+                    publish_past<(STAGES - 2) * S::kOps>(newer);
+                    newer = 0;
+                    cstage = cstage + 1 == STAGES ? 0 : cstage + 1;
+                    st = lds0 + cstage * S::kStage;
+                    fetch_w(0);  // (behind the last step: of the next tile, or stale; not used)
                 }
 #pragma unroll
-                for (int j = 0; j < NI - 1; ++j) add(i, j);
+                for (int j = 0; j < NI; ++j) multiply(i, 1, j);
+                __builtin_amdgcn_sched_barrier(0);
+                if (i + 1 < RB) {
+                    fetch(i + 1, 1);
+#pragma unroll
+                    for (int j = 0; j < NI - 1; ++j) add(i, j, wscale[GLU ? j : 0]);
+                } else {
+                    issue();
+#pragma unroll
+                    for (int j = 0; j < NI - 1; ++j) add(i, j, wscale[GLU ? j : 0]);
+                    fetch(0, 0);
+                    fetch_scale(0, bn);
+                    fetch_w(1);
+                    fetch(0, 1);
+                    fetch_scales();
+                }
                 __builtin_amdgcn_sched_barrier(0);
             }
-            add(RB - 1, NI - 1);
-            if (++cstage == STAGES) cstage = 0;
+          }
         }
+        add(RB - 1, NI - 1, wlast);
         };
         const int mine = (blocks + WM - 1) / WM;
         if constexpr (MI >= 4)
@@ -384,135 +447,183 @@ __global__ __launch_bounds__(kThreads) void fp8_tile_kernel(Fp8Product p) {
             if (mine == 2) steps(std::integral_constant<int, 2>{});
         if (mine == 1) steps(std::integral_constant<int, 1>{});
 
-        // ---- output: a lane's runs of four columns, joined to eight with the other half of the wave
-        auto store = [&](void *base, int64_t at, const float (&v)[16], int n0) {
-#pragma unroll
-            for (int t = 0; t < 4; t += 2) {
+        // ---- output.  A lane holds runs of four columns of one row; a wave turns them in its 2 KiB of LDS into whole lines of a
+        // row (FWD, DX: 16 rows of 128 bytes at a time; gated: 32 rows of 64): stores of 32-byte pieces took as long as the
+        // multiplication of a tile of six steps (7 us; a request is a request whatever its size).
+        auto store16 = [&](void *base, int64_t row, int n, const uint4_t v) {
+            TO *dst = (TO *)base + row * cols + n;
+            if (cols % 8 == 0) {
+                if (n < cols) *(uint4_t *)dst = v;
+            } else {
                 union {
-                    TO e[4];
-                    uint32_t u[2];
-                } a, bq;
+                    uint4_t v;
+                    TO e[8];
+                } u;
+                u.v = v;
 #pragma unroll
-                for (int q = 0; q < 4; ++q) a.e[q] = from_f32<TO>(v[4 * t + q]), bq.e[q] = from_f32<TO>(v[4 * t + 4 + q]);
-                const auto x0 = __builtin_amdgcn_permlane32_swap(a.u[0], bq.u[0], false, false);
-                const auto x1 = __builtin_amdgcn_permlane32_swap(a.u[1], bq.u[1], false, false);
-                const int n = n0 + 8 * (t + half);
-                TO *dst = (TO *)base + at + n;
-                const uint4_t out = {x0[0], x1[0], x0[1], x1[1]};
-                if (cols % 8 == 0) {
-                    if (n < cols) *(uint4_t *)dst = out;
-                } else {
-                    union {
-                        uint4_t v;
-                        TO e[8];
-                    } u;
-                    u.v = out;
-#pragma unroll
-                    for (int q = 0; q < 8; ++q)
-                        if (n + q < cols) dst[q] = u.e[q];
-                }
+                for (int q = 0; q < 8; ++q)
+                    if (n + q < cols) dst[q] = u.e[q];
             }
         };
+        unsigned char *const place = turn + wave * S::kOut;
+        auto pack = [&](const float (&v)[4]) {
+            union {
+                TO e[4];
+                uint2_t u;
+            } a;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) a.e[q] = from_f32<TO>(v[q]);
+            return a.u;
+        };
+        // 32 columns of a row block, from f(q), the lane's q-th value
+        auto store_narrow = [&](void *base, int i, auto f) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const float v[4] = {f(4 * t), f(4 * t + 1), f(4 * t + 2), f(4 * t + 3)};
+                *(uint2_t *)(place + l * 64 + ((t ^ ((l >> 1) & 3)) * 16) + half * 8) = pack(v);
+            }
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int r = 16 * u + (lane >> 2), c = lane & 3, row = (i * WM + wm) * 32 + r;
+                const uint4_t v = *(const uint4_t *)(place + r * 64 + ((c ^ ((r >> 1) & 3)) * 16));
+                if (row < cur.rows) store16(base, cur.row0 + row, cur.col0 + acol0 + c * 8, v);
+            }
+            __builtin_amdgcn_wave_barrier();
+        };
+        // (whole row blocks only: what is issued for certain)
+        int whole = (cur.rows / 32 - wm + WM - 1) / WM;
+        if (whole < 0 || cols % BNC != 0) whole = 0;
 #pragma unroll
         for (int i = 0; i < MI; ++i) {
-            const int r = (i * WM + wm) * 32 + l;
             if (i * WM + wm < blocks) {
-                const bool live = r < cur.rows;
-                const int64_t at = (int64_t)(cur.row0 + r) * cols;
                 if (GLU) {
-                    const int n0 = cur.col0 + acol0;
-                    float e[16], g[16], v[16];
+                    if (p.e_out != nullptr) store_narrow(p.e_out, i, [&](int q) { return acc[i][0][q]; });
+                    if (p.g_out != nullptr) store_narrow(p.g_out, i, [&](int q) { return acc[i][NI - 1][q]; });
 #pragma unroll
-                    for (int q = 0; q < 16; ++q) {
-                        e[q] = acc[i][0][q], g[q] = acc[i][NI - 1][q];
-                        v[q] = e[q] * sigmoid_f32(e[q]) * g[q];
-                    }
-                    if (p.e_out != nullptr && live) store(p.e_out, at, e, n0);
-                    if (p.g_out != nullptr && live) store(p.g_out, at, g, n0);
+                    for (int q = 0; q < 16; ++q) acc[i][0][q] = acc[i][0][q] * sigmoid_f32(acc[i][0][q]) * acc[i][NI - 1][q];
                     if (!HQ) {
-                        if (live) store(p.out, at, v, n0);
+                        store_narrow(p.out, i, [&](int q) { return acc[i][0][q]; });
                     } else {
-                        float a = 0.0f;
+                        uint32_t a = 0u;
 #pragma unroll
                         for (int q = 0; q < 16; ++q) {
-                            if (n0 + 8 * (q / 4) + 4 * half + q % 4 >= cols) v[q] = 0.0f;  // (the padding of the rows)
-                            a = __builtin_fmaxf(a, fp8_finite_abs(v[q]));
-                            acc[i][0][q] = v[q];
+                            if (cols % kFp8Block != 0 && cur.col0 + acol0 + 8 * (q / 4) + 4 * half + q % 4 >= cols) acc[i][0][q] = 0.0f;  // (the rows' padding)
+                            a = fp8_wider(a, acc[i][0][q]);
                         }
-                        a = __builtin_fmaxf(a, __shfl_xor(a, 32));
-                        if (half == 0) amax[r * WN + wn] = a;
+                        if (__any(fp8_unusual(a))) {
+                            a = 0u;
+#pragma unroll
+                            for (int q = 0; q < 16; ++q) a = fp8_wider(a, fp8_finite_abs(acc[i][0][q])), acc[i][0][q] = fp8_finite(acc[i][0][q]);
+                        }
+                        const uint32_t other = (uint32_t)__shfl_xor((int)a, 32);
+                        if (half == 0) amax[((i * WM + wm) * 32 + l) * WN + wn] = a > other ? a : other;
                     }
                 } else {
+                    static_assert(GLU || NI == 2, "a wave's columns are a line of 16-bit values");
 #pragma unroll
-                    for (int j = 0; j < NI; ++j) {
-                        float v[16];
+                    for (int h = 0; h < 2; ++h) {
+                        if (l >> 4 == h) {
 #pragma unroll
-                        for (int q = 0; q < 16; ++q) v[q] = acc[i][j][q];
-                        if (live) store(p.out, at, v, cur.col0 + acol0 + j * 32);
+                            for (int j = 0; j < NI; ++j)
+#pragma unroll
+                                for (int t = 0; t < 4; ++t) {
+                                    const float v[4] = {acc[i][j][4 * t], acc[i][j][4 * t + 1], acc[i][j][4 * t + 2], acc[i][j][4 * t + 3]};
+                                    *(uint2_t *)(place + (l & 15) * 128 + (((4 * j + t) ^ (l & 7)) * 16) + half * 8) = pack(v);
+                                }
+                        }
+                        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            const int r = 8 * u + (lane >> 3), c = lane & 7, row = (i * WM + wm) * 32 + 16 * h + r;
+                            const uint4_t v = *(const uint4_t *)(place + r * 128 + ((c ^ (r & 7)) * 16));
+                            if (row < cur.rows) store16(p.out, cur.row0 + row, cur.col0 + acol0 + c * 8, v);
+                        }
+                        __builtin_amdgcn_wave_barrier();
                     }
                 }
             }
         }
+        newer = GLU ? whole * 2 * ((HQ ? 0 : 1) + (p.e_out != nullptr) + (p.g_out != nullptr)) : whole * 4;
         if (HQ) {
-            // a row's 128 columns are with the WN waves of its wave row: the largest magnitude goes through LDS
+            // a row's 128 columns are with the WN waves of its wave row: the largest magnitude goes through LDS, and so do the
+            // quantised rows, kWaves * 16 of them at a time, which leave as whole lines
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
             const int64_t ldh = fp8_ld(cols), ldh_scale = fp8_ld_scale(cols);
+            constexpr int kRound = kWaves * S::kOut / 128;  // rows
+            static_assert(kRound % (32 * WM) == 0, "whole row blocks of every wave row");
 #pragma unroll
             for (int i = 0; i < MI; ++i) {
                 const int r = (i * WM + wm) * 32 + l;
-                if (i * WM + wm < blocks && r < cur.rows) {
-                    float a = 0.0f;
+                unsigned char *const line = turn + r % kRound * 128;
+                if (i * WM + wm < blocks) {
+                    uint32_t a = 0u;
 #pragma unroll
-                    for (int w = 0; w < WN; ++w) a = __builtin_fmaxf(a, amax[r * WN + w]);
+                    for (int w = 0; w < WN; ++w) a = a > amax[r * WN + w] ? a : amax[r * WN + w];
                     const int byte = fp8_scale_byte(a);
                     const float inverse = fp8_inverse_of(byte);
-                    uint8_t *dst = p.hq + (cur.row0 + r) * ldh + cur.col0 + acol0;
-                    if (wn == 0 && half == 0) p.hq_scale[(cur.row0 + r) * ldh_scale + cur.col0 / kFp8Block] = (uint8_t)byte;
+                    if (wn == 0 && half == 0 && r < cur.rows)
+                        p.hq_scale[(cur.row0 + r) * ldh_scale + cur.col0 / kFp8Block] = (uint8_t)byte;
 #pragma unroll
-                    for (int t = 0; t < 4; t += 2) {
+                    for (int t = 0; t < 4; ++t) {
                         const floatx16 &v = acc[i][0];
-                        const uint32_t x = fp8_pack4(v[4 * t], v[4 * t + 1], v[4 * t + 2], v[4 * t + 3], inverse);
-                        const uint32_t y = fp8_pack4(v[4 * t + 4], v[4 * t + 5], v[4 * t + 6], v[4 * t + 7], inverse);
-                        const auto z = __builtin_amdgcn_permlane32_swap(x, y, false, false);
-                        *(uint2_t *)(dst + 8 * (t + half)) = uint2_t{z[0], z[1]};
+                        const int c = 2 * wn + t / 2;  // 16-byte chunk of the line
+                        *(uint32_t *)(line + ((c ^ (r & 7)) * 16) + t % 2 * 8 + half * 4) =
+                            fp8_pack4(v[4 * t], v[4 * t + 1], v[4 * t + 2], v[4 * t + 3], inverse);
                     }
+                }
+                constexpr int kBlocks = kRound / (32 * WM);  // row blocks of a wave in a round
+                if (i % kBlocks == kBlocks - 1 || i == MI - 1) {
+                    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
+                    const int first = i / kBlocks * kRound;
+#pragma unroll
+                    for (int u = 0; u < kRound / 8 / kWaves; ++u) {
+                        const int rr = (u * kWaves + wave) * 8 + (lane >> 3), c = lane & 7;
+                        if (first + rr < cur.rows)
+                            *(uint4_t *)(p.hq + (cur.row0 + first + rr) * ldh + cur.col0 + c * 16) =
+                                *(const uint4_t *)(turn + rr * 128 + ((c ^ (rr & 7)) * 16));
+                    }
+                    if (i != MI - 1) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
                 }
             }
         }
-        cur.index += stride;
-        if (cur.index >= last) break;
-        decode(cur);
+        if (!follows) break;
+        cur = nt;
     }
+    publish<0>();  // (no copy is on its way into this LDS when the workgroup ends)
 }
 
-template <bool DX, bool GLU, bool HQ, int WM, int WN, int MI, int NI, int STAGES, typename TO>
+template <bool DX, bool GLU, bool HQ, bool PARTIAL, int WM, int WN, int MI, int NI, int STAGES, typename TO>
 int launch(const Fp8Product &p, hipStream_t stream) {
     using S = Shape<WM, WN, MI, NI, STAGES>;
     constexpr int kLds = S::kLds + (HQ ? S::BM * WN * 4 : 0);
     static_assert(kLds <= 160 * 1024, "a CU's LDS");
     constexpr int kPerCu = 160 * 1024 / kLds < 2 ? 1 : 2;
-    auto kern = fp8_tile_kernel<DX, GLU, HQ, WM, WN, MI, NI, STAGES, TO>;
+    auto kern = fp8_tile_kernel<DX, GLU, HQ, PARTIAL, WM, WN, MI, NI, STAGES, TO>;
     static PerDeviceOnce once;
     const hipError_t e = once.run([&] {
         return hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
     });
     if (e != hipSuccess) return (int)e;
     const int grid = device_info().cu_count / kXcd * kXcd * kPerCu;
-    kern<<<grid, kThreads, kLds, stream>>>(p);
+    kern<<<grid, S::kThreads, kLds, stream>>>(p);
     return launch_status();
 }
 
-template <int WM, int WN, int MI, int NI, int STAGES, typename TO>
+template <bool PARTIAL, int WM, int WN, int MI, int NI, int STAGES, typename TO>
 int launch_mode(const Fp8Product &p, hipStream_t stream) {
-    if (p.dx) return launch<true, false, false, WM, WN, MI, NI, STAGES, TO>(p, stream);
-    if (p.glu) return p.hq != nullptr ? launch<false, true, true, WM, WN, MI, NI, STAGES, TO>(p, stream)
-                                        : launch<false, true, false, WM, WN, MI, NI, STAGES, TO>(p, stream);
-    return launch<false, false, false, WM, WN, MI, NI, STAGES, TO>(p, stream);
+    if (p.dx) return launch<true, false, false, PARTIAL, WM, WN, MI, NI, STAGES, TO>(p, stream);
+    if (p.glu) return launch<false, true, false, PARTIAL, WM, WN, MI, NI, STAGES, TO>(p, stream);
+    return launch<false, false, false, PARTIAL, WM, WN, MI, NI, STAGES, TO>(p, stream);
 }
 
 template <typename TO>
 int launch_shape(const Fp8Product &p, hipStream_t stream) {
-    return launch_mode<2, 4, 4, 2, 2, TO>(p, stream);
+    const int red = p.dx ? p.N : p.K;
+    if (fp8_blocks(red) * (p.dx ? p.terms : 1) < 2) return MFL_ERR_UNSUPPORTED;
+    if (p.hq == nullptr)
+        return red % kFp8Block != 0 ? launch_mode<true, 2, 2, 2, 2, 2, TO>(p, stream) : launch_mode<false, 2, 2, 2, 2, 2, TO>(p, stream);
+    return red % kFp8Block != 0 ? launch<false, true, true, true, 2, 4, 4, 2, 2, TO>(p, stream) : launch<false, true, true, false, 2, 4, 4, 2, 2, TO>(p, stream);
 }
 
 }  // namespace

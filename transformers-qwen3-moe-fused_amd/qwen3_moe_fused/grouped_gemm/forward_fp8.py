@@ -7,7 +7,6 @@ past ``sum(m_sizes)`` left unwritten, ``m_sizes`` stays on the device.  The refe
 """
 from __future__ import annotations
 
-import ctypes
 from typing import Optional
 
 import torch
@@ -18,9 +17,13 @@ from ._common import is_int_tensor
 
 # MFL_FP8_*: whose workspace is asked for
 FWD, DX, GLU, GLU_BWD, MLP = 0, 1, 2, 3, 4
+_NO_WORKSPACE = -5  # MFL_ERR_WORKSPACE
+# Rows per expert up to which the forward product and the gated unit are called without scratch memory first: decode sizes do
+# without, and asking for it and allocating it is a fifth of such a call's time on the host.
+_DECODE_ROWS = 8
 
 
-def fp8_weight(weight: torch.Tensor, scale: torch.Tensor) -> "ctypes._Pointer":
+def fp8_weight(weight: torch.Tensor, scale: torch.Tensor) -> "_lib.Fp8Weight":
     return _lib.Fp8Weight(weight.data_ptr(), scale.data_ptr())
 
 
@@ -31,6 +34,16 @@ def fp8_workspace(op: int, like: torch.Tensor, src_rows: int, rows: int, n: int,
         return None, None, 0
     ws = torch.empty(size, device=like.device, dtype=torch.uint8)
     return ws, ws.data_ptr(), size
+
+
+def call_with_workspace(call, op: int, like: torch.Tensor, src_rows: int, rows: int, n: int, k: int, experts: int) -> int:
+    """``call(address, size)``'s status, with scratch memory where it needs some."""
+    if rows <= _DECODE_ROWS * experts:
+        rc = call(None, 0)
+        if rc != _NO_WORKSPACE:
+            return rc
+    _keep, ws, size = fp8_workspace(op, like, src_rows, rows, n, k, experts)
+    return call(ws, size)
 
 
 def check_rows(m_sizes: torch.Tensor, *rows: torch.Tensor) -> None:
@@ -54,10 +67,10 @@ def grouped_gemm_forward_fp8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Te
     with _lib.on_device_of(x):
         y = torch.empty((rows, n), device=x.device, dtype=x.dtype if dtype is None else dtype)
         ms = _lib.as_index_tensor(m_sizes)
-        _keep, ws, ws_bytes = fp8_workspace(FWD, x, rows, rows, n, k, experts)
-        rc = _lib.lib().mfl_gemm_fwd_fp8(x.data_ptr(), rows, None, 1, fp8_weight(w, w_scale), ms.data_ptr(),
-                                         _lib.itype_code(ms.dtype), y.data_ptr(), rows, n, k, experts,
-                                         _lib.dtype_code(x.dtype), _lib.dtype_code(y.dtype), ws, ws_bytes, _lib.stream())
+        entry, weight = _lib.lib().mfl_gemm_fwd_fp8, fp8_weight(w, w_scale)
+        args = (x.data_ptr(), rows, None, 1, weight, ms.data_ptr(), _lib.itype_code(ms.dtype), y.data_ptr(), rows, n, k, experts,
+                _lib.dtype_code(x.dtype), _lib.dtype_code(y.dtype))
+        rc = call_with_workspace(lambda ws, size: entry(*args, ws, size, _lib.stream()), FWD, x, rows, rows, n, k, experts)
     _lib.check(rc, "mfl_gemm_fwd_fp8")
     return y
 
