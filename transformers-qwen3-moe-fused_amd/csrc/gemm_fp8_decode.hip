@@ -94,13 +94,19 @@ __global__ __launch_bounds__(kWaves * 64, 2) void fp8_decode_kernel(Fp8Product p
     const int c = lane & 15, g = lane >> 4;
     int e, rows;
     int64_t row0;
+    // (up to 64 rows, the whole index is read along with the row counts: what a call of a few rows takes is the number of loads
+    // one behind the other)
+    const bool early = p.row_idx != nullptr && p.R <= 64;
+    int index = 0;
+    if (early) index = p.row_idx[lane < p.R ? lane : 0];
     if (!find_rows(p, blockIdx.y, lane, e, row0, rows)) return;
     const int n0 = blockIdx.x * 16 * TILES;
     const int blocks = fp8_blocks(p.K), nbn = fp8_blocks(p.N);
 
     int64_t src = row0 + (c < rows ? c : rows - 1);
     int looked_up = 0;
-    if (p.row_idx != nullptr) looked_up = p.row_idx[src];
+    if (early) looked_up = __shfl(index, (int)src);
+    else if (p.row_idx != nullptr) looked_up = p.row_idx[src];
 
     union Frag {
         uint4_t v[2];
@@ -131,6 +137,16 @@ __global__ __launch_bounds__(kWaves * 64, 2) void fp8_decode_kernel(Fp8Product p
 #pragma unroll
     for (int t = 0; t < PIECES; ++t) acc[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
     for (int b0 = wave; b0 < blocks; b0 += kWaves * AHEAD) {
+        // the weights' scales of the chunk: lane t AHEAD + u that of piece t in block b0 + 4 u
+        static_assert(PIECES * AHEAD <= 64, "one scale a lane");
+        float scales = 0.0f;
+        {
+            const int t = lane / AHEAD, b = b0 + kWaves * (lane % AHEAD);
+            int nb = (n0 + 16 * (GLU ? t / 2 : t)) / kFp8Block;
+            if (nb >= nbn) nb = nbn - 1;
+            if (t < PIECES && b < blocks)
+                scales = (GLU && t & 1 ? p.w[1].scale : p.w[0].scale)[((int64_t)e * nbn + nb) * blocks + b];
+        }
 #pragma unroll
         for (int t = 0; t < kBuffers - 1 && t < PIECES; ++t) load(t, b0);
         // the rows' blocks, quantised
@@ -186,16 +202,13 @@ __global__ __launch_bounds__(kWaves * 64, 2) void fp8_decode_kernel(Fp8Product p
 #pragma unroll
         for (int t = 0; t < PIECES; ++t) {
             if (t + kBuffers - 1 < PIECES) load(t + kBuffers - 1, b0);
-            int nb = (n0 + 16 * (GLU ? t / 2 : t)) / kFp8Block;
-            if (nb >= nbn) nb = nbn - 1;
-            const float *scale = p.w[GLU ? t & 1 : 0].scale + ((int64_t)e * nbn + nb) * blocks;
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
                 const int b = b0 + kWaves * u;
                 if (b < blocks) {
                     const floatx4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
                     const floatx4 part = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw[t % kBuffers][u].i, q[u], zero, 0, 0, 0, 127, 0, byte[u]);
-                    const float s = scale[b];
+                    const float s = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(scales), t * AHEAD + u));
 #pragma unroll
                     for (int i = 0; i < 4; ++i) acc[t][i] = __builtin_fmaf(s, part[i], acc[t][i]);
                 }

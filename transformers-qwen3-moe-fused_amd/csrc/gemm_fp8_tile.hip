@@ -4,7 +4,7 @@
 //   gated           the same for two matrices, out = silu(gate) * up
 //   input gradient  out[r, k] = sum_b S[e, b, k / 128] sd[r, b] sum_{n in block b} d[r, n] w[e, n, k], of one or two terms
 //
-// A workgroup of eight waves owns a tile of BM rows and BN columns of one expert and walks the reduction in steps of one scale
+// A workgroup of four or eight waves owns a tile of BM rows and BN columns of one expert and walks the reduction in steps of one scale
 // block, 128 bytes of every row.  A stage in LDS is one such step: BM x 128 row bytes, BN x 128 weight bytes, and the dwords
 // that hold the rows' scale bytes.  Everything arrives by direct copies (global_load_lds) that the wave counts itself; one
 // barrier a step publishes the stage that has landed and frees the one before.  The tiles of a workgroup are one stream of
@@ -92,8 +92,7 @@ struct Shape {
     static constexpr int kACopies = kA / 1024 / kWaves, kBCopies = kB / 1024 / kWaves;
     static constexpr int kOps = kACopies + kBCopies + 1;  // vector-memory operations a wave issues for a stage
     static constexpr int kTables = (2 * (kMaxExperts + 1) * 4 + 127) / 128 * 128;
-    static constexpr int kOut = 2048;  // a wave's place for turning its output
-    static constexpr int kLds = STAGES * kStage + kTables + kWaves * kOut;
+    static constexpr int kLds = STAGES * kStage + kTables;
     static_assert(kA % (1024 * kWaves) == 0 && kB % (1024 * kWaves) == 0 && kSLanes + 2 <= 64, "whole copies");
 };
 
@@ -108,8 +107,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void fp8_tile_kernel(Fp8Product p)
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
     int *const tab_rows = (int *)(smem + STAGES * S::kStage);
     int *const tab_tiles = tab_rows + kMaxExperts + 1;
-    unsigned char *const turn = smem + STAGES * S::kStage + S::kTables;         // the waves' places
-    uint32_t *const amax = (uint32_t *)(smem + S::kLds);                            // (HQ) per row and wave column
+    uint32_t *const amax = (uint32_t *)(smem + S::kLds);  // (HQ) per row and wave column
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave % WM, wn = wave / WM;
@@ -447,9 +445,9 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void fp8_tile_kernel(Fp8Product p)
             if (mine == 2) steps(std::integral_constant<int, 2>{});
         if (mine == 1) steps(std::integral_constant<int, 1>{});
 
-        // ---- output.  A lane holds runs of four columns of one row; a wave turns them in its 2 KiB of LDS into whole lines of a
-        // row (FWD, DX: 16 rows of 128 bytes at a time; gated: 32 rows of 64): stores of 32-byte pieces took as long as the
-        // multiplication of a tile of six steps (7 us; a request is a request whatever its size).
+        // ---- output.  A lane holds runs of four columns of one row, joined to eight with the other half of the wave.  (Turned in
+        // LDS first, so that whole lines of a row leave at once, the output took as long or longer: 43 against 39 thousand
+        // clocks for a tile of six steps.  Streaming stores: 159 against 148 us for the forward product of 32768 rows.)
         auto store16 = [&](void *base, int64_t row, int n, const uint4_t v) {
             TO *dst = (TO *)base + row * cols + n;
             if (cols % 8 == 0) {
@@ -465,7 +463,6 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void fp8_tile_kernel(Fp8Product p)
                     if (n + q < cols) dst[q] = u.e[q];
             }
         };
-        unsigned char *const place = turn + wave * S::kOut;
         auto pack = [&](const float (&v)[4]) {
             union {
                 TO e[4];
@@ -475,21 +472,18 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void fp8_tile_kernel(Fp8Product p)
             for (int q = 0; q < 4; ++q) a.e[q] = from_f32<TO>(v[q]);
             return a.u;
         };
-        // 32 columns of a row block, from f(q), the lane's q-th value
-        auto store_narrow = [&](void *base, int i, auto f) {
+        // 32 columns of a row block from the wave's column n0 on, from f(q), the lane's q-th value
+        auto store_block = [&](void *base, int i, auto f, int n0) {
+            const int r = (i * WM + wm) * 32 + l;
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const float v[4] = {f(4 * t), f(4 * t + 1), f(4 * t + 2), f(4 * t + 3)};
-                *(uint2_t *)(place + l * 64 + ((t ^ ((l >> 1) & 3)) * 16) + half * 8) = pack(v);
+            for (int t = 0; t < 4; t += 2) {
+                const float va[4] = {f(4 * t), f(4 * t + 1), f(4 * t + 2), f(4 * t + 3)};
+                const float vb[4] = {f(4 * t + 4), f(4 * t + 5), f(4 * t + 6), f(4 * t + 7)};
+                const uint2_t a = pack(va), b = pack(vb);
+                const auto x0 = __builtin_amdgcn_permlane32_swap(a[0], b[0], false, false);
+                const auto x1 = __builtin_amdgcn_permlane32_swap(a[1], b[1], false, false);
+                if (r < cur.rows) store16(base, cur.row0 + r, cur.col0 + acol0 + n0 + 8 * (t + half), uint4_t{x0[0], x1[0], x0[1], x1[1]});
             }
-            __builtin_amdgcn_wave_barrier();
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int r = 16 * u + (lane >> 2), c = lane & 3, row = (i * WM + wm) * 32 + r;
-                const uint4_t v = *(const uint4_t *)(place + r * 64 + ((c ^ ((r >> 1) & 3)) * 16));
-                if (row < cur.rows) store16(base, cur.row0 + row, cur.col0 + acol0 + c * 8, v);
-            }
-            __builtin_amdgcn_wave_barrier();
         };
         // (whole row blocks only: what is issued for certain)
         int whole = (cur.rows / 32 - wm + WM - 1) / WM;
@@ -498,12 +492,12 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void fp8_tile_kernel(Fp8Product p)
         for (int i = 0; i < MI; ++i) {
             if (i * WM + wm < blocks) {
                 if (GLU) {
-                    if (p.e_out != nullptr) store_narrow(p.e_out, i, [&](int q) { return acc[i][0][q]; });
-                    if (p.g_out != nullptr) store_narrow(p.g_out, i, [&](int q) { return acc[i][NI - 1][q]; });
+                    if (p.e_out != nullptr) store_block(p.e_out, i, [&](int q) { return acc[i][0][q]; }, 0);
+                    if (p.g_out != nullptr) store_block(p.g_out, i, [&](int q) { return acc[i][NI - 1][q]; }, 0);
 #pragma unroll
                     for (int q = 0; q < 16; ++q) acc[i][0][q] = acc[i][0][q] * sigmoid_f32(acc[i][0][q]) * acc[i][NI - 1][q];
                     if (!HQ) {
-                        store_narrow(p.out, i, [&](int q) { return acc[i][0][q]; });
+                        store_block(p.out, i, [&](int q) { return acc[i][0][q]; }, 0);
                     } else {
                         uint32_t a = 0u;
 #pragma unroll
@@ -520,70 +514,37 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void fp8_tile_kernel(Fp8Product p)
                         if (half == 0) amax[((i * WM + wm) * 32 + l) * WN + wn] = a > other ? a : other;
                     }
                 } else {
-                    static_assert(GLU || NI == 2, "a wave's columns are a line of 16-bit values");
+                    
+
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if (l >> 4 == h) {
-#pragma unroll
-                            for (int j = 0; j < NI; ++j)
-#pragma unroll
-                                for (int t = 0; t < 4; ++t) {
-                                    const float v[4] = {acc[i][j][4 * t], acc[i][j][4 * t + 1], acc[i][j][4 * t + 2], acc[i][j][4 * t + 3]};
-                                    *(uint2_t *)(place + (l & 15) * 128 + (((4 * j + t) ^ (l & 7)) * 16) + half * 8) = pack(v);
-                                }
-                        }
-                        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            const int r = 8 * u + (lane >> 3), c = lane & 7, row = (i * WM + wm) * 32 + 16 * h + r;
-                            const uint4_t v = *(const uint4_t *)(place + r * 128 + ((c ^ (r & 7)) * 16));
-                            if (row < cur.rows) store16(p.out, cur.row0 + row, cur.col0 + acol0 + c * 8, v);
-                        }
-                        __builtin_amdgcn_wave_barrier();
-                    }
+                    for (int j = 0; j < NI; ++j) store_block(p.out, i, [&](int q) { return acc[i][j][q]; }, j * 32);
                 }
             }
         }
         newer = GLU ? whole * 2 * ((HQ ? 0 : 1) + (p.e_out != nullptr) + (p.g_out != nullptr)) : whole * 4;
         if (HQ) {
-            // a row's 128 columns are with the WN waves of its wave row: the largest magnitude goes through LDS, and so do the
-            // quantised rows, kWaves * 16 of them at a time, which leave as whole lines
+            // a row's 128 columns are with the WN waves of its wave row: the largest magnitude goes through LDS
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
             const int64_t ldh = fp8_ld(cols), ldh_scale = fp8_ld_scale(cols);
-            constexpr int kRound = kWaves * S::kOut / 128;  // rows
-            static_assert(kRound % (32 * WM) == 0, "whole row blocks of every wave row");
 #pragma unroll
             for (int i = 0; i < MI; ++i) {
                 const int r = (i * WM + wm) * 32 + l;
-                unsigned char *const line = turn + r % kRound * 128;
-                if (i * WM + wm < blocks) {
+                if (i * WM + wm < blocks && r < cur.rows) {
                     uint32_t a = 0u;
 #pragma unroll
                     for (int w = 0; w < WN; ++w) a = a > amax[r * WN + w] ? a : amax[r * WN + w];
                     const int byte = fp8_scale_byte(a);
                     const float inverse = fp8_inverse_of(byte);
-                    if (wn == 0 && half == 0 && r < cur.rows)
-                        p.hq_scale[(cur.row0 + r) * ldh_scale + cur.col0 / kFp8Block] = (uint8_t)byte;
+                    uint8_t *const dst = p.hq + (cur.row0 + r) * ldh + cur.col0 + acol0;
+                    if (wn == 0 && half == 0) p.hq_scale[(cur.row0 + r) * ldh_scale + cur.col0 / kFp8Block] = (uint8_t)byte;
 #pragma unroll
-                    for (int t = 0; t < 4; ++t) {
+                    for (int t = 0; t < 4; t += 2) {
                         const floatx16 &v = acc[i][0];
-                        const int c = 2 * wn + t / 2;  // 16-byte chunk of the line
-                        *(uint32_t *)(line + ((c ^ (r & 7)) * 16) + t % 2 * 8 + half * 4) =
-                            fp8_pack4(v[4 * t], v[4 * t + 1], v[4 * t + 2], v[4 * t + 3], inverse);
+                        const uint32_t x = fp8_pack4(v[4 * t], v[4 * t + 1], v[4 * t + 2], v[4 * t + 3], inverse);
+                        const uint32_t y = fp8_pack4(v[4 * t + 4], v[4 * t + 5], v[4 * t + 6], v[4 * t + 7], inverse);
+                        const auto z = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+                        *(uint2_t *)(dst + 8 * (t + half)) = uint2_t{z[0], z[1]};
                     }
-                }
-                constexpr int kBlocks = kRound / (32 * WM);  // row blocks of a wave in a round
-                if (i % kBlocks == kBlocks - 1 || i == MI - 1) {
-                    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
-                    const int first = i / kBlocks * kRound;
-#pragma unroll
-                    for (int u = 0; u < kRound / 8 / kWaves; ++u) {
-                        const int rr = (u * kWaves + wave) * 8 + (lane >> 3), c = lane & 7;
-                        if (first + rr < cur.rows)
-                            *(uint4_t *)(p.hq + (cur.row0 + first + rr) * ldh + cur.col0 + c * 16) =
-                                *(const uint4_t *)(turn + rr * 128 + ((c ^ (rr & 7)) * 16));
-                    }
-                    if (i != MI - 1) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
                 }
             }
         }
@@ -619,11 +580,25 @@ int launch_mode(const Fp8Product &p, hipStream_t stream) {
 
 template <typename TO>
 int launch_shape(const Fp8Product &p, hipStream_t stream) {
-    const int red = p.dx ? p.N : p.K;
-    if (fp8_blocks(red) * (p.dx ? p.terms : 1) < 2) return MFL_ERR_UNSUPPORTED;
-    if (p.hq == nullptr)
-        return red % kFp8Block != 0 ? launch_mode<true, 2, 2, 2, 2, 2, TO>(p, stream) : launch_mode<false, 2, 2, 2, 2, 2, TO>(p, stream);
-    return red % kFp8Block != 0 ? launch<false, true, true, true, 2, 4, 4, 2, 2, TO>(p, stream) : launch<false, true, true, false, 2, 4, 4, 2, 2, TO>(p, stream);
+    const int cols = p.dx ? p.K : p.N, red = p.dx ? p.N : p.K;
+    const int steps = fp8_blocks(red) * (p.dx ? p.terms : 1);
+    if (steps < 2) return MFL_ERR_UNSUPPORTED;  // (a tile has at least as many steps as there are stages)
+    const bool partial = red % kFp8Block != 0;
+    // Quantised output: the 128 columns of a scale block, of both matrices, are one tile.  Three stages of 128 rows against two of
+    // 256: the expert MLP of 131072 rows 947 against 1054 us, of 24008 under Zipf(1) 289 against 330.
+    if (p.hq != nullptr) {
+        if (steps < 3) return partial ? launch<false, true, true, true, 2, 4, 2, 2, 2, TO>(p, stream) : launch<false, true, true, false, 2, 4, 2, 2, 2, TO>(p, stream);
+        return partial ? launch<false, true, true, true, 2, 4, 2, 2, 3, TO>(p, stream) : launch<false, true, true, false, 2, 4, 2, 2, 3, TO>(p, stream);
+    }
+    // 256 x 256 tiles, one workgroup a CU, where experts have many rows and there are tiles for two rounds; else 128 x 128, two
+    // workgroups a CU, whose output and waiting lie under each other's steps.  128 experts, hidden 2048, inner 768, us for
+    // 128 / 256, quantisation included: gated unit with products 352 / 343 at 512 rows per expert, 673 / 617 at 1024, its backward
+    // pass 376 / 345, 704 / 642, forward product 233 / 226, 440 / 420; but 129 / 141 at 256 rows and 43 / 55 at 32; 8 experts of
+    // 1024 rows 35 / 49.
+    const int64_t large = (p.R / 256) * ceil_div(cols, p.glu ? 128 : 256);
+    if (p.R >= (int64_t)448 * p.E && large >= (int64_t)2 * device_info().cu_count)
+        return partial ? launch_mode<true, 2, 4, 4, 2, 2, TO>(p, stream) : launch_mode<false, 2, 4, 4, 2, 2, TO>(p, stream);
+    return partial ? launch_mode<true, 2, 2, 2, 2, 2, TO>(p, stream) : launch_mode<false, 2, 2, 2, 2, 2, TO>(p, stream);
 }
 
 }  // namespace
