@@ -21,10 +21,14 @@ def p():
 def test_workspaces():
     lib = _lib.lib()
     # values 256 bytes a row, scales 4 bytes a row, each rounded up to 256
-    assert lib.mfl_fp8_workspace(0, 10, 80, 64, 200, 4) == 2560 + 256
-    assert lib.mfl_fp8_workspace(1, 10, 80, 64, 200, 4) == 80 * 128 + 512
-    assert lib.mfl_fp8_workspace(3, 0, 80, 64, 200, 4) == 2 * (80 * 128 + 512)
-    assert lib.mfl_fp8_workspace(4, 10, 80, 64, 200, 4) >= 2560 + 256 + 80 * 128 + 512
+    assert lib.mfl_fp8_workspace(0, 10, 80, 64, 208, 4) == 2560 + 256
+    assert lib.mfl_fp8_workspace(1, 10, 80, 64, 208, 4) == 80 * 128 + 512
+    assert lib.mfl_fp8_workspace(3, 0, 80, 64, 208, 4) == 2 * (80 * 128 + 512)
+    assert lib.mfl_fp8_workspace(4, 10, 80, 64, 208, 4) >= 2560 + 256 + 80 * 128 + 512
+    # weights in rows of 200 bytes are copied to rows of 208 where there are four rows per expert and more
+    assert lib.mfl_fp8_workspace(0, 16, 16, 64, 200, 4) == 4096 + 256 + 4 * 64 * 208
+    assert lib.mfl_fp8_workspace(2, 16, 16, 64, 200, 4) == 4096 + 256 + 2 * 4 * 64 * 208
+    assert lib.mfl_fp8_workspace(0, 15, 15, 64, 200, 4) == 15 * 256 + 256
     for bad in ((0, 10, 0, 64, 200, 4), (0, -1, 8, 64, 200, 4), (0, 8, 8, 0, 200, 4), (9, 8, 8, 64, 200, 4), (0, 8, 8, 64, 200, 0)):
         assert lib.mfl_fp8_workspace(*bad) == 0
 

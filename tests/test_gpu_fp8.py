@@ -552,3 +552,63 @@ def test_lora_over_8_bit_weights():
         assert torch.equal(u, v)
     with pytest.raises(NotImplementedError):
         get_lora_parameters(lora)
+
+
+# ---- sizes at which another kernel or tile takes over ---------------------------------------------------------------------
+
+TAKEOVERS = [
+    # rows, experts, out, in: rows whose bytes no 16-byte access fits, with rows for most experts (the weights are copied to
+    # padded rows) and without; one step of the reduction; large tiles, partial rows and columns among them
+    (700, 9, 200, 331),
+    (700, 9, 331, 200),
+    (700, 9, 47, 129),
+    (20, 9, 200, 331),
+    (600, 5, 256, 112),
+    (600, 5, 112, 256),
+    (9000, 8, 2000, 2064),
+    (36000, 6, 2064, 288),
+    (36000, 6, 288, 2064),
+]
+
+
+@pytest.mark.parametrize("rows,experts,n,k", TAKEOVERS)
+def test_product_where_another_kernel_takes_over(rows, experts, n, k):
+    from qwen3_moe_fused.grouped_gemm.forward_fp8 import grouped_gemm_forward_fp8, grouped_gemm_forward_transposed_fp8
+
+    counts = counts_of(rows, experts, "spread", 60)
+    x, dy = make_rows(rows, k, torch.bfloat16, 61, spread=False), make_rows(rows, n, torch.bfloat16, 62, spread=False)
+    w, s = make_weight(experts, n, k, 63)
+    full = dense(w, s)
+    for out, given, transposed in ((grouped_gemm_forward_fp8(x, w, s, sizes(counts)), x, False),
+                                   (grouped_gemm_forward_transposed_fp8(dy, w, s, sizes(counts)), dy, True)):
+        q, _, slack = quantize(given.double())
+        assert_within(out, *product(q, slack, full, counts, transposed, True), "input gradient" if transposed else "forward")
+
+
+@pytest.mark.parametrize("tokens,k,experts,hidden,inter", [(300, 3, 7, 331, 200), (300, 3, 7, 200, 331), (5000, 4, 6, 1040, 1168),
+                                                           (400, 2, 5, 256, 144), (300, 2, 4, 100, 80)])
+def test_gated_unit_and_mlp_where_another_kernel_takes_over(tokens, k, experts, hidden, inter):
+    from qwen3_moe_fused.fused_mlp import moe_fused_mlp_fp8
+    from qwen3_moe_fused.grouped_gemm.fused import grouped_glu_backward_fp8, grouped_glu_forward_fp8
+
+    m_sizes, sort_idx, inv, counts = routed(tokens, k, experts, 64)
+    x = make_rows(tokens, hidden, torch.bfloat16, 65, spread=False)
+    w = mlp_weights(experts, hidden, inter, 66)
+    h, e, g = grouped_glu_forward_fp8(x, *w[:4], m_sizes, sort_idx, k, return_products=True)
+    re, de, rg, dg = gated_reference(x, ((w[0], w[1]), (w[2], w[3])), sort_idx, k, counts)
+    assert_within(e, re, de, "gate projection")
+    assert_within(g, rg, dg, "up projection")
+    rh, dh = gated(re, de, rg, dg)
+    assert_within(h, rh, dh, "gated unit")
+    q, _, slack = quantize(rh, dh)
+    y = moe_fused_mlp_fp8(x, *w, m_sizes, sort_idx, inv, k)
+    assert_within(y, *product(q, slack, dense(w[4], w[5]), counts, cut=True), "expert MLP")
+    dh = make_rows(tokens * k, inter, torch.bfloat16, 67, spread=False)
+    dx = grouped_glu_backward_fp8(dh, e, g, *w[:4], m_sizes)
+    a, ea, b, eb = gated_backward(dh.double(), e.double(), g.double())
+    total, bound = 0, 0
+    for v, err, (wq, s) in ((a, ea, w[0:2]), (b, eb, w[2:4])):
+        qv, _, slack = quantize(v, err)
+        t, bd = product(qv, slack, dense(wq, s), counts, True, True)
+        total, bound = total + t, bound + 2 * bd
+    assert_within(dx, total, bound, "gradient of the rows")

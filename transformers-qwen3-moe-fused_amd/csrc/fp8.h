@@ -45,10 +45,13 @@ struct Fp8Product {
     int ms_i64;
     void *out, *e_out, *g_out;
     int out_dtype;
-    uint8_t *hq, *hq_scale;  // (glu) where given, `out` is not written but quantised rows, made from the fp32 values
-    float *h32;              // (glu; not on tiles) where given, `out` is not written but these fp32 values
+    // (glu) where hq is given, `out` is not written: the tiles write quantised rows, made from the fp32 values; the other kernels
+    // leave those in h32
+    uint8_t *hq, *hq_scale;
+    float *h32;
     int64_t R;
     int N, K, E;
+    int ldw;  // bytes from one row of the weights to the next: K, or (tiles only) K rounded up to 16 with zeros behind column K
 };
 
 // A few rows per expert (kFp8DecodeRowsPerExpert on average), forward and gated, 16-bit outputs, K % 16 == 0: the rows come as
@@ -57,7 +60,8 @@ struct Fp8Product {
 constexpr int kFp8DecodeRowsPerExpert = 8;
 bool gemm_fp8_decodes(const Fp8Product &p);
 int gemm_fp8_decode(const Fp8Product &p, const void *x, int x_dtype, hipStream_t stream);
-// Tiles in LDS, 16-bit outputs, K % 16 == 0; MFL_ERR_UNSUPPORTED for the rest.
+// Tiles in LDS, 16-bit outputs, ldw % 16 == 0; MFL_ERR_UNSUPPORTED for the rest.
+bool gemm_fp8_tiles(const Fp8Product &p);  // whether it takes the product
 int gemm_fp8_tile(const Fp8Product &p, hipStream_t stream);
 // Any shape; MFL_OK or a launch error.
 int gemm_fp8_generic(const Fp8Product &p, hipStream_t stream);
@@ -68,6 +72,8 @@ int fp8_dequant_rows(const uint8_t *q, const uint8_t *scale, int64_t R, int K, v
 int fp8_silu_bwd_quant(const void *dh, const void *e, const void *g, int dtype, int64_t R, int N, uint8_t *de_q,
                        uint8_t *de_scale, uint8_t *dg_q, uint8_t *dg_scale, hipStream_t stream);
 int fp8_quant_blocks(const void *w, int dtype, int E, int N, int K, uint8_t *q, float *scale, hipStream_t stream);
+// (rows, K) bytes to rows of ldw bytes, zeros behind column K; out 16-byte aligned, ldw a multiple of 16.
+int fp8_pad_rows(const uint8_t *w, int64_t rows, int K, int ldw, uint8_t *out, hipStream_t stream);
 int fp8_dequant_blocks(const uint8_t *q, const float *scale, int E, int N, int K, void *out, int out_dtype, hipStream_t stream);
 
 typedef __attribute__((ext_vector_type(8))) int intx8;

@@ -159,6 +159,28 @@ __global__ __launch_bounds__(256) void dequant_blocks_kernel(const uint8_t *__re
         for (int r = threadIdx.x >> 7; r < rows; r += 2) out[base + (int64_t)r * K] = from_f32<T>(fp8_value(q[base + (int64_t)r * K]) * s);
 }
 
+__global__ __launch_bounds__(256) void pad_rows_kernel(const uint8_t *__restrict__ w, int64_t pieces, int K, int per_row,
+                                                       uint8_t *__restrict__ out) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < pieces; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / per_row;
+        const int k = (int)(i - row * per_row) * 16;
+        const uint8_t *src = w + row * K + k;
+        union {
+            uint4_t v;
+            uint8_t b[16];
+        } u;
+        if (k + 16 <= K) {
+            __builtin_memcpy(&u.v, src, 16);
+        } else {
+            u.v = uint4_t{0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int j = 0; j < 15; ++j)
+                if (k + j < K) u.b[j] = src[j];
+        }
+        *(uint4_t *)(out + i * 16) = u.v;
+    }
+}
+
 template <typename T>
 bool wide_rows(const T *x, int K) {
     return K % 8 == 0 && aligned(x, 16);
@@ -206,6 +228,12 @@ int fp8_quant_blocks(const void *w, int dtype, int E, int N, int K, uint8_t *q, 
     const int64_t blocks = (int64_t)E * fp8_blocks(N) * fp8_blocks(K);
     if (blocks > 0x7fffffff) return MFL_ERR_SHAPE;
     MFL_DISPATCH_FLOAT(dtype, T, { quant_blocks_kernel<T><<<(unsigned)blocks, 256, 0, stream>>>((const T *)w, N, K, q, scale); });
+    return launch_status();
+}
+
+int fp8_pad_rows(const uint8_t *w, int64_t rows, int K, int ldw, uint8_t *out, hipStream_t stream) {
+    const int64_t pieces = rows * (ldw / 16), want = (pieces + 255) / 256;
+    pad_rows_kernel<<<(unsigned)(want < 65536 ? want : 65536), 256, 0, stream>>>(w, pieces, K, ldw / 16, out);
     return launch_status();
 }
 

@@ -1,4 +1,4 @@
-// Expert products in 8-bit floating point on LDS tiles: 16-bit outputs, rows of whole 16-byte pieces (K % 16 == 0).
+// Expert products in 8-bit floating point on LDS tiles: 16-bit outputs, weights in rows of whole 16-byte pieces.
 //
 //   forward         out[r, n] = sum_b S[e, n / 128, b] sx[r, b] sum_{k in block b} x[r, k] w[e, n, k]
 //   gated           the same for two matrices, out = silu(gate) * up
@@ -228,19 +228,19 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void fp8_tile_kernel(Fp8Product p)
                 const int r = load * 8 + (lane >> 3);
                 int n = GLU ? r % BNC : r;
                 if (pt.col0 + n >= p.N) n = p.N - 1 - pt.col0;  // (columns that are not stored)
-                boff[c] = (uint32_t)n * (uint32_t)p.K + ((lane & 7) ^ ((r >> 1) & 7)) * 16;
+                boff[c] = (uint32_t)n * (uint32_t)p.ldw + ((lane & 7) ^ ((r >> 1) & 7)) * 16;
             } else {
                 constexpr int CPR = BN / 16;  // chunks of a row of the reduction
                 const int r = (load * 64 + lane) / CPR;
                 int k = ((lane % CPR) ^ spread(r)) * 16;
-                if (pt.col0 + k >= p.K) k = p.K - 16 - pt.col0;  // (columns that are not stored)
-                boff[c] = (uint32_t)r * (uint32_t)p.K + k;
+                if (pt.col0 + k >= p.ldw) k = p.ldw - 16 - pt.col0;  // (columns that are not stored)
+                boff[c] = (uint32_t)r * (uint32_t)p.ldw + k;
             }
         }
         const Fp8Rows a = p.a[0];
-        const int64_t first = gathered ? 0 : pt.row0, mat = (int64_t)pt.expert * p.N * p.K;
+        const int64_t first = gathered ? 0 : pt.row0, mat = (int64_t)pt.expert * p.N * p.ldw;
         abase = a.q + first * lda;
-        bbase = p.w[0].q + mat + (DX ? pt.col0 : (int64_t)pt.col0 * p.K);
+        bbase = p.w[0].q + mat + (DX ? pt.col0 : (int64_t)pt.col0 * p.ldw);
         const float *ws = (GLU && lane > S::kSLanes ? p.w[1].scale : p.w[0].scale) + (int64_t)pt.expert * nbn * kbk;
         ws += DX ? scale_block(pt) : (int64_t)scale_block(pt) * kbk;
         sptr = lane < S::kSLanes ? a.scale + (first + src_row) * lds_ : (const uint8_t *)ws;
@@ -267,12 +267,12 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void fp8_tile_kernel(Fp8Product p)
             }
         }
         copy4(sptr, st + S::kA + S::kB + wave * S::kSWave);
-        int64_t a_step = 128, b_step = DX ? (int64_t)128 * p.K : 128, row_step = (b & 3) == 3 ? 4 : 0, w_step = DX ? kbk * 4 : 4;
+        int64_t a_step = 128, b_step = DX ? (int64_t)128 * p.ldw : 128, row_step = (b & 3) == 3 ? 4 : 0, w_step = DX ? kbk * 4 : 4;
         if (DX) {
             // to the second term's operands
             const bool jump = pstep + 1 == steps_of_term && p.terms == 2;
             a_step = jump ? p.a[1].q - p.a[0].q - (int64_t)(steps_of_term - 1) * 128 : a_step;
-            b_step = jump ? p.w[1].q - p.w[0].q - (int64_t)(steps_of_term - 1) * 128 * p.K : b_step;
+            b_step = jump ? p.w[1].q - p.w[0].q - (int64_t)(steps_of_term - 1) * 128 * p.ldw : b_step;
             row_step = jump ? p.a[1].scale - p.a[0].scale - (steps_of_term - 1) / 4 * 4 : row_step;
             w_step = jump ? (const uint8_t *)p.w[1].scale - (const uint8_t *)p.w[0].scale - (int64_t)(steps_of_term - 1) * kbk * 4 : w_step;
         }
@@ -582,7 +582,6 @@ template <typename TO>
 int launch_shape(const Fp8Product &p, hipStream_t stream) {
     const int cols = p.dx ? p.K : p.N, red = p.dx ? p.N : p.K;
     const int steps = fp8_blocks(red) * (p.dx ? p.terms : 1);
-    if (steps < 2) return MFL_ERR_UNSUPPORTED;  // (a tile has at least as many steps as there are stages)
     const bool partial = red % kFp8Block != 0;
     // Quantised output: the 128 columns of a scale block, of both matrices, are one tile.  Three stages of 128 rows against two of
     // 256: the expert MLP of 131072 rows 947 against 1054 us, of 24008 under Zipf(1) 289 against 330.
@@ -603,16 +602,20 @@ int launch_shape(const Fp8Product &p, hipStream_t stream) {
 
 }  // namespace
 
-int gemm_fp8_tile(const Fp8Product &p, hipStream_t stream) {
-    if (p.out_dtype == MFL_F32 || p.K % 16 != 0 || p.E > kMaxExperts) return MFL_ERR_UNSUPPORTED;
+bool gemm_fp8_tiles(const Fp8Product &p) {
+    if (p.out_dtype == MFL_F32 || p.ldw % 16 != 0 || p.E > kMaxExperts) return false;
     const int cols = p.dx ? p.K : p.N, red = p.dx ? p.N : p.K;
+    if (fp8_blocks(red) * (p.dx ? p.terms : 1) < 2) return false;  // (a tile has at least as many steps as there are stages)
     for (int i = 0; i < (p.glu || p.terms == 2 ? 2 : 1); ++i)
-        if (!aligned(p.w[i].q, 16)) return MFL_ERR_UNSUPPORTED;
-    if (cols % 8 == 0 && (!aligned(p.out, 16) || !aligned(p.e_out, 16) || !aligned(p.g_out, 16))) return MFL_ERR_UNSUPPORTED;
+        if (!aligned(p.w[i].q, 16)) return false;
+    if (cols % 8 == 0 && (!aligned(p.out, 16) || !aligned(p.e_out, 16) || !aligned(p.g_out, 16))) return false;
     // 32-bit offsets of a lane: 256 rows (or all, gathered) of the left operand, 256 of the weights; 32-bit counts of tiles
-    if ((p.row_idx != nullptr ? p.src_rows : 256) * fp8_ld(red) > 0xffffffffll || (int64_t)256 * p.K > 0xffffffffll)
-        return MFL_ERR_UNSUPPORTED;
-    if ((p.R / 64 + p.E) * (int64_t)ceil_div(cols, 64) > 0x3fffffff) return MFL_ERR_UNSUPPORTED;
+    if ((p.row_idx != nullptr ? p.src_rows : 256) * fp8_ld(red) > 0xffffffffll || (int64_t)256 * p.ldw > 0xffffffffll) return false;
+    return (p.R / 64 + p.E) * (int64_t)ceil_div(cols, 64) <= 0x3fffffff;
+}
+
+int gemm_fp8_tile(const Fp8Product &p, hipStream_t stream) {
+    if (!gemm_fp8_tiles(p)) return MFL_ERR_UNSUPPORTED;
     return p.out_dtype == MFL_BF16 ? launch_shape<bf16_t>(p, stream) : launch_shape<f16_t>(p, stream);
 }
 
