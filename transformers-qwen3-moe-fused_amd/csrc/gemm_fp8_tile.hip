@@ -314,7 +314,8 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void fp8_tile_kernel(Fp8Product p)
         if (follows) decode(nt);
         else nt = cur;
         look_up();
-        // the steps of a tile whose waves have `rb` row blocks each (the last wave row one less)
+        // the steps of a tile of which this wave has `rb` row blocks (others may have one less: what the waves of a workgroup have
+        // to agree in is the number of barriers, one a step)
         auto steps = [&](auto rb) {
         constexpr int RB = decltype(rb)::value;
 #pragma unroll
@@ -436,7 +437,20 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void fp8_tile_kernel(Fp8Product p)
         }
         add(RB - 1, NI - 1, wlast);
         };
-        const int mine = (blocks + WM - 1) / WM;
+        // a wave without row blocks in this tile: its part of the copies, and the barriers
+        auto no_steps = [&]() {
+            int step = 0;
+            for (int end = KT - STAGES; step < KT; end = KT) {
+                if (step == KT - STAGES) start_tile();
+                for (; step < end; ++step) {
+                    publish_past<(STAGES - 2) * S::kOps>(newer);
+                    newer = 0;
+                    cstage = cstage + 1 == STAGES ? 0 : cstage + 1;
+                    issue();
+                }
+            }
+        };
+        const int mine = (blocks - wm + WM - 1) / WM;
         if constexpr (MI >= 4)
             if (mine == 4) steps(std::integral_constant<int, 4>{});
         if constexpr (MI >= 3)
@@ -444,6 +458,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void fp8_tile_kernel(Fp8Product p)
         if constexpr (MI >= 2)
             if (mine == 2) steps(std::integral_constant<int, 2>{});
         if (mine == 1) steps(std::integral_constant<int, 1>{});
+        if (mine == 0) no_steps();
 
         // ---- output.  A lane holds runs of four columns of one row, joined to eight with the other half of the wave.  (Turned in
         // LDS first, so that whole lines of a row leave at once, the output took as long or longer: 43 against 39 thousand
