@@ -136,3 +136,19 @@ def test_module_loads_only_what_it_can_hold():
     with pytest.raises(RuntimeError):
         m.load_state_dict({"weight": good["weight"]})
     assert m.to(torch.bfloat16).weight.dtype == torch.float8_e4m3fn
+
+
+def test_widths_past_what_is_counted(p):
+    """2^30 columns at most: more would not be countable in whole blocks."""
+    lib, w, big = _lib.lib(), _lib.Fp8Weight(p, p), 2 ** 30 + 1
+    assert lib.mfl_fp8_workspace(0, 1, 1, 1, 2 ** 31 - 1, 1) == 0
+    for n, k in ((big, 8), (8, big), (8, 2 ** 31 - 1)):
+        assert lib.mfl_gemm_fwd_fp8(p, 1, None, 1, w, p, I32, p, 1, n, k, 1, BF16, BF16, p, 4096, None) == SHAPE
+        assert lib.mfl_gemm_dx_fp8(p, w, p, I32, p, 1, n, k, 1, BF16, BF16, p, 4096, None) == SHAPE
+        assert lib.mfl_glu_fwd_fp8(p, 1, None, 1, w, w, p, I32, p, None, None, 1, n, k, 1, BF16, p, 4096, None) == SHAPE
+        assert lib.mfl_glu_bwd_fp8(p, p, p, w, w, p, I32, p, 1, n, k, 1, BF16, p, 4096, None) == SHAPE
+        assert lib.mfl_mlp_fwd_fp8(p, 1, None, 1, w, w, w, p, I32, p, None, None, 1, n, k, 1, BF16, p, 4096, None) == SHAPE
+        assert lib.mfl_fp8_quant_blocks(p, BF16, 1, n, k, p, p, None) == SHAPE
+        assert lib.mfl_fp8_dequant_blocks(p, p, 1, n, k, p, BF16, None) == SHAPE
+    assert lib.mfl_fp8_quant_rows(p, BF16, 1, big, p, p, None) == SHAPE
+    assert lib.mfl_fp8_dequant_rows(p, p, 1, big, p, BF16, None) == SHAPE

@@ -612,3 +612,124 @@ def test_gated_unit_and_mlp_where_another_kernel_takes_over(tokens, k, experts, 
         t, bd = product(qv, slack, dense(wq, s), counts, True, True)
         total, bound = total + t, bound + 2 * bd
     assert_within(dx, total, bound, "gradient of the rows")
+
+
+# ---- calls that lie a little apart ----------------------------------------------------------------------------------------
+
+def off_grid(t):
+    """The same values, contiguous, one element behind a 16-byte boundary."""
+    raw = torch.empty(t.numel() + 1, dtype=torch.uint8 if t.dtype == FP8 else t.dtype, device=DEV)[1:]
+    view = (raw.view(FP8) if t.dtype == FP8 else raw).view(t.shape)
+    view.copy_(t)
+    assert view.is_contiguous() and view.data_ptr() % 16 != 0
+    return view
+
+
+@pytest.mark.parametrize("rows", [6, 300])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_operands_off_the_16_byte_grid(rows, dtype):
+    from qwen3_moe_fused.grouped_gemm.forward_fp8 import grouped_gemm_forward_fp8, grouped_gemm_forward_transposed_fp8
+
+    n, k, counts = 272, 384, [rows - 4, 0, 4]
+    x, dy = make_rows(rows, k, dtype, 70, spread=False), make_rows(rows, n, dtype, 71, spread=False)
+    w, s = make_weight(3, n, k, 72)
+    for wi, xi, di in ((w, off_grid(x), off_grid(dy)), (off_grid(w), x, dy), (off_grid(w), off_grid(x), off_grid(dy))):
+        for out, given, transposed in ((grouped_gemm_forward_fp8(xi, wi, s, sizes(counts)), x, False),
+                                       (grouped_gemm_forward_transposed_fp8(di, wi, s, sizes(counts)), dy, True)):
+            q, _, slack = quantize(given.double())
+            assert_within(out, *product(q, slack, dense(w, s), counts, transposed, cut_in(out)))
+
+
+@pytest.mark.parametrize("tokens", [3, 200])
+def test_mlp_operands_off_the_16_byte_grid(tokens):
+    from qwen3_moe_fused.fused_mlp import moe_fused_mlp_fp8
+
+    m_sizes, sort_idx, inv, counts = routed(tokens, 2, 8, 73)
+    x, w = make_rows(tokens, 256, torch.bfloat16, 74, spread=False), mlp_weights(8, 256, 128, 75)
+    h, dh = gated(*gated_reference(x, ((w[0], w[1]), (w[2], w[3])), sort_idx, 2, counts))
+    q, _, slack = quantize(h, dh)
+    expect = product(q, slack, dense(w[4], w[5]), counts, cut=True)
+    shifted = [off_grid(t) for t in w[::2]]
+    for xi, weights in ((off_grid(x), w), (x, [shifted[0], *w[1:]]), (x, [*w[:4], shifted[2], w[5]])):
+        assert_within(moe_fused_mlp_fp8(xi, *weights, m_sizes, sort_idx, inv, 2), *expect)
+
+
+@pytest.mark.parametrize("rows,experts,n,k", [(40, 3, 192, 9280), (40, 3, 9280, 192), (600, 3, 192, 9280), (600, 3, 9280, 192),
+                                              (5000, 512, 128, 288), (5000, 513, 128, 288), (4096, 511, 128, 288)])
+def test_long_reductions_and_many_experts(rows, experts, n, k):
+    from qwen3_moe_fused.grouped_gemm.forward_fp8 import grouped_gemm_forward_fp8, grouped_gemm_forward_transposed_fp8
+
+    counts = counts_of(rows, experts, "spread", 76)
+    x, dy = make_rows(rows, k, torch.bfloat16, 77, spread=False), make_rows(rows, n, torch.bfloat16, 78, spread=False)
+    w, s = make_weight(experts, n, k, 79)
+    for out, given, transposed in ((grouped_gemm_forward_fp8(x, w, s, sizes(counts, torch.int64)), x, False),
+                                   (grouped_gemm_forward_transposed_fp8(dy, w, s, sizes(counts, torch.int64)), dy, True)):
+        q, _, slack = quantize(given.double())
+        assert_within(out, *product(q, slack, dense(w, s), counts, transposed, True))
+
+
+def test_mlp_over_a_full_table_of_experts():
+    from qwen3_moe_fused.fused_mlp import moe_fused_mlp_fp8
+
+    m_sizes, sort_idx, inv, counts = routed(1500, 4, 512, 80)
+    x, w = make_rows(1500, 512, torch.bfloat16, 81, spread=False), mlp_weights(512, 512, 128, 82)
+    h, dh = gated(*gated_reference(x, ((w[0], w[1]), (w[2], w[3])), sort_idx, 4, counts))
+    q, _, slack = quantize(h, dh)
+    assert_within(moe_fused_mlp_fp8(x, *w, m_sizes, sort_idx, inv, 4), *product(q, slack, dense(w[4], w[5]), counts, cut=True))
+
+
+@pytest.mark.parametrize("rows", [5, 300])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_scales_whose_product_overflows(rows, dtype):
+    """Huge rows on weights of zeros with huge scales are zero, and tiny scales of either kind meet huge ones of the other."""
+    from qwen3_moe_fused.grouped_gemm.forward_fp8 import grouped_gemm_forward_fp8
+
+    x = make_rows(rows, 256, torch.float32, 83, spread=False)
+    w, s = make_weight(2, 128, 256, 84)
+    counts = [rows - 2, 2]
+    zero = torch.zeros_like(w.float()).to(FP8)
+    y = grouped_gemm_forward_fp8((x * 2.0 ** 110).to(dtype), zero, torch.full_like(s, 2.0 ** 40), sizes(counts))
+    assert (y == 0).all()
+    base = grouped_gemm_forward_fp8(x.to(dtype), w, s, sizes(counts))
+    for up in (90, -90):
+        y = grouped_gemm_forward_fp8((x * 2.0 ** up).to(dtype), w, s * 2.0 ** -up, sizes(counts))
+        assert torch.equal(y, base)
+
+
+def test_training_steps_in_a_graph_and_on_two_streams_at_once():
+    from qwen3_moe_fused.fused_mlp import moe_fused_glu_fp8, moe_fused_mlp_fp8
+    from qwen3_moe_fused.quantize.layer_fp8 import moe_fused_linear_fp8
+
+    m_sizes, sort_idx, inv, _ = routed(300, 2, 8, 85)
+    w = mlp_weights(8, 256, 128, 86)
+    x = make_rows(300, 256, torch.bfloat16, 87, spread=False).requires_grad_()
+    rows = make_rows(600, 256, torch.bfloat16, 88, spread=False).requires_grad_()
+    dy, dh = make_rows(600, 256, torch.bfloat16, 89, False), make_rows(600, 128, torch.bfloat16, 90, False)
+
+    def step():
+        y = moe_fused_mlp_fp8(x, *w, m_sizes, sort_idx, inv, 2)
+        h = moe_fused_glu_fp8(x, *w[:4], m_sizes, sort_idx, inv, 2)
+        p = moe_fused_linear_fp8(rows, w[0], w[1], m_sizes)
+        grads = [torch.autograd.grad(o, i, d)[0] for o, i, d in ((y, x, dy), (h, x, dh), (p, rows, dh))]
+        return [t.detach() for t in (y, h, p)] + grads
+
+    expect = step()
+    streams, results = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        for s, r in zip(streams, results):
+            with torch.cuda.stream(s):
+                r.append(step())
+    torch.cuda.synchronize()
+    for r in results:
+        assert all(torch.equal(a, b) for got in r for a, b in zip(got, expect))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for turn in range(3):
+        with torch.no_grad():
+            x.mul_(-1), rows.mul_(0.5)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, step())), turn

@@ -15,7 +15,9 @@ struct RowsRoom {
     Fp8Rows rows() const { return {q, scale}; }
 };
 
-bool sizes_ok(int64_t R, int N, int K, int E) { return R >= 0 && R <= 0x7fffffff && N > 0 && K > 0 && E > 0; }
+// (columns counted in int, rounded up to whole blocks)
+bool width_ok(int n) { return n > 0 && n <= 1 << 30; }
+bool sizes_ok(int64_t R, int N, int K, int E) { return R >= 0 && R <= 0x7fffffff && width_ok(N) && width_ok(K) && E > 0; }
 
 int check_call(const void *m_sizes, int ms_dtype, int64_t R, int N, int K, int E, int in_dtype, int out_dtype) {
     if (!sizes_ok(R, N, K, E)) return MFL_ERR_SHAPE;
@@ -244,7 +246,7 @@ int mfl_mlp_fwd_fp8(const void *x, int64_t src_rows, const int32_t *row_idx, int
 }
 
 int mfl_fp8_quant_rows(const void *x, int dtype, int64_t R, int K, void *q, uint8_t *scale, void *stream) {
-    if (R < 0 || K <= 0) return MFL_ERR_SHAPE;
+    if (R < 0 || !width_ok(K)) return MFL_ERR_SHAPE;
     if (!dtype_ok(dtype)) return MFL_ERR_DTYPE;
     if (R == 0) return MFL_OK;
     if (!x || !q || !scale) return MFL_ERR_NULL;
@@ -253,7 +255,7 @@ int mfl_fp8_quant_rows(const void *x, int dtype, int64_t R, int K, void *q, uint
 }
 
 int mfl_fp8_dequant_rows(const void *q, const uint8_t *scale, int64_t R, int K, void *out, int out_dtype, void *stream) {
-    if (R < 0 || K <= 0) return MFL_ERR_SHAPE;
+    if (R < 0 || !width_ok(K)) return MFL_ERR_SHAPE;
     if (!dtype_ok(out_dtype)) return MFL_ERR_DTYPE;
     if (R == 0) return MFL_OK;
     if (!q || !scale || !out) return MFL_ERR_NULL;
@@ -262,7 +264,7 @@ int mfl_fp8_dequant_rows(const void *q, const uint8_t *scale, int64_t R, int K, 
 }
 
 int mfl_fp8_quant_blocks(const void *w, int dtype, int E, int N, int K, void *q, float *scale, void *stream) {
-    if (E <= 0 || N <= 0 || K <= 0) return MFL_ERR_SHAPE;
+    if (E <= 0 || !width_ok(N) || !width_ok(K)) return MFL_ERR_SHAPE;
     if (!dtype_ok(dtype)) return MFL_ERR_DTYPE;
     if (!w || !q || !scale) return MFL_ERR_NULL;
     if (!aligned(w, dtype_size(dtype)) || !aligned(scale, 4)) return MFL_ERR_ALIGN;
@@ -270,7 +272,7 @@ int mfl_fp8_quant_blocks(const void *w, int dtype, int E, int N, int K, void *q,
 }
 
 int mfl_fp8_dequant_blocks(const void *q, const float *scale, int E, int N, int K, void *out, int out_dtype, void *stream) {
-    if (E <= 0 || N <= 0 || K <= 0) return MFL_ERR_SHAPE;
+    if (E <= 0 || !width_ok(N) || !width_ok(K)) return MFL_ERR_SHAPE;
     if (!dtype_ok(out_dtype)) return MFL_ERR_DTYPE;
     if (!q || !scale || !out) return MFL_ERR_NULL;
     if (!aligned(scale, 4) || !aligned(out, dtype_size(out_dtype))) return MFL_ERR_ALIGN;

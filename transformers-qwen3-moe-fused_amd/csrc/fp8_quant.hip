@@ -181,6 +181,8 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(const uint8_t *__restrict
     }
 }
 
+constexpr int64_t kMaxGroups = 0xffffff;  // a launch's threads are counted in 32 bits
+
 template <typename T>
 bool wide_rows(const T *x, int K) {
     return K % 8 == 0 && aligned(x, 16);
@@ -191,7 +193,7 @@ bool wide_rows(const T *x, int K) {
 int fp8_quant_rows(const void *x, int dtype, int64_t R, int K, uint8_t *q, uint8_t *scale, hipStream_t stream) {
     const int kb = fp8_blocks(K);
     const int64_t blocks = R * kb, grid = (blocks + kGroups * kPerGroup - 1) / (kGroups * kPerGroup);
-    if (grid > 0x7fffffff) return MFL_ERR_SHAPE;
+    if (grid > kMaxGroups) return MFL_ERR_SHAPE;
     MFL_DISPATCH_FLOAT(dtype, T, {
         if (wide_rows((const T *)x, K))
             quant_rows_kernel<T, true><<<(unsigned)grid, 256, 0, stream>>>((const T *)x, blocks, K, kb, q, scale);
@@ -205,7 +207,7 @@ int fp8_silu_bwd_quant(const void *dh, const void *e, const void *g, int dtype, 
                        uint8_t *de_scale, uint8_t *dg_q, uint8_t *dg_scale, hipStream_t stream) {
     const int nb = fp8_blocks(N);
     const int64_t blocks = R * nb, grid = (blocks + kGroups - 1) / kGroups;
-    if (grid > 0x7fffffff) return MFL_ERR_SHAPE;
+    if (grid > kMaxGroups) return MFL_ERR_SHAPE;
     MFL_DISPATCH_FLOAT(dtype, T, {
         if (wide_rows((const T *)dh, N) && wide_rows((const T *)e, N) && wide_rows((const T *)g, N))
             silu_bwd_quant_kernel<T, true><<<(unsigned)grid, 256, 0, stream>>>((const T *)dh, (const T *)e, (const T *)g, blocks, N,
@@ -226,7 +228,7 @@ int fp8_dequant_rows(const uint8_t *q, const uint8_t *scale, int64_t R, int K, v
 
 int fp8_quant_blocks(const void *w, int dtype, int E, int N, int K, uint8_t *q, float *scale, hipStream_t stream) {
     const int64_t blocks = (int64_t)E * fp8_blocks(N) * fp8_blocks(K);
-    if (blocks > 0x7fffffff) return MFL_ERR_SHAPE;
+    if (blocks > kMaxGroups) return MFL_ERR_SHAPE;
     MFL_DISPATCH_FLOAT(dtype, T, { quant_blocks_kernel<T><<<(unsigned)blocks, 256, 0, stream>>>((const T *)w, N, K, q, scale); });
     return launch_status();
 }
@@ -239,7 +241,7 @@ int fp8_pad_rows(const uint8_t *w, int64_t rows, int K, int ldw, uint8_t *out, h
 
 int fp8_dequant_blocks(const uint8_t *q, const float *scale, int E, int N, int K, void *out, int out_dtype, hipStream_t stream) {
     const int64_t blocks = (int64_t)E * fp8_blocks(N) * fp8_blocks(K);
-    if (blocks > 0x7fffffff) return MFL_ERR_SHAPE;
+    if (blocks > kMaxGroups) return MFL_ERR_SHAPE;
     MFL_DISPATCH_FLOAT(out_dtype, T, { dequant_blocks_kernel<T><<<(unsigned)blocks, 256, 0, stream>>>(q, scale, N, K, (T *)out); });
     return launch_status();
 }

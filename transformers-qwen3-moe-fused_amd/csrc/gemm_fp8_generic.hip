@@ -132,7 +132,7 @@ __global__ __launch_bounds__(256) void fp8_generic_kernel(Fp8Product p) {
             for (int c = 0; c < CB; ++c) {
                 const Fp8Matrix &m = p.w[DX ? term : c];
                 const int64_t at = DX ? ((int64_t)e * nbn + b) * kbk + col0 / kFp8Block : ((int64_t)e * nbn + col0 / kFp8Block) * kbk + b;
-                const float scale = m.scale[at] * row_scale;
+                const float scale = m.scale[at];
                 floatx16 part;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) part[i] = 0.0f;
@@ -143,7 +143,7 @@ __global__ __launch_bounds__(256) void fp8_generic_kernel(Fp8Product p) {
                     part = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fw, fa, part, 0, 0, 0);
                 }
 #pragma unroll
-                for (int i = 0; i < 16; ++i) acc[c][i] = __builtin_fmaf(scale, part[i], acc[c][i]);
+                for (int i = 0; i < 16; ++i) acc[c][i] = __builtin_fmaf(scale, part[i] * row_scale, acc[c][i]);  // (the product of the two scales may overflow by itself)
             }
         }
     }
@@ -173,7 +173,7 @@ __global__ __launch_bounds__(256) void fp8_generic_kernel(Fp8Product p) {
 int gemm_fp8_generic(const Fp8Product &p, hipStream_t stream) {
     const int64_t tiles = fp8_max_tiles(p.R, p.E, kTile);
     const dim3 grid((unsigned)tiles, (unsigned)ceil_div(p.dx ? p.K : p.N, kTile));
-    if (grid.y > 65535u) return MFL_ERR_SHAPE;
+    if (grid.y > 65535u || tiles > 0xffffff) return MFL_ERR_SHAPE;  // (a launch's threads are counted in 32 bits)
     MFL_DISPATCH_FLOAT(p.out_dtype, TO, {
         if (p.dx)
             fp8_generic_kernel<true, false, TO><<<grid, 256, 0, stream>>>(p);
