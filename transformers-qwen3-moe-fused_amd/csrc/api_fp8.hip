@@ -48,7 +48,8 @@ Fp8Matrix matrix(const mfl_fp8_weight *w) { return {(const uint8_t *)w->q, w->sc
 int64_t source_rows(int64_t src_rows, const int32_t *row_idx, int64_t R) { return row_idx != nullptr ? src_rows : R; }
 
 // Weights whose rows no 16-byte access fits are copied to rows that one does where the call has rows for most experts: 60
-// experts, 333 x 1001, 1999 rows, forward and input gradient kernels of 56 and 71 us for any shape, 13 and 15 on tiles behind the copies (5 us each).
+// experts, 333 x 1001, 1999 rows, fp16, forward and input gradient 56 and 71 us in the kernels for any shape, 13 and 15 on tiles
+// behind copies of 13.
 int padded_row(int K) { return (K + 15) / 16 * 16; }
 size_t padded_bytes(int64_t R, int N, int K, int E) {
     return K % 16 != 0 && R >= (int64_t)4 * E ? up256((size_t)E * N * padded_row(K)) : 0;
@@ -57,7 +58,7 @@ size_t padded_bytes(int64_t R, int N, int K, int E) {
 // One product; `room` holds padded_bytes() for each of its matrices.
 int run_product(Fp8Product p, uint8_t *room, hipStream_t stream) {
     const size_t bytes = padded_bytes(p.R, p.N, p.K, p.E);
-    if (bytes != 0 && p.out_dtype != MFL_F32) {
+    if (bytes != 0) {
         Fp8Product padded = p;
         padded.ldw = padded_row(p.K);
         const int matrices = p.glu || p.terms == 2 ? 2 : 1;

@@ -60,7 +60,7 @@ struct Fp8Product {
 constexpr int kFp8DecodeRowsPerExpert = 8;
 bool gemm_fp8_decodes(const Fp8Product &p);
 int gemm_fp8_decode(const Fp8Product &p, const void *x, int x_dtype, hipStream_t stream);
-// Tiles in LDS, 16-bit outputs, ldw % 16 == 0; MFL_ERR_UNSUPPORTED for the rest.
+// Tiles in LDS, ldw % 16 == 0, two steps of the reduction at least; MFL_ERR_UNSUPPORTED for the rest.
 bool gemm_fp8_tiles(const Fp8Product &p);  // whether it takes the product
 int gemm_fp8_tile(const Fp8Product &p, hipStream_t stream);
 // Any shape; MFL_OK or a launch error.

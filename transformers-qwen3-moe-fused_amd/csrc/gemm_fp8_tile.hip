@@ -1,4 +1,4 @@
-// Expert products in 8-bit floating point on LDS tiles: 16-bit outputs, weights in rows of whole 16-byte pieces.
+// Expert products in 8-bit floating point on LDS tiles: weights in rows of whole 16-byte pieces.
 //
 //   forward         out[r, n] = sum_b S[e, n / 128, b] sx[r, b] sum_{k in block b} x[r, k] w[e, n, k]
 //   gated           the same for two matrices, out = silu(gate) * up
@@ -15,13 +15,14 @@
 //   16 multiply-adds by the weights' scale (uniform: 128 x 128) add it to the running fp32 sum.
 //
 // The instruction adds its products in groups of eight and cuts them off 2^-13 below the group's largest (measured): 3e-6 of
-// the sum of magnitudes on average, where the rounding of a 16-bit output is 2e-4 or 2e-3 of the sum itself.  fp32 outputs
-// are not taken here.
+// the sum of magnitudes on average, where the rounding of a 16-bit output is 2e-4 or 2e-3 of the sum itself.  For fp32 outputs
+// the fragments are widened to bf16 in registers, which holds every e4m3 value times its row's scale, and multiplied by
+// v_mfma_f32_32x32x16_bf16 (1e-9): half the rate, and 16 conversions a fragment.
 //
 // LDS layouts.  Rows of 128 bytes along the reduction: 16-byte chunk c of row r at c ^ ((r >> 1) & 7).  A lane's 32 bytes of a
 // 64-wide sub-step are chunks 4 s + h and 4 s + 2 + h (h: its half of the wave); which reduction element sits where in the
 // instruction does not matter as long as both operands agree.  Input gradient: the weights lie as in memory, 128 rows of the
-// reduction by BN columns, chunk c of row n at c ^ ((n & 7) << 1) (BN 128: ^ ((n & 6)), and are read with ds_read_b64_tr_b8 (a group of 16 lanes
+// reduction by BN columns, chunk c of row n at c ^ ((n & 7) << 1) (BN 128: c ^ (n & 6)), and are read with ds_read_b64_tr_b8 (a group of 16 lanes
 // reads 8 rows of 16 bytes and gets 8 rows of one column each), four of them for the same 32 elements.
 #include <type_traits>
 
@@ -96,12 +97,28 @@ struct Shape {
     static_assert(kA % (1024 * kWaves) == 0 && kB % (1024 * kWaves) == 0 && kSLanes + 2 <= 64, "whole copies");
 };
 
+// 8 e4m3 values times the power of two `scale`, as bf16 (exact)
+__device__ __forceinline__ bf16x8 widen(const intx2 v, float scale) {
+    typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+    union {
+        bf16x2 p[4];
+        bf16x8 all;
+    } u;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        u.p[2 * i] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[i], scale, false);
+        u.p[2 * i + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[i], scale, true);
+    }
+    return u.all;
+}
+
 // HQ: the gated unit's result leaves as quantised rows.  PARTIAL: the reduction ends inside a block of 128.
 template <bool DX, bool GLU, bool HQ, bool PARTIAL, int WM, int WN, int MI, int NI, int STAGES, typename TO>
 __global__ __launch_bounds__(WM * WN * 64, 2) void fp8_tile_kernel(Fp8Product p) {
     using S = Shape<WM, WN, MI, NI, STAGES>;
     constexpr int BM = S::BM, BN = S::BN, kWaves = S::kWaves;
     constexpr int BNC = GLU ? BN / 2 : BN;  // output columns of a tile
+    constexpr bool kWide = sizeof(TO) == 4;  // fp32 outputs: bf16 products
     static_assert(!GLU || NI == 2, "gated: a wave holds one block of either matrix");
     static_assert(!HQ || (GLU && BNC == kFp8Block), "quantised output: a tile's columns are one scale block");
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
@@ -317,125 +334,132 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void fp8_tile_kernel(Fp8Product p)
         // the steps of a tile of which this wave has `rb` row blocks (others may have one less: what the waves of a workgroup have
         // to agree in is the number of barriers, one a step)
         auto steps = [&](auto rb) {
-        constexpr int RB = decltype(rb)::value;
+            constexpr int RB = decltype(rb)::value;
 #pragma unroll
-        for (int i = 0; i < RB; ++i)
+            for (int i = 0; i < RB; ++i)
 #pragma unroll
-            for (int j = 0; j < NI; ++j)
+                for (int j = 0; j < NI; ++j)
 #pragma unroll
-                for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.0f;
-        union Frag {
-            uint4_t v[2];
-            intx2 t[4];
-            intx8 i;
-        };
-        Frag fw[NI][2], fa[2];
-        int xscale[2];
-        float wscale[2], wlast = 0.0f;  // the weights' scales of this step, and of the last one's last block
-        floatx16 part[NI];
-        uint32_t st = lds0 + cstage * S::kStage;
-        auto fetch_w = [&](int s) {
+                    for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.0f;
+            union Frag {
+                uint4_t v[2];
+                intx2 t[4];
+                intx8 i;
+            };
+            Frag fw[NI][2], fa[2];
+            int xscale[2];
+            float wscale[2], wlast = 0.0f;  // the weights' scales of this step, and of the last one's last block
+            floatx16 part[NI];
+            uint32_t st = lds0 + cstage * S::kStage;
+            auto fetch_w = [&](int s) {
 #pragma unroll
-            for (int j = 0; j < NI; ++j) {
-                if (!DX) {
-                    constexpr int kNext = GLU ? BNC * 128 : 32 * 128;  // to the wave's next block of columns
+                for (int j = 0; j < NI; ++j) {
+                    if (!DX) {
+                        constexpr int kNext = GLU ? BNC * 128 : 32 * 128;  // to the wave's next block of columns
 #pragma unroll
-                    for (int u = 0; u < 2; ++u)
-                        fw[j][s].v[u] = *(lds_uint4_ptr)(uintptr_t)(((st + woff) ^ (64 * s + 32 * u)) + j * kNext);
+                        for (int u = 0; u < 2; ++u)
+                            fw[j][s].v[u] = *(lds_uint4_ptr)(uintptr_t)(((st + woff) ^ (64 * s + 32 * u)) + j * kNext);
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+                            fw[j][s].t[q] = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                                (lds_intx2_ptr)(uintptr_t)(((st + woff) ^ (32 * j)) + (s * 64 + (q >> 1) * 32 + (q & 1) * 8) * BN));
+                    }
+                }
+            };
+            auto fetch_scales = [&]() {
+#pragma unroll
+                for (int j = 0; j < (GLU ? 2 : 1); ++j)
+                    wscale[j] = *(lds_float_ptr)(uintptr_t)(st + S::kA + S::kB + wave * S::kSWave + (S::kSLanes + j) * 4);
+            };
+            auto fetch = [&](int i, int s) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+                    fa[s].v[u] = *(lds_uint4_ptr)(uintptr_t)(((st + xoff) ^ (64 * s + 32 * u)) + i * WM * 32 * 128);
+            };
+            auto fetch_scale = [&](int i, int b) {
+                xscale[i & 1] = (int)(*(lds_uint32_ptr)(uintptr_t)(st + soff + i * WM * 32 / S::kSLanes * S::kSWave) >> ((b & 3) * 8));
+            };
+            auto multiply = [&](int i, int s, int j) {
+                if (s == 0) {
+#pragma unroll
+                    for (int q = 0; q < 16; ++q) part[j][q] = 0.0f;
+                }
+                if constexpr (!kWide) {
+                    part[j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fw[j][s].i, fa[s].i, part[j], 0, 0, 0, 127, 0, xscale[i & 1]);
                 } else {
+                    const float row_scale = fp8_scale_of(xscale[i & 1] & 255);
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
-                        fw[j][s].t[q] = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                            (lds_intx2_ptr)(uintptr_t)(((st + woff) ^ (32 * j)) + (s * 64 + (q >> 1) * 32 + (q & 1) * 8) * BN));
+                        part[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(widen(fw[j][s].t[q], 1.0f), widen(fa[s].t[q], row_scale), part[j], 0, 0, 0);
+                }
+            };
+            auto add = [&](int i, int j, float scale) {
+#pragma unroll
+                for (int q = 0; q < 16; ++q) acc[i][j][q] = __builtin_fmaf(scale, part[j][q], acc[i][j][q]);
+            };
+            // The matrix unit never waits for the additions: a block's partial sum is added to its running sum while the next block's
+            // second half, or the next row block's first, is multiplied.  A row block's fragments of a sub-step are asked for as soon
+            // as those of the row block before have gone into the unit, those of the next step behind the barrier, which lies before
+            // the step's last sub-step.
+#pragma unroll
+            for (int q = 0; q < 16; ++q) part[NI - 1][q] = 0.0f;
+            fetch_w(0);
+            fetch(0, 0);
+            fetch_scale(0, 0);
+            fetch_scales();
+            fetch_w(1);
+            fetch(0, 1);
+            // (the last steps' copies are the next tile's first; behind the last tile this one's again, which nobody reads)
+            int step = 0;
+            for (int end = KT - STAGES; step < KT; end = KT) {
+                if (step == KT - STAGES) start_tile();
+                for (; step < end; ++step) {
+                    const int b = DX && step >= steps_of_term ? step - steps_of_term : step;
+#pragma unroll
+                    for (int i = 0; i < RB; ++i) {
+                        multiply(i, 0, 0);
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (i == 0) add(RB - 1, NI - 1, wlast);
+                        else add(i - 1, NI - 1, wscale[GLU ? NI - 1 : 0]);
+                        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                        for (int j = 1; j < NI; ++j) multiply(i, 0, j);
+                        __builtin_amdgcn_sched_barrier(0);
+                        const int bn = DX && step + 1 >= steps_of_term ? step + 1 - steps_of_term : step + 1;
+                        if (i + 1 < RB) {
+                            fetch(i + 1, 0);
+                            fetch_scale(i + 1, b);
+                        } else {
+                            wlast = wscale[GLU ? NI - 1 : 0];
+                            publish_past<(STAGES - 2) * S::kOps>(newer);
+                            newer = 0;
+                            cstage = cstage + 1 == STAGES ? 0 : cstage + 1;
+                            st = lds0 + cstage * S::kStage;
+                            fetch_w(0);  // (behind the last step: of the next tile, or stale; not used)
+                        }
+#pragma unroll
+                        for (int j = 0; j < NI; ++j) multiply(i, 1, j);
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (i + 1 < RB) {
+                            fetch(i + 1, 1);
+#pragma unroll
+                            for (int j = 0; j < NI - 1; ++j) add(i, j, wscale[GLU ? j : 0]);
+                        } else {
+                            issue();
+#pragma unroll
+                            for (int j = 0; j < NI - 1; ++j) add(i, j, wscale[GLU ? j : 0]);
+                            fetch(0, 0);
+                            fetch_scale(0, bn);
+                            fetch_w(1);
+                            fetch(0, 1);
+                            fetch_scales();
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
                 }
             }
-        };
-        auto fetch_scales = [&]() {
-#pragma unroll
-            for (int j = 0; j < (GLU ? 2 : 1); ++j)
-                wscale[j] = *(lds_float_ptr)(uintptr_t)(st + S::kA + S::kB + wave * S::kSWave + (S::kSLanes + j) * 4);
-        };
-        auto fetch = [&](int i, int s) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-                fa[s].v[u] = *(lds_uint4_ptr)(uintptr_t)(((st + xoff) ^ (64 * s + 32 * u)) + i * WM * 32 * 128);
-        };
-        auto fetch_scale = [&](int i, int b) {
-            xscale[i & 1] = (int)(*(lds_uint32_ptr)(uintptr_t)(st + soff + i * WM * 32 / S::kSLanes * S::kSWave) >> ((b & 3) * 8));
-        };
-        auto multiply = [&](int i, int s, int j) {
-            if (s == 0) {
-#pragma unroll
-                for (int q = 0; q < 16; ++q) part[j][q] = 0.0f;
-            }
-            part[j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fw[j][s].i, fa[s].i, part[j], 0, 0, 0, 127, 0, xscale[i & 1]);
-        };
-        auto add = [&](int i, int j, float scale) {
-#pragma unroll
-            for (int q = 0; q < 16; ++q) acc[i][j][q] = __builtin_fmaf(scale, part[j][q], acc[i][j][q]);
-        };
-        // The matrix unit never waits for the additions: a block's partial sum is added to its running sum while the next block's
-        // second half, or the next row block's first, is multiplied.  A row block's fragments of a sub-step are asked for as soon
-        // as those of the row block before have gone into the unit, those of the next step behind the barrier, which lies before
-        // the step's last sub-step.
-#pragma unroll
-        for (int q = 0; q < 16; ++q) part[NI - 1][q] = 0.0f;
-        fetch_w(0);
-        fetch(0, 0);
-        fetch_scale(0, 0);
-        fetch_scales();
-        fetch_w(1);
-        fetch(0, 1);
-        // (the last steps' copies are the next tile's first; behind the last tile this one's again, which nobody reads)
-        int step = 0;
-        for (int end = KT - STAGES; step < KT; end = KT) {
-          if (step == KT - STAGES) start_tile();
-          for (; step < end; ++step) {
-            const int b = DX && step >= steps_of_term ? step - steps_of_term : step;
-#pragma unroll
-            for (int i = 0; i < RB; ++i) {
-                multiply(i, 0, 0);
-                __builtin_amdgcn_sched_barrier(0);
-                if (i == 0) add(RB - 1, NI - 1, wlast);
-                else add(i - 1, NI - 1, wscale[GLU ? NI - 1 : 0]);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int j = 1; j < NI; ++j) multiply(i, 0, j);
-                __builtin_amdgcn_sched_barrier(0);
-                const int bn = DX && step + 1 >= steps_of_term ? step + 1 - steps_of_term : step + 1;
-                if (i + 1 < RB) {
-                    fetch(i + 1, 0);
-                    fetch_scale(i + 1, b);
-                } else {
-                    wlast = wscale[GLU ? NI - 1 : 0];
-                    publish_past<(STAGES - 2) * S::kOps>(newer);
-                    newer = 0;
-                    cstage = cstage + 1 == STAGES ? 0 : cstage + 1;
-                    st = lds0 + cstage * S::kStage;
-                    fetch_w(0);  // (behind the last step: of the next tile, or stale; not used)
-                }
-#pragma unroll
-                for (int j = 0; j < NI; ++j) multiply(i, 1, j);
-                __builtin_amdgcn_sched_barrier(0);
-                if (i + 1 < RB) {
-                    fetch(i + 1, 1);
-#pragma unroll
-                    for (int j = 0; j < NI - 1; ++j) add(i, j, wscale[GLU ? j : 0]);
-                } else {
-                    issue();
-#pragma unroll
-                    for (int j = 0; j < NI - 1; ++j) add(i, j, wscale[GLU ? j : 0]);
-                    fetch(0, 0);
-                    fetch_scale(0, bn);
-                    fetch_w(1);
-                    fetch(0, 1);
-                    fetch_scales();
-                }
-                __builtin_amdgcn_sched_barrier(0);
-            }
-          }
-        }
-        add(RB - 1, NI - 1, wlast);
+            add(RB - 1, NI - 1, wlast);
         };
         // a wave without row blocks in this tile: its part of the copies, and the barriers
         auto no_steps = [&]() {
@@ -490,6 +514,23 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void fp8_tile_kernel(Fp8Product p)
         // 32 columns of a row block from the wave's column n0 on, from f(q), the lane's q-th value
         auto store_block = [&](void *base, int i, auto f, int n0) {
             const int r = (i * WM + wm) * 32 + l;
+            if constexpr (kWide) {
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    const int n = cur.col0 + acol0 + n0 + 8 * t + 4 * half;
+                    float *dst = (float *)base + (int64_t)(cur.row0 + r) * cols + n;
+                    const floatx4 v = {f(4 * t), f(4 * t + 1), f(4 * t + 2), f(4 * t + 3)};
+                    if (r >= cur.rows) continue;
+                    if (cols % 4 == 0) {
+                        if (n < cols) *(floatx4 *)dst = v;
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+                            if (n + q < cols) dst[q] = v[q];
+                    }
+                }
+                return;
+            }
 #pragma unroll
             for (int t = 0; t < 4; t += 2) {
                 const float va[4] = {f(4 * t), f(4 * t + 1), f(4 * t + 2), f(4 * t + 3)};
@@ -529,14 +570,13 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void fp8_tile_kernel(Fp8Product p)
                         if (half == 0) amax[((i * WM + wm) * 32 + l) * WN + wn] = a > other ? a : other;
                     }
                 } else {
-                    
-
 #pragma unroll
                     for (int j = 0; j < NI; ++j) store_block(p.out, i, [&](int q) { return acc[i][j][q]; }, j * 32);
                 }
             }
         }
         newer = GLU ? whole * 2 * ((HQ ? 0 : 1) + (p.e_out != nullptr) + (p.g_out != nullptr)) : whole * 4;
+        if (kWide) newer *= 2;
         if (HQ) {
             // a row's 128 columns are with the WN waves of its wave row: the largest magnitude goes through LDS
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
@@ -609,21 +649,23 @@ int launch_shape(const Fp8Product &p, hipStream_t stream) {
     // 128 / 256, quantisation included: gated unit with products 352 / 343 at 512 rows per expert, 673 / 617 at 1024, its backward
     // pass 376 / 345, 704 / 642, forward product 233 / 226, 440 / 420; but 129 / 141 at 256 rows and 43 / 55 at 32; 8 experts of
     // 1024 rows 35 / 49.
+    // (fp32 outputs: 128 x 128)
     const int64_t large = (p.R / 256) * ceil_div(cols, p.glu ? 128 : 256);
-    if (p.R >= (int64_t)448 * p.E && large >= (int64_t)2 * device_info().cu_count)
-        return partial ? launch_mode<true, 2, 4, 4, 2, 2, TO>(p, stream) : launch_mode<false, 2, 4, 4, 2, 2, TO>(p, stream);
+    if constexpr (sizeof(TO) == 2)
+        if (p.R >= (int64_t)448 * p.E && large >= (int64_t)2 * device_info().cu_count)
+            return partial ? launch_mode<true, 2, 4, 4, 2, 2, TO>(p, stream) : launch_mode<false, 2, 4, 4, 2, 2, TO>(p, stream);
     return partial ? launch_mode<true, 2, 2, 2, 2, 2, TO>(p, stream) : launch_mode<false, 2, 2, 2, 2, 2, TO>(p, stream);
 }
 
 }  // namespace
 
 bool gemm_fp8_tiles(const Fp8Product &p) {
-    if (p.out_dtype == MFL_F32 || p.ldw % 16 != 0 || p.E > kMaxExperts) return false;
+    if (p.ldw % 16 != 0 || p.E > kMaxExperts) return false;
     const int cols = p.dx ? p.K : p.N, red = p.dx ? p.N : p.K;
     if (fp8_blocks(red) * (p.dx ? p.terms : 1) < 2) return false;  // (a tile has at least as many steps as there are stages)
     for (int i = 0; i < (p.glu || p.terms == 2 ? 2 : 1); ++i)
         if (!aligned(p.w[i].q, 16)) return false;
-    if (cols % 8 == 0 && (!aligned(p.out, 16) || !aligned(p.e_out, 16) || !aligned(p.g_out, 16))) return false;
+    if (cols % (p.out_dtype == MFL_F32 ? 4 : 8) == 0 && (!aligned(p.out, 16) || !aligned(p.e_out, 16) || !aligned(p.g_out, 16))) return false;
     // 32-bit offsets of a lane: 256 rows (or all, gathered) of the left operand, 256 of the weights; 32-bit counts of tiles
     if ((p.row_idx != nullptr ? p.src_rows : 256) * fp8_ld(red) > 0xffffffffll || (int64_t)256 * p.ldw > 0xffffffffll) return false;
     return (p.R / 64 + p.E) * (int64_t)ceil_div(cols, 64) <= 0x3fffffff;
@@ -631,7 +673,8 @@ bool gemm_fp8_tiles(const Fp8Product &p) {
 
 int gemm_fp8_tile(const Fp8Product &p, hipStream_t stream) {
     if (!gemm_fp8_tiles(p)) return MFL_ERR_UNSUPPORTED;
-    return p.out_dtype == MFL_BF16 ? launch_shape<bf16_t>(p, stream) : launch_shape<f16_t>(p, stream);
+    MFL_DISPATCH_FLOAT(p.out_dtype, TO, { return launch_shape<TO>(p, stream); });
+    return MFL_ERR_DTYPE;
 }
 
 }  // namespace mfl
