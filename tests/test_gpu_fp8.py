@@ -733,3 +733,28 @@ def test_training_steps_in_a_graph_and_on_two_streams_at_once():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, step())), turn
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tokens", [5, 90])
+def test_nan_and_infinity_in_every_type_and_through_the_mlp(dtype, tokens):
+    """A token with an element that is no finite number comes out as NaN, the others as without it; a gated unit that overflows
+    (its fp32 values are infinite) does the same to its rows."""
+    from qwen3_moe_fused.fused_mlp import moe_fused_mlp_fp8
+    from qwen3_moe_fused.grouped_gemm.forward_fp8 import grouped_gemm_forward_fp8
+
+    m_sizes, sort_idx, inv, counts = routed(tokens, 2, 8, 91)
+    x, w = make_rows(tokens, 400, dtype, 92, spread=False), mlp_weights(8, 400, 272, 93)
+    clean, rows = moe_fused_mlp_fp8(x, *w, m_sizes, sort_idx, inv, 2), x[sort_idx.long() // 2].contiguous()
+    flat = grouped_gemm_forward_fp8(rows, w[0], w[1], m_sizes)
+    x[1, 399], x[2, 130] = float("inf"), float("nan")
+    bad = ((sort_idx // 2 == 1) | (sort_idx // 2 == 2)).cpu()
+    for out, expect in ((moe_fused_mlp_fp8(x, *w, m_sizes, sort_idx, inv, 2), clean),
+                        (grouped_gemm_forward_fp8(x[sort_idx.long() // 2].contiguous(), w[0], w[1], m_sizes), flat)):
+        assert torch.equal(out.isnan().cpu(), bad[:, None].expand(out.shape)) and torch.equal(out[~bad], expect[~bad])
+    x = make_rows(tokens, 400, dtype, 92, spread=False)
+    up = w[3].clone()
+    up[int((m_sizes > 0).nonzero()[0])] = 3e38  # the first expert with rows
+    out = moe_fused_mlp_fp8(x, *w[:3], up, *w[4:], m_sizes, sort_idx, inv, 2)
+    first = next(c for c in counts if c)
+    assert out[:first].isnan().all() and torch.equal(out[first:], clean[first:])

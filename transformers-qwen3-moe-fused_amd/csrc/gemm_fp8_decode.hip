@@ -8,8 +8,14 @@
 // multiplied.  A lane holds bytes 16 g .. 16 g + 15 and 64 + 16 g .. of a row of the block (g: its quarter of the wave), so that
 // four lanes read 64 bytes of a row together; the rows are loaded in the same order, their largest magnitude found over the
 // four lanes, and rounded to e4m3 in registers (the order within the block does not matter as long as both operands agree).
-// The waves' sums meet in LDS.  Bound by the weights' bytes, or by latency (row counts, row index, rows, weights one behind
-// the other) where there are few of them.
+// The waves' sums meet in LDS.
+//
+// Bound by the weights' bytes: 32 tokens of 8 of 128 experts, 2048 to 2 x 768, 66 us for 349 MB, 5.3 TB/s.  Of a single token's
+// 12 us (25 MB) a wave spends 0.8 finding its rows, 5 to 7 until the weights are there, 0.6 multiplying; instructions fetched for
+// the first time count too, which is why the conversions are the packed ones (16 for a block's 32 elements) and a chunk that is
+// whole asks nothing: with conversions one by one 3.5 us of the 12 were the rows' quantisation, now 1.4.
+#include <type_traits>
+
 #include "fp8.h"
 
 namespace mfl {
@@ -19,10 +25,17 @@ namespace {
 constexpr int kRows = 16, kWaves = 4;
 constexpr int kBuffers = 3;  // pieces of weights in registers
 
-// 16 elements of a row, where they lie inside it
+// 16 elements of a row.  `widest`: the largest magnitude's bits as of a float, in `bits` and these (16-bit types: compared as
+// they are, two at a time).  `finite`: the same of the finite ones.  `pack`: four of them by the power of two `scale` as e4m3,
+// infinities as NaN: v_cvt_scalef32_pk_fp8_* give what dividing and rounding gives (all values of the 16-bit types, at 13 scales).
 template <typename T>
 struct Piece {
-    uint4_t q[sizeof(T)];
+    static constexpr int kDwords = 4 * sizeof(T);
+    union {
+        uint4_t q[sizeof(T)];
+        uint32_t d[kDwords];
+        T e[16];
+    };
     __device__ __forceinline__ void load(const T *p) {
 #pragma unroll
         for (int i = 0; i < (int)sizeof(T); ++i) q[i] = ((const uint4_t *)p)[i];
@@ -31,22 +44,59 @@ struct Piece {
 #pragma unroll
         for (int i = 0; i < (int)sizeof(T); ++i) q[i] = uint4_t{0u, 0u, 0u, 0u};
     }
-    __device__ __forceinline__ float at(int i) const {
-        union {
-            uint4_t v;
-            T e[16 / sizeof(T)];
-        } u;
-        u.v = q[i / (16 / (int)sizeof(T))];
-        return to_f32(u.e[i % (16 / (int)sizeof(T))]);
+    __device__ __forceinline__ uint32_t widest(uint32_t bits) const {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) bits = fp8_wider(bits, e[i]);
+            return bits;
+        } else {
+            typedef __attribute__((ext_vector_type(2))) uint16_t ushortx2;
+            ushortx2 m = {0, 0};
+#pragma unroll
+            for (int i = 0; i < kDwords; ++i) {
+                const uint32_t w = d[i] & 0x7fff7fffu;
+                m = __builtin_elementwise_max(m, __builtin_bit_cast(ushortx2, w));
+            }
+            const uint16_t top = m[0] > m[1] ? m[0] : m[1];
+            return fp8_wider(bits, to_f32(__builtin_bit_cast(T, top)));
+        }
+    }
+    __device__ __forceinline__ uint32_t finite(uint32_t bits) const {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) bits = fp8_wider(bits, fp8_finite_abs(to_f32(e[i])));
+        return bits;
+    }
+    // (all first halves of the results, then all second ones: a half behind the other half of the same register has to wait)
+    __device__ __forceinline__ void pack(int (&out)[4], float scale) const {
+        typedef __attribute__((ext_vector_type(2))) short shortx2;
+        typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+        typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+        shortx2 r[4] = {};
+        auto half = [&](auto second) {
+            constexpr bool S = decltype(second)::value;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (sizeof(T) == 4)
+                    r[i] = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r[i], e[4 * i + 2 * S], e[4 * i + 2 * S + 1], scale, S);
+                else if constexpr (std::is_same<T, bf16_t>::value)
+                    r[i] = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r[i], __builtin_bit_cast(bf16x2, d[2 * i + S]), scale, S);
+                else
+                    r[i] = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r[i], __builtin_bit_cast(f16x2, d[2 * i + S]), scale, S);
+            }
+        };
+        half(std::false_type{});
+        half(std::true_type{});
+#pragma unroll
+        for (int i = 0; i < 4; ++i) out[i] = __builtin_bit_cast(int, r[i]);
     }
 };
 
 // The largest of the four lanes that hold a row's block, in all of them.
 __device__ __forceinline__ uint32_t over_block(uint32_t a) {
-    uint32_t b = (uint32_t)__shfl_xor((int)a, 16);
-    a = a > b ? a : b;
-    b = (uint32_t)__shfl_xor((int)a, 32);
-    return a > b ? a : b;
+    const auto x = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+    a = x[0] > x[1] ? x[0] : x[1];
+    const auto y = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+    return y[0] > y[1] ? y[0] : y[1];
 }
 
 // The sizes of up to 256 experts at once (their loads in flight together), then 64 at a time.
@@ -101,7 +151,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void fp8_decode_kernel(Fp8Product p
     if (early) index = p.row_idx[lane < p.R ? lane : 0];
     if (!find_rows(p, blockIdx.y, lane, e, row0, rows)) return;
     const int n0 = blockIdx.x * 16 * TILES;
-    const int blocks = fp8_blocks(p.K), nbn = fp8_blocks(p.N);
+    const int blocks = fp8_blocks(p.K), nbn = fp8_blocks(p.N), full = p.K / kFp8Block;
 
     int64_t src = row0 + (c < rows ? c : rows - 1);
     int looked_up = 0;
@@ -112,31 +162,30 @@ __global__ __launch_bounds__(kWaves * 64, 2) void fp8_decode_kernel(Fp8Product p
         uint4_t v[2];
         intx8 i;
     };
-    // piece t: columns n0 + 16 (t / 2) of matrix t % 2 where gated, else n0 + 16 t.  Columns past the last are not stored.
-    Frag fw[kBuffers][AHEAD];
-    auto load = [&](int t, int b0) {
-        const Fp8Matrix &m = p.w[GLU ? t & 1 : 0];
-        int n = n0 + 16 * (GLU ? t / 2 : t) + c;
-        if (n >= p.N) n = p.N - 1;
-        const uint8_t *w = m.q + ((int64_t)e * p.N + n) * p.K + 16 * g;
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            const int b = b0 + kWaves * u;
-            if (b < blocks) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int k = b * kFp8Block + 64 * h;
-                    if (k + 16 * g < p.K) fw[t % kBuffers][u].v[h] = *(const uint4_t *)(w + k);  // (K is a multiple of 16)
-                    else fw[t % kBuffers][u].v[h] = uint4_t{0u, 0u, 0u, 0u};
-                }
-            }
-        }
-    };
-
+    // A chunk of the reduction, blocks b0, b0 + 4, ...  Whole: all of them are there to the end, and nothing is asked about them (a
+    // short call takes as long as its instructions take to arrive).
+    // Piece t: columns n0 + 16 (t / 2) of matrix t % 2 where gated, else n0 + 16 t.  Columns past the last are not stored.
     floatx4 acc[PIECES];
 #pragma unroll
     for (int t = 0; t < PIECES; ++t) acc[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int b0 = wave; b0 < blocks; b0 += kWaves * AHEAD) {
+    auto chunk = [&](int b0, auto whole) {
+        constexpr bool W = decltype(whole)::value;
+        Frag fw[kBuffers][AHEAD];
+        auto load = [&](int t) {
+            const Fp8Matrix &m = p.w[GLU ? t & 1 : 0];
+            int n = n0 + 16 * (GLU ? t / 2 : t) + c;
+            if (n >= p.N) n = p.N - 1;
+            const uint8_t *const w = m.q + (int64_t)e * p.N * p.K;
+            const uint32_t at = (uint32_t)n * (uint32_t)p.K + 16 * g;
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int k = (b0 + kWaves * u) * kFp8Block + 64 * h;
+                    if (W || k + 16 * g < p.K) fw[t % kBuffers][u].v[h] = *(const uint4_t *)(w + k + at);  // (K is a multiple of 16)
+                    else fw[t % kBuffers][u].v[h] = uint4_t{0u, 0u, 0u, 0u};
+                }
+        };
         // the weights' scales of the chunk: lane t AHEAD + u that of piece t in block b0 + 4 u
         static_assert(PIECES * AHEAD <= 64, "one scale a lane");
         float scales = 0.0f;
@@ -148,7 +197,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void fp8_decode_kernel(Fp8Product p
                 scales = (GLU && t & 1 ? p.w[1].scale : p.w[0].scale)[((int64_t)e * nbn + nb) * blocks + b];
         }
 #pragma unroll
-        for (int t = 0; t < kBuffers - 1 && t < PIECES; ++t) load(t, b0);
+        for (int t = 0; t < kBuffers - 1 && t < PIECES; ++t) load(t);
         // the rows' blocks, quantised
         intx8 q[AHEAD];
         int byte[AHEAD];
@@ -161,60 +210,42 @@ __global__ __launch_bounds__(kWaves * 64, 2) void fp8_decode_kernel(Fp8Product p
             const TX *const xr = x + row * p.K + 16 * g;
             Piece<TX> fx[AHEAD][2];
 #pragma unroll
-            for (int u = 0; u < AHEAD; ++u) {
-                const int b = b0 + kWaves * u;
+            for (int u = 0; u < AHEAD; ++u)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const int k = b * kFp8Block + 64 * h;
-                    if (b < blocks && k + 16 * g < p.K) fx[u][h].load(xr + k);
+                    const int k = (b0 + kWaves * u) * kFp8Block + 64 * h;
+                    if (W || k + 16 * g < p.K) fx[u][h].load(xr + k);
                     else fx[u][h].clear();
                 }
-            }
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
-                uint32_t a = 0u;
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) a = fp8_wider(a, fx[u][h].at(i));
-                a = over_block(a);
-                const bool unusual = __any(fp8_unusual(a));
-                if (unusual) {
-                    a = 0u;
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) a = fp8_wider(a, fp8_finite_abs(fx[u][h].at(i)));
-                    a = over_block(a);
-                }
+                uint32_t a = over_block(fx[u][1].widest(fx[u][0].widest(0u)));
+                if (__builtin_expect(__any(fp8_unusual(a)), 0)) a = over_block(fx[u][1].finite(fx[u][0].finite(0u)));
                 byte[u] = fp8_scale_byte(a);
-                const float inverse = fp8_inverse_of(byte[u]);
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        q[u][4 * h + i] = (int)(unusual ? fp8_pack4(fp8_finite(fx[u][h].at(4 * i)), fp8_finite(fx[u][h].at(4 * i + 1)),
-                                                                    fp8_finite(fx[u][h].at(4 * i + 2)), fp8_finite(fx[u][h].at(4 * i + 3)), inverse)
-                                                        : fp8_pack4(fx[u][h].at(4 * i), fx[u][h].at(4 * i + 1), fx[u][h].at(4 * i + 2),
-                                                                    fx[u][h].at(4 * i + 3), inverse));
+                const float scale = fp8_scale_of(byte[u]);
+                int lo[4], hi[4];
+                fx[u][0].pack(lo, scale);
+                fx[u][1].pack(hi, scale);
+                q[u] = intx8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
             }
         }
 #pragma unroll
         for (int t = 0; t < PIECES; ++t) {
-            if (t + kBuffers - 1 < PIECES) load(t + kBuffers - 1, b0);
+            if (t + kBuffers - 1 < PIECES) load(t + kBuffers - 1);
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
-                const int b = b0 + kWaves * u;
-                if (b < blocks) {
-                    const floatx4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-                    const floatx4 part = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw[t % kBuffers][u].i, q[u], zero, 0, 0, 0, 127, 0, byte[u]);
-                    const float s = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(scales), t * AHEAD + u));
+                if (!W && b0 + kWaves * u >= blocks) break;
+                const floatx4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+                const floatx4 part = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw[t % kBuffers][u].i, q[u], zero, 0, 0, 0, 127, 0, byte[u]);
+                const float s = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(scales), t * AHEAD + u));
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[t][i] = __builtin_fmaf(s, part[i], acc[t][i]);
-                }
+                for (int i = 0; i < 4; ++i) acc[t][i] = __builtin_fmaf(s, part[i], acc[t][i]);
             }
         }
-    }
+    };
+    int b0 = wave;
+    for (; b0 + kWaves * (AHEAD - 1) < full; b0 += kWaves * AHEAD) chunk(b0, std::true_type{});
+    if (b0 < blocks) chunk(b0, std::false_type{});
 #pragma unroll
     for (int t = 0; t < PIECES; ++t) sums[wave][t][lane] = acc[t];
     __syncthreads();
@@ -276,7 +307,7 @@ int launch(const Fp8Product &p, const TX *x, hipStream_t stream) {
 
 bool gemm_fp8_decodes(const Fp8Product &p) {
     if (p.dx || p.out_dtype == MFL_F32 || p.K % 16 != 0 || p.R > (int64_t)kFp8DecodeRowsPerExpert * p.E) return false;
-    if (fp8_max_tiles(p.R, p.E, kRows) > 65535) return false;
+    if (fp8_max_tiles(p.R, p.E, kRows) > 65535 || (int64_t)p.N * p.K > 0xffffffffll) return false;  // (32-bit offsets in a matrix)
     return aligned(p.w[0].q, 16) && (!p.glu || aligned(p.w[1].q, 16));
 }
 

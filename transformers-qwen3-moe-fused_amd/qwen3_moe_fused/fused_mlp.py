@@ -166,9 +166,10 @@ class _GluGatheredFp8(torch.autograd.Function):
 
 
 def _check_routing(tokens, sort_idx, inv_sort_idx, k):
-    for idx in (sort_idx, inv_sort_idx):
-        assert idx.dtype == torch.int32 and idx.shape == (tokens.shape[0] * k,) and idx.is_contiguous()
-        assert idx.device == tokens.device
+    rows, device = (tokens.shape[0] * k,), tokens.get_device()
+    assert sort_idx.dtype == torch.int32 and sort_idx.shape == rows and sort_idx.is_contiguous()
+    assert inv_sort_idx.dtype == torch.int32 and inv_sort_idx.shape == rows and inv_sort_idx.is_contiguous()
+    assert sort_idx.get_device() == device and inv_sort_idx.get_device() == device
 
 
 def moe_fused_glu_fp8(tokens: torch.Tensor, w_gate: torch.Tensor, gate_scale: torch.Tensor, w_up: torch.Tensor,
@@ -176,7 +177,8 @@ def moe_fused_glu_fp8(tokens: torch.Tensor, w_gate: torch.Tensor, gate_scale: to
                       num_selected: int) -> torch.Tensor:
     """``moe_fused_glu`` on weights in 8-bit floating point with their block scales (frozen), in bf16, fp16 or fp32.
     Differentiable in ``tokens``; the gradients of the two products are quantised like the forward's rows."""
-    assert not any(t.requires_grad for t in (w_gate, gate_scale, w_up, up_scale)), "8-bit expert weights are frozen"
+    assert not (w_gate.requires_grad or gate_scale.requires_grad or w_up.requires_grad or up_scale.requires_grad), \
+        "8-bit expert weights are frozen"
     _check_routing(tokens, sort_idx, inv_sort_idx, num_selected)
     if not (torch.is_grad_enabled() and tokens.requires_grad):
         return grouped_glu_forward_fp8(tokens, w_gate, gate_scale, w_up, up_scale, m_sizes, sort_idx, num_selected)
@@ -207,8 +209,8 @@ def moe_fused_mlp_fp8(tokens: torch.Tensor, w_gate: torch.Tensor, gate_scale: to
     """``moe_fused_mlp`` on weights in 8-bit floating point with their block scales (frozen), in bf16, fp16 or fp32: between
     the gated unit and the down projection there are only quantised rows, made from the unit's fp32 values.  Differentiable
     in ``tokens``."""
-    assert not any(t.requires_grad for t in (w_gate, gate_scale, w_up, up_scale, w_down, down_scale)), \
-        "8-bit expert weights are frozen"
+    assert not (w_gate.requires_grad or gate_scale.requires_grad or w_up.requires_grad or up_scale.requires_grad
+                or w_down.requires_grad or down_scale.requires_grad), "8-bit expert weights are frozen"
     _check_routing(tokens, sort_idx, inv_sort_idx, num_selected)
     if not (torch.is_grad_enabled() and tokens.requires_grad):
         return grouped_mlp_forward_fp8(tokens, w_gate, gate_scale, w_up, up_scale, w_down, down_scale, m_sizes, sort_idx,

@@ -65,7 +65,7 @@ def grouped_gemm_forward_fp8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Te
     experts, n, k_w = check_fp8_weight(x, w, w_scale)
     assert k_w == k and m_sizes.numel() == experts
     with _lib.on_device_of(x):
-        y = torch.empty((rows, n), device=x.device, dtype=x.dtype if dtype is None else dtype)
+        y = x.new_empty(rows, n, dtype=dtype)
         ms = _lib.as_index_tensor(m_sizes)
         entry, weight = _lib.lib().mfl_gemm_fwd_fp8, fp8_weight(w, w_scale)
         args = (x.data_ptr(), rows, None, 1, weight, ms.data_ptr(), _lib.itype_code(ms.dtype), y.data_ptr(), rows, n, k, experts,
@@ -83,7 +83,7 @@ def grouped_gemm_forward_transposed_fp8(dy: torch.Tensor, w: torch.Tensor, w_sca
     experts, n_w, k = check_fp8_weight(dy, w, w_scale)
     assert n_w == n and m_sizes.numel() == experts
     with _lib.on_device_of(dy):
-        dx = torch.empty((rows, k), device=dy.device, dtype=dy.dtype if dtype is None else dtype)
+        dx = dy.new_empty(rows, k, dtype=dtype)
         ms = _lib.as_index_tensor(m_sizes)
         _keep, ws, ws_bytes = fp8_workspace(DX, dy, rows, rows, n, k, experts)
         rc = _lib.lib().mfl_gemm_dx_fp8(dy.data_ptr(), fp8_weight(w, w_scale), ms.data_ptr(), _lib.itype_code(ms.dtype),

@@ -427,7 +427,7 @@ def grouped_glu_forward_fp8(x: torch.Tensor, w_gate: torch.Tensor, gate_scale: t
     assert check_fp8_weight(x, w_up, up_scale) == (experts, n, k) and x.shape[1] == k and m_sizes.numel() == experts
     assert rows == 0 or x.shape[0] > 0
     with _lib.on_device_of(x):
-        h = torch.empty((rows, n), device=x.device, dtype=x.dtype)
+        h = x.new_empty(rows, n)
         e = torch.empty_like(h) if return_products else None
         g = torch.empty_like(h) if return_products else None
         ms = _lib.as_index_tensor(m_sizes)
@@ -450,7 +450,7 @@ def grouped_glu_backward_fp8(dh: torch.Tensor, e: torch.Tensor, g: torch.Tensor,
     experts, n_w, k = check_fp8_weight(dh, w_gate, gate_scale)
     assert check_fp8_weight(dh, w_up, up_scale) == (experts, n, k) and n_w == n and m_sizes.numel() == experts
     with _lib.on_device_of(dh):
-        dx = torch.empty((rows, k), device=dh.device, dtype=dh.dtype)
+        dx = dh.new_empty(rows, k)
         ms = _lib.as_index_tensor(m_sizes)
         _keep, ws, ws_bytes = fp8_workspace(GLU_BWD, dh, rows, rows, n, k, experts)
         rc = _lib.lib().mfl_glu_bwd_fp8(dh.data_ptr(), e.data_ptr(), g.data_ptr(), fp8_weight(w_gate, gate_scale),
@@ -472,8 +472,8 @@ def grouped_mlp_forward_fp8(x: torch.Tensor, w_gate: torch.Tensor, gate_scale: t
     assert x.shape[1] == k and m_sizes.numel() == experts
     assert rows == 0 or x.shape[0] > 0
     with _lib.on_device_of(x):
-        y = torch.empty((rows, k), device=x.device, dtype=x.dtype)
-        e = torch.empty((rows, n), device=x.device, dtype=x.dtype) if return_products else None
+        y = x.new_empty(rows, k)
+        e = x.new_empty(rows, n) if return_products else None
         g = torch.empty_like(e) if return_products else None
         ms = _lib.as_index_tensor(m_sizes)
         _keep, ws, ws_bytes = fp8_workspace(MLP, x, x.shape[0], rows, n, k, experts)

@@ -26,9 +26,10 @@ def check_fp8_weight(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor)
     """The checks that the products share; returns the weight's (experts, out features, in features)."""
     assert weight.dtype == FP8 and weight.ndim == 3, "expert weights are (E, out, in) float8_e4m3fn"
     experts, n, k = weight.shape
-    assert scale.dtype == torch.float32 and scale.shape == (experts, blocks_of(n), blocks_of(k))
-    for t in (weight, scale):
-        assert t.device == x.device and t.is_contiguous()
+    assert scale.dtype == torch.float32 and scale.shape == (experts, (n + 127) // 128, (k + 127) // 128)
+    device = x.get_device()  # (x is on a GPU; an index compares faster than a device)
+    assert weight.get_device() == device and scale.get_device() == device
+    assert weight.is_contiguous() and scale.is_contiguous()
     return experts, n, k
 
 
