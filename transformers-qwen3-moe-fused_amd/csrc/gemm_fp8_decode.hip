@@ -11,9 +11,9 @@
 // The waves' sums meet in LDS.
 //
 // Bound by the weights' bytes: 32 tokens of 8 of 128 experts, 2048 to 2 x 768, 66 us for 349 MB, 5.3 TB/s.  Of a single token's
-// 12 us (25 MB) a wave spends 0.8 finding its rows, 5 to 7 until the weights are there, 0.6 multiplying; instructions fetched for
-// the first time count too, which is why the conversions are the packed ones (16 for a block's 32 elements) and a chunk that is
-// whole asks nothing: with conversions one by one 3.5 us of the 12 were the rows' quantisation, now 1.4.
+// 10 us (25 MB) a wave spends 0.8 finding its rows, 3 (weights in the caches) to 7 until weights and rows are there and quantised, 0.8
+// multiplying and joining; instructions fetched for the first time count too, which is why the conversions are the packed ones (16
+// for a block's 32 elements) and a chunk that is whole asks nothing: 12.4 us with conversions one by one.
 #include <type_traits>
 
 #include "fp8.h"
