@@ -758,3 +758,17 @@ def test_nan_and_infinity_in_every_type_and_through_the_mlp(dtype, tokens):
     out = moe_fused_mlp_fp8(x, *w[:3], up, *w[4:], m_sizes, sort_idx, inv, 2)
     first = next(c for c in counts if c)
     assert out[:first].isnan().all() and torch.equal(out[first:], clean[first:])
+
+
+@pytest.mark.parametrize("k", [9, 15, 17, 31, 135])
+def test_narrow_odd_rows_of_weights(k):
+    """Rows shorter than 16 bytes, and rows whose last piece has every kind of length, copied to padded rows."""
+    from qwen3_moe_fused.grouped_gemm.forward_fp8 import grouped_gemm_forward_fp8, grouped_gemm_forward_transposed_fp8
+
+    counts = counts_of(700, 9, "spread", 94)
+    x, dy = make_rows(700, k, torch.bfloat16, 95, spread=False), make_rows(700, 300, torch.bfloat16, 96, spread=False)
+    w, s = make_weight(9, 300, k, 97)
+    for out, given, transposed in ((grouped_gemm_forward_fp8(x, w, s, sizes(counts)), x, False),
+                                   (grouped_gemm_forward_transposed_fp8(dy, w, s, sizes(counts)), dy, True)):
+        q, _, slack = quantize(given.double())
+        assert_within(out, *product(q, slack, dense(w, s), counts, transposed, True), "input gradient" if transposed else "forward")

@@ -49,7 +49,7 @@ int64_t source_rows(int64_t src_rows, const int32_t *row_idx, int64_t R) { retur
 
 // Weights whose rows no 16-byte access fits are copied to rows that one does where the call has rows for most experts: 60
 // experts, 333 x 1001, 1999 rows, fp16, forward and input gradient 56 and 71 us in the kernels for any shape, 13 and 15 on tiles
-// behind copies of 13.
+// behind copies of 12.
 int padded_row(int K) { return (K + 15) / 16 * 16; }
 size_t padded_bytes(int64_t R, int N, int K, int E) {
     return K % 16 != 0 && R >= (int64_t)4 * E ? up256((size_t)E * N * padded_row(K)) : 0;

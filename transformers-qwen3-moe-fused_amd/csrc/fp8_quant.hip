@@ -164,18 +164,22 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(const uint8_t *__restrict
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < pieces; i += (int64_t)gridDim.x * 256) {
         const int64_t row = i / per_row;
         const int k = (int)(i - row * per_row) * 16;
-        const uint8_t *src = w + row * K + k;
         union {
             uint4_t v;
+            uint64_t q[2];
             uint8_t b[16];
         } u;
-        if (k + 16 <= K) {
-            __builtin_memcpy(&u.v, src, 16);
+        if (K >= 16) {
+            // (the row's last piece: its last 16 bytes, moved down; byte by byte they would be a load behind the other)
+            const int at = k + 16 <= K ? k : K - 16, moved = (k - at) * 8;
+            __builtin_memcpy(&u.v, w + row * K + at, 16);
+            if (moved >= 64) u.q[0] = u.q[1] >> (moved - 64), u.q[1] = 0u;
+            else if (moved > 0) u.q[0] = u.q[0] >> moved | u.q[1] << (64 - moved), u.q[1] >>= moved;
         } else {
             u.v = uint4_t{0u, 0u, 0u, 0u};
 #pragma unroll
             for (int j = 0; j < 15; ++j)
-                if (k + j < K) u.b[j] = src[j];
+                if (j < K) u.b[j] = w[row * K + j];
         }
         *(uint4_t *)(out + i * 16) = u.v;
     }
