@@ -501,6 +501,7 @@ typedef struct mfl_fp8_weight {
 #define MFL_FP8_GLU 2 /* mfl_glu_fwd_fp8 */
 #define MFL_FP8_GLU_BWD 3 /* mfl_glu_bwd_fp8 (src_rows is not used) */
 #define MFL_FP8_MLP 4 /* mfl_mlp_fwd_fp8, N the intermediate and K the hidden size */
+#define MFL_FP8_MLP_OFF_GRID 5 /* the same where gate, up, e_out or g_out lie off the 16-byte grid (at least as much) */
 MFL_API size_t mfl_fp8_workspace(int op, int64_t src_rows, int64_t R, int N, int K, int E);
 
 /* y[r,n] = sum_k w[e(r),n,k] x[s(r),k], e(r) from m_sizes as in mfl_gemm_fwd, s(r) = row_idx[r] / idx_div of src_rows rows

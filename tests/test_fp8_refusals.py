@@ -152,3 +152,24 @@ def test_widths_past_what_is_counted(p):
         assert lib.mfl_fp8_dequant_blocks(p, p, 1, n, k, p, BF16, None) == SHAPE
     assert lib.mfl_fp8_quant_rows(p, BF16, 1, big, p, p, None) == SHAPE
     assert lib.mfl_fp8_dequant_rows(p, p, 1, big, p, BF16, None) == SHAPE
+
+
+def test_mlp_workspace_holds_fp32_values_only_where_they_are_needed(p):
+    """Tiles take the unit's result to quantised rows themselves: nothing of 4 bytes an element, 131072 rows of 768."""
+    lib, w = _lib.lib(), _lib.Fp8Weight(p, p)
+    rows = 16384 * 2048 + 16384 * 16 + 131072 * 768 + 131072 * 8
+    assert lib.mfl_fp8_workspace(4, 16384, 131072, 768, 2048, 128) == rows
+    assert lib.mfl_fp8_workspace(5, 16384, 131072, 768, 2048, 128) == rows + 131072 * 768 * 4
+    values = 40 * 64 * 4
+    for args, needed in (((10, 40, 64, 208, 4), False), ((10, 32, 64, 208, 4), True), ((10, 40, 64, 128, 4), True)):
+        r, n, k = args[1:4]
+        up = lambda b: -(-b // 256) * 256
+        least = up(10 * (-(-k // 128) * 128)) + up(10 * 4) + up(r * 128) + up(r * 4)
+        assert lib.mfl_fp8_workspace(4, *args) == least + (up(r * n * 4) if needed else 0)
+        assert lib.mfl_fp8_workspace(5, *args) == least + up(r * n * 4)
+    # weights off the grid need the larger one, and say so before anything is launched
+    off = _lib.Fp8Weight(p + 1, p)
+    small = lib.mfl_fp8_workspace(4, 10, 40, 64, 208, 4)
+    assert lib.mfl_mlp_fwd_fp8(p, 10, p, 4, off, w, w, p, I32, p, None, None, 40, 64, 208, 4, BF16, p, small, None) == WORKSPACE
+    assert lib.mfl_mlp_fwd_fp8(p, 10, p, 4, w, w, w, p, I32, p, p + 2, p + 2, 40, 64, 208, 4, BF16, p, small, None) == WORKSPACE
+    assert values == lib.mfl_fp8_workspace(5, 10, 40, 64, 208, 4) - small

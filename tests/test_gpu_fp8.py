@@ -772,3 +772,33 @@ def test_narrow_odd_rows_of_weights(k):
                                    (grouped_gemm_forward_transposed_fp8(dy, w, s, sizes(counts)), dy, True)):
         q, _, slack = quantize(given.double())
         assert_within(out, *product(q, slack, dense(w, s), counts, transposed, True), "input gradient" if transposed else "forward")
+
+
+@pytest.mark.parametrize("shift", [0, 1])
+def test_mlp_through_the_c_interface_writes_its_workspace_only(shift):
+    """Outputs on and off the 16-byte grid, with a workspace of the size that is asked for and guard bytes behind it."""
+    from qwen3_moe_fused import _lib
+    from qwen3_moe_fused.grouped_gemm.forward_fp8 import MLP, MLP_OFF_GRID, fp8_weight
+    from qwen3_moe_fused.grouped_gemm.fused import grouped_mlp_forward_fp8
+
+    m_sizes, sort_idx, _, counts = routed(300, 2, 8, 98)
+    for hidden, inter in ((256, 136), (331, 200)):
+        x, w = make_rows(300, hidden, torch.bfloat16, 99, spread=False), mlp_weights(8, hidden, inter, 100)
+        y, e, g = grouped_mlp_forward_fp8(x, *w, m_sizes, sort_idx, 2, return_products=True)
+        ours = torch.full((3, 600 * max(hidden, inter) + 8), 7.0, device=DEV, dtype=torch.bfloat16)
+        out = [ours[i, shift:shift + t.numel()].view(t.shape) for i, t in enumerate((y, e, g))]
+        size = _lib.lib().mfl_fp8_workspace(MLP_OFF_GRID if shift else MLP, 300, 600, inter, hidden, 8)
+        ws = torch.full((size + 4096,), 171, device=DEV, dtype=torch.uint8)
+        rc = _lib.lib().mfl_mlp_fwd_fp8(x.data_ptr(), 300, sort_idx.data_ptr(), 2, *(fp8_weight(*w[i:i + 2]) for i in (0, 2, 4)),
+                                        m_sizes.data_ptr(), _lib.I32, *(t.data_ptr() for t in out), 600, inter, hidden, 8,
+                                        _lib.BF16, ws.data_ptr(), size, _lib.stream())
+        assert rc == 0 and (ws[size:] == 171).all()
+        for t, buf in zip(out, ours):
+            assert (buf[:shift] == 7).all() and (buf[shift + t.numel():] == 7).all()
+        re, de, rg, dg = gated_reference(x, ((w[0], w[1]), (w[2], w[3])), sort_idx, 2, counts)
+        assert_within(out[1], re, de, "gate projection")
+        assert_within(out[2], rg, dg, "up projection")
+        q, _, slack = quantize(*gated(re, de, rg, dg))
+        assert_within(out[0], *product(q, slack, dense(w[4], w[5]), counts, cut=True), "expert MLP")
+        if not shift:
+            assert all(torch.equal(a, b) for a, b in zip(out, (y, e, g)))

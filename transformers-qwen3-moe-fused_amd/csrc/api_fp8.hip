@@ -73,8 +73,27 @@ int run_product(Fp8Product p, uint8_t *room, hipStream_t stream) {
     }
     int rc = gemm_fp8_tile(p, stream);
     if (rc != MFL_ERR_UNSUPPORTED) return rc;
+    if (p.hq != nullptr && p.h32 == nullptr) return MFL_ERR_WORKSPACE;  // (no such call: mlp_needs_values)
     rc = gemm_fp8_generic(p, stream);
     return rc || p.hq == nullptr ? rc : fp8_quant_rows(p.h32, MFL_F32, p.R, p.N, p.hq, p.hq_scale, stream);
+}
+
+// Whether the expert MLP's gated unit leaves fp32 values in the workspace (the tiles write quantised rows, the other kernels do
+// not).  `on_grid`: gate, up and the products' outputs lie on the 16-byte grid.
+bool mlp_needs_values(int64_t src_rows, int64_t R, int N, int K, int E, bool on_grid) {
+    if (R <= (int64_t)kFp8DecodeRowsPerExpert * E || !on_grid) return true;
+    static const int32_t gathered = 0;
+    Fp8Product p = {};
+    p.glu = true, p.terms = 1, p.row_idx = &gathered, p.src_rows = src_rows > 256 ? src_rows : 256, p.out_dtype = MFL_F32;
+    p.R = R, p.N = N, p.K = K, p.E = E, p.ldw = padded_bytes(R, N, K, E) != 0 ? padded_row(K) : K;
+    return !gemm_fp8_tiles(p);
+}
+size_t mlp_values_bytes(bool needed, int64_t R, int N) { return needed ? up256((size_t)R * N * 4) : 0; }
+// (the down projection's padded copy takes the place of the others')
+size_t mlp_bytes(int64_t src_rows, int64_t R, int N, int K, int E, bool on_grid) {
+    const size_t front = 2 * padded_bytes(R, N, K, E), back = padded_bytes(R, K, N, E);
+    return rows_bytes(src_rows, K) + rows_bytes(R, N) + mlp_values_bytes(mlp_needs_values(src_rows, R, N, K, E, on_grid), R, N) +
+           (front > back ? front : back);
 }
 
 }  // namespace
@@ -92,11 +111,10 @@ size_t mfl_fp8_workspace(int op, int64_t src_rows, int64_t R, int N, int K, int 
             return rows_bytes(R, N) + padded_bytes(R, N, K, E);
         case MFL_FP8_GLU_BWD:
             return 2 * rows_bytes(R, N) + 2 * padded_bytes(R, N, K, E);
-        case MFL_FP8_MLP: {
-            // (the down projection's copy takes the place of the others')
-            const size_t front = 2 * padded_bytes(R, N, K, E), back = padded_bytes(R, K, N, E);
-            return rows_bytes(src_rows, K) + rows_bytes(R, N) + up256((size_t)R * N * 4) + (front > back ? front : back);
-        }
+        case MFL_FP8_MLP:
+            return mlp_bytes(src_rows, R, N, K, E, true);
+        case MFL_FP8_MLP_OFF_GRID:
+            return mlp_bytes(src_rows, R, N, K, E, false);
         default:
             return 0;
     }
@@ -219,12 +237,14 @@ int mfl_mlp_fwd_fp8(const void *x, int64_t src_rows, const int32_t *row_idx, int
     const size_t size = dtype_size(dtype);
     if (!aligned(x, size) || !aligned(y, size) || !aligned(e_out, size) || !aligned(g_out, size)) return MFL_ERR_ALIGN;
     if ((e_out == nullptr) != (g_out == nullptr)) return MFL_ERR_NULL;
-    rc = check_workspace(MFL_FP8_MLP, src_rows, R, I, H, E, workspace, ws_bytes);
+    const bool on_grid = aligned(gate->q, 16) && aligned(up->q, 16) && aligned(e_out, 16) && aligned(g_out, 16);
+    rc = check_workspace(on_grid ? MFL_FP8_MLP : MFL_FP8_MLP_OFF_GRID, src_rows, R, I, H, E, workspace, ws_bytes);
     if (rc) return rc;
+    const size_t values = mlp_values_bytes(mlp_needs_values(src_rows, R, I, H, E, on_grid), R, I);
     const int64_t used = source_rows(src_rows, row_idx, R);
     const RowsRoom room((uint8_t *)workspace, used, H), hidden((uint8_t *)workspace + rows_bytes(src_rows, H), R, I);
     void *const h = (uint8_t *)workspace + rows_bytes(src_rows, H) + rows_bytes(R, I);
-    uint8_t *const padding = (uint8_t *)h + up256((size_t)R * I * 4);
+    uint8_t *const padding = (uint8_t *)h + values;
     Fp8Product p = {};
     p.glu = true, p.terms = 1, p.a[0] = room.rows(), p.w[0] = matrix(gate), p.w[1] = matrix(up);
     p.row_idx = row_idx, p.idx_div = idx_div, p.src_rows = used;
@@ -241,7 +261,7 @@ int mfl_mlp_fwd_fp8(const void *x, int64_t src_rows, const int32_t *row_idx, int
     }
     rc = fp8_quant_rows(x, dtype, used, H, room.q, room.scale, (hipStream_t)stream);
     if (rc) return rc;
-    p.hq = hidden.q, p.hq_scale = hidden.scale, p.h32 = (float *)h;
+    p.hq = hidden.q, p.hq_scale = hidden.scale, p.h32 = values != 0 ? (float *)h : nullptr;
     rc = run_product(p, padding, (hipStream_t)stream);
     return rc ? rc : run_product(d, padding, (hipStream_t)stream);
 }

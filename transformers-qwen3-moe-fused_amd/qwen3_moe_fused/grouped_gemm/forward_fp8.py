@@ -16,7 +16,7 @@ from ..quantize.fp8 import check_fp8_weight
 from ._common import is_int_tensor
 
 # MFL_FP8_*: whose workspace is asked for
-FWD, DX, GLU, GLU_BWD, MLP = 0, 1, 2, 3, 4
+FWD, DX, GLU, GLU_BWD, MLP, MLP_OFF_GRID = 0, 1, 2, 3, 4, 5
 _NO_WORKSPACE = -5  # MFL_ERR_WORKSPACE
 # Rows per expert up to which the forward product and the gated unit are called without scratch memory first: decode sizes do
 # without, and asking for it and allocating it is a fifth of such a call's time on the host.

@@ -28,7 +28,7 @@ from ._common import check_operands, is_int_tensor
 from .forward import grouped_gemm_forward
 from ..quantize.fp8 import check_fp8_weight
 from .forward_4bit import UNSUPPORTED, check_packed, grouped_gemm_forward_4bit
-from .forward_fp8 import GLU, GLU_BWD, MLP, call_with_workspace, check_rows, fp8_weight, fp8_workspace
+from .forward_fp8 import GLU, GLU_BWD, MLP, MLP_OFF_GRID, call_with_workspace, check_rows, fp8_weight, fp8_workspace
 
 
 def _gather(x_src: torch.Tensor, row_idx: torch.Tensor, idx_div: int) -> torch.Tensor:
@@ -476,7 +476,8 @@ def grouped_mlp_forward_fp8(x: torch.Tensor, w_gate: torch.Tensor, gate_scale: t
         e = x.new_empty(rows, n) if return_products else None
         g = torch.empty_like(e) if return_products else None
         ms = _lib.as_index_tensor(m_sizes)
-        _keep, ws, ws_bytes = fp8_workspace(MLP, x, x.shape[0], rows, n, k, experts)
+        on_grid = (w_gate.data_ptr() | w_up.data_ptr()) % 16 == 0
+        _keep, ws, ws_bytes = fp8_workspace(MLP if on_grid else MLP_OFF_GRID, x, x.shape[0], rows, n, k, experts)
         rc = _lib.lib().mfl_mlp_fwd_fp8(x.data_ptr(), x.shape[0], _lib.ptr(row_idx), idx_div, fp8_weight(w_gate, gate_scale),
                                         fp8_weight(w_up, up_scale), fp8_weight(w_down, down_scale), ms.data_ptr(),
                                         _lib.itype_code(ms.dtype), y.data_ptr(), _lib.ptr(e), _lib.ptr(g), rows, n, k, experts,
