@@ -802,3 +802,33 @@ def test_mlp_through_the_c_interface_writes_its_workspace_only(shift):
         assert_within(out[0], *product(q, slack, dense(w[4], w[5]), counts, cut=True), "expert MLP")
         if not shift:
             assert all(torch.equal(a, b) for a, b in zip(out, (y, e, g)))
+
+
+# ---- how far the expert MLP is from its definition as a whole ---------------------------------------------------------------
+
+# The gated unit's values are rounded to the 8-bit grid from computed sums.  A value that is off by d lands on the other side of a
+# border with probability d / step and is then off by a step, 1/8 of the value at most, so the mean square of what that adds is
+# d |h| / 8.  For e, g of unit variance and sums off by s on average that is 1.8 s / 8 of the mean square of h (E[|silu'(e) silu(e)|] =
+# 0.36, E[silu(e)^2] = 0.36, E|g| = 0.8), and the down projection keeps the ratio.  fp32 sums: some 24 roundings one behind the
+# other, each with a standard deviation of 2^-24 / sqrt(3), so s = 0.8 * 1.7e-7, which gives 1.7e-4; twice that for the few values
+# of a test.  Products cut off 2^-13 below the largest of eight (bf16 rows, more than 8 per expert): s <= 0.8 * 2^-13 sqrt(8 / 3)
+# (the reference's CUT), 6.0e-3.
+BORDERS, BORDERS_CUT = 3.5e-4, 6e-3
+
+
+@pytest.mark.parametrize("tokens,k,experts", [(128, 8, 128), (300, 4, 8)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_expert_mlp_is_as_near_as_its_type(tokens, k, experts, dtype):
+    """Over the norm, and beyond the rounding of the output itself."""
+    from qwen3_moe_fused.fused_mlp import moe_fused_mlp_fp8
+
+    m_sizes, sort_idx, inv, counts = routed(tokens, k, experts, 101)
+    x, w = make_rows(tokens, 2048, dtype, 102, spread=False), mlp_weights(experts, 2048, 256, 103)
+    y = moe_fused_mlp_fp8(x, *w, m_sizes, sort_idx, inv, k)
+    rows = quantize(x.double())[0][sort_idx.long() // k]
+    e, g = (grouped(rows, dense(w[i], w[i + 1]), counts) for i in (0, 2))
+    exact = grouped(quantize(e * torch.sigmoid(e) * g)[0], dense(w[4], w[5]), counts)
+    off = [((t.double() - exact).norm() / exact.norm()).item() for t in (y, exact.to(dtype))]
+    beyond = max(off[0] ** 2 - off[1] ** 2, 0.0) ** 0.5
+    tiles_in_8_bit = dtype == torch.bfloat16 and tokens * k > 8 * experts
+    assert beyond <= (BORDERS_CUT if tiles_in_8_bit else BORDERS), (beyond, *off)

@@ -8,7 +8,8 @@
 // multiplied.  A lane holds bytes 16 g .. 16 g + 15 and 64 + 16 g .. of a row of the block (g: its quarter of the wave), so that
 // four lanes read 64 bytes of a row together; the rows are loaded in the same order, their largest magnitude found over the
 // four lanes, and rounded to e4m3 in registers (the order within the block does not matter as long as both operands agree).
-// The waves' sums meet in LDS.
+// The waves' sums meet in LDS.  The gated unit's operands are widened to bf16 and multiplied by v_mfma_f32_16x16x32_bf16 (fp8.h
+// says why): 32 tokens 67.0 against 65.8 us, one token's MLP 22.3 either way.
 //
 // Bound by the weights' bytes: 32 tokens of 8 of 128 experts, 2048 to 2 x 768, 66 us for 349 MB, 5.3 TB/s.  Of a single token's
 // 10 us (25 MB) a wave spends 0.8 finding its rows, 3 (weights in the caches) to 7 until weights and rows are there and quantised, 0.8
@@ -133,7 +134,7 @@ __device__ __forceinline__ bool find_rows(const Fp8Product &p, int slot, int lan
     return false;
 }
 
-// AHEAD: blocks of the reduction that a wave holds of the rows, and of every piece, at a time.
+// AHEAD: blocks of the reduction that a wave holds of the rows, and of every piece, at a time.  Gated: bf16 products.
 template <bool GLU, int PIECES, int AHEAD, typename TX, typename TO>
 __global__ __launch_bounds__(kWaves * 64, 2) void fp8_decode_kernel(Fp8Product p, const TX *__restrict__ x) {
     static_assert(!GLU || PIECES % 2 == 0, "gated: blocks of columns of both matrices");
@@ -160,6 +161,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void fp8_decode_kernel(Fp8Product p
 
     union Frag {
         uint4_t v[2];
+        intx2 t[4];
         intx8 i;
     };
     // A chunk of the reduction, blocks b0, b0 + 4, ...  Whole: all of them are there to the end, and nothing is asked about them (a
@@ -199,7 +201,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void fp8_decode_kernel(Fp8Product p
 #pragma unroll
         for (int t = 0; t < kBuffers - 1 && t < PIECES; ++t) load(t);
         // the rows' blocks, quantised
-        intx8 q[AHEAD];
+        Frag q[AHEAD];
+        bf16x8 wide[AHEAD][4];  // (gated)
         int byte[AHEAD];
         {
             int64_t row = src;
@@ -226,7 +229,11 @@ __global__ __launch_bounds__(kWaves * 64, 2) void fp8_decode_kernel(Fp8Product p
                 int lo[4], hi[4];
                 fx[u][0].pack(lo, scale);
                 fx[u][1].pack(hi, scale);
-                q[u] = intx8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                q[u].i = intx8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                if constexpr (GLU) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) wide[u][i] = fp8_widen(q[u].t[i], scale);
+                }
             }
         }
 #pragma unroll
@@ -235,8 +242,15 @@ __global__ __launch_bounds__(kWaves * 64, 2) void fp8_decode_kernel(Fp8Product p
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
                 if (!W && b0 + kWaves * u >= blocks) break;
-                const floatx4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-                const floatx4 part = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw[t % kBuffers][u].i, q[u], zero, 0, 0, 0, 127, 0, byte[u]);
+                const Frag &w = fw[t % kBuffers][u];
+                floatx4 part = {0.0f, 0.0f, 0.0f, 0.0f};
+                if constexpr (GLU) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp8_widen(w.t[i], 1.0f), wide[u][i], part, 0, 0, 0);
+                } else {
+                    part = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.i, q[u].i, part, 0, 0, 0, 127, 0, byte[u]);
+                }
                 const float s = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(scales), t * AHEAD + u));
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[t][i] = __builtin_fmaf(s, part[i], acc[t][i]);

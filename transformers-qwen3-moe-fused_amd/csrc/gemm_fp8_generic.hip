@@ -6,11 +6,8 @@
 //   input gradient  out[r, k] = sum_b S[e, b, k / 128] sd[r, b] sum_{n in block b} d[r, n] w[e, n, k]
 //
 // A step is one block of 128 of the reduction: eight bf16 matrix instructions into fresh accumulators, and a multiply-add by
-// both scales into the running fp32 sums.  bf16 and not the 8-bit matrix instruction, because the latter adds its products in
-// groups of eight with all but 14 bits below the group's largest product cut off (measured: 2^-13 of the largest survives,
-// 2^-14 does not; 3e-6 of the sum of magnitudes on average, 1.7e-5 at most, against 1e-9 and 1.5e-8 with bf16): far below a
-// 16-bit output's rounding, far above an fp32 one's.  The weights are the first operand, so that a lane's accumulators belong
-// to one row (its scale is the lane's) and to runs of four columns.  For widths that no 16-byte access fits the weights are
+// both scales into the running fp32 sums (bf16 products for every output: fp8.h).  The weights are the first operand, so that
+// a lane's accumulators belong to one row (its scale is the lane's) and to runs of four columns.  For widths that no 16-byte access fits the weights are
 // read byte by byte; that, and the plain load-wait-multiply order, is what bounds it: 32768 rows, 128 experts, 2048 to 768,
 // fp32, weights off the grid 1226 us, its input gradient 2763 (tiles, weights on the grid: 213 and 200).
 #include "fp8.h"

@@ -14,10 +14,8 @@
 //   scale it hands to the instruction) and to runs of four columns.  Two instructions make a block's partial sum over a step,
 //   16 multiply-adds by the weights' scale (uniform: 128 x 128) add it to the running fp32 sum.
 //
-// The instruction adds its products in groups of eight and cuts them off 2^-13 below the group's largest (measured): 3e-6 of
-// the sum of magnitudes on average, where the rounding of a 16-bit output is 2e-4 or 2e-3 of the sum itself.  For fp32 outputs
-// the fragments are widened to bf16 in registers, which holds every e4m3 value times its row's scale, and multiplied by
-// v_mfma_f32_32x32x16_bf16 (1e-9): half the rate, and 16 conversions a fragment.
+// For fp32 outputs and the quantised gated unit in fp16 the fragments are widened to bf16 in registers and multiplied by
+// v_mfma_f32_32x32x16_bf16: half the rate, and 16 conversions a fragment (fp8.h says why).
 //
 // LDS layouts.  Rows of 128 bytes along the reduction: 16-byte chunk c of row r at c ^ ((r >> 1) & 7).  A lane's 32 bytes of a
 // 64-wide sub-step are chunks 4 s + h and 4 s + 2 + h (h: its half of the wave); which reduction element sits where in the
@@ -33,7 +31,6 @@ namespace mfl {
 namespace {
 
 typedef __attribute__((address_space(3))) void *lds_void_ptr;
-typedef __attribute__((ext_vector_type(2))) int intx2;
 typedef __attribute__((address_space(3))) intx2 *lds_intx2_ptr;
 typedef const __attribute__((address_space(3))) uint4_t *lds_uint4_ptr;
 typedef const __attribute__((address_space(3))) uint32_t *lds_uint32_ptr;
@@ -97,28 +94,14 @@ struct Shape {
     static_assert(kA % (1024 * kWaves) == 0 && kB % (1024 * kWaves) == 0 && kSLanes + 2 <= 64, "whole copies");
 };
 
-// 8 e4m3 values times the power of two `scale`, as bf16 (exact)
-__device__ __forceinline__ bf16x8 widen(const intx2 v, float scale) {
-    typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
-    union {
-        bf16x2 p[4];
-        bf16x8 all;
-    } u;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        u.p[2 * i] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[i], scale, false);
-        u.p[2 * i + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[i], scale, true);
-    }
-    return u.all;
-}
-
 // HQ: the gated unit's result leaves as quantised rows.  PARTIAL: the reduction ends inside a block of 128.
 template <bool DX, bool GLU, bool HQ, bool PARTIAL, int WM, int WN, int MI, int NI, int STAGES, typename TO>
 __global__ __launch_bounds__(WM * WN * 64, 2) void fp8_tile_kernel(Fp8Product p) {
     using S = Shape<WM, WN, MI, NI, STAGES>;
     constexpr int BM = S::BM, BN = S::BN, kWaves = S::kWaves;
     constexpr int BNC = GLU ? BN / 2 : BN;  // output columns of a tile
-    constexpr bool kWide = sizeof(TO) == 4;  // fp32 outputs: bf16 products
+    constexpr bool kF32 = sizeof(TO) == 4;
+    constexpr bool kBf16 = kF32 || (HQ && std::is_same<TO, f16_t>::value);  // bf16 products
     static_assert(!GLU || NI == 2, "gated: a wave holds one block of either matrix");
     static_assert(!HQ || (GLU && BNC == kFp8Block), "quantised output: a tile's columns are one scale block");
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
@@ -385,13 +368,13 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void fp8_tile_kernel(Fp8Product p)
 #pragma unroll
                     for (int q = 0; q < 16; ++q) part[j][q] = 0.0f;
                 }
-                if constexpr (!kWide) {
+                if constexpr (!kBf16) {
                     part[j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fw[j][s].i, fa[s].i, part[j], 0, 0, 0, 127, 0, xscale[i & 1]);
                 } else {
                     const float row_scale = fp8_scale_of(xscale[i & 1] & 255);
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
-                        part[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(widen(fw[j][s].t[q], 1.0f), widen(fa[s].t[q], row_scale), part[j], 0, 0, 0);
+                        part[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fp8_widen(fw[j][s].t[q], 1.0f), fp8_widen(fa[s].t[q], row_scale), part[j], 0, 0, 0);
                 }
             };
             auto add = [&](int i, int j, float scale) {
@@ -514,7 +497,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void fp8_tile_kernel(Fp8Product p)
         // 32 columns of a row block from the wave's column n0 on, from f(q), the lane's q-th value
         auto store_block = [&](void *base, int i, auto f, int n0) {
             const int r = (i * WM + wm) * 32 + l;
-            if constexpr (kWide) {
+            if constexpr (kF32) {
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
                     const int n = cur.col0 + acol0 + n0 + 8 * t + 4 * half;
@@ -576,7 +559,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void fp8_tile_kernel(Fp8Product p)
             }
         }
         newer = GLU ? whole * 2 * ((HQ ? 0 : 1) + (p.e_out != nullptr) + (p.g_out != nullptr)) : whole * 4;
-        if (kWide) newer *= 2;
+        if (kF32) newer *= 2;
         if (HQ) {
             // a row's 128 columns are with the WN waves of its wave row: the largest magnitude goes through LDS
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
