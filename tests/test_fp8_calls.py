@@ -1,0 +1,120 @@
+"""How the 8-bit floating-point products are called, on the CPU: the tensors claim to be on the GPU, and the library is a
+stand-in that sums every row of the left operand."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+import torch.autograd.forward_ad as forward_ad
+
+from qwen3_moe_fused import _lib
+from qwen3_moe_fused.fused_mlp import moe_fused_glu_fp8, moe_fused_mlp_fp8
+from qwen3_moe_fused.quantize.layer_fp8 import moe_fused_linear_fp8
+
+FP8 = torch.float8_e4m3fn
+TOKENS, K, EXPERTS, HIDDEN, INTER = 4, 2, 3, 256, 128
+ROWS = TOKENS * K
+
+
+def _array(address, *shape):
+    return np.ctypeslib.as_array((ctypes.c_float * int(np.prod(shape))).from_address(address)).reshape(shape)
+
+
+class _RowSums:
+    """Every output's row r is filled with the sum of the row that it is made of (fp32 only)."""
+
+    def __init__(self):
+        self.calls = []
+
+    def mfl_fp8_workspace(self, *sizes):
+        return 0
+
+    def _run(self, name, x, src_rows, idx, div, width, outs, rows):
+        self.calls.append(name)
+        source = _array(x, src_rows, width).sum(axis=1)
+        index = np.arange(rows) if idx is None else np.ctypeslib.as_array((ctypes.c_int32 * rows).from_address(idx)) // div
+        for at, n in outs:
+            if at is not None:
+                _array(at, rows, n)[:] = source[index][:, None]
+        return 0
+
+    def mfl_gemm_fwd_fp8(self, x, src, idx, div, w, ms, it, y, rows, n, k, *rest):
+        return self._run("gemm_fwd", x, src, idx, div, k, [(y, n)], rows)
+
+    def mfl_gemm_dx_fp8(self, dy, w, ms, it, dx, rows, n, k, *rest):
+        return self._run("gemm_dx", dy, rows, None, 1, n, [(dx, k)], rows)
+
+    def mfl_glu_fwd_fp8(self, x, src, idx, div, gate, up, ms, it, h, e, g, rows, n, k, *rest):
+        return self._run("glu_fwd", x, src, idx, div, k, [(h, n), (e, n), (g, n)], rows)
+
+    def mfl_glu_bwd_fp8(self, dh, e, g, gate, up, ms, it, dx, rows, n, k, *rest):
+        return self._run("glu_bwd", dh, rows, None, 1, n, [(dx, k)], rows)
+
+    def mfl_mlp_fwd_fp8(self, x, src, idx, div, gate, up, down, ms, it, y, e, g, rows, inter, hidden, *rest):
+        return self._run("mlp_fwd", x, src, idx, div, hidden, [(y, hidden), (e, inter), (g, inter)], rows)
+
+    def mfl_combine_rows(self, *args):
+        self.calls.append("combine")
+        return 0
+
+
+@pytest.fixture
+def library(monkeypatch):
+    stand_in = _RowSums()
+    monkeypatch.setattr(torch.Tensor, "is_cuda", True)
+    monkeypatch.setattr(_lib, "lib", lambda: stand_in)
+    monkeypatch.setattr(_lib, "stream", lambda: 0)
+    return stand_in
+
+
+def _weights():
+    out = []
+    for n, k in ((INTER, HIDDEN), (INTER, HIDDEN), (HIDDEN, INTER)):
+        out += [torch.zeros((EXPERTS, n, k), dtype=torch.uint8).view(FP8), torch.ones(EXPERTS, n // 128, k // 128)]
+    return out
+
+
+def _call(which):
+    """(a function of the left operand, its rows)"""
+    w, sizes = _weights(), torch.tensor([3, 4, 1], dtype=torch.int32)
+    idx = torch.arange(ROWS, dtype=torch.int32)
+    if which == "linear":
+        return lambda x: moe_fused_linear_fp8(x, w[0], w[1], sizes), ROWS
+    if which == "glu":
+        return lambda x: moe_fused_glu_fp8(x, *w[:4], sizes, idx, idx.clone(), K), TOKENS
+    return lambda x: moe_fused_mlp_fp8(x, *w, sizes, idx, idx.clone(), K), TOKENS
+
+
+WHICH = pytest.mark.parametrize("which", ["linear", "glu", "mlp"])
+
+
+@WHICH
+def test_a_trace_holds_the_call(library, which):
+    call, rows = _call(which)
+    a, b = torch.randn(rows, HIDDEN), torch.randn(rows, HIDDEN)
+    with torch.no_grad():
+        traced = torch.jit.trace(call, (a,), check_trace=False)
+        del library.calls[:]
+        got = traced(b)
+        assert len(library.calls) == 1
+        assert torch.equal(got, call(b)) and not torch.equal(got, call(a))
+
+
+@WHICH
+@pytest.mark.parametrize("grad", [False, True])
+def test_tangents_are_refused(library, which, grad):
+    call, rows = _call(which)
+    x = torch.randn(rows, HIDDEN, requires_grad=grad)
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        with pytest.raises((NotImplementedError, RuntimeError)):
+            call(forward_ad.make_dual(x, torch.ones_like(x)))
+
+
+@WHICH
+def test_a_plain_call_without_gradients_is_one_library_call(library, which):
+    call, rows = _call(which)
+    x = torch.randn(rows, HIDDEN)
+    out = call(x)
+    expect = x.sum(1) if which == "linear" else x.sum(1).repeat_interleave(K)
+    assert len(library.calls) == 1 and not out.requires_grad
+    assert torch.allclose(out, expect[:, None].expand_as(out), rtol=1e-4, atol=1e-4)

@@ -151,8 +151,11 @@ def moe_fused_glu_4bit(tokens: torch.Tensor, gate_weight: torch.Tensor, up_weigh
 class _GluGatheredFp8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, tokens, w_gate, gate_scale, w_up, up_scale, m_sizes, sort_idx, inv_sort_idx, k):
-        h, e, g = grouped_glu_forward_fp8(tokens, w_gate, gate_scale, w_up, up_scale, m_sizes, sort_idx, k,
-                                          return_products=True)
+        need = ctx.needs_input_grad[0]
+        out = grouped_glu_forward_fp8(tokens, w_gate, gate_scale, w_up, up_scale, m_sizes, sort_idx, k, return_products=need)
+        if not need:
+            return out
+        h, e, g = out
         ctx.save_for_backward(w_gate, gate_scale, w_up, up_scale, m_sizes, inv_sort_idx, e, g)
         ctx.k, ctx.n_tokens = k, tokens.shape[0]
         return h
@@ -180,7 +183,7 @@ def moe_fused_glu_fp8(tokens: torch.Tensor, w_gate: torch.Tensor, gate_scale: to
     assert not (w_gate.requires_grad or gate_scale.requires_grad or w_up.requires_grad or up_scale.requires_grad), \
         "8-bit expert weights are frozen"
     _check_routing(tokens, sort_idx, inv_sort_idx, num_selected)
-    if not (torch.is_grad_enabled() and tokens.requires_grad):
+    if not (torch.is_grad_enabled() and tokens.requires_grad) and _lib.plain_call():  # (as in moe_fused_linear_fp8)
         return grouped_glu_forward_fp8(tokens, w_gate, gate_scale, w_up, up_scale, m_sizes, sort_idx, num_selected)
     return _GluGatheredFp8.apply(tokens, w_gate, gate_scale, w_up, up_scale, m_sizes, sort_idx, inv_sort_idx, num_selected)
 
@@ -188,8 +191,12 @@ def moe_fused_glu_fp8(tokens: torch.Tensor, w_gate: torch.Tensor, gate_scale: to
 class _MlpGatheredFp8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, tokens, w_gate, gate_scale, w_up, up_scale, w_down, down_scale, m_sizes, sort_idx, inv_sort_idx, k):
-        y, e, g = grouped_mlp_forward_fp8(tokens, w_gate, gate_scale, w_up, up_scale, w_down, down_scale, m_sizes, sort_idx, k,
-                                          return_products=True)
+        need = ctx.needs_input_grad[0]
+        out = grouped_mlp_forward_fp8(tokens, w_gate, gate_scale, w_up, up_scale, w_down, down_scale, m_sizes, sort_idx, k,
+                                      return_products=need)
+        if not need:
+            return out
+        y, e, g = out
         ctx.save_for_backward(w_gate, gate_scale, w_up, up_scale, w_down, down_scale, m_sizes, inv_sort_idx, e, g)
         ctx.k, ctx.n_tokens = k, tokens.shape[0]
         return y
@@ -212,7 +219,7 @@ def moe_fused_mlp_fp8(tokens: torch.Tensor, w_gate: torch.Tensor, gate_scale: to
     assert not (w_gate.requires_grad or gate_scale.requires_grad or w_up.requires_grad or up_scale.requires_grad
                 or w_down.requires_grad or down_scale.requires_grad), "8-bit expert weights are frozen"
     _check_routing(tokens, sort_idx, inv_sort_idx, num_selected)
-    if not (torch.is_grad_enabled() and tokens.requires_grad):
+    if not (torch.is_grad_enabled() and tokens.requires_grad) and _lib.plain_call():  # (as in moe_fused_linear_fp8)
         return grouped_mlp_forward_fp8(tokens, w_gate, gate_scale, w_up, up_scale, w_down, down_scale, m_sizes, sort_idx,
                                        num_selected)
     return _MlpGatheredFp8.apply(tokens, w_gate, gate_scale, w_up, up_scale, w_down, down_scale, m_sizes, sort_idx,

@@ -12,6 +12,7 @@ from typing import Optional
 import torch
 from torch import nn
 
+from .. import _lib
 from ..grouped_gemm.forward_fp8 import grouped_gemm_forward_fp8, grouped_gemm_forward_transposed_fp8
 from ..modular_qwen3_moe_fused import MoeFusedLinear
 from .fp8 import FP8, blocks_of, quantize_fp8_blocks
@@ -39,7 +40,8 @@ def moe_fused_linear_fp8(input: torch.Tensor, weight: torch.Tensor, weight_scale
     """``moe_fused_linear`` on ``weight`` (E, out, in) float8_e4m3fn with ``weight_scale`` (E, ceil(out / 128),
     ceil(in / 128)) fp32; both frozen.  Differentiable in ``input``."""
     assert not weight.requires_grad and not weight_scale.requires_grad, "8-bit expert weights are frozen"
-    if not (torch.is_grad_enabled() and input.requires_grad):
+    # (past autograd only where nobody watches: a tracer has to record the call, a forward-mode level has to refuse it)
+    if not (torch.is_grad_enabled() and input.requires_grad) and _lib.plain_call():
         return grouped_gemm_forward_fp8(input, weight, weight_scale, m_sizes)
     return _GroupedGemmFp8.apply(input, weight, weight_scale, m_sizes)
 
