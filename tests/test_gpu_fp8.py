@@ -832,3 +832,31 @@ def test_expert_mlp_is_as_near_as_its_type(tokens, k, experts, dtype):
     beyond = max(off[0] ** 2 - off[1] ** 2, 0.0) ** 0.5
     tiles_in_8_bit = dtype == torch.bfloat16 and tokens * k > 8 * experts
     assert beyond <= (BORDERS_CUT if tiles_in_8_bit else BORDERS), (beyond, *off)
+
+
+@pytest.mark.parametrize("rows,width", [(24, 256), (400, 256), (400, 128)])  # decode kernel, tiles, any shape's kernel
+@pytest.mark.parametrize("index", [torch.int32, torch.int64])
+def test_counts_past_every_integer_are_cut_at_the_last_row(rows, width, index):
+    from qwen3_moe_fused import _lib
+    from qwen3_moe_fused.grouped_gemm.forward_fp8 import DX, FWD, fp8_weight, fp8_workspace
+
+    x = make_rows(rows, width, torch.bfloat16, 104, spread=False)
+    w, s = make_weight(4, width, width, 105)
+    top = torch.iinfo(index).max
+    q, _, slack = quantize(x.double())
+    for counts in ([7, top, top, 5], [top, top, 5, top], [-top, 3, top - 2, top], [0, top, -1, 1]):
+        taken, left = [], rows
+        for c in counts:
+            taken.append(min(max(c, 0), left))
+            left -= taken[-1]
+        for transposed in (False, True):
+            out = torch.full((rows + 512, width), 7.0, device=DEV, dtype=torch.bfloat16)
+            _keep, ws, size = fp8_workspace(DX if transposed else FWD, x, rows, rows, width, width, 4)
+            ms = sizes(counts, index)
+            args = (ms.data_ptr(), _lib.itype_code(index), out.data_ptr(), rows, width, width, 4, _lib.BF16, _lib.BF16, ws, size,
+                    _lib.stream())
+            source = () if transposed else (rows, None, 1)
+            call = _lib.lib().mfl_gemm_dx_fp8 if transposed else _lib.lib().mfl_gemm_fwd_fp8
+            assert call(x.data_ptr(), *source, fp8_weight(w, s), *args) == 0
+            assert_within(out[:rows], *product(q, slack, dense(w, s), taken, transposed, True))
+            assert (out[rows:] == 7.0).all()

@@ -24,6 +24,7 @@
 // 1 % (weights' bytes); the tiles of that unit in bf16 have 8-bit ones (the MLP of 131072 rows 910 us against 1190).
 #pragma once
 #include "common.h"
+#include "fp8_counts.h"
 
 namespace mfl {
 
@@ -153,31 +154,52 @@ __device__ __forceinline__ uint32_t fp8_max16(uint32_t x) {
     return fp8_dpp_max<0x121>(x);
 }
 
-// Where tile `slot` of the row tiles of BM rows lies: every wave scans the row counts, 64 experts at a time.  Sizes that sum to
-// more than R rows are cut at R, negative ones count as none.  False past the last tile.
+// An expert's row count, 0 past the last expert; 64 of them, a lane each, cut at `room` rows: the lane's first row, the row behind
+// its last one, and (in every lane) that of the last lane.
+__device__ __forceinline__ uint32_t fp8_load_count(const void *m_sizes, int ms_i64, int e, int E, int64_t R) {
+    if (e >= E) return 0u;
+    return fp8_count_of(ms_i64 ? ((const int64_t *)m_sizes)[e] : ((const int32_t *)m_sizes)[e], (uint32_t)R);
+}
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ uint32_t fp8_dpp_sum(uint32_t x) {
+    return fp8_sum(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROW_MASK, 0xf, true));
+}
+struct Fp8Counted {
+    int begin, end, all;
+};
+__device__ __forceinline__ Fp8Counted fp8_cut(uint32_t count, uint32_t room) {
+    uint32_t x = count;  // (the order of wave_inclusive_scan)
+    x = fp8_dpp_sum<0x111, 0xf>(x);
+    x = fp8_dpp_sum<0x112, 0xf>(x);
+    x = fp8_dpp_sum<0x114, 0xf>(x);
+    x = fp8_dpp_sum<0x118, 0xf>(x);
+    x = fp8_dpp_sum<0x142, 0xa>(x);
+    x = fp8_dpp_sum<0x143, 0xc>(x);
+    const int end = (int)fp8_end(x, room);
+    return {(int)fp8_begin(x, count, room), end, wave_last(end)};
+}
+__device__ __forceinline__ int fp8_tiles_of(int rows, int bm) { return (int)(((uint32_t)rows + (uint32_t)bm - 1u) / (uint32_t)bm); }
+
+// Where tile `slot` of the row tiles of BM rows lies: every wave scans the row counts, 64 experts at a time.  False past the last
+// tile.
 template <int BM>
 __device__ __forceinline__ bool fp8_find_tile(const void *m_sizes, int ms_i64, int E, int64_t R, int slot, int lane, int &expert,
                                               int64_t &row0, int &rows) {
-    int tiles_before = 0;
-    int64_t rows_before = 0;
+    int tiles_before = 0, rows_before = 0;
     for (int e0 = 0; e0 < E; e0 += 64) {
-        const int e = e0 + lane;
-        int m = e < E ? load_msize(m_sizes, ms_i64, e) : 0;
-        if (m < 0) m = 0;
-        const int t = ceil_div(m, BM);
-        const int mi = wave_inclusive_scan(m), ti = wave_inclusive_scan(t);
+        const Fp8Counted c = fp8_cut(fp8_load_count(m_sizes, ms_i64, e0 + lane, E, R), (uint32_t)R - (uint32_t)rows_before);
+        const int t = fp8_tiles_of(c.end - c.begin, BM), ti = wave_inclusive_scan(t);
         const uint64_t past = __ballot(tiles_before + ti > slot);
         if (past) {
             const int src = __ffsll((unsigned long long)past) - 1;
-            const int m_e = __builtin_amdgcn_readlane(m, src);
             const int tile = slot - (tiles_before + __builtin_amdgcn_readlane(ti, src) - __builtin_amdgcn_readlane(t, src));
+            const int begin = __builtin_amdgcn_readlane(c.begin, src) + tile * BM, end = __builtin_amdgcn_readlane(c.end, src);
             expert = e0 + src;
-            row0 = rows_before + __builtin_amdgcn_readlane(mi, src) - m_e + (int64_t)tile * BM;
-            rows = m_e - tile * BM < BM ? m_e - tile * BM : BM;
-            if (row0 + rows > R) rows = (int)(R - row0);
-            return rows > 0;
+            row0 = (int64_t)rows_before + begin;
+            rows = end - begin < BM ? end - begin : BM;
+            return true;
         }
-        rows_before += wave_last(mi);
+        rows_before += c.all;
         tiles_before += wave_last(ti);
     }
     return false;

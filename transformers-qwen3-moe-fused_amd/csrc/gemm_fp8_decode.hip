@@ -102,32 +102,26 @@ __device__ __forceinline__ uint32_t over_block(uint32_t a) {
 
 // The sizes of up to 256 experts at once (their loads in flight together), then 64 at a time.
 __device__ __forceinline__ bool find_rows(const Fp8Product &p, int slot, int lane, int &expert, int64_t &row0, int &rows) {
-    int tiles_before = 0;
-    int64_t rows_before = 0;
+    int tiles_before = 0, rows_before = 0;
     for (int e0 = 0; e0 < p.E; e0 += 256) {
-        int m[4];
+        uint32_t count[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) count[i] = fp8_load_count(p.m_sizes, p.ms_i64, e0 + 64 * i + lane, p.E, p.R);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int e = e0 + 64 * i + lane;
-            m[i] = e < p.E ? load_msize(p.m_sizes, p.ms_i64, e) : 0;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (m[i] < 0) m[i] = 0;
-            const int t = ceil_div(m[i], kRows);
-            const int mi = wave_inclusive_scan(m[i]), ti = wave_inclusive_scan(t);
+            const Fp8Counted c = fp8_cut(count[i], (uint32_t)p.R - (uint32_t)rows_before);
+            const int t = fp8_tiles_of(c.end - c.begin, kRows), ti = wave_inclusive_scan(t);
             const uint64_t past = __ballot(tiles_before + ti > slot);
             if (past) {
                 const int src = __ffsll((unsigned long long)past) - 1;
-                const int m_e = __builtin_amdgcn_readlane(m[i], src);
                 const int tile = slot - (tiles_before + __builtin_amdgcn_readlane(ti, src) - __builtin_amdgcn_readlane(t, src));
+                const int begin = __builtin_amdgcn_readlane(c.begin, src) + tile * kRows, end = __builtin_amdgcn_readlane(c.end, src);
                 expert = e0 + 64 * i + src;
-                row0 = rows_before + __builtin_amdgcn_readlane(mi, src) - m_e + (int64_t)tile * kRows;
-                rows = m_e - tile * kRows < kRows ? m_e - tile * kRows : kRows;
-                if (row0 + rows > p.R) rows = (int)(p.R - row0);
-                return rows > 0;
+                row0 = (int64_t)rows_before + begin;
+                rows = end - begin < kRows ? end - begin : kRows;
+                return true;
             }
-            rows_before += wave_last(mi);
+            rows_before += c.all;
             tiles_before += wave_last(ti);
         }
     }

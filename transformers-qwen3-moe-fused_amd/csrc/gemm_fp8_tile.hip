@@ -123,21 +123,15 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void fp8_tile_kernel(Fp8Product p)
     static_assert(!DX || BN == 128 || BN == 256, "rows of half or all of the banks");
     auto spread = [](int n) { return BN == 128 ? ((n >> 1) & 3) << 1 : (n & 7) << 1; };
 
-    // ---- rows and row tiles before every expert; an expert's rows are cut into tiles of equal height, a multiple of 32
+    // ---- rows and row tiles before every expert, cut at row R; an expert's rows come in tiles of equal height, a multiple of 32
     {
         int row_carry = 0, tile_carry = 0;
         for (int e0 = 0; e0 < p.E; e0 += 64) {
             const int e = e0 + lane;
-            int m = e < p.E ? load_msize(p.m_sizes, p.ms_i64, e) : 0;
-            if (m < 0) m = 0;
-            const int64_t room = p.R - row_carry;  // sizes that sum to more than R rows are cut there
-            const int before = wave_inclusive_scan(m) - m;
-            if (before >= room) m = 0;
-            else if (before + m > room) m = (int)(room - before);
-            const int t = ceil_div(m, BM);
-            const int mi = wave_inclusive_scan(m), ti = wave_inclusive_scan(t);
-            if (wave == 0 && e < p.E) tab_rows[e] = row_carry + mi - m, tab_tiles[e] = tile_carry + ti - t;
-            row_carry += wave_last(mi), tile_carry += wave_last(ti);
+            const Fp8Counted c = fp8_cut(fp8_load_count(p.m_sizes, p.ms_i64, e, p.E, p.R), (uint32_t)p.R - (uint32_t)row_carry);
+            const int t = fp8_tiles_of(c.end - c.begin, BM), ti = wave_inclusive_scan(t);
+            if (wave == 0 && e < p.E) tab_rows[e] = row_carry + c.begin, tab_tiles[e] = tile_carry + ti - t;
+            row_carry += c.all, tile_carry += wave_last(ti);
         }
         if (tid == 0) tab_rows[p.E] = row_carry, tab_tiles[p.E] = tile_carry;
         __syncthreads();
