@@ -118,3 +118,23 @@ def test_a_plain_call_without_gradients_is_one_library_call(library, which):
     expect = x.sum(1) if which == "linear" else x.sum(1).repeat_interleave(K)
     assert len(library.calls) == 1 and not out.requires_grad
     assert torch.allclose(out, expect[:, None].expand_as(out), rtol=1e-4, atol=1e-4)
+
+
+def test_an_adapter_over_8_bit_weights_keeps_its_type_whatever_the_base_class(monkeypatch):
+    """The base class may move an adapter to the type of the base weight, as it does for 16-bit ones."""
+    from qwen3_moe_fused import lora
+    from qwen3_moe_fused.modular_qwen3_moe_fused import MoeFusedLinear
+    from qwen3_moe_fused.quantize.layer_fp8 import MoeFusedLinearFp8
+
+    def move(self, adapter_name, device=None):
+        weight = self.get_base_layer().weight
+        for adapters in (self.lora_A, self.lora_B):
+            adapters[adapter_name].to(device=weight.device, dtype=weight.dtype)
+
+    monkeypatch.setattr(lora.LoraLayer, "_move_adapter_to_device_of_base_layer", move)
+    over = lora.LoraMoeFusedLinear(MoeFusedLinearFp8(32, 16, 2), "default", r=4)
+    assert {p.dtype for p in (over.lora_A["default"].weight, over.lora_B["default"].weight)} == {torch.float32}
+    over._move_adapter_to_device_of_base_layer("default", torch.device("cpu"))
+    assert over.lora_A["default"].weight.dtype == torch.float32
+    plain = lora.LoraMoeFusedLinear(MoeFusedLinear(32, 16, 2).to(torch.bfloat16), "default", r=4)
+    assert plain.lora_A["default"].weight.dtype == torch.bfloat16

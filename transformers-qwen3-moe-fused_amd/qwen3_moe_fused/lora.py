@@ -80,8 +80,7 @@ except ImportError:
 
         def _move_adapter_to_device_of_base_layer(self, adapter_name: str) -> None:
             weight = self.base_layer.weight
-            # (packed and 8-bit floating-point base weights leave the adapter in its own type)
-            dtype = weight.dtype if weight.dtype.is_floating_point and weight.dtype.itemsize > 1 else None
+            dtype = weight.dtype if weight.dtype.is_floating_point else None  # (packed weights: the adapter's own)
             self.lora_A[adapter_name].to(device=weight.device, dtype=dtype)
             self.lora_B[adapter_name].to(device=weight.device, dtype=dtype)
 
@@ -119,6 +118,15 @@ class LoraMoeFusedLinear(nn.Module, LoraLayer):
             self.reset_lora_parameters(adapter_name, init_lora_weights)
         self._move_adapter_to_device_of_base_layer(adapter_name)
         self.set_adapter(self.active_adapters)
+
+    def _move_adapter_to_device_of_base_layer(self, adapter_name: str, device: Optional[torch.device] = None) -> None:
+        weight = self.get_base_layer().weight
+        if not (weight.dtype.is_floating_point and weight.dtype.itemsize == 1):
+            args = () if device is None else (device,)
+            return super()._move_adapter_to_device_of_base_layer(adapter_name, *args)
+        # 8-bit floating-point weights mean nothing without their scales: the adapter only changes its place
+        for adapters in (self.lora_A, self.lora_B):
+            adapters[adapter_name].to(device=weight.device if device is None else device)
 
     def reset_lora_parameters(self, adapter_name: str, init_lora_weights: Union[bool, str]) -> None:
         if init_lora_weights is False or adapter_name not in self.lora_A:
