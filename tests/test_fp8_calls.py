@@ -138,3 +138,32 @@ def test_an_adapter_over_8_bit_weights_keeps_its_type_whatever_the_base_class(mo
     assert over.lora_A["default"].weight.dtype == torch.float32
     plain = lora.LoraMoeFusedLinear(MoeFusedLinear(32, 16, 2).to(torch.bfloat16), "default", r=4)
     assert plain.lora_A["default"].weight.dtype == torch.bfloat16
+
+
+def _step(which, x):
+    call, _ = _call(which)
+    return call(x)
+
+
+@WHICH
+def test_saved_tensors_that_come_back_in_other_strides(library, monkeypatch, which):
+    """A saved-tensor hook may hand equal tensors back that are laid out otherwise."""
+    from qwen3_moe_fused import fused_mlp
+
+    monkeypatch.setattr(fused_mlp, "_combine", lambda dx, inv, *a: dx.view(TOKENS, K, -1).sum(1))
+
+    def strided(t):
+        raw = torch.empty((*t.shape, 2), dtype=torch.uint8 if t.dtype == FP8 else t.dtype)
+        out = (raw.view(FP8) if t.dtype == FP8 else raw)[..., 0]
+        assert out.is_contiguous() == (out.numel() < 2)
+        return out.copy_(t)
+
+    _, rows = _call(which)
+    grads = []
+    for unpack in (lambda t: t, strided):
+        x = torch.ones(rows, HIDDEN, requires_grad=True)
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            out = _step(which, x)
+            out.backward(torch.arange(out.numel(), dtype=torch.float32).view_as(out))
+        grads.append(x.grad)
+    assert torch.equal(*grads)

@@ -162,8 +162,9 @@ class _GluGatheredFp8(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dh):
-        w_gate, gate_scale, w_up, up_scale, m_sizes, inv_sort_idx, e, g = ctx.saved_tensors
-        dx = grouped_glu_backward_fp8(dh.contiguous(), e, g, w_gate, gate_scale, w_up, up_scale, m_sizes)
+        # (a saved-tensor hook may hand equal tensors back in other strides)
+        w_gate, gate_scale, w_up, up_scale, m_sizes, inv_sort_idx, e, g = (_lib.dense(t) for t in ctx.saved_tensors)
+        dx = grouped_glu_backward_fp8(_lib.dense(dh), e, g, w_gate, gate_scale, w_up, up_scale, m_sizes)
         with _lib.on_device_of(dx):
             return _combine(dx, inv_sort_idx, None, ctx.n_tokens, ctx.k), *(None,) * 8
 
@@ -203,8 +204,9 @@ class _MlpGatheredFp8(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        w_gate, gate_scale, w_up, up_scale, w_down, down_scale, m_sizes, inv_sort_idx, e, g = ctx.saved_tensors
-        dh = grouped_gemm_forward_transposed_fp8(dy.contiguous(), w_down, down_scale, m_sizes)
+        w_gate, gate_scale, w_up, up_scale, w_down, down_scale, m_sizes, inv_sort_idx, e, g = (
+            _lib.dense(t) for t in ctx.saved_tensors)
+        dh = grouped_gemm_forward_transposed_fp8(_lib.dense(dy), w_down, down_scale, m_sizes)
         dx = grouped_glu_backward_fp8(dh, e, g, w_gate, gate_scale, w_up, up_scale, m_sizes)
         with _lib.on_device_of(dx):
             return _combine(dx, inv_sort_idx, None, ctx.n_tokens, ctx.k), *(None,) * 10

@@ -30,8 +30,9 @@ class _GroupedGemmFp8(torch.autograd.Function):
     def backward(ctx, dy):
         dx = None
         if ctx.needs_input_grad[0]:
-            weight, weight_scale, m_sizes = ctx.saved_tensors
-            dx = grouped_gemm_forward_transposed_fp8(dy.contiguous(), weight, weight_scale, m_sizes, ctx.dtype)
+            # (a saved-tensor hook may hand equal tensors back in other strides)
+            weight, weight_scale, m_sizes = (_lib.dense(t) for t in ctx.saved_tensors)
+            dx = grouped_gemm_forward_transposed_fp8(_lib.dense(dy), weight, weight_scale, m_sizes, ctx.dtype)
         return dx, None, None, None
 
 
