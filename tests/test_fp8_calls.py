@@ -167,3 +167,20 @@ def test_saved_tensors_that_come_back_in_other_strides(library, monkeypatch, whi
             out.backward(torch.arange(out.numel(), dtype=torch.float32).view_as(out))
         grads.append(x.grad)
     assert torch.equal(*grads)
+
+
+@WHICH
+def test_second_derivatives_and_batches_of_gradients_are_refused(library, monkeypatch, which):
+    """A gradient that kernels have written is no function of anything for autograd: a second derivative would leave it out."""
+    from qwen3_moe_fused import fused_mlp
+
+    monkeypatch.setattr(fused_mlp, "_combine", lambda dx, inv, *a: dx.view(TOKENS, K, -1).sum(1))
+    _, rows = _call(which)
+    x = torch.ones(rows, HIDDEN, requires_grad=True)
+    out = _step(which, x)
+    dx, = torch.autograd.grad(out, x, torch.ones_like(out).requires_grad_(), create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        (dx.sum() + x.square().sum()).backward()
+    out = _step(which, x)
+    with pytest.raises((RuntimeError, AssertionError, NotImplementedError)):
+        torch.autograd.grad(out, x, torch.ones(2, *out.shape), is_grads_batched=True)
