@@ -97,3 +97,67 @@ def test_lora_directories_round_trip(tmp_path):
     convert.convert_lora_to_unfused(fused, back)
     sd2 = safetensors.torch.load_file(os.path.join(back, "adapter_model.safetensors"))
     assert sd2.keys() == ref.keys() and all(torch.equal(sd2[k], ref[k]) for k in ref)
+
+
+def _quantised_state(prefix="model.", inter=136, hidden=256):
+    """Expert matrices in e4m3 with a scale per 128 x 128 block, as block-quantised checkpoints carry them."""
+    g = torch.Generator().manual_seed(2)
+    sd = {prefix + "embed_tokens.weight": torch.randn(10, hidden, generator=g),
+          f"{prefix}layers.0.self_attn.q_proj.weight": torch.randn(hidden, hidden, generator=g).to(torch.float8_e4m3fn),
+          f"{prefix}layers.0.self_attn.q_proj.weight_scale_inv": torch.rand(2, 2, generator=g)}
+    for layer in range(L):
+        for e in range(E):
+            for proj, (n, k) in (("gate_proj", (inter, hidden)), ("up_proj", (inter, hidden)), ("down_proj", (hidden, inter))):
+                key = f"{prefix}layers.{layer}.mlp.experts.{e}.{proj}.weight"
+                sd[key] = (torch.randn(n, k, generator=g) * 40).clamp(-448, 448).to(torch.float8_e4m3fn)
+                sd[key + "_scale_inv"] = torch.rand(-(-n // 128), -(-k // 128), generator=g)
+    return sd
+
+
+def _same(a, b):
+    raw = (lambda t: t.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t)
+    return a.dtype == b.dtype and torch.equal(raw(a), raw(b))
+
+
+def test_block_quantised_experts_keep_their_scales(tmp_path):
+    """Both ways through directories, and into the modules that take such weights."""
+    from types import SimpleNamespace
+
+    from qwen3_moe_fused.modular_qwen3_moe_fused import Qwen3MoeFusedSparseMoeBlock
+    from qwen3_moe_fused.quantize.layer_fp8 import MoeFusedLinearFp8
+
+    src, fused, back = (str(tmp_path / n) for n in ("src", "fused", "back"))
+    os.makedirs(src)
+    ref = _quantised_state()
+    safetensors.torch.save_file(ref, os.path.join(src, "model.safetensors"))
+    with open(os.path.join(src, "config.json"), "w") as f:
+        json.dump({"architectures": ["Qwen3MoeForCausalLM"], "num_hidden_layers": L, "num_experts": E,
+                   "quantization_config": {"quant_method": "fp8", "weight_block_size": [128, 128]}}, f)
+    convert.convert_model_to_fused(src, fused)
+    sd = convert.load_sharded_state_dict(fused)
+    assert not any(".experts." in k for k in sd)
+    assert _same(sd["model.layers.0.self_attn.q_proj.weight_scale_inv"], ref["model.layers.0.self_attn.q_proj.weight_scale_inv"])
+    block = Qwen3MoeFusedSparseMoeBlock(SimpleNamespace(num_experts=E, num_experts_per_tok=2, norm_topk_prob=True,
+                                                        hidden_size=256, moe_intermediate_size=136, hidden_act="silu"))
+    for name in convert.EXPERT_PROJECTIONS:
+        old = getattr(block, name)
+        setattr(block, name, MoeFusedLinearFp8(old.in_features, old.out_features, old.num_experts))
+    prefix = "model.layers.1.mlp."
+    state = {k[len(prefix):]: v for k, v in sd.items() if k.startswith(prefix)}
+    missing, unexpected = block.load_state_dict(state, strict=False)
+    assert missing == ["gate.weight"] and not unexpected
+    for name in convert.EXPERT_PROJECTIONS:
+        module = getattr(block, name)
+        for e in range(E):
+            key = f"{prefix}experts.{e}.{name}.weight"
+            assert _same(module.weight[e], ref[key]) and _same(module.weight_scale_inv[e], ref[key + "_scale_inv"])
+    convert.convert_model_to_unfused(fused, back)
+    sd2 = convert.load_sharded_state_dict(back)
+    assert sd2.keys() == ref.keys() and all(_same(sd2[k], ref[k]) for k in ref)
+
+
+def test_an_expert_without_its_scale_is_reported():
+    sd = _quantised_state()
+    del sd["model.layers.1.mlp.experts.2.up_proj.weight_scale_inv"]
+    with pytest.raises(KeyError):
+        convert.convert_state_dict_to_fused_(sd, param_names=convert.EXPERT_PROJECTIONS, num_hidden_layers=L, num_experts=E)

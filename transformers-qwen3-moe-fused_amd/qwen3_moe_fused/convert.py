@@ -51,23 +51,29 @@ def find_key_prefix(state_dict: TStateDict, *, is_fused: bool) -> str:
     raise RuntimeError("Key prefix not found.")
 
 
-def _fused_key(prefix: str, layer: int, param: str) -> str:
-    return f"{prefix}layers.{layer}.mlp.{param}.weight"
+# what a projection has: its matrix and, in block-quantised checkpoints (e4m3), the matrix's scales
+_ENTRIES = ("weight", "weight_scale_inv")
 
 
-def _expert_key(prefix: str, layer: int, expert: int, param: str) -> str:
-    return f"{prefix}layers.{layer}.mlp.experts.{expert}.{param}.weight"
+def _fused_key(prefix: str, layer: int, param: str, entry: str = "weight") -> str:
+    return f"{prefix}layers.{layer}.mlp.{param}.{entry}"
+
+
+def _expert_key(prefix: str, layer: int, expert: int, param: str, entry: str = "weight") -> str:
+    return f"{prefix}layers.{layer}.mlp.experts.{expert}.{param}.{entry}"
 
 
 def convert_state_dict_to_fused_(state_dict: TStateDict, *, param_names: Iterable[str], num_hidden_layers: int,
                                  num_experts: int) -> None:
     """In place: the ``num_experts`` per-expert tensors of every (layer, param) become one stacked
-    tensor with the expert index in front."""
+    tensor with the expert index in front, and so do their scales where there are any."""
     prefix = find_key_prefix(state_dict, is_fused=False)
     for layer in range(num_hidden_layers):
         for param in param_names:
-            per_expert = [state_dict.pop(_expert_key(prefix, layer, e, param)) for e in range(num_experts)]
-            state_dict[_fused_key(prefix, layer, param)] = torch.stack(per_expert)
+            for entry in _ENTRIES:
+                keys = [_expert_key(prefix, layer, e, param, entry) for e in range(num_experts)]
+                if entry == "weight" or any(key in state_dict for key in keys):
+                    state_dict[_fused_key(prefix, layer, param, entry)] = torch.stack([state_dict.pop(key) for key in keys])
 
 
 def convert_state_dict_to_unfused_(state_dict: TStateDict, *, param_names: Iterable[str], num_hidden_layers: int,
@@ -77,10 +83,13 @@ def convert_state_dict_to_unfused_(state_dict: TStateDict, *, param_names: Itera
     prefix = find_key_prefix(state_dict, is_fused=True)
     for layer in range(num_hidden_layers):
         for param in param_names:
-            fused = state_dict.pop(_fused_key(prefix, layer, param))
-            assert fused.shape[0] == num_experts, (fused.shape, num_experts)
-            for e in range(num_experts):
-                state_dict[_expert_key(prefix, layer, e, param)] = fused[e].clone()
+            for entry in _ENTRIES:
+                key = _fused_key(prefix, layer, param, entry)
+                if entry == "weight" or key in state_dict:
+                    fused = state_dict.pop(key)
+                    assert fused.shape[0] == num_experts, (fused.shape, num_experts)
+                    for e in range(num_experts):
+                        state_dict[_expert_key(prefix, layer, e, param, entry)] = fused[e].clone()
 
 
 # ---------------------------------------------------------------------------- whole models
