@@ -485,8 +485,10 @@ MFL_API int mfl_moe_block_bwd(const mfl_moe_block *b, const void *dout, const vo
  * finite value.  The left operand comes in bf16 / fp16 / fp32 and is quantised by the call: one scale per row and 128
  * elements of the reduction, the smallest power of two, 2^-117 at least, that brings the largest finite magnitude of the
  * block to 448 or below; every element is rounded once (nearest, ties to even); elements that are infinite or no number
- * become NaN and leave the scale to the others.  Sums are fp32, rounded once to out_dtype.  N and K are 2^30 at most.  The
- * reference has no counterpart.
+ * become NaN and leave the scale to the others.  Sums are fp32, rounded once to out_dtype; a sum over 128 elements is taken with
+ * the row's scale and without the weights', so that rows (and gradients) of magnitudes past 2^111 (2.6e33) may overflow where
+ * small weights' scales would bring the product back.  N and K are 2^30 at most.  Row counts (m_sizes) that are negative count as
+ * none, and those that sum to more than R are cut at row R.  The reference has no counterpart.
  *
  * workspace: mfl_fp8_workspace(...) bytes, 256-byte aligned (NULL where that is 0); it is scratch: nothing is kept in it
  * from one call to the next, and calls that can overlap in time need one each.  The forward product and the gated unit do

@@ -860,3 +860,17 @@ def test_counts_past_every_integer_are_cut_at_the_last_row(rows, width, index):
             assert call(x.data_ptr(), *source, fp8_weight(w, s), *args) == 0
             assert_within(out[:rows], *product(q, slack, dense(w, s), taken, transposed, True))
             assert (out[rows:] == 7.0).all()
+
+
+@pytest.mark.parametrize("rows,n", [(6, 128), (300, 128), (300, 64)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_up_to_the_largest_magnitude_that_is_promised(rows, n, dtype):
+    """2^111 against the largest weights, in both directions; every sum is a power of two times 7, which fp32 and bf16 hold."""
+    from qwen3_moe_fused.grouped_gemm.forward_fp8 import grouped_gemm_forward_fp8, grouped_gemm_forward_transposed_fp8
+
+    w = torch.full((2, n, 256), 448.0, device=DEV).to(FP8)
+    s = torch.full((2, 1, 2), 2.0 ** -60, device=DEV)
+    for out, red in ((grouped_gemm_forward_fp8(torch.full((rows, 256), 2.0 ** 111, device=DEV, dtype=dtype), w, s, sizes([rows - 1, 1])), 256),
+                     (grouped_gemm_forward_transposed_fp8(torch.full((rows, n), 2.0 ** 111, device=DEV, dtype=dtype), w, s,
+                                                          sizes([rows - 1, 1])), n)):
+        assert (out == red * 448.0 * 2.0 ** 51).all()

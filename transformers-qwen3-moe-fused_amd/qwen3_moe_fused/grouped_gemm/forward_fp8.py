@@ -2,8 +2,9 @@
 
 Host wrappers over ``mfl_gemm_fwd_fp8`` / ``mfl_gemm_dx_fp8``.  ``w`` (E, out, in) float8_e4m3fn with fp32 scales per 128 x 128
 block; the rows (bf16, fp16 or fp32) are quantised by the call, one power-of-two scale per row and 128 elements of the
-reduction (``quantize/fp8.py``).  The contract is otherwise that of ``grouped_gemm_forward``: output freshly allocated, rows
-past ``sum(m_sizes)`` left unwritten, ``m_sizes`` stays on the device.  The reference has no counterpart.
+reduction (``quantize/fp8.py``).  Rows of magnitudes past 2^111 may overflow before the weights' scales are applied.  The contract
+is otherwise that of ``grouped_gemm_forward``: output freshly allocated, rows past ``sum(m_sizes)`` left unwritten, ``m_sizes``
+stays on the device.  The reference has no counterpart.
 """
 from __future__ import annotations
 
