@@ -874,3 +874,114 @@ def test_rows_up_to_the_largest_magnitude_that_is_promised(rows, n, dtype):
                      (grouped_gemm_forward_transposed_fp8(torch.full((rows, n), 2.0 ** 111, device=DEV, dtype=dtype), w, s,
                                                           sizes([rows - 1, 1])), n)):
         assert (out == red * 448.0 * 2.0 ** 51).all()
+
+
+# ---- the decode kernel's own quantiser ------------------------------------------------------------------------------------
+
+def blocks_around_their_largest(dtype):
+    """Rows of 128 (a block each): a largest value at and next to the borders of the scale, and below it values of every exponent
+    that the grid tells apart, down to what becomes zero, among them the middles between two neighbours."""
+    g = torch.Generator().manual_seed(106)
+    bits = {torch.bfloat16: 7, torch.float16: 10, torch.float32: 23}[dtype]
+    down = torch.arange(0, 22).repeat_interleave(64)
+    mantissa = torch.cat([torch.arange(32) / 32.0, torch.randint(0, 2 ** bits, (32,), generator=g) / 2.0 ** bits]).repeat(22)
+    below = (1 + mantissa.double()) * torch.exp2(-down.double() - 1)
+    below = torch.cat([below, -below])
+    blocks = []
+    for top in (1.0, 1.5, 1.75, 1.75 + 2.0 ** -bits, 2.0 - 2.0 ** -bits):
+        for lo in range(0, below.numel(), 127):
+            v = below[lo:lo + 127]
+            blocks.append(torch.cat([torch.tensor([top], dtype=torch.float64), v, torch.zeros(127 - v.numel())])[
+                torch.randperm(128, generator=g)])
+    x = torch.stack(blocks)
+    # (fp16: the least values are subnormal, others next to the largest)
+    low, high = (-3, 13) if dtype == torch.float16 else (-100, 100)
+    x = x * torch.exp2(torch.randint(low, high, (x.shape[0], 1), generator=g).double())
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_decode_kernel_quantises_like_the_quantiser(dtype):
+    """Weights of ones on the diagonal: what comes out are the quantised rows, bit for bit (every sum has one term)."""
+    from qwen3_moe_fused.grouped_gemm.forward_fp8 import grouped_gemm_forward_fp8
+    from qwen3_moe_fused.quantize.fp8 import dequantize_fp8_rows, quantize_fp8_rows
+
+    k, experts = 1024, 16
+    values = [blocks_around_their_largest(dtype).reshape(-1)]
+    if dtype != torch.float32:  # every finite value of the type, next to its neighbours and in any order
+        every = torch.arange(-2 ** 15, 2 ** 15, dtype=torch.int32).to(torch.int16).view(dtype)
+        every = every[every.isfinite()]
+        # (16-bit outputs: quantised values past the type's largest would be infinite)
+        every = every[every.abs() <= torch.finfo(dtype).max / 2]
+        values += [every, every[torch.randperm(every.numel(), generator=torch.Generator().manual_seed(107))]]
+    else:
+        g = torch.Generator().manual_seed(108)
+        bits = torch.randint(-2 ** 31, 2 ** 31, (2 ** 16,), generator=g).to(torch.int32).view(torch.float32)
+        values.append(bits[bits.abs() <= 2.0 ** 120])
+    out = torch.float16 if dtype == torch.float16 else torch.bfloat16
+    w = torch.eye(k, device=DEV).to(FP8).expand(experts, k, k).contiguous()
+    s = torch.ones((experts, k // 128, k // 128), device=DEV)
+    for v in values:
+        rows = -(-v.numel() // k)
+        x = torch.zeros(rows * k, dtype=dtype)
+        x[:v.numel()] = v
+        x = x.view(rows, k).to(DEV)
+        for part in x.split(8 * experts):
+            part = part.contiguous()
+            counts = [min(8, max(0, part.shape[0] - 8 * e)) for e in range(experts)]
+            y = grouped_gemm_forward_fp8(part, w, s, sizes(counts), out)
+            expect = dequantize_fp8_rows(*quantize_fp8_rows(part), out)
+            assert expect.isfinite().all()
+            assert torch.equal(y, expect)
+
+
+# ---- whole tiles, several of them a workgroup -----------------------------------------------------------------------------
+
+# A workgroup that goes on to another tile waits for that tile's copies behind the stores of whole row blocks, which it counts
+# only where the columns are whole tiles: 128 x 128 tiles (564 and 768 for 512 workgroups) and 256 x 256 ones (1152 for 256), in
+# reductions of whole blocks.
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,experts,n,k", [(6000, 16, 2048, 512), (6000, 16, 512, 2048), (36000, 6, 2048, 256), (36000, 6, 256, 2048)])
+def test_products_in_whole_tiles_one_behind_the_other(rows, experts, n, k, dtype):
+    from qwen3_moe_fused.grouped_gemm.forward_fp8 import grouped_gemm_forward_fp8, grouped_gemm_forward_transposed_fp8
+
+    counts = counts_of(rows, experts, "spread", 109)
+    w, s = make_weight(experts, n, k, 110)
+    full = dense(w, s)
+    x, dy = make_rows(rows, k, dtype, 111, spread=False), make_rows(rows, n, dtype, 112, spread=False)
+    for out, given, transposed in ((grouped_gemm_forward_fp8(x, w, s, sizes(counts)), x, False),
+                                   (grouped_gemm_forward_transposed_fp8(dy, w, s, sizes(counts)), dy, True)):
+        q, _, slack = quantize(given.double())
+        assert_within(out, *product(q, slack, full, counts, transposed, cut_in(out)), "input gradient" if transposed else "forward")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("tokens,k,experts,hidden,inter", [(1500, 4, 16, 512, 1024), (1500, 4, 16, 256, 1024), (9000, 4, 6, 256, 2048),
+                                                           (9000, 4, 6, 2048, 256)])
+def test_gated_unit_and_mlp_in_whole_tiles_one_behind_the_other(tokens, k, experts, hidden, inter, dtype):
+    """The quantised unit's kernel with and without the two products, 128 x (128 + 128) tiles, 384 and more for 256 workgroups."""
+    from qwen3_moe_fused.grouped_gemm.fused import grouped_glu_backward_fp8, grouped_glu_forward_fp8, grouped_mlp_forward_fp8
+
+    m_sizes, sort_idx, _, counts = routed(tokens, k, experts, 113)
+    x, w = make_rows(tokens, hidden, dtype, 114, spread=False), mlp_weights(experts, hidden, inter, 115)
+    re, de, rg, dg = gated_reference(x, ((w[0], w[1]), (w[2], w[3])), sort_idx, k, counts)
+    rh, dh = gated(re, de, rg, dg)
+    h, e, g = grouped_glu_forward_fp8(x, *w[:4], m_sizes, sort_idx, k, return_products=True)
+    y, e2, g2 = grouped_mlp_forward_fp8(x, *w, m_sizes, sort_idx, k, return_products=True)
+    for what, at, out in (("gate projection", (re, de), e), ("up projection", (rg, dg), g), ("gated unit", (rh, dh), h),
+                          ("gate projection", (re, de), e2), ("up projection", (rg, dg), g2)):
+        assert_within(out, *at, what)
+    q, _, slack = quantize(rh, dh)
+    assert_within(y, *product(q, slack, dense(w[4], w[5]), counts, cut=cut_in(y)), "expert MLP")
+    assert torch.equal(y, grouped_mlp_forward_fp8(x, *w, m_sizes, sort_idx, k))
+    del re, de, rg, dg, rh, dh, q, slack
+    dh = make_rows(tokens * k, inter, dtype, 116, spread=False)
+    dx = grouped_glu_backward_fp8(dh, e, g, *w[:4], m_sizes)
+    a, ea, b, eb = gated_backward(dh.double(), e.double(), g.double())
+    total, bound = 0, 0
+    for v, err, (wq, s) in ((a, ea, w[0:2]), (b, eb, w[2:4])):
+        qv, _, slack = quantize(v, err)
+        t, bd = product(qv, slack, dense(wq, s), counts, True, cut_in(dx))
+        total, bound = total + t, bound + 2 * bd
+    assert_within(dx, total, bound, "gradient of the rows")
