@@ -492,12 +492,14 @@ MFL_API int mfl_moe_block_bwd(const mfl_moe_block *b, const void *dout, const vo
  *
  * workspace: mfl_fp8_workspace(...) bytes, 256-byte aligned (NULL where that is 0); it is scratch: nothing is kept in it
  * from one call to the next, and calls that can overlap in time need one each.  The forward product and the gated unit do
- * without at decode sizes; a call that needs one and has none answers MFL_ERR_WORKSPACE before it enqueues anything. */
+ * without at decode sizes (MFL_FP8_DECODE_ROWS rows per expert on average and fewer, 16-bit types, K a multiple of 16, operands on the
+ * 16-byte grid); a call that needs one and has none answers MFL_ERR_WORKSPACE before it enqueues anything. */
 typedef struct mfl_fp8_weight {
     const void *q;      /* e4m3 bytes */
     const float *scale; /* NaN scales make their block's products NaN */
 } mfl_fp8_weight;
 
+#define MFL_FP8_DECODE_ROWS 8
 #define MFL_FP8_FWD 0 /* mfl_gemm_fwd_fp8: (src_rows, K) quantised; R, N, K, E of the product */
 #define MFL_FP8_DX 1  /* mfl_gemm_dx_fp8 (src_rows is not used) */
 #define MFL_FP8_GLU 2 /* mfl_glu_fwd_fp8 */

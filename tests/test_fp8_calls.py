@@ -184,3 +184,14 @@ def test_second_derivatives_and_batches_of_gradients_are_refused(library, monkey
     out = _step(which, x)
     with pytest.raises((RuntimeError, AssertionError, NotImplementedError)):
         torch.autograd.grad(out, x, torch.ones(2, *out.shape), is_grads_batched=True)
+
+
+def test_the_decode_sizes_are_the_librarys():
+    import os
+    import re
+
+    from qwen3_moe_fused.grouped_gemm import forward_fp8
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    with open(os.path.join(root, "include", "moe_fused_linear.h")) as f:
+        assert re.findall(r"#define MFL_FP8_DECODE_ROWS (\d+)", f.read()) == [str(forward_fp8._DECODE_ROWS)]

@@ -47,9 +47,11 @@ Fp8Matrix matrix(const mfl_fp8_weight *w) { return {(const uint8_t *)w->q, w->sc
 // the rows of the left operand that a product reads
 int64_t source_rows(int64_t src_rows, const int32_t *row_idx, int64_t R) { return row_idx != nullptr ? src_rows : R; }
 
-// Weights whose rows no 16-byte access fits are copied to rows that one does where the call has rows for most experts: 60
-// experts, 333 x 1001, 1999 rows, fp16, forward and input gradient 56 and 71 us in the kernels for any shape, 13 and 15 on tiles
-// behind copies of 12.
+// Weights whose rows no 16-byte access fits are copied to rows that one does where the call has rows for most experts.  The copy
+// reads every expert's, the kernels for any shape only those of experts with rows: us of forward / input gradient with copies,
+// and without, 60 experts of 333 x 1001: 30 / 29 and 58 / 73 at one row for every expert, 29 / 29 and 61 / 77 at four, 31 / 31 and
+// 63 / 78 at 32; 128 of 768 x 2041: 123 / 122 and 364 / 688, 124 / 124 and 365 / 672, 133 / 144 and 380 / 686.  So they pay where
+// a third to a half of the experts have rows; with four rows per expert nearly all do, unless they are very unequal.
 int padded_row(int K) { return (K + 15) / 16 * 16; }
 size_t padded_bytes(int64_t R, int N, int K, int E) {
     return K % 16 != 0 && R >= (int64_t)4 * E ? up256((size_t)E * N * padded_row(K)) : 0;

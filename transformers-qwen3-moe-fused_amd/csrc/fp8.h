@@ -72,7 +72,12 @@ struct Fp8Product {
 // A few rows per expert (kFp8DecodeRowsPerExpert on average), forward and gated, 16-bit outputs, K % 16 == 0: the rows come as
 // they are (x, of the output's type or fp32) and are quantised on the way; p.a is not read.  MFL_ERR_UNSUPPORTED for the rest;
 // gemm_fp8_decodes: whether it takes the product with an aligned x.
-constexpr int kFp8DecodeRowsPerExpert = 8;
+// The line: 128 experts, 2048 to 768, us of a launch with the same rows for every expert, this kernel / tiles behind the
+// quantiser, product and gated unit: 42.6 / 50.8 and 75 / 81 at 8 rows per expert, 46.6 / 53.1 and 83 / 86 at 16, 73 / 55 and
+// 130 / 90 at 24, where an expert's weights are read twice (16 rows at a time).  The sizes are known on the device only, and
+// skewed ones have experts past 16 rows well before: 8 per expert under Zipf(1) 46.6 / 50.0 and 77 / 79, under Zipf(1.5)
+// 34 / 29 and 63 / 54, all on one expert 24 / 22 and 36 / 24; 2 per expert there 23 / 22 and 32 / 29, 14 / 21 and 15 / 22.
+constexpr int kFp8DecodeRowsPerExpert = MFL_FP8_DECODE_ROWS;
 bool gemm_fp8_decodes(const Fp8Product &p);
 int gemm_fp8_decode(const Fp8Product &p, const void *x, int x_dtype, hipStream_t stream);
 // Tiles in LDS, ldw % 16 == 0, two steps of the reduction at least; MFL_ERR_UNSUPPORTED for the rest.

@@ -21,7 +21,7 @@ FWD, DX, GLU, GLU_BWD, MLP, MLP_OFF_GRID = 0, 1, 2, 3, 4, 5
 _NO_WORKSPACE = -5  # MFL_ERR_WORKSPACE
 # Rows per expert up to which the forward product and the gated unit are called without scratch memory first: decode sizes do
 # without, and asking for it and allocating it is a fifth of such a call's time on the host.
-_DECODE_ROWS = 8
+_DECODE_ROWS = 8  # MFL_FP8_DECODE_ROWS
 
 
 def fp8_weight(weight: torch.Tensor, scale: torch.Tensor) -> "_lib.Fp8Weight":
