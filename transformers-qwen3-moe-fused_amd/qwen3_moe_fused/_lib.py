@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import os
 from typing import Optional
 
@@ -234,6 +235,18 @@ def plain_call() -> bool:
             and _transforms() is None and _tracing_state() is None
             and (_function_modes() == 0 or all(isinstance(torch._C._get_function_stack_at(i), DeviceContext)
                                                for i in range(_function_modes()))))
+
+
+def once_differentiable(backward):
+    """torch's decorator of that name, which refuses second derivatives, asked for only where a graph of the gradients is being made
+    (the gradient mode that it sets in every call is 3 us of a backward pass)."""
+    refusing = torch.autograd.function.once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        return refusing(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return run
 
 
 def dense(t: torch.Tensor) -> torch.Tensor:

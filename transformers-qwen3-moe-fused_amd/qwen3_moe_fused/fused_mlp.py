@@ -12,7 +12,6 @@ from __future__ import annotations
 import ctypes
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .grouped_gemm.backward_dw import grouped_gemm_backward_dw
@@ -162,7 +161,7 @@ class _GluGatheredFp8(torch.autograd.Function):
         return h
 
     @staticmethod
-    @once_differentiable
+    @_lib.once_differentiable
     def backward(ctx, dh):
         # (a saved-tensor hook may hand equal tensors back in other strides)
         w_gate, gate_scale, w_up, up_scale, m_sizes, inv_sort_idx, e, g = (_lib.dense(t) for t in ctx.saved_tensors)
@@ -205,7 +204,7 @@ class _MlpGatheredFp8(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_lib.once_differentiable
     def backward(ctx, dy):
         w_gate, gate_scale, w_up, up_scale, w_down, down_scale, m_sizes, inv_sort_idx, e, g = (
             _lib.dense(t) for t in ctx.saved_tensors)

@@ -11,7 +11,6 @@ from typing import Optional
 
 import torch
 from torch import nn
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from ..grouped_gemm.forward_fp8 import grouped_gemm_forward_fp8, grouped_gemm_forward_transposed_fp8
@@ -28,7 +27,7 @@ class _GroupedGemmFp8(torch.autograd.Function):
         return grouped_gemm_forward_fp8(x, weight, weight_scale, m_sizes)
 
     @staticmethod
-    @once_differentiable
+    @_lib.once_differentiable
     def backward(ctx, dy):
         dx = None
         if ctx.needs_input_grad[0]:
