@@ -20,8 +20,8 @@
 // 8-bit grid.  With 8-bit products the MLP of 24008 rows, 2048 and 768, is 2.3e-3 from the definition in bf16 (1.66e-3 are its
 // rounding) and 1.5e-3 in fp16 (2.07e-4), with bf16 products 1.68e-3 and 2.16e-4.  Either neighbour across a border is as near to
 // the unit's real value: against the MLP without the rounding to the grid it is 2.65e-2 either way.  So that unit has bf16 products
-// in fp16, which is chosen for its digits (24008 rows 247 -> 306 us), and the gated unit at decode sizes has them in any type, at
-// 1 % (weights' bytes); the tiles of that unit in bf16 have 8-bit ones (the MLP of 131072 rows 910 us against 1190).
+// in fp16, which is chosen for its digits (24008 rows 247 -> 301 us), and the gated unit at decode sizes has them in any type (32
+// tokens' unit 1 %, bound by the weights' bytes; one token's MLP in a graph 15.2 -> 15.9 us); the tiles of that unit in bf16 have 8-bit ones (the MLP of 131072 rows 910 us against 1190).
 #pragma once
 #include "common.h"
 #include "fp8_counts.h"
@@ -159,12 +159,25 @@ __device__ __forceinline__ uint32_t fp8_max16(uint32_t x) {
     return fp8_dpp_max<0x121>(x);
 }
 
-// An expert's row count, 0 past the last expert; 64 of them, a lane each, cut at `room` rows: the lane's first row, the row behind
-// its last one, and (in every lane) that of the last lane.
-__device__ __forceinline__ uint32_t fp8_load_count(const void *m_sizes, int ms_i64, int e, int E, int64_t R) {
-    if (e >= E) return 0u;
-    return fp8_count_of(ms_i64 ? ((const int64_t *)m_sizes)[e] : ((const int32_t *)m_sizes)[e], (uint32_t)R);
+// The row counts of experts e, e + 64, ..., 0 past the last expert, their loads all in flight together.
+template <int N>
+__device__ __forceinline__ void fp8_load_counts(const void *m_sizes, int ms_i64, int e, int E, int64_t R, uint32_t (&count)[N]) {
+    int64_t size[N];
+    if (ms_i64) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) size[i] = ((const int64_t *)m_sizes)[e + 64 * i < E ? e + 64 * i : E - 1];
+    } else {
+        int32_t narrow[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) narrow[i] = ((const int32_t *)m_sizes)[e + 64 * i < E ? e + 64 * i : E - 1];
+#pragma unroll
+        for (int i = 0; i < N; ++i) size[i] = narrow[i];
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) count[i] = e + 64 * i < E ? fp8_count_of(size[i], (uint32_t)R) : 0u;
 }
+// 64 counts, a lane each, cut at `room` rows: the lane's first row, the row behind its last one, and (in every lane) that of the
+// last lane.
 template <int CTRL, int ROW_MASK>
 __device__ __forceinline__ uint32_t fp8_dpp_sum(uint32_t x) {
     return fp8_sum(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROW_MASK, 0xf, true));
@@ -192,7 +205,9 @@ __device__ __forceinline__ bool fp8_find_tile(const void *m_sizes, int ms_i64, i
                                               int64_t &row0, int &rows) {
     int tiles_before = 0, rows_before = 0;
     for (int e0 = 0; e0 < E; e0 += 64) {
-        const Fp8Counted c = fp8_cut(fp8_load_count(m_sizes, ms_i64, e0 + lane, E, R), (uint32_t)R - (uint32_t)rows_before);
+        uint32_t count[1];
+        fp8_load_counts(m_sizes, ms_i64, e0 + lane, E, R, count);
+        const Fp8Counted c = fp8_cut(count[0], (uint32_t)R - (uint32_t)rows_before);
         const int t = fp8_tiles_of(c.end - c.begin, BM), ti = wave_inclusive_scan(t);
         const uint64_t past = __ballot(tiles_before + ti > slot);
         if (past) {

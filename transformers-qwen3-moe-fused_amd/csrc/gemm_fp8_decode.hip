@@ -9,7 +9,7 @@
 // four lanes read 64 bytes of a row together; the rows are loaded in the same order, their largest magnitude found over the
 // four lanes, and rounded to e4m3 in registers (the order within the block does not matter as long as both operands agree).
 // The waves' sums meet in LDS.  The gated unit's operands are widened to bf16 and multiplied by v_mfma_f32_16x16x32_bf16 (fp8.h
-// says why): 32 tokens 67.0 against 65.8 us, one token's MLP 22.3 either way.
+// says why): in a graph 32 tokens' unit 63.9 against 63.5 us, one token's MLP 15.9 against 15.2.
 //
 // Bound by the weights' bytes: 32 tokens of 8 of 128 experts, 2048 to 2 x 768, 66 us for 349 MB, 5.3 TB/s.  Of a single token's
 // 10 us (25 MB) a wave spends 0.8 finding its rows, 3 (weights in the caches) to 7 until weights and rows are there and quantised, 0.8
@@ -100,28 +100,32 @@ __device__ __forceinline__ uint32_t over_block(uint32_t a) {
     return y[0] > y[1] ? y[0] : y[1];
 }
 
-// The sizes of up to 256 experts at once (their loads in flight together), then 64 at a time.
+// The row counts of up to 256 experts at once (their loads in flight together), then 64 at a time.  A launch has at most 2^16
+// tiles and so fewer than 2^20 rows: 64 counts of no more than that each sum to less than 2^31, and the two sums, which need not
+// wait for each other, are never taken past the first expert whose tiles pass `slot`.
 __device__ __forceinline__ bool find_rows(const Fp8Product &p, int slot, int lane, int &expert, int64_t &row0, int &rows) {
     int tiles_before = 0, rows_before = 0;
     for (int e0 = 0; e0 < p.E; e0 += 256) {
         uint32_t count[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) count[i] = fp8_load_count(p.m_sizes, p.ms_i64, e0 + 64 * i + lane, p.E, p.R);
+        fp8_load_counts(p.m_sizes, p.ms_i64, e0 + lane, p.E, p.R, count);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const Fp8Counted c = fp8_cut(count[i], (uint32_t)p.R - (uint32_t)rows_before);
-            const int t = fp8_tiles_of(c.end - c.begin, kRows), ti = wave_inclusive_scan(t);
+            const int m = (int)count[i], t = ceil_div(m, kRows);
+            const int mi = wave_inclusive_scan(m), ti = wave_inclusive_scan(t);
             const uint64_t past = __ballot(tiles_before + ti > slot);
             if (past) {
                 const int src = __ffsll((unsigned long long)past) - 1;
+                const int m_e = __builtin_amdgcn_readlane(m, src);
                 const int tile = slot - (tiles_before + __builtin_amdgcn_readlane(ti, src) - __builtin_amdgcn_readlane(t, src));
-                const int begin = __builtin_amdgcn_readlane(c.begin, src) + tile * kRows, end = __builtin_amdgcn_readlane(c.end, src);
+                const int first = rows_before + __builtin_amdgcn_readlane(mi, src) - m_e + tile * kRows;
+                const int left = m_e - tile * kRows, room = (int)p.R - first;  // (counts that sum to more than the rows are cut there)
                 expert = e0 + 64 * i + src;
-                row0 = (int64_t)rows_before + begin;
-                rows = end - begin < kRows ? end - begin : kRows;
-                return true;
+                row0 = first;
+                rows = left < kRows ? left : kRows;
+                if (rows > room) rows = room;
+                return rows > 0;
             }
-            rows_before += c.all;
+            rows_before += wave_last(mi);
             tiles_before += wave_last(ti);
         }
     }

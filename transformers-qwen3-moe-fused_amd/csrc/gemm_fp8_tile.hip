@@ -128,7 +128,9 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void fp8_tile_kernel(Fp8Product p)
         int row_carry = 0, tile_carry = 0;
         for (int e0 = 0; e0 < p.E; e0 += 64) {
             const int e = e0 + lane;
-            const Fp8Counted c = fp8_cut(fp8_load_count(p.m_sizes, p.ms_i64, e, p.E, p.R), (uint32_t)p.R - (uint32_t)row_carry);
+            uint32_t count[1];
+            fp8_load_counts(p.m_sizes, p.ms_i64, e, p.E, p.R, count);
+            const Fp8Counted c = fp8_cut(count[0], (uint32_t)p.R - (uint32_t)row_carry);
             const int t = fp8_tiles_of(c.end - c.begin, BM), ti = wave_inclusive_scan(t);
             if (wave == 0 && e < p.E) tab_rows[e] = row_carry + c.begin, tab_tiles[e] = tile_carry + ti - t;
             row_carry += c.all, tile_carry += wave_last(ti);
