@@ -21,7 +21,8 @@
 // rounding) and 1.5e-3 in fp16 (2.07e-4), with bf16 products 1.68e-3 and 2.16e-4.  Either neighbour across a border is as near to
 // the unit's real value: against the MLP without the rounding to the grid it is 2.65e-2 either way.  So that unit has bf16 products
 // in fp16, which is chosen for its digits (24008 rows 247 -> 301 us), and the gated unit at decode sizes has them in any type (32
-// tokens' unit 1 %, bound by the weights' bytes; one token's MLP in a graph 15.2 -> 15.9 us); the tiles of that unit in bf16 have 8-bit ones (the MLP of 131072 rows 910 us against 1190).
+// tokens' unit 1 %, bound by the weights' bytes; one token's MLP in a graph 15.2 -> 15.9 us); the tiles of that unit in bf16 have
+// 8-bit ones (the MLP of 131072 rows 910 us against 1190).
 #pragma once
 #include "common.h"
 #include "fp8_counts.h"
