@@ -7,9 +7,9 @@
 //
 // A step is one block of 128 of the reduction: eight bf16 matrix instructions into fresh accumulators, and a multiply-add by
 // both scales into the running fp32 sums (bf16 products for every output: fp8.h).  The weights are the first operand, so that
-// a lane's accumulators belong to one row (its scale is the lane's) and to runs of four columns.  For widths that no 16-byte access fits the weights are
-// read byte by byte; that, and the plain load-wait-multiply order, is what bounds it: 32768 rows, 128 experts, 2048 to 768,
-// fp32, weights off the grid 1226 us, its input gradient 2763 (tiles, weights on the grid: 213 and 200).
+// a lane's accumulators belong to one row (its scale is the lane's) and to runs of four columns.  For widths that no 16-byte
+// access fits the weights are read byte by byte; that, and the plain load-wait-multiply order, is what bounds it: 32768 rows, 128
+// experts, 2048 to 768, fp32, weights off the grid 1226 us, its input gradient 2763 (tiles, weights on the grid: 217 and 197).
 #include "fp8.h"
 
 namespace mfl {
