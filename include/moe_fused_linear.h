@@ -533,6 +533,13 @@ MFL_API int mfl_mlp_fwd_fp8(const void *x, int64_t src_rows, const int32_t *row_
                     void *e_out, void *g_out, int64_t R, int I, int H, int E, int dtype, void *workspace,
                     size_t ws_bytes, void *stream);
 
+/* mfl_mlp_fwd_fp8 with x quantised already: xq (16-byte aligned) and xq_scale (4-byte) are what mfl_fp8_quant_rows or
+ * mfl_add_rms_norm_fp8 made of x, for all src_rows rows.  The decode kernels read x itself and find the same values. */
+MFL_API int mfl_mlp_fwd_fp8_rows(const void *x, const void *xq, const uint8_t *xq_scale, int64_t src_rows, const int32_t *row_idx,
+                         int idx_div, const mfl_fp8_weight *gate, const mfl_fp8_weight *up, const mfl_fp8_weight *down,
+                         const void *m_sizes, int m_sizes_dtype, void *y, void *e_out, void *g_out, int64_t R, int I, int H,
+                         int E, int dtype, void *workspace, size_t ws_bytes, void *stream);
+
 /* Quantised rows by themselves: q (R, 128 ceil(K/128)) bytes, zeros behind column K, and scale (R, 4 ceil(ceil(K/128)/4))
  * biased exponent bytes (the scale is 2^(byte - 127)), of which the first ceil(K/128) of a row are written. */
 MFL_API int mfl_fp8_quant_rows(const void *x, int dtype, int64_t R, int K, void *q, uint8_t *scale, void *stream);
@@ -540,6 +547,51 @@ MFL_API int mfl_fp8_dequant_rows(const void *q, const uint8_t *scale, int64_t R,
 /* Weights: q (E,N,K) and scales by the rule of the rows, over 128 x 128 blocks. */
 MFL_API int mfl_fp8_quant_blocks(const void *w, int dtype, int E, int N, int K, void *q, float *scale, void *stream);
 MFL_API int mfl_fp8_dequant_blocks(const void *q, const float *scale, int E, int N, int K, void *out, int out_dtype, void *stream);
+
+/* ---- norm and the whole expert layer -------------------------------------------------- */
+
+/* s = x + residual, rounded to dtype; y = s / sqrt(mean(s^2) + eps) * weight along rows of H, rounded once behind sums and products
+ * in 64 bits (to 32 bits and from there to dtype).  residual NULL: s is x, and the s given is not written.  weight (H) of dtype or
+ * MFL_F32.  y may be x, s may be x or residual (no other overlap).  H is MFL_NORM_WIDTH at most (MFL_ERR_LIMIT).  The stock layers'
+ * norm rounds once more between the two products. */
+#define MFL_NORM_WIDTH 32768
+MFL_API int mfl_add_rms_norm(const void *x, const void *residual, const void *weight, void *y, void *s, int64_t R, int H, float eps,
+                     int dtype, int weight_dtype, void *stream);
+/* Its gradients from dy and, where not NULL, ds (what arrives for s): dx (R,H), which is the residual's gradient too, and dw (H) in
+ * weight_dtype, where not NULL.  s (R,H) as the forward call left it.  workspace: mfl_add_rms_norm_bwd_workspace(R, H) bytes where dw
+ * is asked for, 16-byte aligned.  Same bits from run to run.  dx may be dy, ds or s. */
+MFL_API size_t mfl_add_rms_norm_bwd_workspace(int64_t R, int H);
+MFL_API int mfl_add_rms_norm_bwd(const void *dy, const void *ds, const void *s, const void *weight, void *dx, void *dw, int64_t R,
+                         int H, float eps, int dtype, int weight_dtype, void *workspace, size_t ws_bytes, void *stream);
+/* mfl_add_rms_norm with y as quantised rows: q and scale are what mfl_fp8_quant_rows makes of y as rounded to dtype, laid out the
+ * same; y itself where not NULL. */
+MFL_API int mfl_add_rms_norm_fp8(const void *x, const void *residual, const void *weight, void *q, uint8_t *scale, void *y, void *s,
+                         int64_t R, int H, float eps, int dtype, int weight_dtype, void *stream);
+
+/* The whole sparse expert layer for up to MFL_LAYER_TOKENS tokens: logits = rows router^T (sums in 64 bits, rounded
+ * once to dtype), softmax, the k largest (of the rounded logits; equal ones: lower expert id), their weights brought to a sum of one
+ * where renorm; out = sum over the chosen experts of weight * down(silu(gate row) * (up row)), in fp32 without a rounding in between
+ * (bf16: the gated unit's result as the sum of two bf16 values), rounded once.
+ * norm_weight NULL: rows = x, residual has to be NULL.  Else rows = y of mfl_add_rms_norm(x, residual, norm_weight) and its s is added
+ * to out.
+ * s_gate, s_up, s_down given: expert weights are e4m3 bytes with these block scales, and the rows and the gated unit's result are
+ * quantised as mfl_mlp_fwd_fp8 quantises them; else they are of dtype.  x, residual, norm_weight, router, out, logits of dtype.
+ * A token whose logits hold a NaN, or an infinity as the largest, chooses no expert; its row of out is NaN, the others are what they
+ * are without it.  E up to 1024, k up to 64, H and I up to 2^24 (MFL_ERR_LIMIT).  out and logits overlap nothing else.
+ * workspace: mfl_moe_layer_workspace bytes (0: shape not taken), 256-byte aligned, scratch.  Replaces
+ * qwen3_moe_fused/modular_qwen3_moe_fused.py:72-118 at decode sizes. */
+#define MFL_LAYER_TOKENS 16
+typedef struct mfl_moe_layer {
+    const void *x, *residual, *norm_weight; /* (T,H), (T,H) or NULL, (H) or NULL */
+    const void *router;                     /* (E,H) */
+    const void *w_gate, *w_up, *w_down;     /* (E,I,H), (E,I,H), (E,H,I) */
+    const float *s_gate, *s_up, *s_down;    /* all or none */
+    int64_t T;
+    int E, k, H, I, renorm, dtype;
+    float eps;
+} mfl_moe_layer;
+MFL_API size_t mfl_moe_layer_workspace(const mfl_moe_layer *p);
+MFL_API int mfl_moe_layer_fwd(const mfl_moe_layer *p, void *out, void *logits, void *workspace, size_t ws_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,323 @@
+"""The residual's addition with the norm behind it, forward, backward and to 8-bit rows, against 64 bits."""
+import pytest
+import torch
+
+import layer_reference as ref
+from qwen3_moe_fused import _lib
+from qwen3_moe_fused.kernels.norm import add_rms_norm, add_rms_norm_backward, add_rms_norm_fp8
+from qwen3_moe_fused.quantize.fp8 import dequantize_fp8_rows, quantize_fp8_rows
+
+pytestmark = pytest.mark.gpu
+DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+EPS = 1e-6
+# widths around every change of a row's threads, and such as no 16-byte access fits
+WIDTHS = (1, 7, 8, 129, 512, 513, 1001, 1024, 1032, 2048, 2049, 4096, 4100, 8192, 8200, 16384, 20000, 32768)
+
+
+def _inputs(rows, width, dtype, seed=0, residual=True, weight_dtype=None, std=1.0):
+    g = torch.Generator().manual_seed(seed)
+    x = (torch.randn((rows, width), generator=g) * std).to(dtype)
+    r = (torch.randn((rows, width), generator=g) * 0.5 * std).to(dtype) if residual else None
+    w = (1.0 + 0.1 * torch.randn(width, generator=g)).to(weight_dtype or dtype)
+    return x, r, w, g
+
+
+def _cuda(*ts):
+    return [None if t is None else t.cuda() for t in ts]
+
+
+def _check(y, s, x, r, w, dtype, eps=EPS):
+    want_s = ref.stream(x, r)
+    assert torch.equal(s.cpu().double(), want_s)
+    want, _, _ = ref.norm(want_s, w, eps)
+    assert ((y.cpu().double() - want).abs() <= ref.half_step(want, dtype)).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("width", WIDTHS)
+@pytest.mark.parametrize("rows", (1, 5))
+def test_forward(dtype, width, rows):
+    for residual in (True, False):
+        x, r, w, _ = _inputs(rows, width, dtype, width, residual)
+        y, s = add_rms_norm(*_cuda(x, r, w), EPS)
+        _check(y, s, x, r, w, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_leading_dimensions_other_weights_and_no_rows(dtype):
+    x, r, w, _ = _inputs(12, 96, dtype, weight_dtype=torch.float32)
+    y, s = add_rms_norm(x.view(3, 4, 96).cuda(), r.view(3, 4, 96).cuda(), w.cuda(), 1e-5)
+    assert y.shape == s.shape == (3, 4, 96)
+    _check(y.view(12, 96), s.view(12, 96), x, r, w, dtype, 1e-5)
+    empty = torch.empty((0, 96), device="cuda", dtype=dtype)
+    y, s = add_rms_norm(empty, empty.clone(), w.cuda())
+    assert y.shape == s.shape == (0, 96)
+    values, scales, s = add_rms_norm_fp8(empty, None, w.cuda())
+    assert values.shape == (0, 96) and scales.shape == (0, 1)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("off", (1, 3))
+def test_rows_off_the_16_byte_grid(dtype, off):
+    x, r, w, _ = _inputs(6, 264, dtype)
+
+    def moved(t):
+        room = torch.empty(t.numel() + off, device="cuda", dtype=t.dtype)
+        room[off:] = t.flatten().cuda()
+        return room[off:].view(t.shape)
+
+    y, s = add_rms_norm(moved(x), moved(r), moved(w), EPS)
+    _check(y, s, x, r, w, dtype)
+    dy = torch.randn(x.shape, generator=torch.Generator().manual_seed(1)).to(dtype)
+    a = add_rms_norm_backward(moved(dy), moved(dy), moved(s.cpu()), moved(w), EPS)
+    b = add_rms_norm_backward(dy.cuda(), dy.cuda(), s, w.cuda(), EPS)
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float32))
+@pytest.mark.parametrize("std", (1e30, 1e-30))
+def test_magnitudes_whose_squares_32_bits_do_not_hold(dtype, std):
+    x, r, w, g = _inputs(4, 300, dtype, std=std)
+    eps = 0.0 if std < 1 else EPS
+    y, s = add_rms_norm(*_cuda(x, r, w), eps)
+    _check(y, s, x, r, w, dtype, eps)
+    if std > 1:  # (rows of 1e-30 without eps have gradients of 1e30)
+        dy = torch.randn(x.shape, generator=g).to(dtype)
+        dx, dw = add_rms_norm_backward(dy.cuda(), None, s, w.cuda(), eps)
+        want = ref.norm_gradients(dy, None, s.cpu().double(), w, eps)
+        bounds = ref.norm_gradient_bounds(dy, None, s.cpu().double(), w, eps, dtype, dtype)
+        for a, b, c in zip((dx, dw), want, bounds):
+            assert ((a.cpu().double() - b).abs() <= c).all()
+
+
+def test_a_row_without_a_finite_length_leaves_the_others_alone():
+    x, r, w, _ = _inputs(9, 700, torch.bfloat16)
+    x[2, 5], x[4, 699], x[6] = float("nan"), float("inf"), 0.0
+    r[6] = 0.0
+    y, s = add_rms_norm(*_cuda(x, r, w), EPS)
+    keep = [0, 1, 3, 5, 6, 7, 8]
+    _check(y[keep], s[keep], x[keep], r[keep], w, torch.bfloat16)
+    assert y[2].isnan().all() and (y[6] == 0).all()
+    # an infinite element: 1 / length is zero, and the element itself no number
+    assert y[4, 699].isnan() and (y[4, :699] == 0).all()
+
+
+# ---- 8-bit rows
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("width", (1, 17, 128, 130, 1001, 2048, 2050, 4096, 8200, 20000))
+def test_quantised_rows_are_those_of_the_normed_rows(dtype, width):
+    x, r, w, _ = _inputs(5, width, dtype, width)
+    if width > 1000:
+        x[1, 3], x[2, 500], x[3, 128:256] = float("nan"), float("inf"), 0.0
+        r[3, 128:256] = 0.0
+    x, r, w = _cuda(x, r, w)
+    values, scales, s, y = add_rms_norm_fp8(x, r, w, EPS, return_normed=True)
+    want_y, want_s = add_rms_norm(x, r, w, EPS)
+    assert torch.equal(y.view(torch.uint8), want_y.view(torch.uint8)) and torch.equal(s.view(torch.uint8), want_s.view(torch.uint8))
+    want, want_scales = quantize_fp8_rows(y)
+    assert values.stride() == want.stride() and scales.stride() == want_scales.stride()
+    assert torch.equal(values.view(torch.uint8), want.view(torch.uint8))
+    assert torch.equal(scales.view(torch.uint8), want_scales.view(torch.uint8))
+    padded = torch.as_strided(values.view(torch.uint8), (5, values.stride(0)), (values.stride(0), 1))[:, width:]
+    assert (padded == 0).all()  # zeros behind the last column
+    other, other_scales, s = add_rms_norm_fp8(x, None, w, EPS)
+    assert s is x and torch.equal(dequantize_fp8_rows(other, other_scales, torch.float32).nan_to_num(),
+                                  dequantize_fp8_rows(*quantize_fp8_rows(add_rms_norm(x, None, w, EPS)[0]), torch.float32).nan_to_num())
+
+
+# ---- backward
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("width", WIDTHS)
+def test_backward(dtype, width):
+    rows = 7 if width > 2100 else 37
+    x, r, w, g = _inputs(rows, width, dtype, width)
+    dy, ds = (torch.randn(x.shape, generator=g).to(dtype) for _ in range(2))
+    leaves = [t.cuda().requires_grad_() for t in (x, r, w)]
+    y, s = add_rms_norm(*leaves, EPS)
+    got = torch.autograd.grad((y, s), leaves, (dy.cuda(), ds.cuda()))
+    s64 = ref.stream(x, r)
+    dx, dw = ref.norm_gradients(dy, ds, s64, w, EPS)
+    bound, bound_w = ref.norm_gradient_bounds(dy, ds, s64, w, EPS, dtype, dtype)
+    assert torch.equal(got[0], got[1])
+    assert ((got[0].cpu().double() - dx).abs() <= bound).all()
+    assert ((got[2].cpu().double() - dw).abs() <= bound_w).all()
+
+
+@pytest.mark.parametrize("rows", (1, 2, 3000, 20011))
+def test_backward_over_many_rows_is_the_same_every_time(rows):
+    x, _, w, g = _inputs(rows, 136, torch.bfloat16, residual=False, weight_dtype=torch.float32)
+    dy = torch.randn(x.shape, generator=g).to(torch.bfloat16)
+    leaves = [x.cuda().requires_grad_(), w.cuda().requires_grad_()]
+    y, s = add_rms_norm(leaves[0], None, leaves[1], EPS)
+    assert s is leaves[0]
+    got = torch.autograd.grad(y, leaves, dy.cuda(), retain_graph=True)
+    dx, dw = ref.norm_gradients(dy, None, x.double(), w, EPS)
+    bound, bound_w = ref.norm_gradient_bounds(dy, None, x.double(), w, EPS, torch.bfloat16, torch.float32)
+    assert ((got[0].cpu().double() - dx).abs() <= bound).all() and ((got[1].cpu().double() - dw).abs() <= bound_w).all()
+    again = torch.autograd.grad(y, leaves, dy.cuda())
+    assert all(torch.equal(a, b) for a, b in zip(got, again))
+
+
+def test_gradient_against_differences():
+    """Central differences of the definition in 64 bits: off by about h^2 times the third derivative, a few 1e-9 here."""
+    x, r, w, g = _inputs(2, 24, torch.float32)
+    dy, ds = torch.randn(x.shape, generator=g), torch.randn(x.shape, generator=g)
+    leaves = [t.cuda().requires_grad_() for t in (x, r, w)]
+    got = torch.autograd.grad(add_rms_norm(*leaves, EPS), leaves, (dy.cuda(), ds.cuda()))
+
+    def loss(x, r, w):
+        s = x + r
+        return ((ref.norm(s, w, EPS)[0] * dy.double()).sum() + (s * ds.double()).sum()).item()
+
+    h = 1e-5
+    for which, grad in enumerate(got):
+        flat = grad.cpu().double().flatten()
+        for i in range(0, flat.numel(), 5):
+            sides = []
+            for sign in (1, -1):
+                args = [t.double().clone() for t in (x, r, w)]
+                args[which].view(-1)[i] += sign * h
+                sides.append(loss(*args))
+            slope = (sides[0] - sides[1]) / (2 * h)
+            assert abs(flat[i].item() - slope) <= 2e-5 * (1 + abs(slope))
+
+
+@pytest.mark.parametrize("needs", [(True, False, False), (False, True, False), (False, False, True), (True, False, True)])
+def test_gradients_that_are_asked_for(needs):
+    x, r, w, g = _inputs(11, 72, torch.float32)
+    dy, ds = (torch.randn(x.shape, generator=g).cuda() for _ in range(2))
+    everything = [t.cuda().requires_grad_() for t in (x, r, w)]
+    want = torch.autograd.grad(add_rms_norm(*everything, EPS), everything, (dy, ds))
+    some = [t.cuda().requires_grad_(n) for t, n in zip((x, r, w), needs)]
+    got = torch.autograd.grad(add_rms_norm(*some, EPS), [t for t, n in zip(some, needs) if n], (dy, ds))
+    assert all(torch.equal(a, b) for a, b in zip(got, [t for t, n in zip(want, needs) if n]))
+
+
+def test_one_result_used_alone_and_shared_inputs():
+    x, r, w, g = _inputs(5, 40, torch.float32)
+    dy = torch.randn(x.shape, generator=g)
+    leaves = [t.cuda().requires_grad_() for t in (x, r, w)]
+    _, s = add_rms_norm(*leaves, EPS)
+    got = torch.autograd.grad(s, leaves, dy.cuda(), allow_unused=True)  # the addition's gradient
+    assert torch.equal(got[0].cpu(), dy) and torch.equal(got[1].cpu(), dy) and (got[2] is None or (got[2] == 0).all())
+    y, _ = add_rms_norm(*leaves, EPS)
+    got = torch.autograd.grad(y, leaves, dy.cuda())
+    dx, _ = ref.norm_gradients(dy, None, ref.stream(x, r), w, EPS)
+    bound, _ = ref.norm_gradient_bounds(dy, None, ref.stream(x, r), w, EPS, torch.float32, torch.float32)
+    assert ((got[0].cpu().double() - dx).abs() <= bound).all()
+    # the same tensor twice: both of its gradients
+    one = x.cuda().requires_grad_()
+    y, _ = add_rms_norm(one, one, w.cuda(), EPS)
+    (grad,) = torch.autograd.grad(y, one, dy.cuda())
+    dx, _ = ref.norm_gradients(dy, None, ref.stream(x, x), w, EPS)
+    bound, _ = ref.norm_gradient_bounds(dy, None, ref.stream(x, x), w, EPS, torch.float32, torch.float32)
+    assert ((grad.cpu().double() - 2 * dx).abs() <= 2 * bound + 2.0 ** -23 * dx.abs()).all()
+
+
+def test_backward_through_the_quantised_form():
+    x, r, w, g = _inputs(6, 200, torch.bfloat16)
+    dy, ds = (torch.randn(x.shape, generator=g).to(torch.bfloat16).cuda() for _ in range(2))
+    leaves = [t.cuda().requires_grad_() for t in (x, r, w)]
+    want = torch.autograd.grad(add_rms_norm(*leaves, EPS), leaves, (dy, ds))
+    values, scales, s, y = add_rms_norm_fp8(*leaves, EPS, return_normed=True)
+    assert not values.requires_grad and not scales.requires_grad
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad((y, s), leaves, (dy, ds)), want))
+    values, scales, s = add_rms_norm_fp8(*leaves, EPS)
+    got = torch.autograd.grad(s, leaves[:2], ds)
+    assert torch.equal(got[0], ds) and torch.equal(got[1], ds)
+
+
+def test_second_derivatives_and_tangents_are_refused():
+    x, r, w, _ = _inputs(3, 16, torch.float32)
+    leaves = [t.cuda().requires_grad_() for t in (x, r, w)]
+    y, _ = add_rms_norm(*leaves, EPS)
+    (grad,) = torch.autograd.grad(y.sum(), leaves[:1], create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(grad.sum(), leaves[:1])
+    from torch.autograd import forward_ad
+
+    with forward_ad.dual_level(), pytest.raises(RuntimeError):
+        add_rms_norm(forward_ad.make_dual(x.cuda(), r.cuda()), None, w.cuda(), EPS)
+
+
+# ---- streams, graphs, in place
+
+def test_captured_and_replayed_with_eager_passes_between():
+    x, r, w, g = _inputs(33, 2048, torch.bfloat16)
+    dy, ds = (torch.randn(x.shape, generator=g).to(torch.bfloat16).cuda() for _ in range(2))
+    leaves = [t.cuda().requires_grad_() for t in (x, r, w)]
+
+    def step():
+        out = add_rms_norm(*leaves, EPS)
+        return (*out, *torch.autograd.grad(out, leaves, (dy, ds)))
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            step()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for seed in range(3):
+        with torch.no_grad():
+            leaves[0].copy_(torch.randn(x.shape, generator=torch.Generator().manual_seed(seed)).to(torch.bfloat16))
+        graph.replay()
+        got = [t.detach().clone() for t in captured]
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_on_another_stream_than_the_default():
+    x, r, w, _ = _inputs(64, 2048, torch.bfloat16)
+    x, r, w = _cuda(x, r, w)
+    want = add_rms_norm(x, r, w, EPS)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        a = add_rms_norm(x, r, w, EPS)
+    b = add_rms_norm(x, r, w, EPS)
+    torch.cuda.synchronize()
+    for got in (a, b):
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_results_in_the_place_of_operands():
+    x, r, w, g = _inputs(19, 1001, torch.float16)
+    xc, rc, wc = _cuda(x, r, w)
+    y, s = add_rms_norm(xc, rc, wc, EPS)
+    dy, ds = (torch.randn(x.shape, generator=g).to(torch.float16).cuda() for _ in range(2))
+    dx, _ = add_rms_norm_backward(dy, ds, s, wc, EPS)
+    a, b, lib = xc.clone(), rc.clone(), _lib.lib()
+    _lib.check(lib.mfl_add_rms_norm(a.data_ptr(), b.data_ptr(), wc.data_ptr(), a.data_ptr(), b.data_ptr(), 19, 1001, EPS, _lib.F16,
+                                    _lib.F16, _lib.stream()), "norm")
+    assert torch.equal(a, y) and torch.equal(b, s)
+    for place in range(3):
+        ops = [dy.clone(), ds.clone(), s.clone()]
+        _lib.check(lib.mfl_add_rms_norm_bwd(*(t.data_ptr() for t in ops), wc.data_ptr(), ops[place].data_ptr(), None, 19, 1001, EPS,
+                                            _lib.F16, _lib.F16, None, 0, _lib.stream()), "norm backward")
+        assert torch.equal(ops[place], dx)
+
+
+def test_more_elements_than_32_bits_count():
+    rows, width = (1 << 31) // 2048 + 3, 2048
+    x = torch.zeros((rows, width), device="cuda", dtype=torch.bfloat16)
+    tail, _, w, _ = _inputs(5, width, torch.bfloat16, residual=False)
+    x[-5:] = tail.cuda()
+    wc = w.cuda()
+    y, _ = add_rms_norm(x, None, wc, EPS)
+    _check(y[-5:], x[-5:], tail, None, w, torch.bfloat16)
+    del y
+    values, scales, _ = add_rms_norm_fp8(x, None, wc, EPS)
+    want, want_scales = quantize_fp8_rows(add_rms_norm(tail.cuda(), None, wc, EPS)[0])
+    assert torch.equal(values[-5:].view(torch.uint8), want.view(torch.uint8))
+    assert torch.equal(scales[-5:].view(torch.uint8), want_scales.view(torch.uint8))
+    dy = torch.zeros_like(x)
+    dy[-5:] = tail.flip(0).cuda()
+    dx, _ = add_rms_norm_backward(dy, None, x, wc, EPS, need_dw=False)
+    want, _ = ref.norm_gradients(tail.flip(0), None, tail.double(), w, EPS)
+    bound, _ = ref.norm_gradient_bounds(tail.flip(0), None, tail.double(), w, EPS, torch.bfloat16, torch.bfloat16)
+    assert ((dx[-5:].cpu().double() - want).abs() <= bound).all()

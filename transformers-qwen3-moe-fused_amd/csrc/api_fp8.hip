@@ -98,6 +98,52 @@ size_t mlp_bytes(int64_t src_rows, int64_t R, int N, int K, int E, bool on_grid)
            (front > back ? front : back);
 }
 
+int mlp_fwd(const void *x, const Fp8Rows *given, int64_t src_rows, const int32_t *row_idx, int idx_div, const mfl_fp8_weight *gate,
+                    const mfl_fp8_weight *up, const mfl_fp8_weight *down, const void *m_sizes, int m_sizes_dtype, void *y,
+                    void *e_out, void *g_out, int64_t R, int I, int H, int E, int dtype, void *workspace, size_t ws_bytes,
+                    void *stream) {
+    int rc = check_call(m_sizes, m_sizes_dtype, R, I, H, E, dtype, dtype);
+    if (!rc) rc = check_source(src_rows, row_idx, idx_div, R);
+    if (rc) return rc;
+    if (R == 0) return MFL_OK;
+    if (!x || !y) return MFL_ERR_NULL;
+    rc = check_weight(gate);
+    if (!rc) rc = check_weight(up);
+    if (!rc) rc = check_weight(down);
+    if (rc) return rc;
+    const size_t size = dtype_size(dtype);
+    if (!aligned(x, size) || !aligned(y, size) || !aligned(e_out, size) || !aligned(g_out, size)) return MFL_ERR_ALIGN;
+    if ((e_out == nullptr) != (g_out == nullptr)) return MFL_ERR_NULL;
+    const bool on_grid = aligned(gate->q, 16) && aligned(up->q, 16) && aligned(e_out, 16) && aligned(g_out, 16);
+    rc = check_workspace(on_grid ? MFL_FP8_MLP : MFL_FP8_MLP_OFF_GRID, src_rows, R, I, H, E, workspace, ws_bytes);
+    if (rc) return rc;
+    const size_t values = mlp_values_bytes(mlp_needs_values(src_rows, R, I, H, E, on_grid), R, I);
+    const int64_t used = source_rows(src_rows, row_idx, R);
+    const RowsRoom room((uint8_t *)workspace, used, H), hidden((uint8_t *)workspace + rows_bytes(src_rows, H), R, I);
+    void *const h = (uint8_t *)workspace + rows_bytes(src_rows, H) + rows_bytes(R, I);
+    uint8_t *const padding = (uint8_t *)h + values;
+    Fp8Product p = {};
+    p.glu = true, p.terms = 1, p.a[0] = room.rows(), p.w[0] = matrix(gate), p.w[1] = matrix(up);
+    p.row_idx = row_idx, p.idx_div = idx_div, p.src_rows = used;
+    p.m_sizes = m_sizes, p.ms_i64 = m_sizes_dtype == MFL_I64;
+    p.e_out = e_out, p.g_out = g_out, p.out_dtype = dtype, p.R = R, p.N = I, p.K = p.ldw = H, p.E = E;
+    Fp8Product d = p;  // the down projection
+    d.glu = false, d.a[0] = hidden.rows(), d.w[0] = matrix(down), d.row_idx = nullptr, d.src_rows = R;
+    d.out = y, d.e_out = d.g_out = nullptr, d.N = H, d.K = d.ldw = I;
+    if (gemm_fp8_decodes(p) && gemm_fp8_decodes(d) && aligned(x, 16)) {
+        // a few rows: both kernels quantise their rows themselves, from the fp32 values between them
+        p.h32 = (float *)h;
+        rc = gemm_fp8_decode(p, x, dtype, (hipStream_t)stream);
+        return rc ? rc : gemm_fp8_decode(d, h, MFL_F32, (hipStream_t)stream);
+    }
+    if (given != nullptr) p.a[0] = *given;
+    else rc = fp8_quant_rows(x, dtype, used, H, room.q, room.scale, (hipStream_t)stream);
+    if (rc) return rc;
+    p.hq = hidden.q, p.hq_scale = hidden.scale, p.h32 = values != 0 ? (float *)h : nullptr;
+    rc = run_product(p, padding, (hipStream_t)stream);
+    return rc ? rc : run_product(d, padding, (hipStream_t)stream);
+}
+
 }  // namespace
 
 extern "C" {
@@ -227,45 +273,19 @@ int mfl_mlp_fwd_fp8(const void *x, int64_t src_rows, const int32_t *row_idx, int
                     const mfl_fp8_weight *up, const mfl_fp8_weight *down, const void *m_sizes, int m_sizes_dtype, void *y,
                     void *e_out, void *g_out, int64_t R, int I, int H, int E, int dtype, void *workspace, size_t ws_bytes,
                     void *stream) {
-    int rc = check_call(m_sizes, m_sizes_dtype, R, I, H, E, dtype, dtype);
-    if (!rc) rc = check_source(src_rows, row_idx, idx_div, R);
-    if (rc) return rc;
-    if (R == 0) return MFL_OK;
-    if (!x || !y) return MFL_ERR_NULL;
-    rc = check_weight(gate);
-    if (!rc) rc = check_weight(up);
-    if (!rc) rc = check_weight(down);
-    if (rc) return rc;
-    const size_t size = dtype_size(dtype);
-    if (!aligned(x, size) || !aligned(y, size) || !aligned(e_out, size) || !aligned(g_out, size)) return MFL_ERR_ALIGN;
-    if ((e_out == nullptr) != (g_out == nullptr)) return MFL_ERR_NULL;
-    const bool on_grid = aligned(gate->q, 16) && aligned(up->q, 16) && aligned(e_out, 16) && aligned(g_out, 16);
-    rc = check_workspace(on_grid ? MFL_FP8_MLP : MFL_FP8_MLP_OFF_GRID, src_rows, R, I, H, E, workspace, ws_bytes);
-    if (rc) return rc;
-    const size_t values = mlp_values_bytes(mlp_needs_values(src_rows, R, I, H, E, on_grid), R, I);
-    const int64_t used = source_rows(src_rows, row_idx, R);
-    const RowsRoom room((uint8_t *)workspace, used, H), hidden((uint8_t *)workspace + rows_bytes(src_rows, H), R, I);
-    void *const h = (uint8_t *)workspace + rows_bytes(src_rows, H) + rows_bytes(R, I);
-    uint8_t *const padding = (uint8_t *)h + values;
-    Fp8Product p = {};
-    p.glu = true, p.terms = 1, p.a[0] = room.rows(), p.w[0] = matrix(gate), p.w[1] = matrix(up);
-    p.row_idx = row_idx, p.idx_div = idx_div, p.src_rows = used;
-    p.m_sizes = m_sizes, p.ms_i64 = m_sizes_dtype == MFL_I64;
-    p.e_out = e_out, p.g_out = g_out, p.out_dtype = dtype, p.R = R, p.N = I, p.K = p.ldw = H, p.E = E;
-    Fp8Product d = p;  // the down projection
-    d.glu = false, d.a[0] = hidden.rows(), d.w[0] = matrix(down), d.row_idx = nullptr, d.src_rows = R;
-    d.out = y, d.e_out = d.g_out = nullptr, d.N = H, d.K = d.ldw = I;
-    if (gemm_fp8_decodes(p) && gemm_fp8_decodes(d) && aligned(x, 16)) {
-        // a few rows: both kernels quantise their rows themselves, from the fp32 values between them
-        p.h32 = (float *)h;
-        rc = gemm_fp8_decode(p, x, dtype, (hipStream_t)stream);
-        return rc ? rc : gemm_fp8_decode(d, h, MFL_F32, (hipStream_t)stream);
-    }
-    rc = fp8_quant_rows(x, dtype, used, H, room.q, room.scale, (hipStream_t)stream);
-    if (rc) return rc;
-    p.hq = hidden.q, p.hq_scale = hidden.scale, p.h32 = values != 0 ? (float *)h : nullptr;
-    rc = run_product(p, padding, (hipStream_t)stream);
-    return rc ? rc : run_product(d, padding, (hipStream_t)stream);
+    return mlp_fwd(x, nullptr, src_rows, row_idx, idx_div, gate, up, down, m_sizes, m_sizes_dtype, y, e_out, g_out, R, I, H, E, dtype,
+                   workspace, ws_bytes, stream);
+}
+
+int mfl_mlp_fwd_fp8_rows(const void *x, const void *xq, const uint8_t *xq_scale, int64_t src_rows, const int32_t *row_idx, int idx_div,
+                         const mfl_fp8_weight *gate, const mfl_fp8_weight *up, const mfl_fp8_weight *down, const void *m_sizes,
+                         int m_sizes_dtype, void *y, void *e_out, void *g_out, int64_t R, int I, int H, int E, int dtype,
+                         void *workspace, size_t ws_bytes, void *stream) {
+    if (R > 0 && (!xq || !xq_scale)) return MFL_ERR_NULL;
+    if (!aligned(xq, 16) || !aligned(xq_scale, 4)) return MFL_ERR_ALIGN;
+    const Fp8Rows given = {(const uint8_t *)xq, xq_scale};
+    return mlp_fwd(x, &given, src_rows, row_idx, idx_div, gate, up, down, m_sizes, m_sizes_dtype, y, e_out, g_out, R, I, H, E, dtype,
+                   workspace, ws_bytes, stream);
 }
 
 int mfl_fp8_quant_rows(const void *x, int dtype, int64_t R, int K, void *q, uint8_t *scale, void *stream) {

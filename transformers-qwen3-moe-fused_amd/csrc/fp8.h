@@ -160,6 +160,51 @@ __device__ __forceinline__ uint32_t fp8_max16(uint32_t x) {
     return fp8_dpp_max<0x121>(x);
 }
 
+// Eight values of a block, which 16 lanes hold (all of them here together), to q, the block's scale byte to scale by the lane that
+// is its first.
+__device__ __forceinline__ void fp8_store_block(float (&v)[8], uint8_t *q, uint8_t *scale, bool first) {
+    uint32_t a = 0u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a = fp8_wider(a, v[i]);
+    a = fp8_max16(a);
+    if (fp8_unusual(a)) {
+        a = 0u;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a = fp8_wider(a, fp8_finite_abs(v[i])), v[i] = fp8_finite(v[i]);
+        a = fp8_max16(a);
+    }
+    const int byte = fp8_scale_byte(a);
+    const float inverse = fp8_inverse_of(byte);
+    *(uint2_t *)q = uint2_t{fp8_pack4(v[0], v[1], v[2], v[3], inverse), fp8_pack4(v[4], v[5], v[6], v[7], inverse)};
+    if (first) *scale = (uint8_t)byte;
+}
+
+// The same, but what the rounded values stand for, in bf16 (exact below 2^128).
+__device__ __forceinline__ void fp8_store_wide(float (&v)[8], bf16_t *to) {
+    uint32_t a = 0u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a = fp8_wider(a, v[i]);
+    a = fp8_max16(a);
+    if (fp8_unusual(a)) {
+        a = 0u;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a = fp8_wider(a, fp8_finite_abs(v[i])), v[i] = fp8_finite(v[i]);
+        a = fp8_max16(a);
+    }
+    const int byte = fp8_scale_byte(a);
+    const float inverse = fp8_inverse_of(byte);
+    const intx2 q = {(int)fp8_pack4(v[0], v[1], v[2], v[3], inverse), (int)fp8_pack4(v[4], v[5], v[6], v[7], inverse)};
+    *(bf16x8 *)to = fp8_widen(q, fp8_scale_of(byte));
+}
+
+// The largest of the four lanes lane % 16, + 16, + 32, + 48, in all of them.
+__device__ __forceinline__ uint32_t fp8_over_quarters(uint32_t a) {
+    const auto x = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+    a = x[0] > x[1] ? x[0] : x[1];
+    const auto y = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+    return y[0] > y[1] ? y[0] : y[1];
+}
+
 // The row counts of experts e, e + 64, ..., 0 past the last expert, their loads all in flight together.
 template <int N>
 __device__ __forceinline__ void fp8_load_counts(const void *m_sizes, int ms_i64, int e, int E, int64_t R, uint32_t (&count)[N]) {

@@ -28,24 +28,6 @@ __device__ __forceinline__ void load8(const T *row, int k, int K, float (&v)[8])
     }
 }
 
-// The lane's 8 values of a block (16 lanes) to q, the block's scale byte to scale.
-__device__ __forceinline__ void store_block(float (&v)[8], uint8_t *q, uint8_t *scale, bool first) {
-    uint32_t a = 0u;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) a = fp8_wider(a, v[i]);
-    a = fp8_max16(a);
-    if (fp8_unusual(a)) {
-        a = 0u;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) a = fp8_wider(a, fp8_finite_abs(v[i])), v[i] = fp8_finite(v[i]);
-        a = fp8_max16(a);
-    }
-    const int byte = fp8_scale_byte(a);
-    const float inverse = fp8_inverse_of(byte);
-    *(uint2_t *)q = uint2_t{fp8_pack4(v[0], v[1], v[2], v[3], inverse), fp8_pack4(v[4], v[5], v[6], v[7], inverse)};
-    if (first) *scale = (uint8_t)byte;
-}
-
 // Blocks of a launch are numbered row by row; a group of 16 lanes takes kPerGroup of them, a workgroup's groups side by side.
 constexpr int kGroups = 16, kPerGroup = 4;
 
@@ -67,7 +49,7 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const T *__restrict__ x
     for (int i = 0; i < kPerGroup; ++i) {
         const int64_t at = ((int64_t)blockIdx.x * kPerGroup + i) * kGroups + group;
         if (at < blocks)  // (the same for the 16 lanes of a group)
-            store_block(v[i], q + row[i] * ld + b[i] * kFp8Block + lane * 8, scale + row[i] * ld_scale + b[i], lane == 0);
+            fp8_store_block(v[i], q + row[i] * ld + b[i] * kFp8Block + lane * 8, scale + row[i] * ld_scale + b[i], lane == 0);
     }
 }
 
@@ -94,8 +76,8 @@ __global__ __launch_bounds__(256) void silu_bwd_quant_kernel(const T *__restrict
         ev[i] = de;
     }
     const int64_t out = row * fp8_ld(N) + n, out_scale = row * fp8_ld_scale(N) + b;
-    store_block(ev, de_q + out, de_scale + out_scale, lane == 0);
-    store_block(gv, dg_q + out, dg_scale + out_scale, lane == 0);
+    fp8_store_block(ev, de_q + out, de_scale + out_scale, lane == 0);
+    fp8_store_block(gv, dg_q + out, dg_scale + out_scale, lane == 0);
 }
 
 __device__ __forceinline__ float fp8_value(uint32_t byte) { return __builtin_amdgcn_cvt_f32_fp8((int)byte, 0); }

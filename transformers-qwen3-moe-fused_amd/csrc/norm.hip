@@ -1,0 +1,276 @@
+// The residual's addition and the root-mean-square norm behind it, forward and backward, and with rows in 8-bit blocks as the
+// result (norm_parts.h has the arithmetic).
+#include "fp8.h"
+#include "norm_parts.h"
+#include "ops.h"
+
+namespace mfl {
+
+namespace {
+
+// ---- forward --------------------------------------------------------------------------------------------------------------
+// A row belongs to LANES threads, which hold it in registers, 8 C elements each in C runs of 8: one pass over memory.
+template <typename T, typename TW, int LANES, int C, bool FP8, bool WHOLE>
+__global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_fwd_kernel(const T *__restrict__ x, const T *__restrict__ residual,
+                                                                           const TW *__restrict__ weight, T *__restrict__ y,
+                                                                           T *__restrict__ s, uint8_t *__restrict__ q,
+                                                                           uint8_t *__restrict__ scale, int64_t R, int H,
+                                                                           double eps) {
+    constexpr int ROWS = LANES < 256 ? 256 / LANES : 1, WAVES = LANES / 64;
+    __shared__ double part[ROWS * WAVES];
+    const int i = threadIdx.x % LANES;
+    int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES;
+    const bool in = row < R;
+    if (!in) row = R - 1;  // (computed along, not stored)
+    x += row * H;
+    Eight<T, WHOLE> v[C];
+    Eight<TW, WHOLE> w[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) v[c].load(x, (c * LANES + i) * 8, H);
+    if (residual != nullptr) {
+        Eight<T, WHOLE> o[C];
+#pragma unroll
+        for (int c = 0; c < C; ++c) o[c].load(residual + row * H, (c * LANES + i) * 8, H);
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            add_rounded(v[c], o[c]);
+            if (in) v[c].store(s + row * H, (c * LANES + i) * 8, H);
+        }
+    }
+    double sum = 0.0;
+#pragma unroll
+    for (int c = 0; c < C; ++c) sum = sum_of_squares(v[c], sum);
+#pragma unroll
+    for (int c = 0; c < C; ++c) w[c].load(weight, (c * LANES + i) * 8, H);
+    sum = wave_sum(sum);
+    if (LANES > 64) {
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = sum;
+        __syncthreads();
+        sum = 0.0;
+#pragma unroll
+        for (int u = 0; u < WAVES; ++u) sum += part[threadIdx.x / LANES * WAVES + u];
+    }
+    const double r = inverse_root(sum / (double)H + eps);
+    if (!in) return;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const int k = (c * LANES + i) * 8;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[c].v[u] = normed(v[c].v[u], r, w[c].v[u]);
+        if (y != nullptr) v[c].store(y + row * H, k, H);
+        if constexpr (FP8) {
+            float f[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) f[u] = k + u < H ? to_f32(v[c].v[u]) : 0.0f;
+            if (k < fp8_ld(H))  // (the 16 lanes of a block alike)
+                fp8_store_block(f, q + row * fp8_ld(H) + k, scale + row * fp8_ld_scale(H) + k / kFp8Block, (i & 15) == 0);
+        }
+    }
+}
+
+// ---- backward -------------------------------------------------------------------------------------------------------------
+// With u = s r and g = dy w: dx = r (g - u mean(g u)) + ds, dw = sum over the rows of dy u.  s is read as the forward pass left
+// it and its r found again, which costs a sum beside the one that is needed anyway.  A group of LANES threads takes every
+// gridDim.x * GROUPS-th row and keeps its columns' share of dw in registers; the groups of a workgroup meet in LDS, the workgroups
+// in `partial` (workgroup, H), which a second kernel adds up in order.
+template <typename T, typename TW, int LANES, int C, int THREADS, bool WHOLE>
+__global__ __launch_bounds__(THREADS) void norm_bwd_kernel(const T *__restrict__ dy, const T *__restrict__ ds, const T *__restrict__ s,
+                                                          const TW *__restrict__ weight, T *__restrict__ dx,
+                                                          float *__restrict__ partial, int64_t R, int H, double eps) {
+    constexpr int GROUPS = THREADS / LANES, WAVES = LANES / 64;
+    __shared__ double squares[2][GROUPS * WAVES];
+    __shared__ float alongs[2][GROUPS * WAVES];
+    extern __shared__ float shared_dw[];  // (GROUPS - 1, LANES * C * 8) where the groups are many
+    const int i = threadIdx.x % LANES, group = threadIdx.x / LANES;
+    float dw[C][8];
+    Eight<TW, WHOLE> w[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        w[c].load(weight, (c * LANES + i) * 8, H);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) dw[c][u] = 0.0f;
+    }
+    int turn = 0;
+    // (every group of a workgroup takes as many turns: the rows' sums wait for one another where a row has several waves)
+    for (int64_t row0 = (int64_t)blockIdx.x * GROUPS; row0 < R; row0 += (int64_t)gridDim.x * GROUPS, turn ^= 1) {
+        const int64_t row = row0 + group;
+        const bool in = row < R;
+        const int64_t at = (in ? row : R - 1) * H;
+        Eight<T, WHOLE> sv[C], g[C], d[C];
+#pragma unroll
+        for (int c = 0; c < C; ++c) sv[c].load(s + at, (c * LANES + i) * 8, H);
+#pragma unroll
+        for (int c = 0; c < C; ++c) g[c].load(dy + at, (c * LANES + i) * 8, H);
+        if (ds != nullptr && dx != nullptr) {
+#pragma unroll
+            for (int c = 0; c < C; ++c) d[c].load(ds + at, (c * LANES + i) * 8, H);
+        }
+        double square = 0.0;  // (32 bits hold no square of a 32-bit or bf16 value past 2^64)
+        float along = 0.0f;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const float a = to_f32(sv[c].v[u]);
+                square = __builtin_fma((double)a, (double)a, square);
+                along = __builtin_fmaf(to_f32(g[c].v[u]) * to_f32(w[c].v[u]), a, along);
+            }
+#pragma unroll
+        for (int step = 32; step; step >>= 1) along += __shfl_xor(along, step);
+        square = wave_sum(square);
+        if (WAVES > 1) {
+            if ((threadIdx.x & 63) == 0) squares[turn][threadIdx.x >> 6] = square, alongs[turn][threadIdx.x >> 6] = along;
+            __syncthreads();  // (two tables in turn: one barrier a row)
+            square = 0.0, along = 0.0f;
+#pragma unroll
+            for (int u = 0; u < WAVES; ++u) square += squares[turn][group * WAVES + u], along += alongs[turn][group * WAVES + u];
+        }
+        const double root = inverse_root(square / (double)H + eps);
+        const float r = (float)root, back = (float)((double)along / (double)H * root * root);  // dx = r (g - s back) + ds
+        if (!in) continue;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const float a = to_f32(sv[c].v[u]), b = to_f32(g[c].v[u]);
+                dw[c][u] = __builtin_fmaf(b, a * r, dw[c][u]);
+                float o = r * __builtin_fmaf(-a, back, b * to_f32(w[c].v[u]));
+                if (ds != nullptr && dx != nullptr) o += to_f32(d[c].v[u]);
+                sv[c].v[u] = from_f32<T>(o);
+            }
+            if (dx != nullptr) sv[c].store(dx + at, (c * LANES + i) * 8, H);
+        }
+    }
+    if (partial == nullptr) return;
+    if (GROUPS > 1) {
+        constexpr int WIDTH = LANES * C * 8;
+        if (group > 0) {
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int u = 0; u < 8; ++u) shared_dw[(group - 1) * WIDTH + (c * 8 + u) * LANES + i] = dw[c][u];
+        }
+        __syncthreads();
+        if (group > 0) return;
+        for (int o = 0; o < GROUPS - 1; ++o)
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int u = 0; u < 8; ++u) dw[c][u] += shared_dw[o * WIDTH + (c * 8 + u) * LANES + i];
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const int k = (c * LANES + i) * 8;
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (k + u < H) partial[(int64_t)blockIdx.x * H + k + u] = dw[c][u];
+    }
+}
+
+// dw (H) = the sum of `parts` rows of partial; 16 columns a workgroup, 16 threads a column.
+template <typename TW>
+__global__ __launch_bounds__(256) void norm_dw_kernel(const float *__restrict__ partial, TW *__restrict__ dw, int parts, int H) {
+    __shared__ float sums[16][17];
+    const int col = threadIdx.x & 15, part = threadIdx.x >> 4, k = blockIdx.x * 16 + col;
+    float sum = 0.0f;
+    if (k < H)
+        for (int p = part; p < parts; p += 16) sum += partial[(int64_t)p * H + k];
+    sums[part][col] = sum;
+    __syncthreads();
+    if (part != 0 || k >= H) return;
+    sum = 0.0f;
+#pragma unroll
+    for (int p = 0; p < 16; ++p) sum += sums[p][col];
+    dw[k] = from_f32<TW>(sum);
+}
+
+static_assert(MFL_NORM_WIDTH == 1024 * 4 * 8, "1024 threads of four runs");
+constexpr int kBwdThreads = 512;
+
+// threads of a row, and the backward kernel's workgroups
+int lanes_of(int H) { return H <= 512 ? 64 : H <= 1024 ? 128 : H <= 2048 ? 256 : H <= 4096 ? 512 : 1024; }
+int bwd_grid(int64_t R, int H) {
+    const int lanes = lanes_of(H), groups = lanes < kBwdThreads ? kBwdThreads / lanes : 1;
+    const int64_t want = (R + groups - 1) / groups, most = 2 * device_info().cu_count;
+    return (int)(want < most ? want : most);
+}
+
+template <typename T, typename TW, bool FP8, bool WHOLE>
+int launch_fwd(const NormCall &n, hipStream_t stream) {
+#define MFL_NORM(L, C)                                                                                                          \
+    norm_fwd_kernel<T, TW, L, C, FP8, WHOLE><<<(unsigned)((n.R + (L < 256 ? 256 / L : 1) - 1) / (L < 256 ? 256 / L : 1)),               \
+                                        L < 256 ? 256 : L, 0, stream>>>((const T *)n.x, (const T *)n.residual,                   \
+                                                                       (const TW *)n.weight, (T *)n.y, (T *)n.s, n.q, n.scale,   \
+                                                                       n.R, n.H, (double)n.eps)
+    const int H = n.H;
+    if (H <= 512) MFL_NORM(64, 1);
+    else if (H <= 1024) MFL_NORM(128, 1);
+    else if (H <= 2048) MFL_NORM(256, 1);
+    else if (H <= 4096) MFL_NORM(512, 1);
+    else if (H <= 8192) MFL_NORM(1024, 1);
+    else if (H <= 16384) MFL_NORM(1024, 2);
+    else MFL_NORM(1024, 4);
+#undef MFL_NORM
+    return launch_status();
+}
+
+template <typename T, typename TW, bool WHOLE>
+int launch_bwd(const NormCall &n, const void *dy, const void *ds, void *dx, void *dw, float *partial, hipStream_t stream) {
+    const int grid = bwd_grid(n.R, n.H), H = n.H;
+#define MFL_NORM(L, C)                                                                                                         \
+    {                                                                                                                          \
+        constexpr int threads = L < kBwdThreads ? kBwdThreads : L;                                                             \
+        constexpr int room = (threads / L - 1) * L * C * 8 * 4;  /* 14 KB at most */                                           \
+        auto kernel = norm_bwd_kernel<T, TW, L, C, threads, WHOLE>;                                                            \
+        kernel<<<grid, threads, room, stream>>>((const T *)dy, (const T *)ds, (const T *)n.s, (const TW *)n.weight, (T *)dx,    \
+                                                dw != nullptr ? partial : nullptr, n.R, H, (double)n.eps);                             \
+    }
+    if (H <= 512) MFL_NORM(64, 1)
+    else if (H <= 1024) MFL_NORM(128, 1)
+    else if (H <= 2048) MFL_NORM(256, 1)
+    else if (H <= 4096) MFL_NORM(512, 1)
+    else if (H <= 8192) MFL_NORM(1024, 1)
+    else if (H <= 16384) MFL_NORM(1024, 2)
+    else MFL_NORM(1024, 4)
+#undef MFL_NORM
+    if (dw != nullptr) norm_dw_kernel<TW><<<ceil_div(H, 16), 256, 0, stream>>>(partial, (TW *)dw, grid, H);
+    return launch_status();
+}
+
+template <typename T, typename TW>
+int fwd(const NormCall &n, hipStream_t stream) {
+    if (n.H % 8 == 0) return n.q ? launch_fwd<T, TW, true, true>(n, stream) : launch_fwd<T, TW, false, true>(n, stream);
+    return n.q ? launch_fwd<T, TW, true, false>(n, stream) : launch_fwd<T, TW, false, false>(n, stream);
+}
+template <typename T, typename TW>
+int bwd(const NormCall &n, const void *dy, const void *ds, void *dx, void *dw, float *partial, hipStream_t stream) {
+    if (n.H % 8 == 0) return launch_bwd<T, TW, true>(n, dy, ds, dx, dw, partial, stream);
+    return launch_bwd<T, TW, false>(n, dy, ds, dx, dw, partial, stream);
+}
+
+}  // namespace
+
+int add_rms_norm(const NormCall &n, hipStream_t stream) {
+    // (a launch's threads are counted in 32 bits)
+    const int64_t lanes = lanes_of(n.H);
+    if (n.R > 0xffffffffll / lanes - 1024) return MFL_ERR_LIMIT;
+    int rc = MFL_OK;
+    MFL_DISPATCH_FLOAT(n.dtype, T, {
+        if (n.weight_dtype == n.dtype) rc = fwd<T, T>(n, stream);
+        else rc = fwd<T, float>(n, stream);
+    });
+    return rc;
+}
+
+size_t add_rms_norm_bwd_workspace(int64_t R, int H) { return (size_t)bwd_grid(R, H) * H * sizeof(float); }
+
+int add_rms_norm_bwd(const NormCall &n, const void *dy, const void *ds, void *dx, void *dw, float *partial, hipStream_t stream) {
+    int rc = MFL_OK;
+    MFL_DISPATCH_FLOAT(n.dtype, T, {
+        if (n.weight_dtype == n.dtype) rc = bwd<T, T>(n, dy, ds, dx, dw, partial, stream);
+        else rc = bwd<T, float>(n, dy, ds, dx, dw, partial, stream);
+    });
+    return rc;
+}
+
+}  // namespace mfl

@@ -33,6 +33,25 @@ int nf4_unnest_absmax(const UnnestScales *s, int count, hipStream_t stream);
 int nf4_quant(const void *w, int w_dtype, int64_t n, int blocksize, const float *code16, uint8_t *wq, float *absmax,
               hipStream_t stream);
 
+// s = x + residual (x itself, not written, where residual is null), y = s / sqrt(mean(s^2) + eps) * weight; y, and its 8-bit blocks
+// q with their scale bytes, where given.  H up to MFL_NORM_WIDTH.
+struct NormCall {
+    const void *x, *residual, *weight;
+    void *y, *s;
+    uint8_t *q, *scale;
+    int64_t R;
+    int H;
+    float eps;
+    int dtype, weight_dtype;
+};
+int add_rms_norm(const NormCall &n, hipStream_t stream);
+size_t add_rms_norm_bwd_workspace(int64_t R, int H);
+// n.s: the stream that the forward pass left (read); dx, dw where wanted, ds may be null.
+int add_rms_norm_bwd(const NormCall &n, const void *dy, const void *ds, void *dx, void *dw, float *partial, hipStream_t stream);
+
+size_t moe_layer_workspace(const mfl_moe_layer &p);
+int moe_layer_fwd(const mfl_moe_layer &p, void *out, void *logits, void *workspace, hipStream_t stream);
+
 int router_fwd(const void *x, const void *w, void *logits, int64_t T, int H, int E, int out_dtype, hipStream_t stream);
 size_t router_dw_workspace(int64_t T, int H, int E);
 int router_dw(const void *x, const void *dlogits, void *dw, int64_t T, int H, int E, void *workspace, size_t ws_bytes,

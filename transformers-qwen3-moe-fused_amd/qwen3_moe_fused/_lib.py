@@ -66,6 +66,16 @@ class BlockCopy(ctypes.Structure):
     _fields_ = [("src", _vp), ("dst", _vp), ("blocks", _i64), ("bytes", _i64), ("src_stride", _i64), ("dst_stride", _i64)]
 
 
+class MoeLayer(ctypes.Structure):
+    """``mfl_moe_layer``: the whole sparse layer for a few tokens."""
+
+    _fields_ = [("x", _vp), ("residual", _vp), ("norm_weight", _vp), ("router", _vp), ("w_gate", _vp), ("w_up", _vp),
+                ("w_down", _vp), ("s_gate", _vp), ("s_up", _vp), ("s_down", _vp), ("T", _i64), ("E", _i), ("k", _i), ("H", _i),
+                ("I", _i), ("renorm", _i), ("dtype", _i), ("eps", _f)]
+
+
+_layerp = ctypes.POINTER(MoeLayer)
+
 # name -> (restype, argtypes); mirrors include/moe_fused_linear.h
 _SIGNATURES = {
     "mfl_abi_version": (_i, []),
@@ -137,6 +147,14 @@ _SIGNATURES = {
     "mfl_moe_block_workspace": (_sz, [_blockp]),
     "mfl_moe_block_fwd": (_i, [_blockp, _vp, _vp, _sz, _vp]),
     "mfl_moe_block_bwd_workspace": (_sz, [_blockp]),
+    "mfl_mlp_fwd_fp8_rows": (_i, [_vp, _vp, _vp, _i64, _vp, _i, _fp8p, _fp8p, _fp8p, _vp, _i, _vp, _vp, _vp, _i64, _i, _i, _i, _i,
+                                  _vp, _sz, _vp]),
+    "mfl_add_rms_norm": (_i, [_vp, _vp, _vp, _vp, _vp, _i64, _i, _f, _i, _i, _vp]),
+    "mfl_add_rms_norm_bwd_workspace": (_sz, [_i64, _i]),
+    "mfl_add_rms_norm_bwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i, _f, _i, _i, _vp, _sz, _vp]),
+    "mfl_add_rms_norm_fp8": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i, _f, _i, _i, _vp]),
+    "mfl_moe_layer_workspace": (_sz, [_layerp]),
+    "mfl_moe_layer_fwd": (_i, [_layerp, _vp, _vp, _vp, _sz, _vp]),
     "mfl_moe_block_bwd": (_i, [_blockp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
 }
 

@@ -10,6 +10,7 @@ re-gathers the token rows instead of keeping a (rows, hidden) copy alive.
 from __future__ import annotations
 
 import ctypes
+from typing import Optional, Tuple
 
 import torch
 
@@ -23,6 +24,7 @@ from .grouped_gemm.fused import (grouped_gemm_forward_transposed_dual, grouped_g
 from .kernels.routing import _combine, _gather, _scatter
 from .kernels.silu_mul import silu_mul_backward
 from .grouped_gemm.forward_4bit import UNSUPPORTED, check_packed, grouped_gemm_forward_transposed_4bit
+from .quantize.fp8 import check_fp8_weight
 from .quantize.nf4 import packed_weight
 
 
@@ -192,10 +194,11 @@ def moe_fused_glu_fp8(tokens: torch.Tensor, w_gate: torch.Tensor, gate_scale: to
 
 class _MlpGatheredFp8(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, tokens, w_gate, gate_scale, w_up, up_scale, w_down, down_scale, m_sizes, sort_idx, inv_sort_idx, k):
+    def forward(ctx, tokens, w_gate, gate_scale, w_up, up_scale, w_down, down_scale, m_sizes, sort_idx, inv_sort_idx, k,
+                values, value_scales):
         need = ctx.needs_input_grad[0]
         out = grouped_mlp_forward_fp8(tokens, w_gate, gate_scale, w_up, up_scale, w_down, down_scale, m_sizes, sort_idx, k,
-                                      return_products=need)
+                                      return_products=need, quantized=None if values is None else (values, value_scales))
         if not need:
             return out
         y, e, g = out
@@ -211,23 +214,24 @@ class _MlpGatheredFp8(torch.autograd.Function):
         dh = grouped_gemm_forward_transposed_fp8(_lib.dense(dy), w_down, down_scale, m_sizes)
         dx = grouped_glu_backward_fp8(dh, e, g, w_gate, gate_scale, w_up, up_scale, m_sizes)
         with _lib.on_device_of(dx):
-            return _combine(dx, inv_sort_idx, None, ctx.n_tokens, ctx.k), *(None,) * 10
+            return _combine(dx, inv_sort_idx, None, ctx.n_tokens, ctx.k), *(None,) * 12
 
 
 def moe_fused_mlp_fp8(tokens: torch.Tensor, w_gate: torch.Tensor, gate_scale: torch.Tensor, w_up: torch.Tensor,
                       up_scale: torch.Tensor, w_down: torch.Tensor, down_scale: torch.Tensor, m_sizes: torch.Tensor,
-                      sort_idx: torch.Tensor, inv_sort_idx: torch.Tensor, num_selected: int) -> torch.Tensor:
+                      sort_idx: torch.Tensor, inv_sort_idx: torch.Tensor, num_selected: int,
+                      quantized: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> torch.Tensor:
     """``moe_fused_mlp`` on weights in 8-bit floating point with their block scales (frozen), in bf16, fp16 or fp32: between
     the gated unit and the down projection there are only quantised rows, made from the unit's fp32 values.  Differentiable
-    in ``tokens``."""
+    in ``tokens``.  ``quantized``: what ``add_rms_norm_fp8`` (or ``quantize_fp8_rows``) made of ``tokens`` already."""
     assert not (w_gate.requires_grad or gate_scale.requires_grad or w_up.requires_grad or up_scale.requires_grad
                 or w_down.requires_grad or down_scale.requires_grad), "8-bit expert weights are frozen"
     _check_routing(tokens, sort_idx, inv_sort_idx, num_selected)
     if not (torch.is_grad_enabled() and tokens.requires_grad) and _lib.plain_call():  # (as in moe_fused_linear_fp8)
         return grouped_mlp_forward_fp8(tokens, w_gate, gate_scale, w_up, up_scale, w_down, down_scale, m_sizes, sort_idx,
-                                       num_selected)
+                                       num_selected, quantized=quantized)
     return _MlpGatheredFp8.apply(tokens, w_gate, gate_scale, w_up, up_scale, w_down, down_scale, m_sizes, sort_idx,
-                                 inv_sort_idx, num_selected)
+                                 inv_sort_idx, num_selected, *(quantized or (None, None)))
 
 
 class _MoeBlock(torch.autograd.Function):
@@ -327,3 +331,98 @@ def moe_block_4bit(tokens: torch.Tensor, logits: torch.Tensor, w_gate: torch.Ten
                       ctypes.pointer(down), tokens.shape[0], experts, num_selected, hidden, inter, int(bool(renorm)),
                       _lib.dtype_code(tokens.dtype), _lib.dtype_code(logits.dtype), 0)
     return _run_block(b, tokens)
+
+
+# ---- the whole layer for a few tokens --------------------------------------------------------------------------------------
+
+LAYER_TOKENS = 16  # MFL_LAYER_TOKENS
+
+
+def _layer(hidden, w_router, w_gate, w_up, w_down, scales, k, renorm, residual, norm_weight, eps):
+    assert hidden.is_cuda and hidden.ndim == 2 and hidden.is_contiguous(), "the layer runs on the GPU, on a dense matrix of tokens"
+    dtype, device = _lib.dtype_code(hidden.dtype), hidden.get_device()
+    tokens, width = hidden.shape
+    assert tokens <= LAYER_TOKENS, f"the layer in two launches takes up to {LAYER_TOKENS} tokens: more are the block's"
+    experts, inter, in_features = w_gate.shape
+    assert in_features == width and w_up.shape == w_gate.shape and w_down.shape == (experts, width, inter)
+    assert w_router.shape == (experts, width) and 0 < k <= experts
+    dense = [w_router]
+    if scales is None:
+        dense += [w_gate, w_up, w_down]
+        s_gate = s_up = s_down = None
+    else:
+        for w, s in zip((w_gate, w_up, w_down), scales):
+            check_fp8_weight(hidden, w, s)
+        s_gate, s_up, s_down = (s.data_ptr() for s in scales)
+    if norm_weight is not None:
+        assert norm_weight.shape == (width,)
+        dense.append(norm_weight)
+    if residual is not None:
+        assert norm_weight is not None, "a residual is added in front of a norm"
+        assert residual.shape == hidden.shape
+        dense.append(residual)
+    for t in dense:
+        assert t.dtype == hidden.dtype and t.get_device() == device and t.is_contiguous()
+    with _lib.on_device_of(hidden):
+        out, logits = torch.empty_like(hidden), hidden.new_empty(tokens, experts)
+        if tokens == 0:
+            return out, logits
+        call = _lib.MoeLayer(hidden.data_ptr(), _lib.ptr(residual), _lib.ptr(norm_weight), w_router.data_ptr(), w_gate.data_ptr(),
+                             w_up.data_ptr(), w_down.data_ptr(), s_gate, s_up, s_down, tokens, experts, k, width, inter,
+                             int(bool(renorm)), dtype, eps)
+        lib = _lib.lib()
+        size = lib.mfl_moe_layer_workspace(call)
+        ws = torch.empty(size, device=hidden.device, dtype=torch.uint8)
+        rc = lib.mfl_moe_layer_fwd(call, out.data_ptr(), logits.data_ptr(), ws.data_ptr(), size, _lib.stream())
+    _lib.check(rc, "mfl_moe_layer_fwd")
+    return out, logits
+
+
+class _Layer(torch.autograd.Function):
+    """For whoever watches (``_lib.plain_call``): the layer has no backward pass, no tangents and no batching rule."""
+
+    @staticmethod
+    def forward(ctx, hidden, w_router, w_gate, w_up, w_down, s_gate, s_up, s_down, k, renorm, residual, norm_weight, eps):
+        scales = None if s_gate is None else (s_gate, s_up, s_down)
+        out, logits = _layer(hidden, w_router, w_gate, w_up, w_down, scales, k, renorm, residual, norm_weight, eps)
+        ctx.mark_non_differentiable(out, logits)
+        return out, logits
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("the layer for a few tokens has no backward pass")
+
+
+def _call_layer(hidden, w_router, w_gate, w_up, w_down, scales, k, renorm, residual, norm_weight, eps):
+    if torch.is_grad_enabled():
+        assert not any(t is not None and t.requires_grad for t in (hidden, w_router, w_gate, w_up, w_down, residual, norm_weight,
+                                                                   *(scales or ()))), \
+            "the layer for a few tokens has no backward pass: call it under torch.no_grad(), or the block"
+    if _lib.plain_call():
+        return _layer(hidden, w_router, w_gate, w_up, w_down, scales, k, renorm, residual, norm_weight, eps)
+    return _Layer.apply(hidden, w_router, w_gate, w_up, w_down, *(scales or (None,) * 3), k, renorm, residual, norm_weight, eps)
+
+
+def moe_fused_layer(hidden: torch.Tensor, w_router: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
+                    num_selected: int, renorm: bool, residual: Optional[torch.Tensor] = None,
+                    norm_weight: Optional[torch.Tensor] = None, eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The whole sparse block (modular_qwen3_moe_fused.py:72-118) for up to 16 tokens, for serving: ``hidden`` (T, H), ``w_router``
+    (E, H), the three expert matrices, all of one type (bf16, fp16 or fp32).  Returns (out (T, H), router logits (T, E)).
+
+    With ``norm_weight`` (H) the layer's second half as a decoder layer has it: s = hidden + residual (or hidden), the experts get
+    ``add_rms_norm``'s rows, and s is added to what they return.
+
+    Experts are chosen from the logits as rounded to the tensors' type, equal ones by the lower id, as in the block; between there and
+    the output nothing is rounded to 16 bits, so results differ from the block's by its roundings of the gated unit, of each expert's
+    row and of the routing weights."""
+    return _call_layer(hidden, w_router, w_gate, w_up, w_down, None, num_selected, renorm, residual, norm_weight, eps)
+
+
+def moe_fused_layer_fp8(hidden: torch.Tensor, w_router: torch.Tensor, w_gate: torch.Tensor, gate_scale: torch.Tensor,
+                        w_up: torch.Tensor, up_scale: torch.Tensor, w_down: torch.Tensor, down_scale: torch.Tensor,
+                        num_selected: int, renorm: bool, residual: Optional[torch.Tensor] = None,
+                        norm_weight: Optional[torch.Tensor] = None, eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``moe_fused_layer`` on expert weights in 8-bit floating point with their block scales; the rows (not those that the router
+    reads) and the gated unit's result are quantised as in ``moe_fused_mlp_fp8``."""
+    return _call_layer(hidden, w_router, w_gate, w_up, w_down, (gate_scale, up_scale, down_scale), num_selected, renorm, residual,
+                       norm_weight, eps)

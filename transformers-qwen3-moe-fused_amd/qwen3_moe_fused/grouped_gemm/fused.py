@@ -16,7 +16,7 @@ kernels instead.
 """
 from __future__ import annotations
 
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 
@@ -26,7 +26,7 @@ from ..kernels.silu_mul import silu_mul_forward
 from ..quantize.nf4 import packed_weight, resolve_absmax
 from ._common import check_operands, is_int_tensor
 from .forward import grouped_gemm_forward
-from ..quantize.fp8 import check_fp8_weight
+from ..quantize.fp8 import check_fp8_rows, check_fp8_weight
 from .forward_4bit import UNSUPPORTED, check_packed, grouped_gemm_forward_4bit
 from .forward_fp8 import GLU, GLU_BWD, MLP, MLP_OFF_GRID, call_with_workspace, check_rows, fp8_weight, fp8_workspace
 
@@ -462,15 +462,19 @@ def grouped_glu_backward_fp8(dh: torch.Tensor, e: torch.Tensor, g: torch.Tensor,
 
 def grouped_mlp_forward_fp8(x: torch.Tensor, w_gate: torch.Tensor, gate_scale: torch.Tensor, w_up: torch.Tensor,
                             up_scale: torch.Tensor, w_down: torch.Tensor, down_scale: torch.Tensor, m_sizes: torch.Tensor,
-                            row_idx: Optional[torch.Tensor] = None, idx_div: int = 1, return_products: bool = False):
+                            row_idx: Optional[torch.Tensor] = None, idx_div: int = 1, return_products: bool = False,
+                            quantized: Optional[Tuple[torch.Tensor, torch.Tensor]] = None):
     """The gated unit followed by the down projection (``w_down`` (E, hidden, intermediate)); the unit's result goes from its
-    fp32 values to quantised rows.  ``y``, or ``(y, e, g)`` with ``return_products``."""
+    fp32 values to quantised rows.  ``y``, or ``(y, e, g)`` with ``return_products``.  ``quantized``: (values, scales) of ``x`` as
+    ``quantize_fp8_rows`` or ``add_rms_norm_fp8`` left them, which the call then does not make again."""
     check_rows(m_sizes, x)
     rows = _check_gather(x, row_idx, idx_div)
     experts, n, k = check_fp8_weight(x, w_gate, gate_scale)
     assert check_fp8_weight(x, w_up, up_scale) == (experts, n, k) and check_fp8_weight(x, w_down, down_scale) == (experts, k, n)
     assert x.shape[1] == k and m_sizes.numel() == experts
     assert rows == 0 or x.shape[0] > 0
+    if quantized is not None:
+        check_fp8_rows(*quantized, x)
     with _lib.on_device_of(x):
         y = x.new_empty(rows, k)
         e = x.new_empty(rows, n) if return_products else None
@@ -478,9 +482,12 @@ def grouped_mlp_forward_fp8(x: torch.Tensor, w_gate: torch.Tensor, gate_scale: t
         ms = _lib.as_index_tensor(m_sizes)
         on_grid = (w_gate.data_ptr() | w_up.data_ptr()) % 16 == 0
         _keep, ws, ws_bytes = fp8_workspace(MLP if on_grid else MLP_OFF_GRID, x, x.shape[0], rows, n, k, experts)
-        rc = _lib.lib().mfl_mlp_fwd_fp8(x.data_ptr(), x.shape[0], _lib.ptr(row_idx), idx_div, fp8_weight(w_gate, gate_scale),
-                                        fp8_weight(w_up, up_scale), fp8_weight(w_down, down_scale), ms.data_ptr(),
-                                        _lib.itype_code(ms.dtype), y.data_ptr(), _lib.ptr(e), _lib.ptr(g), rows, n, k, experts,
-                                        _lib.dtype_code(x.dtype), ws, ws_bytes, _lib.stream())
+        args = (x.shape[0], _lib.ptr(row_idx), idx_div, fp8_weight(w_gate, gate_scale), fp8_weight(w_up, up_scale),
+                fp8_weight(w_down, down_scale), ms.data_ptr(), _lib.itype_code(ms.dtype), y.data_ptr(), _lib.ptr(e), _lib.ptr(g),
+                rows, n, k, experts, _lib.dtype_code(x.dtype), ws, ws_bytes, _lib.stream())
+        if quantized is None:
+            rc = _lib.lib().mfl_mlp_fwd_fp8(x.data_ptr(), *args)
+        else:
+            rc = _lib.lib().mfl_mlp_fwd_fp8_rows(x.data_ptr(), quantized[0].data_ptr(), quantized[1].data_ptr(), *args)
     _lib.check(rc, "mfl_mlp_fwd_fp8")
     return (y, e, g) if return_products else y

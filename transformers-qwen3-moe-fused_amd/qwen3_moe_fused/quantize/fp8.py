@@ -33,6 +33,20 @@ def check_fp8_weight(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor)
     return experts, n, k
 
 
+def check_fp8_rows(values: torch.Tensor, scale: torch.Tensor, like: torch.Tensor) -> None:
+    """That (values, scale) are quantised rows of ``like``'s shape and device, as ``quantize_fp8_rows`` lays them out."""
+    assert values.dtype == FP8 and scale.dtype == torch.float8_e8m0fnu and values.shape == like.shape and like.ndim == 2
+    rows, k = values.shape
+    blocks = blocks_of(k)
+    assert scale.shape == (rows, blocks)
+    device = like.get_device()
+    assert values.get_device() == device and scale.get_device() == device
+    # (a single row, or none, may have any stride)
+    assert rows <= 1 or (values.stride(0) == blocks * BLOCK and scale.stride(0) == (blocks + 3) // 4 * 4), \
+        "values and scales as quantize_fp8_rows lays them out"
+    assert (k == 1 or values.stride(1) == 1) and (blocks == 1 or scale.stride(1) == 1)
+
+
 def quantize_fp8_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """``x`` (rows, K) in bf16 / fp16 / fp32 -> (values (rows, K) float8_e4m3fn, scales (rows, ceil(K / 128))
     float8_e8m0fnu).  Rows of the values lie a multiple of 128 bytes apart (zeros behind column K), those of the scales a
