@@ -577,7 +577,8 @@ MFL_API int mfl_add_rms_norm_fp8(const void *x, const void *residual, const void
  * s_gate, s_up, s_down given: expert weights are e4m3 bytes with these block scales, and the rows and the gated unit's result are
  * quantised as mfl_mlp_fwd_fp8 quantises them; else they are of dtype.  x, residual, norm_weight, router, out, logits of dtype.
  * A token whose logits hold a NaN, or an infinity as the largest, chooses no expert; its row of out is NaN, the others are what they
- * are without it.  E up to 1024, k up to 64, H and I up to 2^24 (MFL_ERR_LIMIT).  out and logits overlap nothing else.
+ * are without it.  E up to 1024, k up to 64, H and I up to 2^24, T k (I + 16)
+ * up to 2^28 (MFL_ERR_LIMIT).  out and logits overlap nothing else.
  * workspace: mfl_moe_layer_workspace bytes (0: shape not taken), 256-byte aligned, scratch.  Replaces
  * qwen3_moe_fused/modular_qwen3_moe_fused.py:72-118 at decode sizes. */
 #define MFL_LAYER_TOKENS 16

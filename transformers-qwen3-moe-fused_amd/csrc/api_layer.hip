@@ -22,6 +22,12 @@ int check_norm(const NormCall &n) {
     return MFL_OK;
 }
 
+// (the gated unit's rows, T k of them, are addressed with 32 bits)
+bool past_limits(const mfl_moe_layer &p) {
+    return p.T > MFL_LAYER_TOKENS || p.E > 1024 || p.k > 64 || p.H > 1 << 24 || p.I > 1 << 24 ||
+           p.T * p.k * ((int64_t)p.I + 16) > 1 << 28;
+}
+
 }  // namespace
 
 extern "C" {
@@ -69,15 +75,15 @@ int mfl_add_rms_norm_bwd(const void *dy, const void *ds, const void *s, const vo
 }
 
 size_t mfl_moe_layer_workspace(const mfl_moe_layer *p) {
-    if (!p || p->T <= 0 || p->T > MFL_LAYER_TOKENS || p->E <= 0 || p->k <= 0 || p->k > p->E || p->H <= 0 || p->I <= 0) return 0;
-    if (p->E > 1024 || p->k > 64 || p->H > 1 << 24 || p->I > 1 << 24 || !dtype_ok(p->dtype)) return 0;
+    if (!p || p->T <= 0 || p->E <= 0 || p->k <= 0 || p->k > p->E || p->H <= 0 || p->I <= 0) return 0;
+    if (past_limits(*p) || !dtype_ok(p->dtype)) return 0;
     return moe_layer_workspace(*p);
 }
 
 int mfl_moe_layer_fwd(const mfl_moe_layer *p, void *out, void *logits, void *workspace, size_t ws_bytes, void *stream) {
     if (!p) return MFL_ERR_NULL;
     if (p->T < 0 || p->E <= 0 || p->k <= 0 || p->k > p->E || p->H <= 0 || p->I <= 0) return MFL_ERR_SHAPE;
-    if (p->T > MFL_LAYER_TOKENS || p->E > 1024 || p->k > 64 || p->H > 1 << 24 || p->I > 1 << 24) return MFL_ERR_LIMIT;
+    if (past_limits(*p)) return MFL_ERR_LIMIT;
     if (!dtype_ok(p->dtype)) return MFL_ERR_DTYPE;
     if (p->norm_weight && (!(p->eps >= 0.0f) || isinf(p->eps))) return MFL_ERR_SHAPE;
     if (p->T == 0) return MFL_OK;

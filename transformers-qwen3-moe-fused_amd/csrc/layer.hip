@@ -22,101 +22,108 @@ struct Layer {
     const void *rows;    // the rows that the experts read, `ld` apart: normed rows, in 8-bit layers what their blocks stand for in bf16
     void *rows_out;      // where the first kernel leaves them, or null (they are x)
     int64_t ld;
-    float *h;  // (T k, ldh): the gated unit's results, a row per (expert, token) in this order
+    float *h;  // (T k, ldh): the gated unit's results, a row per (expert, token) in this order; bf16: eight columns at a time as eight
+               // high and eight low halves (Halves)
     int64_t ldh;
+    uint32_t *widest;  // 8-bit layers: (T k, blocks of 128) largest finite magnitudes of h, as bits
+    uint32_t *claimed, *done;  // a word per workgroup of the second kernel
+    uint32_t *zeros;           // what the first kernel clears of all these, and how many words
+    int zero_words;
 };
 
 // ---- first kernel: stream, norm, logits -----------------------------------------------------------------------------------
-// A workgroup has two experts and all tokens.  It norms the tokens itself (the rows are read once more per workgroup, from the
-// caches), so that nothing has to wait for another workgroup; token t is written by workgroup t.
-constexpr int kRouterExperts = 2;
-
-template <typename T, int TOKENS, bool FP8, bool WHOLE>
+// A workgroup has a token and EXPERTS experts.  It norms the token itself (the row is read once more per workgroup, from the
+// caches), so that nothing has to wait for another workgroup; the first one of a token writes its rows.  ONE: a row is one run of
+// eight elements a thread, and stays in registers.
+template <typename T, int EXPERTS, bool FP8, bool WHOLE, bool ONE>
 __global__ __launch_bounds__(256) void layer_router_kernel(Layer p) {
-    constexpr int SUMS = kRouterExperts * TOKENS;
-    __shared__ double root[TOKENS];
-    __shared__ double part[4][SUMS];
+    __shared__ double squares[4];
+    __shared__ double part[4][EXPERTS];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int H = p.c.H, E = p.c.E, tokens = (int)p.c.T;
-    const bool norm = p.c.norm_weight != nullptr;
-    const T *const x = (const T *)p.c.x, *const residual = (const T *)p.c.residual, *const weight = (const T *)p.c.norm_weight;
-    const int e0 = blockIdx.x * kRouterExperts;
-    const T *router[kRouterExperts];
-#pragma unroll
-    for (int j = 0; j < kRouterExperts; ++j) router[j] = (const T *)p.c.router + (int64_t)(e0 + j < E ? e0 + j : E - 1) * H;
+    const int H = p.c.H, E = p.c.E, t = blockIdx.y, e0 = blockIdx.x * EXPERTS;
+    const bool norm = p.c.norm_weight != nullptr, writes = blockIdx.x == 0;
+    const T *const x = (const T *)p.c.x + (int64_t)t * H;
+    const T *const residual = p.c.residual != nullptr ? (const T *)p.c.residual + (int64_t)t * H : nullptr;
+    for (int i = (blockIdx.y * gridDim.x + blockIdx.x) * 256 + tid; i < p.zero_words; i += gridDim.x * gridDim.y * 256) p.zeros[i] = 0u;
 
-    auto stream_of = [&](int t, int k) {
+    auto stream_of = [&](int k) {
         Eight<T, WHOLE> v;
-        v.load(x + (int64_t)t * H, k, H);
+        v.load(x, k, H);
         if (residual != nullptr) {
             Eight<T, WHOLE> o;
-            o.load(residual + (int64_t)t * H, k, H);
+            o.load(residual, k, H);
             add_rounded(v, o);
         }
         return v;
     };
+    Eight<T, WHOLE> w, r[EXPERTS], s;
+    auto load_weights = [&](int k) {
+        if (norm) w.load((const T *)p.c.norm_weight, k, H);
+#pragma unroll
+        for (int j = 0; j < EXPERTS; ++j) r[j].load((const T *)p.c.router + (int64_t)(e0 + j < E ? e0 + j : E - 1) * H, k, H);
+    };
+    if (ONE) s = stream_of(tid * 8), load_weights(tid * 8);
+    double length = 0.0;
     if (norm) {
-        for (int t = wave; t < tokens; t += 4) {
-            double sum = 0.0;
-            for (int k = lane * 8; k < H; k += 512) sum = sum_of_squares(stream_of(t, k), sum);
-            sum = wave_sum(sum);
-            if (lane == 0) root[t] = inverse_root(sum / (double)H + (double)p.c.eps);
-        }
+        double sum = 0.0;
+        if (ONE) sum = sum_of_squares(s, sum);
+        else
+            for (int k = tid * 8; k < H; k += 2048) sum = sum_of_squares(stream_of(k), sum);
+        sum = wave_sum(sum);
+        if (lane == 0) squares[wave] = sum;
         __syncthreads();
+        length = inverse_root((squares[0] + squares[1] + squares[2] + squares[3]) / (double)H + (double)p.c.eps);
     }
-    double acc[kRouterExperts][TOKENS];
+    double acc[EXPERTS];
 #pragma unroll
-    for (int j = 0; j < kRouterExperts; ++j)
-#pragma unroll
-        for (int t = 0; t < TOKENS; ++t) acc[j][t] = 0.0;
+    for (int j = 0; j < EXPERTS; ++j) acc[j] = 0.0;
     const int padded = FP8 ? (int)fp8_ld(H) : H;  // (8-bit: whole blocks of 128, the same for the 16 lanes of a block)
     for (int k = tid * 8; k < padded; k += 2048) {
-        Eight<T, WHOLE> w, r[kRouterExperts];
-        if (norm) w.load(weight, k, H);
+        if (!ONE) s = stream_of(k), load_weights(k);
+        Eight<T, WHOLE> v = s;
+        if (norm) {
+            if (writes && p.stream_out != nullptr) s.store((T *)p.stream_out + (int64_t)t * H, k, H);
 #pragma unroll
-        for (int j = 0; j < kRouterExperts; ++j) r[j].load(router[j], k, H);
+            for (int i = 0; i < 8; ++i) v.v[i] = normed(s.v[i], length, w.v[i]);
+        }
+        if (writes && p.rows_out != nullptr) {
+            if constexpr (FP8) {
+                float f[8];
 #pragma unroll
-        for (int t = 0; t < TOKENS; ++t) {
-            Eight<T, WHOLE> v = stream_of(t < tokens ? t : tokens - 1, k);
-            const bool mine = t < tokens && t % gridDim.x == blockIdx.x;
-            if (norm) {
-                if (mine && p.stream_out != nullptr) v.store((T *)p.stream_out + (int64_t)t * H, k, H);
-                const double length = root[t < tokens ? t : tokens - 1];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v.v[i] = normed(v.v[i], length, w.v[i]);
+                for (int i = 0; i < 8; ++i) f[i] = k + i < H ? to_f32(v.v[i]) : 0.0f;
+                fp8_store_wide(f, (bf16_t *)p.rows_out + t * p.ld + k);
+            } else {
+                v.store((T *)p.rows_out + t * p.ld, k, H);
             }
-            if (mine && p.rows_out != nullptr) {
-                if constexpr (FP8) {
-                    float f[8];
+        }
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) f[i] = k + i < H ? to_f32(v.v[i]) : 0.0f;
-                    fp8_store_wide(f, (bf16_t *)p.rows_out + t * p.ld + k);
-                } else {
-                    v.store((T *)p.rows_out + t * p.ld, k, H);
-                }
-            }
+        for (int i = 0; i < 8; ++i) {
+            const double a = (double)to_f32(v.v[i]);
 #pragma unroll
-            for (int j = 0; j < kRouterExperts; ++j)
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    // (behind column H the stream, the weight and the router are zeros; a NaN of the token's stays its own)
-                    acc[j][t] = __builtin_fma((double)to_f32(v.v[i]), (double)to_f32(r[j].v[i]), acc[j][t]);
+            for (int j = 0; j < EXPERTS; ++j)
+                // (behind column H the stream, the weight and the router are zeros)
+                acc[j] = __builtin_fma(a, (double)to_f32(r[j].v[i]), acc[j]);
         }
     }
+    // every step halves the sums that a lane holds: EXPERTS - 1 exchanges and one a step for the rest
+    int step = 32, mine = 0;
 #pragma unroll
-    for (int j = 0; j < kRouterExperts; ++j)
+    for (int half = EXPERTS / 2; half; half /= 2, step /= 2) {
+        const bool upper = lane & step;
+        if (upper) mine += half;
 #pragma unroll
-        for (int t = 0; t < TOKENS; ++t) {
-            const double sum = wave_sum(acc[j][t]);
-            if (lane == 0) part[wave][j * TOKENS + t] = sum;
+        for (int j = 0; j < half; ++j) {
+            const double keep = upper ? acc[j + half] : acc[j], give = upper ? acc[j] : acc[j + half];
+            acc[j] = keep + __shfl_xor(give, step);
         }
+    }
+    const int last = step;
+    for (; step; step /= 2) acc[0] += __shfl_xor(acc[0], step);
+    if ((lane & (2 * last - 1)) == 0) part[wave][mine] = acc[0];
     __syncthreads();
-    if (tid < SUMS) {
-        const int e = e0 + tid / TOKENS, t = tid % TOKENS;
-        if (e < E && t < tokens)
-            ((T *)p.logits)[(int64_t)t * E + e] = from_f32<T>((float)(part[0][tid] + part[1][tid] + part[2][tid] + part[3][tid]));
-    }
+    if (tid < EXPERTS && e0 + tid < E)
+        ((T *)p.logits)[(int64_t)t * E + e0 + tid] = from_f32<T>((float)(part[0][tid] + part[1][tid] + part[2][tid] + part[3][tid]));
 }
 
 // ---- routing, found by every workgroup of the other kernels from the logits -----------------------------------------------
@@ -156,10 +163,13 @@ __device__ __forceinline__ void choose(const T *logits, int t, int E, int k, int
     int key[PER_LANE];  // the order of the values as whole numbers (-0 as 0)
     int top = kNone;
     bool nan = false;
+    T raw[PER_LANE];
+#pragma unroll
+    for (int i = 0; i < PER_LANE; ++i) raw[i] = logits[(int64_t)t * E + (lane + 64 * i < E ? lane + 64 * i : E - 1)];  // (in flight together)
 #pragma unroll
     for (int i = 0; i < PER_LANE; ++i) {
         const int e = lane + 64 * i;
-        v[i] = e < E ? to_f32(logits[(int64_t)t * E + e]) + 0.0f : -INFINITY;
+        v[i] = e < E ? to_f32(raw[i]) + 0.0f : -INFINITY;
         nan |= v[i] != v[i];
         const int bits = __float_as_int(v[i]);
         key[i] = e < E ? bits ^ ((bits >> 31) & 0x7fffffff) : kNone;
@@ -219,7 +229,6 @@ __device__ __forceinline__ void find_routing(const Layer &p, Routing &r) {
     for (int t = wave; t < tokens; t += kWaves) {
         const T *const logits = (const T *)p.logits;
         if (E <= 128) choose<T, 2>(logits, t, E, k, p.c.renorm, r, lane);
-        else if (E <= 256) choose<T, 4>(logits, t, E, k, p.c.renorm, r, lane);
         else choose<T, 16>(logits, t, E, k, p.c.renorm, r, lane);
     }
     __syncthreads();
@@ -261,21 +270,40 @@ struct Weights {
     static constexpr int kRun = 16 / (int)sizeof(Element), kStep = 4 * kRun;
 };
 
-// `count` (a constant) elements of a row from k on; zeros from column K on.  WHOLE: K is a multiple of count.
-template <bool WHOLE, int BYTES, typename E>
-__device__ __forceinline__ void load_run(const E *row, int k, int K, void *to) {
-    constexpr int count = BYTES / (int)sizeof(E);
-    if (WHOLE ? k < K : k + count <= K) {
-        __builtin_memcpy(to, row + k, BYTES);
-    } else {
-#pragma unroll
-        for (int i = 0; i < count; ++i) ((E *)to)[i] = !WHOLE && k + i < K ? row[k + i] : (E)0;
-    }
-}
-
 struct alignas(16) Run {
-    uint4_t v;
+    uint64_t v[2];
 };
+
+// 16 bytes of a row from element k on, zeros from element K on; WHOLE: K is a multiple of what they hold.  Without branches: what lies
+// behind the row's end is loaded from `safe`, or moved down from the row's last 16 bytes.
+template <bool WHOLE, typename E>
+__device__ __forceinline__ Run load_run(const E *row, int k, int K, const E *safe) {
+    constexpr int count = 16 / (int)sizeof(E);
+    Run run;
+    if (WHOLE) {
+        const bool in = k < K;
+        __builtin_memcpy(&run, in ? row + k : safe, 16);
+        run.v[0] = in ? run.v[0] : 0u;
+        run.v[1] = in ? run.v[1] : 0u;
+    } else if (K >= count) {
+        const int at = k + count <= K ? k : K - count, moved = (k - at) * 8 * (int)sizeof(E);
+        __builtin_memcpy(&run, row + at, 16);
+        const uint64_t lo = run.v[0], hi = run.v[1];
+        run.v[0] = moved == 0 ? lo : moved < 64 ? lo >> moved | hi << (64 - moved) : moved < 128 ? hi >> (moved - 64) : 0u;
+        run.v[1] = moved < 64 ? hi >> moved : 0u;
+    } else {
+        run.v[0] = run.v[1] = 0u;
+#pragma unroll 1
+        for (int i = 0; i < count && k + i < K; ++i) {
+            uint64_t bits = 0u;
+            __builtin_memcpy(&bits, row + k + i, sizeof(E));
+            const int at = i * 8 * (int)sizeof(E);
+            if (at < 64) run.v[0] |= bits << at;
+            else run.v[1] |= bits << (at - 64);
+        }
+    }
+    return run;
+}
 
 __device__ __forceinline__ floatx4 mfma_f32(const float (&a)[4], const float (&b)[4], floatx4 acc) {
 #pragma unroll
@@ -283,6 +311,22 @@ __device__ __forceinline__ floatx4 mfma_f32(const float (&a)[4], const float (&b
     return acc;
 }
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+
+// bf16 layers keep a value h of the gated unit as two bf16 ones, h as rounded and what that leaves, as rounded: 2^-17 of it is lost at
+// most, where the output's own rounding is 2^-9.  fp16 weights are widened for h in 32 bits (it need not fit the type), and in 8-bit
+// layers h is quantised where it is read, by which time its blocks' largest magnitudes are known.
+template <typename T, bool FP8>
+constexpr bool kHalves = std::is_same<T, bf16_t>::value && !FP8;
+
+// What workgroups hand to one another within a kernel goes past the L2s of the XCDs, both ways: stores and loads of the device's
+// scope.  (Ordinary ones with a fence before the word that says so write back and invalidate a whole L2 for every wave: 120 us.)
+__device__ __forceinline__ void publish(void *to, uint64_t v) {
+    __hip_atomic_store((uint64_t *)to, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ uint32_t peek(const uint32_t *word) {
+    return __hip_atomic_load(word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+constexpr int kDeviceScope = 16;  // the load's sc1 bit
 
 // ---- gate and up --------------------------------------------------------------------------------------------------------------
 // An item is an expert's eight columns of either matrix, side by side as the 16 rows of one tile, times the expert's tokens as its
@@ -317,22 +361,16 @@ __device__ __forceinline__ void gate_up_item(const Layer &p, const Routing &r, i
     }
     floatx4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int s0 = begin; s0 < end; s0 += U) {
-        Run a[U];
-        struct alignas(16) {
-            X v[kRun];
-        } b[U];
+        Run a[U], b[U][kRowBytes / 16];
         float block_scale[U / 2];
 #pragma unroll
-        for (int u = 0; u < U; ++u) load_run<WHOLE, 16>(w, s0 + u < end ? (s0 + u) * kStep + g * kRun : H, H, &a[u]);
+        for (int u = 0; u < U; ++u) a[u] = load_run<WHOLE>(w, s0 + u < end ? (s0 + u) * kStep + g * kRun : H, H, w);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int k = s0 + u < end ? (s0 + u) * kStep + g * kRun : H;
-            if (FP8) {  // (rows of whole blocks)
-                if (s0 + u < end) __builtin_memcpy(b[u].v, x + k, kRowBytes);
-                else __builtin_memset(b[u].v, 0, kRowBytes);
-            } else {
-                load_run<WHOLE, kRowBytes>(x, k, H, b[u].v);
-            }
+            // (8-bit layers: rows of whole blocks, zeros behind column H)
+            if constexpr (FP8) __builtin_memcpy(b[u], s0 + u < end ? x + k : x, kRowBytes);
+            else b[u][0] = load_run<WHOLE>(x, k, H, x);
         }
         if (FP8) {
 #pragma unroll
@@ -351,7 +389,7 @@ __device__ __forceinline__ void gate_up_item(const Layer &p, const Routing &r, i
 #pragma unroll
                     for (int o = 0; o < 2; ++o) {
                         bf16x8 bv;
-                        __builtin_memcpy(&bv, b[2 * u + q].v + 8 * o, 16);
+                        __builtin_memcpy(&bv, &b[2 * u + q][o], 16);
                         sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp8_widen(f.t[o], 1.0f), bv, sum, 0, 0, 0);
                     }
                 }
@@ -396,7 +434,30 @@ __device__ __forceinline__ void gate_up_item(const Layer &p, const Routing &r, i
             const float h = acc[i] * sigmoid_f32(acc[i]) * up[i];
             acc[i] = tile * 8 + 4 * g + i < I ? h : 0.0f;
         }
-        *(floatx4 *)(p.h + (int64_t)(first + n) * p.ldh + tile * 8 + 4 * g) = acc;
+        float *const to = p.h + (int64_t)(first + n) * p.ldh + tile * 8;
+        if constexpr (kHalves<T, FP8>) {
+            bf16x4 high, low;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                high[i] = (bf16_t)acc[i];
+                low[i] = (bf16_t)(acc[i] - (float)high[i]);
+            }
+            publish((bf16_t *)to + 4 * g, __builtin_bit_cast(uint64_t, high));
+            publish((bf16_t *)to + 8 + 4 * g, __builtin_bit_cast(uint64_t, low));
+        } else {
+            publish(to + 4 * g, __builtin_bit_cast(uint64_t, floatx2{acc[0], acc[1]}));
+            publish(to + 4 * g + 2, __builtin_bit_cast(uint64_t, floatx2{acc[2], acc[3]}));
+        }
+    }
+    if constexpr (FP8) {
+        // the blocks' largest magnitudes: their order is that of the bits, and whoever comes last, the result is the same
+        uint32_t top = 0u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fp8_wider(top, fp8_finite_abs(acc[i]));
+        const uint32_t other = (uint32_t)__shfl_xor((int)top, 16);
+        if (g == 0 && n < rows)
+            __hip_atomic_fetch_max(p.widest + (int64_t)(first + n) * nb + tile * 8 / kFp8Block, top > other ? top : other, __ATOMIC_RELAXED,
+                                   __HIP_MEMORY_SCOPE_AGENT);
     }
 }
 
@@ -407,180 +468,226 @@ __device__ __forceinline__ void gate_up_item(const Layer &p, const Routing &r, i
 // the matrix unit's work are for nothing, but it has a thirtieth of its time to do.)
 typedef float Sums[kWaves][kTokens][4];
 
+// A chunk of an expert's weights for an item: U steps of the lane's row and part.
+template <typename T, bool FP8>
+struct Chunk {
+    static constexpr int U = FP8 ? 4 : 6;
+    Run a[U];
+    float scale[U / 2];
+};
+
 template <typename T, bool FP8, bool WHOLE>
-__device__ __forceinline__ void down_item(const Layer &p, const Routing &r, int tile, float (*sums)[kTokens][4]) {
+struct Down {
     typedef Weights<T, FP8> W;
     typedef typename W::Element Element;
-    constexpr int kRun = W::kRun, kStep = W::kStep;
-    constexpr int U = FP8 ? 4 : 6;
-    constexpr int kUnit = FP8 ? kFp8Block : kRun;
-    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int H = p.c.H, I = p.c.I;
-    const int length = ((I + 3) / 4 + kUnit - 1) / kUnit * kUnit;  // of a part
-    const int steps = (length + kStep - 1) / kStep;
-    const int row = tile * 4 + (n >> 2), from = (n & 3) * length;
-    const int left = I - from < length ? (I - from < 0 ? 0 : I - from) : length;  // of the lane's part, both as row and as column
-    const int nb = fp8_blocks(H), kb = fp8_blocks(I);
-    sums[wave][lane >> 2][lane & 3] = 0.0f;  // (a wave's own: its LDS operations keep their order)
-    const int experts = r.experts;
-    for (int at = wave; at < experts; at += kWaves) {
-        const int e = __builtin_amdgcn_readfirstlane(r.expert[at]);
-        const int first = __builtin_amdgcn_readfirstlane(r.first[at]);
-        const int rows = __builtin_amdgcn_readfirstlane(r.first[at + 1]) - first;
-        const Element *const w = (const Element *)p.c.w_down + ((int64_t)e * H + (row < H ? row : H - 1)) * I + from;
-        const float *const scale = FP8 ? p.c.s_down + ((int64_t)e * nb + tile * 4 / kFp8Block) * kb : nullptr;
-        floatx4 acc[4];
-        float total[4];
+    static constexpr int kRun = W::kRun, kStep = W::kStep, U = Chunk<T, FP8>::U;
+    static constexpr int kUnit = FP8 ? kFp8Block : kRun;
+    const Layer &p;
+    const Routing &r;
+    const int lane, n, g, wave, length, steps, from, left, nb, kb;
+    const uint32_t h_bytes;
+    const __amdgpu_buffer_rsrc_t h;
+
+    __device__ __forceinline__ Down(const Layer &p, const Routing &r)
+        : p(p), r(r), lane(threadIdx.x & 63), n(lane & 15), g(lane >> 4), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)),
+          length(((p.c.I + 3) / 4 + kUnit - 1) / kUnit * kUnit),  // of a part
+          steps((length + kStep - 1) / kStep), from((n & 3) * length),
+          // (of the lane's part, as a row of the weights and as a column of the rows)
+          left(p.c.I - from < length ? (p.c.I - from < 0 ? 0 : p.c.I - from) : length), nb(fp8_blocks(p.c.H)), kb(fp8_blocks(p.c.I)),
+          h_bytes((uint32_t)(p.c.T * p.c.k * p.ldh * 4)), h(__builtin_amdgcn_make_buffer_rsrc(p.h, 0, (int)h_bytes, 0x00020000)) {}
+
+    __device__ __forceinline__ void load(Chunk<T, FP8> &c, int tile, int at, int s0) const {
+        const int row = tile * 4 + (n >> 2), H = p.c.H, e = __builtin_amdgcn_readfirstlane(r.expert[at]);
+        const Element *const w = (const Element *)p.c.w_down + ((int64_t)e * H + (row < H ? row : H - 1)) * p.c.I;
+        // (the lane's part ends where the next begins, or with the row: a run that the row's end cuts is the last one of all)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) acc[q] = floatx4{0.0f, 0.0f, 0.0f, 0.0f}, total[q] = 0.0f;
-        for (int s0 = 0; s0 < steps; s0 += U) {
-            Run a[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) load_run<WHOLE, 16>(w, s0 + u < steps ? (s0 + u) * kStep + g * kRun : left, left, &a[u]);
-            float block_scale[U];
-            if (FP8) {
-#pragma unroll
-                for (int u = 0; u < U / 2; ++u) {
-                    const int b = from / kFp8Block + s0 / 2 + u;
-                    block_scale[u] = (s0 + 2 * u) * kStep < left ? scale[b] : 0.0f;
-                }
-            }
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                if (q * 4 >= rows) break;
-                const int mine = q * 4 + (n >> 2);
-                const float *const h = p.h + (int64_t)(first + (mine < rows ? mine : rows - 1)) * p.ldh + from;
-#pragma unroll
-                for (int u0 = 0; u0 < U; u0 += 2) {
-                    if (s0 + u0 >= steps) break;
-                    struct alignas(16) {
-                        float v[kRun];
-                    } b[2];
-#pragma unroll
-                    for (int o = 0; o < 2; ++o) {
-                        // (rows of h are whole runs long, zeros behind column I)
-                        const int k = (s0 + u0 + o) * kStep + g * kRun;
-                        if (s0 + u0 + o < steps && k < left) __builtin_memcpy(b[o].v, h + k, sizeof(b[o].v));
-                        else __builtin_memset(b[o].v, 0, sizeof(b[o].v));
-                    }
-                    if constexpr (FP8) {
-                        // the block's 128 values: 32 here, the others in the other quarters of the wave
-                        uint32_t top = 0u;
-#pragma unroll
-                        for (int o = 0; o < 2; ++o)
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) top = fp8_wider(top, b[o].v[i]);
-                        top = fp8_over_quarters(top);
-                        if (__builtin_expect(__any(fp8_unusual(top)), 0)) {
-                            top = 0u;
-#pragma unroll
-                            for (int o = 0; o < 2; ++o)
-#pragma unroll
-                                for (int i = 0; i < 16; ++i) top = fp8_wider(top, fp8_finite_abs(b[o].v[i])), b[o].v[i] = fp8_finite(b[o].v[i]);
-                            top = fp8_over_quarters(top);
-                        }
-                        const int byte = fp8_scale_byte(top);
-                        const float inverse = fp8_inverse_of(byte), back = fp8_scale_of(byte);
-                        floatx4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                        for (int o = 0; o < 2; ++o) {
-                            union {
-                                Run r;
-                                intx2 t[2];
-                            } f = {a[u0 + o]};
-#pragma unroll
-                            for (int z = 0; z < 2; ++z) {
-                                const float *const c = b[o].v + 8 * z;
-                                const intx2 packed = {(int)fp8_pack4(c[0], c[1], c[2], c[3], inverse), (int)fp8_pack4(c[4], c[5], c[6], c[7], inverse)};
-                                sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp8_widen(f.t[z], 1.0f), fp8_widen(packed, back), sum, 0, 0, 0);
-                            }
-                        }
-                        const float lo = n & 1 ? sum[1] : sum[0], hi = n & 1 ? sum[3] : sum[2];
-                        total[q] = __builtin_fmaf(block_scale[u0 / 2], n & 2 ? hi : lo, total[q]);
-                    } else {
-#pragma unroll
-                        for (int o = 0; o < 2; ++o) {
-                            if constexpr (std::is_same<T, bf16_t>::value) {
-                                // the fp32 value as the sum of two bf16 ones: 2^-17 of it is lost at most, the output's own rounding is 2^-9
-                                bf16x8 av, high, low;
-                                __builtin_memcpy(&av, &a[u0 + o], 16);
-#pragma unroll
-                                for (int i = 0; i < 8; ++i) {
-                                    high[i] = (bf16_t)b[o].v[i];
-                                    low[i] = (bf16_t)(b[o].v[i] - (float)high[i]);
-                                }
-                                acc[q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, low, acc[q], 0, 0, 0);
-                                acc[q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, high, acc[q], 0, 0, 0);
-                            } else {
-                                // (fp16: widened, since the unit's values need not fit the type)
-                                T narrow[kRun];
-                                __builtin_memcpy(narrow, &a[u0 + o], 16);
-#pragma unroll
-                                for (int z = 0; z < kRun; z += 4) {
-                                    const float av[4] = {to_f32(narrow[z]), to_f32(narrow[z + 1]), to_f32(narrow[z + 2]), to_f32(narrow[z + 3])};
-                                    const float bv[4] = {b[o].v[z], b[o].v[z + 1], b[o].v[z + 2], b[o].v[z + 3]};
-                                    acc[q] = mfma_f32(av, bv, acc[q]);
-                                }
-                            }
-                        }
-                    }
-                }
-            }
+        for (int u = 0; u < U; ++u) {
+            const int k = (s0 + u) * kStep + g * kRun;
+            c.a[u] = load_run<WHOLE>(w, s0 + u < steps && k < length ? from + k : p.c.I, p.c.I, w);
         }
-        // lane (n, g): column g's sum of part i for the token and part of n, in acc[.][i]
+        if (FP8) {
+            const float *const scale = p.c.s_down + ((int64_t)e * nb + tile * 4 / kFp8Block) * kb;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            if (q * 4 >= rows) break;
-            if (!FP8) {
-                const float lo = n & 1 ? acc[q][1] : acc[q][0], hi = n & 1 ? acc[q][3] : acc[q][2];
-                total[q] = n & 2 ? hi : lo;
-            }
-            float v = total[q];
-            v += __shfl_xor(v, 1);
-            v += __shfl_xor(v, 2);
-            const int mine = q * 4 + (n >> 2);
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            if ((n & 3) == 0 && mine < rows) sums[wave][r.token[first + mine]][g] += r.weight[first + mine] * v;
+            for (int u = 0; u < U / 2; ++u) c.scale[u] = (s0 + 2 * u) * kStep < left ? scale[from / kFp8Block + s0 / 2 + u] : 0.0f;
         }
     }
+
+    // acc += the chunk times the lane's row of h (8-bit: total, block by block)
+    __device__ __forceinline__ void multiply(const Chunk<T, FP8> &c, int s0, int pair, floatx4 &acc, float &total) const {
+        struct alignas(16) {
+            float v[kRun];
+        } b[U];
+        uint32_t top[U / 2];
+        // (rows of h are whole runs long, zeros behind column I; behind the last row the loads return zeros)
+        const uint32_t row = (uint32_t)pair * (uint32_t)p.ldh * 4u;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k = (s0 + u) * kStep + g * kRun;
+            const uint32_t at = s0 + u < steps && k < left ? row + (uint32_t)(from + k) * 4u : h_bytes;
+#pragma unroll
+            for (int i = 0; i < kRun; i += 4) {
+                const auto v = __builtin_amdgcn_raw_buffer_load_b128(h, (int)at, i * 4, kDeviceScope);
+                __builtin_memcpy(b[u].v + i, &v, 16);
+            }
+        }
+        if (FP8) {
+            const uint32_t *const widest = p.widest + (int64_t)pair * kb + from / kFp8Block;
+#pragma unroll
+            for (int u = 0; u < U / 2; ++u) top[u] = (s0 + 2 * u) * kStep < left ? peek(widest + s0 / 2 + u) : 0u;
+        }
+        if constexpr (FP8) {
+#pragma unroll
+            for (int u = 0; u < U / 2; ++u) {
+                const float scale = fp8_scale_of(fp8_scale_byte(top[u]));
+                floatx4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int o = 0; o < 2; ++o) {
+                    union {
+                        Run r;
+                        intx2 t[2];
+                    } f = {c.a[2 * u + o]};
+#pragma unroll
+                    for (int z = 0; z < 2; ++z)
+                        sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp8_widen(f.t[z], 1.0f), fp8_rounded(b[2 * u + o].v + 8 * z, scale), sum, 0, 0, 0);
+                }
+                const float lo = n & 1 ? sum[1] : sum[0], hi = n & 1 ? sum[3] : sum[2];
+                total = __builtin_fmaf(c.scale[u], n & 2 ? hi : lo, total);
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if constexpr (kHalves<T, FP8>) {
+                    bf16x8 av, high, low;
+                    __builtin_memcpy(&av, &c.a[u], 16);
+                    __builtin_memcpy(&high, b[u].v, 16);
+                    __builtin_memcpy(&low, b[u].v + 4, 16);
+                    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, low, acc, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, high, acc, 0, 0, 0);
+                } else {
+                    T narrow[kRun];
+                    __builtin_memcpy(narrow, &c.a[u], 16);
+#pragma unroll
+                    for (int z = 0; z < kRun; z += 4) {
+                        const float av[4] = {to_f32(narrow[z]), to_f32(narrow[z + 1]), to_f32(narrow[z + 2]), to_f32(narrow[z + 3])};
+                        const float bv[4] = {b[u].v[z], b[u].v[z + 1], b[u].v[z + 2], b[u].v[z + 3]};
+                        acc = mfma_f32(av, bv, acc);
+                    }
+                }
+            }
+        }
+    }
+
+    // `c`: the wave's first chunk of the item, loaded already where it has one
+    __device__ __forceinline__ void item(Chunk<T, FP8> &c, int tile, float (*sums)[kTokens][4]) const {
+        sums[wave][lane >> 2][lane & 3] = 0.0f;  // (a wave's own: its LDS operations keep their order)
+        const int experts = r.experts;
+        for (int at = wave; at < experts; at += kWaves) {
+            const int first = __builtin_amdgcn_readfirstlane(r.first[at]);
+            const int rows = __builtin_amdgcn_readfirstlane(r.first[at + 1]) - first;
+            // four tokens at a time (hardly any expert has more: its weights are read again then, from the caches)
+            for (int q = 0; q < rows; q += 4) {
+                const int mine = q + (n >> 2), pair = first + (mine < rows ? mine : rows - 1);
+                floatx4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+                float total = 0.0f;
+                for (int s0 = 0; s0 < steps; s0 += U) {
+                    if (at != wave || q != 0 || s0 != 0) load(c, tile, at, s0);
+                    multiply(c, s0, pair, acc, total);
+                }
+                // lane (n, g): column g's sum of part i for the token and part of n, in acc[i]
+                if (!FP8) {
+                    const float lo = n & 1 ? acc[1] : acc[0], hi = n & 1 ? acc[3] : acc[2];
+                    total = n & 2 ? hi : lo;
+                }
+                total += __shfl_xor(total, 1);
+                total += __shfl_xor(total, 2);
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                if ((n & 3) == 0 && mine < rows) sums[wave][r.token[first + mine]][g] += r.weight[first + mine] * total;
+            }
+        }
+        __syncthreads();
+        const int t = threadIdx.x >> 2, col = tile * 4 + (threadIdx.x & 3);
+        if (t < (int)p.c.T && col < p.c.H) {
+            float v = 0.0f;
+#pragma unroll
+            for (int u = 0; u < kWaves; ++u) v += sums[u][t][threadIdx.x & 3];
+            if (p.stream != nullptr) v += to_f32(((const T *)p.stream)[(int64_t)t * p.c.H + col]);
+            if (r.lost >> t & 1u) v = __builtin_nanf("");
+            ((T *)p.out)[(int64_t)t * p.c.H + col] = from_f32<T>(v);
+        }
+    }
+};
+
+// ---- second kernel: both, with one meeting of all workgroups between them -------------------------------------------------------
+// The gated unit's items are dealt out in as many units as there are workgroups: unit b is items b, b + G, ...  A workgroup claims its
+// own unit; before it waits for anything it looks whether there is a unit that nobody has claimed (a workgroup that has not started
+// yet) and does it in the other's place.  So a workgroup waits only for units that running workgroups have claimed, and these wait for
+// nothing before their units are done: every wait ends, however many of the workgroups are there at once.
+template <typename T, bool FP8, bool WHOLE>
+__global__ __launch_bounds__(kThreads, 4) void layer_experts_kernel(Layer p) {
+    __shared__ Routing r;
+    __shared__ union {
+        Parts part;
+        Sums sums[2];
+    } room;
+    __shared__ int unit_found;
+    const int tid = threadIdx.x;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // (asked for before the routing is known: the answer is there by then)
+    uint32_t taken = 0u;
+    if (tid == 0) taken = __hip_atomic_exchange(p.claimed + blockIdx.x, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    find_routing<T>(p, r);
+    const int tiles = (int)(p.ldh / 8), items = r.experts * tiles, G = (int)gridDim.x;
+    const int units = items < G ? items : G;
+    int unit = (int)blockIdx.x, turn = 0;
+    if (tid == 0) unit_found = taken ? -1 : unit;
     __syncthreads();
-    const int t = threadIdx.x >> 2, c = tile * 4 + (threadIdx.x & 3);
-    if (t < (int)p.c.T && c < H) {
-        float v = 0.0f;
-#pragma unroll
-        for (int u = 0; u < kWaves; ++u) v += sums[u][t][threadIdx.x & 3];
-        if (p.stream != nullptr) v += to_f32(((const T *)p.stream)[(int64_t)t * H + c]);
-        if (r.lost >> t & 1u) v = __builtin_nanf("");
-        ((T *)p.out)[(int64_t)t * H + c] = from_f32<T>(v);
+    unit = unit_found < units ? unit_found : -1;
+    for (bool own = true;; own = false) {
+        if (!own) {
+            int free = 0x7fffffff;
+            for (int b = tid; b < units; b += kThreads)
+                if (peek(p.claimed + b) == 0u && b < free) free = b;
+            if (!__syncthreads_or(free != 0x7fffffff)) break;
+            if (tid == 0) unit_found = -1;
+            __syncthreads();
+            if (free != 0x7fffffff) atomicMax(&unit_found, free);  // (any of them)
+            __syncthreads();
+            unit = unit_found;
+            __syncthreads();
+            if (tid == 0) unit_found = __hip_atomic_exchange(p.claimed + unit, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ? -1 : unit;
+            __syncthreads();
+            unit = unit_found;
+        }
+        if (unit < 0) continue;
+        for (int i = unit; i < items; i += G, ++turn)
+            gate_up_item<T, FP8, WHOLE>(p, r, i / tiles, i % tiles, room.part[turn & 1], turn & (kWaves - 1));
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // every wave's rows of h are there, before the word that says so
+        __syncthreads();
+        if (tid == 0) __hip_atomic_store(p.done + unit, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
-}
-
-template <typename T, bool FP8, bool WHOLE>
-__global__ __launch_bounds__(kThreads, 4) void layer_gate_up_kernel(Layer p) {
-    __shared__ Routing r;
-    __shared__ Parts part;
-    find_routing<T>(p, r);
-    const int tiles = (int)(p.ldh / 8), items = r.experts * tiles;
-    int turn = 0;
-    for (int i = blockIdx.x; i < items; i += gridDim.x, ++turn)
-        gate_up_item<T, FP8, WHOLE>(p, r, i / tiles, i % tiles, part[turn & 1], turn & (kWaves - 1));
-}
-
-template <typename T, bool FP8, bool WHOLE>
-__global__ __launch_bounds__(kThreads, 4) void layer_down_kernel(Layer p) {
-    __shared__ Routing r;
-    __shared__ Sums sums[2];
-    find_routing<T>(p, r);
-    const int items = ceil_div(p.c.H, 4);
-    int turn = 0;
-    for (int i = blockIdx.x; i < items; i += gridDim.x, ++turn) down_item<T, FP8, WHOLE>(p, r, i, sums[turn & 1]);
+    const Down<T, FP8, WHOLE> down(p, r);
+    const int last = ceil_div(p.c.H, 4);
+    Chunk<T, FP8> c;
+    if ((int)blockIdx.x < last && wave < r.experts) down.load(c, blockIdx.x, wave, 0);
+    for (;;) {
+        bool all = true;
+        for (int b = tid; b < units; b += kThreads) all = all && peek(p.done + b) != 0u;
+        if (__syncthreads_and(all)) break;
+        __builtin_amdgcn_s_sleep(1);
+    }
+    turn = 0;
+    for (int i = blockIdx.x; i < last; i += G, ++turn) {
+        if (turn != 0 && wave < r.experts) down.load(c, i, wave, 0);
+        down.item(c, i, room.sums[turn & 1]);
+    }
 }
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
+int most_workgroups() { return 2 * device_info().cu_count; }
+
 struct Room {
-    size_t stream, rows, h;  // bytes
+    size_t stream, rows, h, widest, flags;  // bytes
     int64_t ld, ldh;
     explicit Room(const mfl_moe_layer &c) {
         const bool fp8 = c.s_gate != nullptr, norm = c.norm_weight != nullptr;
@@ -589,27 +696,29 @@ struct Room {
         stream = c.residual != nullptr ? up256((size_t)c.T * c.H * dtype_size(c.dtype)) : 0;
         rows = fp8 ? up256((size_t)c.T * ld * 2) : norm ? up256((size_t)c.T * ld * dtype_size(c.dtype)) : 0;
         h = up256((size_t)c.T * c.k * ldh * 4);
+        widest = fp8 ? up256((size_t)c.T * c.k * fp8_blocks(c.I) * 4) : 0;
+        flags = up256((size_t)2 * most_workgroups() * 4);
     }
+    size_t all() const { return stream + rows + h + widest + flags; }
 };
 
 template <typename T, bool FP8, bool WHOLE>
 int launch(const Layer &p, hipStream_t stream) {
     const int tokens = (int)p.c.T;
-    const unsigned routers = (unsigned)ceil_div(p.c.E, kRouterExperts);
-    const bool whole8 = p.c.H % 8 == 0;
-#define MFL_LAYER_ROUTER(N)                                                                             \
-    if (whole8) layer_router_kernel<T, N, FP8, true><<<routers, 256, 0, stream>>>(p);                    \
-    else layer_router_kernel<T, N, FP8, false><<<routers, 256, 0, stream>>>(p);
-    if (tokens == 1) { MFL_LAYER_ROUTER(1) }
-    else if (tokens <= 4) { MFL_LAYER_ROUTER(4) }
-    else if (tokens <= 8) { MFL_LAYER_ROUTER(8) }
-    else { MFL_LAYER_ROUTER(16) }
+    // (few workgroups with two experts each are done before the same with eight would be: 64 x 2 at one token of 128 experts)
+    const bool many = (int64_t)tokens * p.c.E >= 1024, whole8 = p.c.H % 8 == 0, one = p.c.H <= 2048;
+    const dim3 grid(ceil_div(p.c.E, many ? 8 : 2), tokens);
+#define MFL_LAYER_ROUTER(N)                                                                                       \
+    if (whole8 && one) layer_router_kernel<T, N, FP8, true, true><<<grid, 256, 0, stream>>>(p);                    \
+    else if (whole8) layer_router_kernel<T, N, FP8, true, false><<<grid, 256, 0, stream>>>(p);                     \
+    else layer_router_kernel<T, N, FP8, false, false><<<grid, 256, 0, stream>>>(p);
+    if (many) { MFL_LAYER_ROUTER(8) }
+    else { MFL_LAYER_ROUTER(2) }
 #undef MFL_LAYER_ROUTER
-    const int most = 2 * device_info().cu_count;
     const int hits = p.c.T * p.c.k < p.c.E ? (int)p.c.T * p.c.k : p.c.E;
-    const int64_t front = hits * (p.ldh / 8), back = ceil_div(p.c.H, 4);
-    layer_gate_up_kernel<T, FP8, WHOLE><<<(unsigned)(front < most ? front : most), kThreads, 0, stream>>>(p);
-    layer_down_kernel<T, FP8, WHOLE><<<(unsigned)(back < most ? back : most), kThreads, 0, stream>>>(p);
+    const int64_t front = hits * (p.ldh / 8), back = ceil_div(p.c.H, 4), want = front > back ? front : back;
+    const unsigned most = (unsigned)most_workgroups();
+    layer_experts_kernel<T, FP8, WHOLE><<<want < most ? (unsigned)want : most, kThreads, 0, stream>>>(p);
     return launch_status();
 }
 
@@ -626,22 +735,29 @@ int launch_type(const Layer &p, hipStream_t stream) {
 
 }  // namespace
 
-size_t moe_layer_workspace(const mfl_moe_layer &c) {
-    const Room room(c);
-    return room.stream + room.rows + room.h;
-}
+size_t moe_layer_workspace(const mfl_moe_layer &c) { return Room(c).all(); }
 
 int moe_layer_fwd(const mfl_moe_layer &c, void *out, void *logits, void *workspace, hipStream_t stream) {
     const Room room(c);
-    uint8_t *const ws = (uint8_t *)workspace;
+    uint8_t *at = (uint8_t *)workspace;
+    auto take = [&](size_t bytes) {
+        uint8_t *const here = bytes ? at : nullptr;
+        at += bytes;
+        return here;
+    };
     Layer p = {};
     p.c = c, p.out = out, p.logits = logits;
     p.ld = room.ld, p.ldh = room.ldh;
-    p.stream_out = room.stream ? ws : nullptr;
-    p.stream = c.norm_weight == nullptr ? nullptr : room.stream ? p.stream_out : c.x;
-    p.rows_out = room.rows ? ws + room.stream : nullptr;
-    p.rows = room.rows ? p.rows_out : c.x;
-    p.h = (float *)(ws + room.stream + room.rows);
+    p.stream_out = take(room.stream);
+    p.stream = c.norm_weight == nullptr ? nullptr : p.stream_out != nullptr ? p.stream_out : c.x;
+    p.rows_out = take(room.rows);
+    p.rows = p.rows_out != nullptr ? p.rows_out : c.x;
+    p.h = (float *)take(room.h);
+    p.zeros = (uint32_t *)at;
+    p.zero_words = (int)((room.widest + room.flags) / 4);
+    p.widest = (uint32_t *)take(room.widest);
+    p.claimed = (uint32_t *)take(room.flags);
+    p.done = p.claimed + most_workgroups();
     int rc = MFL_OK;
     MFL_DISPATCH_FLOAT(c.dtype, T, { rc = launch_type<T>(p, stream); });
     return rc;
