@@ -12,6 +12,7 @@ namespace {
 
 constexpr int kTokens = MFL_LAYER_TOKENS, kMaxExperts = 1024, kMaxChosen = 64;
 constexpr int kWaves = 8, kThreads = kWaves * 64;
+
 static_assert(kTokens == 16, "an expert's rows are the 16 columns of one matrix instruction");
 
 struct Layer {
@@ -26,7 +27,7 @@ struct Layer {
                // high and eight low halves (Halves)
     int64_t ldh;
     uint32_t *widest;  // 8-bit layers: (T k, blocks of 128) largest finite magnitudes of h, as bits
-    uint32_t *claimed, *done;  // a word per workgroup of the second kernel
+    uint32_t *units;   // a word per unit of the second kernel's work
     uint32_t *zeros;           // what the first kernel clears of all these, and how many words
     int zero_words;
 };
@@ -274,23 +275,18 @@ struct alignas(16) Run {
     uint64_t v[2];
 };
 
-// 16 bytes of a row from element k on, zeros from element K on; WHOLE: K is a multiple of what they hold.  Without branches: what lies
-// behind the row's end is loaded from `safe`, or moved down from the row's last 16 bytes.
+// 16 bytes of a row from element k on, zeros from element K on; WHOLE: K is a multiple of what they hold.  In two steps, so that
+// nothing is computed from what is still on its way: `fetch` loads (the row's last 16 bytes where its end cuts the run), `settle`, called
+// where the values are needed, moves them down.
 template <bool WHOLE, typename E>
-__device__ __forceinline__ Run load_run(const E *row, int k, int K, const E *safe) {
+__device__ __forceinline__ Run fetch(const E *row, int k, int K) {
     constexpr int count = 16 / (int)sizeof(E);
     Run run;
     if (WHOLE) {
-        const bool in = k < K;
-        __builtin_memcpy(&run, in ? row + k : safe, 16);
-        run.v[0] = in ? run.v[0] : 0u;
-        run.v[1] = in ? run.v[1] : 0u;
+        if (k < K) __builtin_memcpy(&run, row + k, 16);
+        else run.v[0] = run.v[1] = 0u;
     } else if (K >= count) {
-        const int at = k + count <= K ? k : K - count, moved = (k - at) * 8 * (int)sizeof(E);
-        __builtin_memcpy(&run, row + at, 16);
-        const uint64_t lo = run.v[0], hi = run.v[1];
-        run.v[0] = moved == 0 ? lo : moved < 64 ? lo >> moved | hi << (64 - moved) : moved < 128 ? hi >> (moved - 64) : 0u;
-        run.v[1] = moved < 64 ? hi >> moved : 0u;
+        __builtin_memcpy(&run, row + (k + count <= K ? k : K - count), 16);
     } else {
         run.v[0] = run.v[1] = 0u;
 #pragma unroll 1
@@ -302,6 +298,16 @@ __device__ __forceinline__ Run load_run(const E *row, int k, int K, const E *saf
             else run.v[1] |= bits << (at - 64);
         }
     }
+    return run;
+}
+template <bool WHOLE, typename E>
+__device__ __forceinline__ Run settle(Run run, int k, int K) {
+    constexpr int count = 16 / (int)sizeof(E);
+    if (WHOLE || K < count) return run;
+    const int moved = k + count <= K ? 0 : (k + count - K) * 8 * (int)sizeof(E);
+    const uint64_t lo = run.v[0], hi = run.v[1];
+    run.v[0] = moved == 0 ? lo : moved < 64 ? lo >> moved | hi << (64 - moved) : moved < 128 ? hi >> (moved - 64) : 0u;
+    run.v[1] = moved < 64 ? hi >> moved : 0u;
     return run;
 }
 
@@ -326,56 +332,76 @@ __device__ __forceinline__ void publish(void *to, uint64_t v) {
 __device__ __forceinline__ uint32_t peek(const uint32_t *word) {
     return __hip_atomic_load(word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-constexpr int kDeviceScope = 16;  // the load's sc1 bit
+
+constexpr int kDeviceScope = 16;  // a buffer load's sc1 bit
 
 // ---- gate and up --------------------------------------------------------------------------------------------------------------
 // An item is an expert's eight columns of either matrix, side by side as the 16 rows of one tile, times the expert's tokens as its
 // 16 columns; the eight waves share the reduction and meet in LDS.  Weights straight from memory into the matrix unit's registers.
+// A column is a token, whether it chose the expert or not: what a wave needs of the tokens is the same for every item, and stays in
+// registers where its share of the reduction is one chunk.  The next item's weights are asked for before the waves meet.
 typedef floatx4 Parts[2][kWaves][64];
 
 template <typename T, bool FP8, bool WHOLE>
-__device__ __forceinline__ void gate_up_item(const Layer &p, const Routing &r, int at, int tile, floatx4 (*part)[64], int finisher) {
+struct GateUp {
     typedef Weights<T, FP8> W;
     typedef typename W::Element Element;
     typedef typename std::conditional<FP8, bf16_t, T>::type X;
-    constexpr int kRun = W::kRun, kStep = W::kStep, kRowBytes = kRun * (int)sizeof(X);
-    constexpr int U = FP8 ? 4 : 8;  // steps whose loads are in flight together
-    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int H = p.c.H, I = p.c.I;
-    const int e = __builtin_amdgcn_readfirstlane(r.expert[at]);
-    const int first = __builtin_amdgcn_readfirstlane(r.first[at]);
-    const int rows = __builtin_amdgcn_readfirstlane(r.first[at + 1]) - first;
-    const int col = tile * 8 + (n & 7);
-    const Element *const w = (const Element *)(n < 8 ? p.c.w_gate : p.c.w_up) + ((int64_t)e * I + (col < I ? col : I - 1)) * H;
-    const X *const x = (const X *)p.rows + r.token[first + (n < rows ? n : rows - 1)] * p.ld;
-    // whole blocks of 128 a wave where weights have scales
-    constexpr int kUnit = FP8 ? 2 : 1;
-    const int steps = (H + kStep - 1) / kStep, share = ((steps + kWaves - 1) / kWaves + kUnit - 1) / kUnit * kUnit;
-    const int begin = wave * share, end = begin + share < steps ? begin + share : steps;
-    const int nb = fp8_blocks(I), kb = fp8_blocks(H);
-    const float *scale = nullptr;
-    if (FP8) {
-        const int64_t block = ((int64_t)e * nb + tile * 8 / kFp8Block) * kb;
-        scale = (g < 2 ? p.c.s_gate : p.c.s_up) + block;  // (of the results that the lane holds, not of the rows that it loads)
+    static constexpr int kRun = W::kRun, kStep = W::kStep, kPieces = kRun * (int)sizeof(X) / 16;
+    static constexpr int U = FP8 ? 4 : 8;      // steps of a chunk: their loads are in flight together
+    static constexpr int D = FP8 ? 4 : 2;      // items whose first chunks are
+    static constexpr int kUnit = FP8 ? 2 : 1;  // (whole blocks of 128 a wave where weights have scales)
+    const Layer &p;
+    const Routing &r;
+    const int lane, n, g, wave, tiles, begin, end, chunks;
+    struct Weight {
+        Run a[U];
+        float scale[U / 2];
+    };
+    Weight w[D];
+    Run b[U][kPieces];
+
+    static __device__ __forceinline__ int share(int H) {
+        const int steps = (H + kStep - 1) / kStep;
+        return ((steps + kWaves - 1) / kWaves + kUnit - 1) / kUnit * kUnit;
     }
-    floatx4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s0 = begin; s0 < end; s0 += U) {
-        Run a[U], b[U][kRowBytes / 16];
-        float block_scale[U / 2];
+    __device__ __forceinline__ GateUp(const Layer &p, const Routing &r)
+        : p(p), r(r), lane(threadIdx.x & 63), n(lane & 15), g(lane >> 4), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)),
+          tiles((int)(p.ldh / 8)), begin(wave * share(p.c.H)),
+          end(begin + share(p.c.H) < (p.c.H + kStep - 1) / kStep ? begin + share(p.c.H) : (p.c.H + kStep - 1) / kStep),
+          chunks((share(p.c.H) + U - 1) / U) {
+        if (chunks == 1) load_rows(begin);
+    }
+
+    // the first element of the lane's run of a step; H behind the wave's share
+    __device__ __forceinline__ int element(int step) const { return step < end ? step * kStep + g * kRun : p.c.H; }
+    __device__ __forceinline__ void load_weights(Weight &to, int item, int s0) const {
+        const int H = p.c.H, I = p.c.I, tile = item % tiles, col = tile * 8 + (n & 7);
+        const int e = __builtin_amdgcn_readfirstlane(r.expert[item / tiles]);
+        const Element *const w = (const Element *)(n < 8 ? p.c.w_gate : p.c.w_up) + ((int64_t)e * I + (col < I ? col : I - 1)) * H;
 #pragma unroll
-        for (int u = 0; u < U; ++u) a[u] = load_run<WHOLE>(w, s0 + u < end ? (s0 + u) * kStep + g * kRun : H, H, w);
+        for (int u = 0; u < U; ++u) to.a[u] = fetch<WHOLE>(w, element(s0 + u), H);
+        if (FP8) {
+            const int64_t block = ((int64_t)e * fp8_blocks(I) + tile * 8 / kFp8Block) * fp8_blocks(H);
+            // (of the results that the lane holds, not of the rows that it loads)
+            const float *const scales = (g < 2 ? p.c.s_gate : p.c.s_up) + block;
+#pragma unroll
+            for (int u = 0; u < U / 2; ++u) to.scale[u] = s0 + 2 * u < end ? scales[(s0 + 2 * u) / 2] : 0.0f;
+        }
+    }
+    __device__ __forceinline__ void load_rows(int s0) {
+        const X *const x = (const X *)p.rows + (n < (int)p.c.T ? n : (int)p.c.T - 1) * p.ld;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int k = s0 + u < end ? (s0 + u) * kStep + g * kRun : H;
             // (8-bit layers: rows of whole blocks, zeros behind column H)
-            if constexpr (FP8) __builtin_memcpy(b[u], s0 + u < end ? x + k : x, kRowBytes);
-            else b[u][0] = load_run<WHOLE>(x, k, H, x);
+            if constexpr (FP8) __builtin_memcpy(b[u], s0 + u < end ? x + (s0 + u) * kStep + g * kRun : x, sizeof(b[u]));
+            else b[u][0] = settle<WHOLE, X>(fetch<WHOLE>(x, element(s0 + u), p.c.H), element(s0 + u), p.c.H);
         }
-        if (FP8) {
+    }
+    __device__ __forceinline__ void multiply(const Weight &weight, int s0, floatx4 &acc) const {
+        Run a[U];
 #pragma unroll
-            for (int u = 0; u < U / 2; ++u) block_scale[u] = s0 + 2 * u < end ? scale[(s0 + 2 * u) / 2] : 0.0f;
-        }
+        for (int u = 0; u < U; ++u) a[u] = settle<WHOLE, Element>(weight.a[u], element(s0 + u), p.c.H);
         if constexpr (FP8) {
 #pragma unroll
             for (int u = 0; u < U / 2; ++u) {
@@ -387,91 +413,111 @@ __device__ __forceinline__ void gate_up_item(const Layer &p, const Routing &r, i
                         intx2 t[2];
                     } f = {a[2 * u + q]};
 #pragma unroll
-                    for (int o = 0; o < 2; ++o) {
-                        bf16x8 bv;
-                        __builtin_memcpy(&bv, &b[2 * u + q][o], 16);
-                        sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp8_widen(f.t[o], 1.0f), bv, sum, 0, 0, 0);
-                    }
+                    for (int o = 0; o < 2; ++o)
+                        sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp8_widen(f.t[o], 1.0f), __builtin_bit_cast(bf16x8, b[2 * u + q][o]), sum, 0, 0, 0);
                 }
-                if (s0 + 2 * u < end)
+                // (behind the wave's share the weights are zeros, and so is the scale)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(block_scale[u], sum[i], acc[i]);
+                for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(weight.scale[u], sum[i], acc[i]);
             }
         } else {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 if constexpr (std::is_same<T, bf16_t>::value) {
-                    bf16x8 av, bv;
-                    __builtin_memcpy(&av, &a[u], 16);
-                    __builtin_memcpy(&bv, &b[u], 16);
-                    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, bv, acc, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a[u]), __builtin_bit_cast(bf16x8, b[u][0]), acc, 0, 0, 0);
                 } else if constexpr (std::is_same<T, f16_t>::value) {
-                    f16x8 av, bv;
-                    __builtin_memcpy(&av, &a[u], 16);
-                    __builtin_memcpy(&bv, &b[u], 16);
-                    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, bv, acc, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a[u]), __builtin_bit_cast(f16x8, b[u][0]), acc, 0, 0, 0);
                 } else {
-                    float av[4], bv[4];
-                    __builtin_memcpy(av, &a[u], 16);
-                    __builtin_memcpy(bv, &b[u], 16);
-                    acc = mfma_f32(av, bv, acc);
+                    const floatx4 av = __builtin_bit_cast(floatx4, a[u]), bv = __builtin_bit_cast(floatx4, b[u][0]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(av[i], bv[i], acc, 0, 0, 0);
                 }
             }
         }
     }
-    part[wave][lane] = acc;
-    __syncthreads();
-    if (wave != finisher) return;
+
+    // Items from, from + by, ... below to; `turn` counts a workgroup's items.
+    __device__ __forceinline__ void run(int from, int to, int by, Parts &parts, int &turn) {
 #pragma unroll
-    for (int v = 0; v < kWaves; ++v) acc = v == 0 ? part[0][lane] : acc + part[v][lane];
+        for (int d = 0; d < D; ++d)
+            if (from + d * by < to) load_weights(w[d], from + d * by, begin);
+        for (int i = from; i < to; i += D * by) {
+#pragma unroll
+            for (int d = 0; d < D; ++d, ++turn) {
+                const int item = i + d * by;
+                if (item >= to) break;
+                floatx4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+                for (int c = 0; c < chunks; ++c) {
+                    if (c != 0) load_weights(w[d], item, begin + c * U);
+                    if (chunks != 1) load_rows(begin + c * U);
+                    multiply(w[d], begin + c * U, acc);
+                }
+                if (item + D * by < to) load_weights(w[d], item + D * by, begin);
+                floatx4(*const part)[64] = parts[turn & 1];
+                part[wave][lane] = acc;
+                __syncthreads();
+                if (wave != (turn & (kWaves - 1))) continue;
+#pragma unroll
+                for (int v = 0; v < kWaves; ++v) acc = v == 0 ? part[0][lane] : acc + part[v][lane];
+                finish(item, acc);
+            }
+        }
+    }
     // lane (token n, g): gate of columns 4 g ... where g < 2, up of columns 4 (g - 2) ... else
-    floatx4 up;
+    __device__ __forceinline__ void finish(int item, floatx4 acc) const {
+        const int tile = item % tiles, e = r.expert[item / tiles];
+        const uint32_t mask = r.mask[e];
+        const bool chosen = mask >> n & 1u;
+        const int pair = (int)(mask >> 16) + __popc(mask & ((1u << n) - 1u));
+        floatx4 up;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) up[i] = __shfl_xor(acc[i], 32);
-    if (g < 2 && n < rows) {
+        for (int i = 0; i < 4; ++i) up[i] = __shfl_xor(acc[i], 32);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float h = acc[i] * sigmoid_f32(acc[i]) * up[i];
-            acc[i] = tile * 8 + 4 * g + i < I ? h : 0.0f;
+            acc[i] = tile * 8 + 4 * g + i < p.c.I ? h : 0.0f;
         }
-        float *const to = p.h + (int64_t)(first + n) * p.ldh + tile * 8;
-        if constexpr (kHalves<T, FP8>) {
-            bf16x4 high, low;
+        if (g < 2 && chosen) {
+            float *const to = p.h + (int64_t)pair * p.ldh + tile * 8;
+            if constexpr (kHalves<T, FP8>) {
+                bf16x4 high, low;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                high[i] = (bf16_t)acc[i];
-                low[i] = (bf16_t)(acc[i] - (float)high[i]);
+                for (int i = 0; i < 4; ++i) {
+                    high[i] = (bf16_t)acc[i];
+                    low[i] = (bf16_t)(acc[i] - (float)high[i]);
+                }
+                publish((bf16_t *)to + 4 * g, __builtin_bit_cast(uint64_t, high));
+                publish((bf16_t *)to + 8 + 4 * g, __builtin_bit_cast(uint64_t, low));
+            } else {
+                publish(to + 4 * g, __builtin_bit_cast(uint64_t, floatx2{acc[0], acc[1]}));
+                publish(to + 4 * g + 2, __builtin_bit_cast(uint64_t, floatx2{acc[2], acc[3]}));
             }
-            publish((bf16_t *)to + 4 * g, __builtin_bit_cast(uint64_t, high));
-            publish((bf16_t *)to + 8 + 4 * g, __builtin_bit_cast(uint64_t, low));
-        } else {
-            publish(to + 4 * g, __builtin_bit_cast(uint64_t, floatx2{acc[0], acc[1]}));
-            publish(to + 4 * g + 2, __builtin_bit_cast(uint64_t, floatx2{acc[2], acc[3]}));
+        }
+        if constexpr (FP8) {
+            // the blocks' largest magnitudes: their order is that of the bits, and whoever comes last, the result is the same
+            uint32_t top = 0u;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = fp8_wider(top, fp8_finite_abs(acc[i]));
+            const uint32_t other = (uint32_t)__shfl_xor((int)top, 16);
+            if (g == 0 && chosen)
+                __hip_atomic_fetch_max(p.widest + (int64_t)pair * fp8_blocks(p.c.I) + tile * 8 / kFp8Block, top > other ? top : other,
+                                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
     }
-    if constexpr (FP8) {
-        // the blocks' largest magnitudes: their order is that of the bits, and whoever comes last, the result is the same
-        uint32_t top = 0u;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top = fp8_wider(top, fp8_finite_abs(acc[i]));
-        const uint32_t other = (uint32_t)__shfl_xor((int)top, 16);
-        if (g == 0 && n < rows)
-            __hip_atomic_fetch_max(p.widest + (int64_t)(first + n) * nb + tile * 8 / kFp8Block, top > other ? top : other, __ATOMIC_RELAXED,
-                                   __HIP_MEMORY_SCOPE_AGENT);
-    }
-}
+};
 
 // ---- down and sum ---------------------------------------------------------------------------------------------------------------
-// An item is four columns of the output, all chosen experts: a wave takes every eighth of them.  A tile's 16 rows are the four
-// columns' weights times four parts of the reduction, its 16 columns four tokens times the same four parts; where the parts agree
-// the result counts, and the four are added.  (With 16 columns an item there would be too few to fill the chip; three quarters of
-// the matrix unit's work are for nothing, but it has a thirtieth of its time to do.)
-typedef float Sums[kWaves][kTokens][4];
+// An item is eight columns of the output, all chosen experts: a wave takes every eighth of them.  A tile's 16 rows are the eight
+// columns' weights times two parts of the reduction, its 16 columns eight tokens times the same two parts; where the parts agree the
+// result counts, and the two are added.  (With 16 columns an item there would be too few to fill the chip; half of the matrix unit's
+// work is for nothing, but it has a thirtieth of its time to do.)
+constexpr int kParts = 2, kColumns = 16 / kParts;
+typedef float Sums[kWaves][kTokens][kColumns];
 
 // A chunk of an expert's weights for an item: U steps of the lane's row and part.
 template <typename T, bool FP8>
 struct Chunk {
-    static constexpr int U = FP8 ? 4 : 6;
+    static constexpr int U = FP8 ? 6 : 12;
     Run a[U];
     float scale[U / 2];
 };
@@ -490,126 +536,149 @@ struct Down {
 
     __device__ __forceinline__ Down(const Layer &p, const Routing &r)
         : p(p), r(r), lane(threadIdx.x & 63), n(lane & 15), g(lane >> 4), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)),
-          length(((p.c.I + 3) / 4 + kUnit - 1) / kUnit * kUnit),  // of a part
-          steps((length + kStep - 1) / kStep), from((n & 3) * length),
+          length(((p.c.I + kParts - 1) / kParts + kUnit - 1) / kUnit * kUnit),  // of a part
+          steps((length + kStep - 1) / kStep), from((n & (kParts - 1)) * length),
           // (of the lane's part, as a row of the weights and as a column of the rows)
           left(p.c.I - from < length ? (p.c.I - from < 0 ? 0 : p.c.I - from) : length), nb(fp8_blocks(p.c.H)), kb(fp8_blocks(p.c.I)),
           h_bytes((uint32_t)(p.c.T * p.c.k * p.ldh * 4)), h(__builtin_amdgcn_make_buffer_rsrc(p.h, 0, (int)h_bytes, 0x00020000)) {}
 
     __device__ __forceinline__ void load(Chunk<T, FP8> &c, int tile, int at, int s0) const {
-        const int row = tile * 4 + (n >> 2), H = p.c.H, e = __builtin_amdgcn_readfirstlane(r.expert[at]);
+        const int row = tile * kColumns + n / kParts, H = p.c.H, e = __builtin_amdgcn_readfirstlane(r.expert[at]);
         const Element *const w = (const Element *)p.c.w_down + ((int64_t)e * H + (row < H ? row : H - 1)) * p.c.I;
         // (the lane's part ends where the next begins, or with the row: a run that the row's end cuts is the last one of all)
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int k = (s0 + u) * kStep + g * kRun;
-            c.a[u] = load_run<WHOLE>(w, s0 + u < steps && k < length ? from + k : p.c.I, p.c.I, w);
+            c.a[u] = fetch<WHOLE>(w, s0 + u < steps && k < length ? from + k : p.c.I, p.c.I);
         }
         if (FP8) {
-            const float *const scale = p.c.s_down + ((int64_t)e * nb + tile * 4 / kFp8Block) * kb;
+            const float *const scale = p.c.s_down + ((int64_t)e * nb + tile * kColumns / kFp8Block) * kb;
 #pragma unroll
             for (int u = 0; u < U / 2; ++u) c.scale[u] = (s0 + 2 * u) * kStep < left ? scale[from / kFp8Block + s0 / 2 + u] : 0.0f;
         }
     }
 
+    __device__ __forceinline__ Run weight(const Chunk<T, FP8> &c, int s0, int u) const {
+        const int k = (s0 + u) * kStep + g * kRun;
+        return settle<WHOLE, Element>(c.a[u], s0 + u < steps && k < length ? from + k : p.c.I, p.c.I);
+    }
+
     // acc += the chunk times the lane's row of h (8-bit: total, block by block)
-    __device__ __forceinline__ void multiply(const Chunk<T, FP8> &c, int s0, int pair, floatx4 &acc, float &total) const {
-        struct alignas(16) {
-            float v[kRun];
-        } b[U];
-        uint32_t top[U / 2];
-        // (rows of h are whole runs long, zeros behind column I; behind the last row the loads return zeros)
-        const uint32_t row = (uint32_t)pair * (uint32_t)p.ldh * 4u;
+    __device__ __forceinline__ void multiply(const Chunk<T, FP8> &c, int s0, int pair, floatx4 &acc, floatx2 &total) const {
+        constexpr int B = FP8 ? 2 : 6;  // steps whose rows are in flight together
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int k = (s0 + u) * kStep + g * kRun;
-            const uint32_t at = s0 + u < steps && k < left ? row + (uint32_t)(from + k) * 4u : h_bytes;
+        for (int u0 = 0; u0 < U; u0 += B) {
+            if (s0 + u0 >= steps) break;
+            struct alignas(16) {
+                float v[kRun];
+            } b[B];
+            // (rows of h are whole runs long, zeros behind column I; behind the last row the loads return zeros)
+            const uint32_t row = (uint32_t)pair * (uint32_t)p.ldh * 4u;
 #pragma unroll
-            for (int i = 0; i < kRun; i += 4) {
-                const auto v = __builtin_amdgcn_raw_buffer_load_b128(h, (int)at, i * 4, kDeviceScope);
-                __builtin_memcpy(b[u].v + i, &v, 16);
+            for (int u = 0; u < B; ++u) {
+                const int k = (s0 + u0 + u) * kStep + g * kRun;
+                const uint32_t at = s0 + u0 + u < steps && k < left ? row + (uint32_t)(from + k) * 4u : h_bytes;
+#pragma unroll
+                for (int i = 0; i < kRun; i += 4) {
+                    const auto v = __builtin_amdgcn_raw_buffer_load_b128(h, (int)at, i * 4, kDeviceScope);
+                    __builtin_memcpy(b[u].v + i, &v, 16);
+                }
             }
-        }
-        if (FP8) {
-            const uint32_t *const widest = p.widest + (int64_t)pair * kb + from / kFp8Block;
-#pragma unroll
-            for (int u = 0; u < U / 2; ++u) top[u] = (s0 + 2 * u) * kStep < left ? peek(widest + s0 / 2 + u) : 0u;
-        }
-        if constexpr (FP8) {
-#pragma unroll
-            for (int u = 0; u < U / 2; ++u) {
-                const float scale = fp8_scale_of(fp8_scale_byte(top[u]));
+            if constexpr (FP8) {
+                const uint32_t top = (s0 + u0) * kStep < left ? peek(p.widest + (int64_t)pair * kb + from / kFp8Block + (s0 + u0) / 2) : 0u;
+                const float scale = fp8_scale_of(fp8_scale_byte(top));
                 floatx4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int o = 0; o < 2; ++o) {
                     union {
                         Run r;
                         intx2 t[2];
-                    } f = {c.a[2 * u + o]};
+                    } f = {weight(c, s0, u0 + o)};
 #pragma unroll
                     for (int z = 0; z < 2; ++z)
-                        sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp8_widen(f.t[z], 1.0f), fp8_rounded(b[2 * u + o].v + 8 * z, scale), sum, 0, 0, 0);
+                        sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp8_widen(f.t[z], 1.0f), fp8_rounded(b[o].v + 8 * z, scale), sum, 0, 0, 0);
                 }
-                const float lo = n & 1 ? sum[1] : sum[0], hi = n & 1 ? sum[3] : sum[2];
-                total = __builtin_fmaf(c.scale[u], n & 2 ? hi : lo, total);
-            }
-        } else {
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if constexpr (kHalves<T, FP8>) {
-                    bf16x8 av, high, low;
-                    __builtin_memcpy(&av, &c.a[u], 16);
-                    __builtin_memcpy(&high, b[u].v, 16);
-                    __builtin_memcpy(&low, b[u].v + 4, 16);
-                    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, low, acc, 0, 0, 0);
-                    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, high, acc, 0, 0, 0);
-                } else {
-                    T narrow[kRun];
-                    __builtin_memcpy(narrow, &c.a[u], 16);
+                for (int i = 0; i < 2; ++i) total[i] = __builtin_fmaf(c.scale[u0 / 2], n & 1 ? sum[2 * i + 1] : sum[2 * i], total[i]);
+            } else {
 #pragma unroll
-                    for (int z = 0; z < kRun; z += 4) {
-                        const float av[4] = {to_f32(narrow[z]), to_f32(narrow[z + 1]), to_f32(narrow[z + 2]), to_f32(narrow[z + 3])};
-                        const float bv[4] = {b[u].v[z], b[u].v[z + 1], b[u].v[z + 2], b[u].v[z + 3]};
-                        acc = mfma_f32(av, bv, acc);
+                for (int u = 0; u < B; ++u) {
+                    if constexpr (kHalves<T, FP8>) {
+                        const bf16x8 av = __builtin_bit_cast(bf16x8, weight(c, s0, u0 + u));
+                        bf16x8 high, low;
+                        __builtin_memcpy(&high, b[u].v, 16);
+                        __builtin_memcpy(&low, b[u].v + 4, 16);
+                        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, low, acc, 0, 0, 0);
+                        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, high, acc, 0, 0, 0);
+                    } else {
+                        const Run run = weight(c, s0, u0 + u);
+                        T narrow[kRun];
+                        __builtin_memcpy(narrow, &run, 16);
+#pragma unroll
+                        for (int z = 0; z < kRun; z += 4) {
+                            const float av[4] = {to_f32(narrow[z]), to_f32(narrow[z + 1]), to_f32(narrow[z + 2]), to_f32(narrow[z + 3])};
+                            const float bv[4] = {b[u].v[z], b[u].v[z + 1], b[u].v[z + 2], b[u].v[z + 3]};
+                            acc = mfma_f32(av, bv, acc);
+                        }
                     }
                 }
             }
         }
     }
 
-    // `c`: the wave's first chunk of the item, loaded already where it has one
-    __device__ __forceinline__ void item(Chunk<T, FP8> &c, int tile, float (*sums)[kTokens][4]) const {
-        sums[wave][lane >> 2][lane & 3] = 0.0f;  // (a wave's own: its LDS operations keep their order)
-        const int experts = r.experts;
-        for (int at = wave; at < experts; at += kWaves) {
-            const int first = __builtin_amdgcn_readfirstlane(r.first[at]);
-            const int rows = __builtin_amdgcn_readfirstlane(r.first[at + 1]) - first;
-            // four tokens at a time (hardly any expert has more: its weights are read again then, from the caches)
-            for (int q = 0; q < rows; q += 4) {
-                const int mine = q + (n >> 2), pair = first + (mine < rows ? mine : rows - 1);
-                floatx4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-                float total = 0.0f;
-                for (int s0 = 0; s0 < steps; s0 += U) {
-                    if (at != wave || q != 0 || s0 != 0) load(c, tile, at, s0);
-                    multiply(c, s0, pair, acc, total);
-                }
-                // lane (n, g): column g's sum of part i for the token and part of n, in acc[i]
-                if (!FP8) {
-                    const float lo = n & 1 ? acc[1] : acc[0], hi = n & 1 ? acc[3] : acc[2];
-                    total = n & 2 ? hi : lo;
-                }
-                total += __shfl_xor(total, 1);
-                total += __shfl_xor(total, 2);
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                if ((n & 3) == 0 && mine < rows) sums[wave][r.token[first + mine]][g] += r.weight[first + mine] * total;
-            }
+    // What a wave multiplies of an item, one after the other: experts, eight tokens at a time (hardly any expert has more: its weights
+    // are read again then, from the caches), chunks of the reduction.
+    struct Place {
+        int at, q, s0;
+    };
+    __device__ __forceinline__ int rows_of(int at) const { return __builtin_amdgcn_readfirstlane(r.first[at + 1]) - __builtin_amdgcn_readfirstlane(r.first[at]); }
+    __device__ __forceinline__ Place after(Place x) const {
+        x.s0 += U;
+        if (x.s0 < steps) return x;
+        x.s0 = 0, x.q += kColumns;
+        if (x.q < rows_of(x.at)) return x;
+        x.q = 0, x.at += kWaves;
+        return x;
+    }
+    __device__ __forceinline__ void one(const Chunk<T, FP8> &c, Place x, floatx4 &acc, floatx2 &total, float (*sums)[kTokens][kColumns]) const {
+        const int first = __builtin_amdgcn_readfirstlane(r.first[x.at]), rows = rows_of(x.at);
+        const int mine = x.q + n / kParts, pair = first + (mine < rows ? mine : rows - 1);
+        if (x.s0 == 0) acc = floatx4{0.0f, 0.0f, 0.0f, 0.0f}, total = floatx2{0.0f, 0.0f};
+        multiply(c, x.s0, pair, acc, total);
+        if (x.s0 + U < steps) return;
+        // lane (n, g): columns 2 g and 2 g + 1, part i % 2 in acc[i], for the token and the part of n
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float v = FP8 ? total[i] : n & 1 ? acc[2 * i + 1] : acc[2 * i];
+            v += __shfl_xor(v, 1);
+            if ((n & 1) == 0 && mine < rows) sums[wave][r.token[first + mine]][2 * g + i] += r.weight[first + mine] * v;
+        }
+    }
+
+    // `c`: the wave's first chunk of the item, loaded already where it has one.  What comes next is asked for before a chunk is multiplied.
+    __device__ __forceinline__ void item(Chunk<T, FP8> &c, int tile, float (*sums)[kTokens][kColumns]) const {
+        static_assert(kTokens * kColumns == 128, "two sums a lane");
+        (&sums[wave][0][0])[lane] = 0.0f;  // (a wave's own: its LDS operations keep their order)
+        (&sums[wave][0][0])[lane + 64] = 0.0f;
+        floatx4 acc;
+        floatx2 total;
+        Chunk<T, FP8> d;
+        for (Place x = {wave, 0, 0}; x.at < r.experts;) {
+            const Place y = after(x);
+            if (y.at < r.experts) load(d, tile, y.at, y.s0);
+            one(c, x, acc, total, sums);
+            if (y.at >= r.experts) break;
+            x = after(y);
+            if (x.at < r.experts) load(c, tile, x.at, x.s0);
+            one(d, y, acc, total, sums);
         }
         __syncthreads();
-        const int t = threadIdx.x >> 2, col = tile * 4 + (threadIdx.x & 3);
+        const int t = threadIdx.x / kColumns, col = tile * kColumns + threadIdx.x % kColumns;
         if (t < (int)p.c.T && col < p.c.H) {
             float v = 0.0f;
 #pragma unroll
-            for (int u = 0; u < kWaves; ++u) v += sums[u][t][threadIdx.x & 3];
+            for (int u = 0; u < kWaves; ++u) v += sums[u][t][threadIdx.x % kColumns];
             if (p.stream != nullptr) v += to_f32(((const T *)p.stream)[(int64_t)t * p.c.H + col]);
             if (r.lost >> t & 1u) v = __builtin_nanf("");
             ((T *)p.out)[(int64_t)t * p.c.H + col] = from_f32<T>(v);
@@ -618,62 +687,64 @@ struct Down {
 };
 
 // ---- second kernel: both, with one meeting of all workgroups between them -------------------------------------------------------
-// The gated unit's items are dealt out in as many units as there are workgroups: unit b is items b, b + G, ...  A workgroup claims its
-// own unit; before it waits for anything it looks whether there is a unit that nobody has claimed (a workgroup that has not started
-// yet) and does it in the other's place.  So a workgroup waits only for units that running workgroups have claimed, and these wait for
-// nothing before their units are done: every wait ends, however many of the workgroups are there at once.
+// The gated unit's items are dealt out in as many units as there are workgroups: unit b is items b, b + G, ...; each unit has a word: 0
+// free, 1 claimed, 2 done.  A workgroup claims its own unit; before it waits for anything it looks whether there is one that nobody has
+// claimed (of a workgroup that has not started yet) and does it in the other's place.  Whoever claims a unit is running, and waits for
+// nothing before the unit is done: every wait ends, however many of the workgroups are there at once.
 template <typename T, bool FP8, bool WHOLE>
-__global__ __launch_bounds__(kThreads, 4) void layer_experts_kernel(Layer p) {
+__global__ __launch_bounds__(kThreads, 2) void layer_experts_kernel(Layer p) {
     __shared__ Routing r;
     __shared__ union {
-        Parts part;
+        Parts parts;
         Sums sums[2];
     } room;
-    __shared__ int unit_found;
-    const int tid = threadIdx.x;
+    __shared__ int found;
+    const int tid = threadIdx.x, G = (int)gridDim.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    // (asked for before the routing is known: the answer is there by then)
-    uint32_t taken = 0u;
-    if (tid == 0) taken = __hip_atomic_exchange(p.claimed + blockIdx.x, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    auto claim = [&](int unit) { return __hip_atomic_fetch_max(p.units + unit, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 0u ? unit : -1; };
+    int unit = -1;
+    if (tid == 0) unit = claim((int)blockIdx.x);  // (asked for before the routing is known: the answer is there by then)
     find_routing<T>(p, r);
-    const int tiles = (int)(p.ldh / 8), items = r.experts * tiles, G = (int)gridDim.x;
-    const int units = items < G ? items : G;
-    int unit = (int)blockIdx.x, turn = 0;
-    if (tid == 0) unit_found = taken ? -1 : unit;
-    __syncthreads();
-    unit = unit_found < units ? unit_found : -1;
-    for (bool own = true;; own = false) {
-        if (!own) {
-            int free = 0x7fffffff;
-            for (int b = tid; b < units; b += kThreads)
-                if (peek(p.claimed + b) == 0u && b < free) free = b;
-            if (!__syncthreads_or(free != 0x7fffffff)) break;
-            if (tid == 0) unit_found = -1;
-            __syncthreads();
-            if (free != 0x7fffffff) atomicMax(&unit_found, free);  // (any of them)
-            __syncthreads();
-            unit = unit_found;
-            __syncthreads();
-            if (tid == 0) unit_found = __hip_atomic_exchange(p.claimed + unit, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ? -1 : unit;
-            __syncthreads();
-            unit = unit_found;
-        }
-        if (unit < 0) continue;
-        for (int i = unit; i < items; i += G, ++turn)
-            gate_up_item<T, FP8, WHOLE>(p, r, i / tiles, i % tiles, room.part[turn & 1], turn & (kWaves - 1));
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // every wave's rows of h are there, before the word that says so
-        __syncthreads();
-        if (tid == 0) __hip_atomic_store(p.done + unit, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
+    const int tiles = (int)(p.ldh / 8), items = r.experts * tiles, units = items < G ? items : G;
+    const int last = ceil_div(p.c.H, kColumns);
+    int turn = 0;
     const Down<T, FP8, WHOLE> down(p, r);
-    const int last = ceil_div(p.c.H, 4);
     Chunk<T, FP8> c;
-    if ((int)blockIdx.x < last && wave < r.experts) down.load(c, blockIdx.x, wave, 0);
+    if ((int)blockIdx.x >= units) unit = -1;
     for (;;) {
-        bool all = true;
-        for (int b = tid; b < units; b += kThreads) all = all && peek(p.done + b) != 0u;
-        if (__syncthreads_and(all)) break;
-        __builtin_amdgcn_s_sleep(1);
+        // (of thread 0: the unit that it claimed)
+        if (tid == 0) found = unit;
+        __syncthreads();
+        const int got = found;
+        if (got >= 0) {
+            GateUp<T, FP8, WHOLE> front(p, r);
+            front.run(got, items, G, room.parts, turn);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // every wave's rows of h are there, before the word that says so
+            __syncthreads();
+            if (tid == 0) __hip_atomic_store(p.units + got, 2u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        if ((int)blockIdx.x < last && wave < r.experts) down.load(c, blockIdx.x, wave, 0);
+        bool all;
+        int any;
+        for (;;) {
+            int least = 2, free = -1;
+            for (int b = tid; b < units; b += kThreads) {
+                const int state = (int)peek(p.units + b);
+                if (state < least) least = state;
+                if (state == 0) free = b;
+            }
+            any = free;
+            all = __syncthreads_and(least == 2);
+            if (all || __syncthreads_or(free >= 0)) break;
+            __builtin_amdgcn_s_sleep(1);
+        }
+        if (all) break;
+        if (tid == 0) found = -1;
+        __syncthreads();
+        if (any >= 0) atomicMax(&found, any);  // (any of them)
+        __syncthreads();
+        if (tid == 0) unit = claim(found);
+        __syncthreads();
     }
     turn = 0;
     for (int i = blockIdx.x; i < last; i += G, ++turn) {
@@ -684,7 +755,7 @@ __global__ __launch_bounds__(kThreads, 4) void layer_experts_kernel(Layer p) {
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
-int most_workgroups() { return 2 * device_info().cu_count; }
+int most_workgroups() { return device_info().cu_count; }
 
 struct Room {
     size_t stream, rows, h, widest, flags;  // bytes
@@ -697,7 +768,7 @@ struct Room {
         rows = fp8 ? up256((size_t)c.T * ld * 2) : norm ? up256((size_t)c.T * ld * dtype_size(c.dtype)) : 0;
         h = up256((size_t)c.T * c.k * ldh * 4);
         widest = fp8 ? up256((size_t)c.T * c.k * fp8_blocks(c.I) * 4) : 0;
-        flags = up256((size_t)2 * most_workgroups() * 4);
+        flags = up256((size_t)most_workgroups() * 4);
     }
     size_t all() const { return stream + rows + h + widest + flags; }
 };
@@ -716,7 +787,7 @@ int launch(const Layer &p, hipStream_t stream) {
     else { MFL_LAYER_ROUTER(2) }
 #undef MFL_LAYER_ROUTER
     const int hits = p.c.T * p.c.k < p.c.E ? (int)p.c.T * p.c.k : p.c.E;
-    const int64_t front = hits * (p.ldh / 8), back = ceil_div(p.c.H, 4), want = front > back ? front : back;
+    const int64_t front = hits * (p.ldh / 8), back = ceil_div(p.c.H, kColumns), want = front > back ? front : back;
     const unsigned most = (unsigned)most_workgroups();
     layer_experts_kernel<T, FP8, WHOLE><<<want < most ? (unsigned)want : most, kThreads, 0, stream>>>(p);
     return launch_status();
@@ -756,8 +827,7 @@ int moe_layer_fwd(const mfl_moe_layer &c, void *out, void *logits, void *workspa
     p.zeros = (uint32_t *)at;
     p.zero_words = (int)((room.widest + room.flags) / 4);
     p.widest = (uint32_t *)take(room.widest);
-    p.claimed = (uint32_t *)take(room.flags);
-    p.done = p.claimed + most_workgroups();
+    p.units = (uint32_t *)take(room.flags);
     int rc = MFL_OK;
     MFL_DISPATCH_FLOAT(c.dtype, T, { rc = launch_type<T>(p, stream); });
     return rc;
