@@ -563,63 +563,68 @@ struct Down {
         return settle<WHOLE, Element>(c.a[u], s0 + u < steps && k < length ? from + k : p.c.I, p.c.I);
     }
 
-    // acc += the chunk times the lane's row of h (8-bit: total, block by block)
-    __device__ __forceinline__ void multiply(const Chunk<T, FP8> &c, int s0, int pair, floatx4 &acc, floatx2 &total) const {
-        constexpr int B = FP8 ? 2 : 6;  // steps whose rows are in flight together
+    // The lane's row of h for a chunk.
+    struct alignas(16) Rows {
+        float v[U][kRun];
+        uint32_t top[U / 2];
+    };
+    __device__ __forceinline__ void load_rows(Rows &b, int s0, int pair) const {
+        // (rows of h are whole runs long, zeros behind column I; behind the last row the loads return zeros)
+        const uint32_t row = (uint32_t)pair * (uint32_t)p.ldh * 4u;
 #pragma unroll
-        for (int u0 = 0; u0 < U; u0 += B) {
-            if (s0 + u0 >= steps) break;
-            struct alignas(16) {
-                float v[kRun];
-            } b[B];
-            // (rows of h are whole runs long, zeros behind column I; behind the last row the loads return zeros)
-            const uint32_t row = (uint32_t)pair * (uint32_t)p.ldh * 4u;
+        for (int u = 0; u < U; ++u) {
+            const int k = (s0 + u) * kStep + g * kRun;
+            const uint32_t at = s0 + u < steps && k < left ? row + (uint32_t)(from + k) * 4u : h_bytes;
 #pragma unroll
-            for (int u = 0; u < B; ++u) {
-                const int k = (s0 + u0 + u) * kStep + g * kRun;
-                const uint32_t at = s0 + u0 + u < steps && k < left ? row + (uint32_t)(from + k) * 4u : h_bytes;
-#pragma unroll
-                for (int i = 0; i < kRun; i += 4) {
-                    const auto v = __builtin_amdgcn_raw_buffer_load_b128(h, (int)at, i * 4, kDeviceScope);
-                    __builtin_memcpy(b[u].v + i, &v, 16);
-                }
+            for (int i = 0; i < kRun; i += 4) {
+                const auto v = __builtin_amdgcn_raw_buffer_load_b128(h, (int)at, i * 4, kDeviceScope);
+                __builtin_memcpy(b.v[u] + i, &v, 16);
             }
-            if constexpr (FP8) {
-                const uint32_t top = (s0 + u0) * kStep < left ? peek(p.widest + (int64_t)pair * kb + from / kFp8Block + (s0 + u0) / 2) : 0u;
-                const float scale = fp8_scale_of(fp8_scale_byte(top));
+        }
+        if (FP8) {
+            const uint32_t *const widest = p.widest + (int64_t)pair * kb + from / kFp8Block + s0 / 2;
+#pragma unroll
+            for (int u = 0; u < U / 2; ++u) b.top[u] = (s0 + 2 * u) * kStep < left ? peek(widest + u) : 0u;
+        }
+    }
+    // acc += the chunk times the lane's row (8-bit: total, block by block)
+    __device__ __forceinline__ void multiply(const Chunk<T, FP8> &c, const Rows &b, int s0, floatx4 &acc, floatx2 &total) const {
+        if constexpr (FP8) {
+#pragma unroll
+            for (int u = 0; u < U; u += 2) {
+                const float scale = fp8_scale_of(fp8_scale_byte(b.top[u / 2]));
                 floatx4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int o = 0; o < 2; ++o) {
                     union {
                         Run r;
                         intx2 t[2];
-                    } f = {weight(c, s0, u0 + o)};
+                    } f = {weight(c, s0, u + o)};
 #pragma unroll
                     for (int z = 0; z < 2; ++z)
-                        sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp8_widen(f.t[z], 1.0f), fp8_rounded(b[o].v + 8 * z, scale), sum, 0, 0, 0);
+                        sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp8_widen(f.t[z], 1.0f), fp8_rounded(b.v[u + o] + 8 * z, scale), sum, 0, 0, 0);
                 }
 #pragma unroll
-                for (int i = 0; i < 2; ++i) total[i] = __builtin_fmaf(c.scale[u0 / 2], n & 1 ? sum[2 * i + 1] : sum[2 * i], total[i]);
-            } else {
+                for (int i = 0; i < 2; ++i) total[i] = __builtin_fmaf(c.scale[u / 2], n & 1 ? sum[2 * i + 1] : sum[2 * i], total[i]);
+            }
+        } else {
 #pragma unroll
-                for (int u = 0; u < B; ++u) {
-                    if constexpr (kHalves<T, FP8>) {
-                        const bf16x8 av = __builtin_bit_cast(bf16x8, weight(c, s0, u0 + u));
-                        bf16x8 high, low;
-                        __builtin_memcpy(&high, b[u].v, 16);
-                        __builtin_memcpy(&low, b[u].v + 4, 16);
-                        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, low, acc, 0, 0, 0);
-                        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, high, acc, 0, 0, 0);
-                    } else {
-                        const Run run = weight(c, s0, u0 + u);
-                        T narrow[kRun];
-                        __builtin_memcpy(narrow, &run, 16);
+            for (int u = 0; u < U; ++u) {
+                const Run run = weight(c, s0, u);
+                if constexpr (kHalves<T, FP8>) {
+                    bf16x8 high, low;
+                    __builtin_memcpy(&high, b.v[u], 16);
+                    __builtin_memcpy(&low, b.v[u] + 4, 16);
+                    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, run), low, acc, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, run), high, acc, 0, 0, 0);
+                } else {
+                    T narrow[kRun];
+                    __builtin_memcpy(narrow, &run, 16);
 #pragma unroll
-                        for (int z = 0; z < kRun; z += 4) {
-                            const float av[4] = {to_f32(narrow[z]), to_f32(narrow[z + 1]), to_f32(narrow[z + 2]), to_f32(narrow[z + 3])};
-                            const float bv[4] = {b[u].v[z], b[u].v[z + 1], b[u].v[z + 2], b[u].v[z + 3]};
-                            acc = mfma_f32(av, bv, acc);
-                        }
+                    for (int z = 0; z < kRun; z += 4) {
+                        const float av[4] = {to_f32(narrow[z]), to_f32(narrow[z + 1]), to_f32(narrow[z + 2]), to_f32(narrow[z + 3])};
+                        const float bv[4] = {b.v[u][z], b.v[u][z + 1], b.v[u][z + 2], b.v[u][z + 3]};
+                        acc = mfma_f32(av, bv, acc);
                     }
                 }
             }
@@ -640,11 +645,16 @@ struct Down {
         x.q = 0, x.at += kWaves;
         return x;
     }
-    __device__ __forceinline__ void one(const Chunk<T, FP8> &c, Place x, floatx4 &acc, floatx2 &total, float (*sums)[kTokens][kColumns]) const {
+    // Place x with its weights in c; those of y, if there is one, are asked for behind the rows of x: loads come back in order.
+    __device__ __forceinline__ void one(const Chunk<T, FP8> &c, Place x, Chunk<T, FP8> &d, Place y, int tile, floatx4 &acc, floatx2 &total,
+                                        float (*sums)[kTokens][kColumns]) const {
         const int first = __builtin_amdgcn_readfirstlane(r.first[x.at]), rows = rows_of(x.at);
         const int mine = x.q + n / kParts, pair = first + (mine < rows ? mine : rows - 1);
         if (x.s0 == 0) acc = floatx4{0.0f, 0.0f, 0.0f, 0.0f}, total = floatx2{0.0f, 0.0f};
-        multiply(c, x.s0, pair, acc, total);
+        Rows b;
+        load_rows(b, x.s0, pair);
+        if (y.at < r.experts) load(d, tile, y.at, y.s0);
+        multiply(c, b, x.s0, acc, total);
         if (x.s0 + U < steps) return;
         // lane (n, g): columns 2 g and 2 g + 1, part i % 2 in acc[i], for the token and the part of n
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -666,12 +676,10 @@ struct Down {
         Chunk<T, FP8> d;
         for (Place x = {wave, 0, 0}; x.at < r.experts;) {
             const Place y = after(x);
-            if (y.at < r.experts) load(d, tile, y.at, y.s0);
-            one(c, x, acc, total, sums);
+            one(c, x, d, y, tile, acc, total, sums);
             if (y.at >= r.experts) break;
             x = after(y);
-            if (x.at < r.experts) load(c, tile, x.at, x.s0);
-            one(d, y, acc, total, sums);
+            one(d, y, c, x, tile, acc, total, sums);
         }
         __syncthreads();
         const int t = threadIdx.x / kColumns, col = tile * kColumns + threadIdx.x % kColumns;
