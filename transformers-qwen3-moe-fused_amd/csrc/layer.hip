@@ -340,7 +340,7 @@ constexpr int kDeviceScope = 16;  // a buffer load's sc1 bit
 // 16 columns; the eight waves share the reduction and meet in LDS.  Weights straight from memory into the matrix unit's registers.
 // A column is a token, whether it chose the expert or not: what a wave needs of the tokens is the same for every item, and stays in
 // registers where its share of the reduction is one chunk.  The next item's weights are asked for before the waves meet.
-typedef floatx4 Parts[2][kWaves][64];
+typedef floatx4 Parts[2][2][kWaves][64];
 
 template <typename T, bool FP8, bool WHOLE>
 struct GateUp {
@@ -350,6 +350,7 @@ struct GateUp {
     static constexpr int kRun = W::kRun, kStep = W::kStep, kPieces = kRun * (int)sizeof(X) / 16;
     static constexpr int U = FP8 ? 4 : 8;      // steps of a chunk: their loads are in flight together
     static constexpr int D = FP8 ? 4 : 2;      // items whose first chunks are
+    static constexpr int kGroup = FP8 ? 2 : 1;
     static constexpr int kUnit = FP8 ? 2 : 1;  // (whole blocks of 128 a wave where weights have scales)
     const Layer &p;
     const Routing &r;
@@ -436,30 +437,43 @@ struct GateUp {
         }
     }
 
-    // Items from, from + by, ... below to; `turn` counts a workgroup's items.
+    // Items from, from + by, ... below to; the waves meet once for kGroup of them.  `turn` counts a workgroup's meetings.
     __device__ __forceinline__ void run(int from, int to, int by, Parts &parts, int &turn) {
 #pragma unroll
         for (int d = 0; d < D; ++d)
             if (from + d * by < to) load_weights(w[d], from + d * by, begin);
         for (int i = from; i < to; i += D * by) {
 #pragma unroll
-            for (int d = 0; d < D; ++d, ++turn) {
+            for (int d = 0; d < D; d += kGroup, ++turn) {
                 const int item = i + d * by;
                 if (item >= to) break;
-                floatx4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-                for (int c = 0; c < chunks; ++c) {
-                    if (c != 0) load_weights(w[d], item, begin + c * U);
-                    if (chunks != 1) load_rows(begin + c * U);
-                    multiply(w[d], begin + c * U, acc);
-                }
-                if (item + D * by < to) load_weights(w[d], item + D * by, begin);
-                floatx4(*const part)[64] = parts[turn & 1];
-                part[wave][lane] = acc;
-                __syncthreads();
-                if (wave != (turn & (kWaves - 1))) continue;
+                floatx4 acc[kGroup];
 #pragma unroll
-                for (int v = 0; v < kWaves; ++v) acc = v == 0 ? part[0][lane] : acc + part[v][lane];
-                finish(item, acc);
+                for (int o = 0; o < kGroup; ++o) acc[o] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+                for (int c = 0; c < chunks; ++c) {
+                    if (c != 0) {
+#pragma unroll
+                        for (int o = 0; o < kGroup; ++o)
+                            if (item + o * by < to) load_weights(w[d + o], item + o * by, begin + c * U);
+                    }
+                    if (chunks != 1) load_rows(begin + c * U);
+#pragma unroll
+                    for (int o = 0; o < kGroup; ++o)
+                        if (item + o * by < to) multiply(w[d + o], begin + c * U, acc[o]);
+                }
+                floatx4(*const part)[kWaves][64] = parts[turn & 1];
+#pragma unroll
+                for (int o = 0; o < kGroup; ++o) {
+                    if (item + (D + o) * by < to) load_weights(w[d + o], item + (D + o) * by, begin);
+                    if (item + o * by < to) part[o][wave][lane] = acc[o];
+                }
+                __syncthreads();
+                // as many waves finish an item each, others every time
+                const int mine = (wave - kGroup * turn) & (kWaves - 1);
+                if (mine >= kGroup || item + mine * by >= to) continue;
+#pragma unroll
+                for (int v = 0; v < kWaves; ++v) acc[0] = v == 0 ? part[mine][0][lane] : acc[0] + part[mine][v][lane];
+                finish(item + mine * by, acc[0]);
             }
         }
     }
@@ -513,11 +527,14 @@ struct GateUp {
 // work is for nothing, but it has a thirtieth of its time to do.)
 constexpr int kParts = 2, kColumns = 16 / kParts;
 typedef float Sums[kWaves][kTokens][kColumns];
+constexpr int kStagedRow = kParts * 6 * 64 + 8;  // (8-bit layers) elements of a staged row: a chunk, and 16 bytes more for the banks
 
 // A chunk of an expert's weights for an item: U steps of the lane's row and part.
-template <typename T, bool FP8>
+// (Six where more would not fit the registers: rows that have to be moved down, and fp16, which is widened: 61 -> 44 us at 5 tokens of
+// 1001 x 333.)
+template <typename T, bool FP8, bool WHOLE>
 struct Chunk {
-    static constexpr int U = FP8 ? 6 : 12;
+    static constexpr int U = FP8 || !WHOLE || std::is_same<T, f16_t>::value ? 6 : 12;
     Run a[U];
     float scale[U / 2];
 };
@@ -526,7 +543,7 @@ template <typename T, bool FP8, bool WHOLE>
 struct Down {
     typedef Weights<T, FP8> W;
     typedef typename W::Element Element;
-    static constexpr int kRun = W::kRun, kStep = W::kStep, U = Chunk<T, FP8>::U;
+    static constexpr int kRun = W::kRun, kStep = W::kStep, U = Chunk<T, FP8, WHOLE>::U;
     static constexpr int kUnit = FP8 ? kFp8Block : kRun;
     const Layer &p;
     const Routing &r;
@@ -542,7 +559,7 @@ struct Down {
           left(p.c.I - from < length ? (p.c.I - from < 0 ? 0 : p.c.I - from) : length), nb(fp8_blocks(p.c.H)), kb(fp8_blocks(p.c.I)),
           h_bytes((uint32_t)(p.c.T * p.c.k * p.ldh * 4)), h(__builtin_amdgcn_make_buffer_rsrc(p.h, 0, (int)h_bytes, 0x00020000)) {}
 
-    __device__ __forceinline__ void load(Chunk<T, FP8> &c, int tile, int at, int s0) const {
+    __device__ __forceinline__ void load(Chunk<T, FP8, WHOLE> &c, int tile, int at, int s0) const {
         const int row = tile * kColumns + n / kParts, H = p.c.H, e = __builtin_amdgcn_readfirstlane(r.expert[at]);
         const Element *const w = (const Element *)p.c.w_down + ((int64_t)e * H + (row < H ? row : H - 1)) * p.c.I;
         // (the lane's part ends where the next begins, or with the row: a run that the row's end cuts is the last one of all)
@@ -558,21 +575,20 @@ struct Down {
         }
     }
 
-    __device__ __forceinline__ Run weight(const Chunk<T, FP8> &c, int s0, int u) const {
+    __device__ __forceinline__ Run weight(const Chunk<T, FP8, WHOLE> &c, int s0, int u) const {
         const int k = (s0 + u) * kStep + g * kRun;
         return settle<WHOLE, Element>(c.a[u], s0 + u < steps && k < length ? from + k : p.c.I, p.c.I);
     }
 
-    // The lane's row of h for a chunk.
+    // The lane's row of h for a chunk.  (8-bit: not here, but in LDS, see stage.)
     struct alignas(16) Rows {
-        float v[U][kRun];
-        uint32_t top[U / 2];
+        float v[FP8 ? 1 : U][kRun];
     };
     __device__ __forceinline__ void load_rows(Rows &b, int s0, int pair) const {
         // (rows of h are whole runs long, zeros behind column I; behind the last row the loads return zeros)
         const uint32_t row = (uint32_t)pair * (uint32_t)p.ldh * 4u;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
+        for (int u = 0; u < (FP8 ? 1 : U); ++u) {
             const int k = (s0 + u) * kStep + g * kRun;
             const uint32_t at = s0 + u < steps && k < left ? row + (uint32_t)(from + k) * 4u : h_bytes;
 #pragma unroll
@@ -581,18 +597,52 @@ struct Down {
                 __builtin_memcpy(b.v[u] + i, &v, 16);
             }
         }
-        if (FP8) {
-            const uint32_t *const widest = p.widest + (int64_t)pair * kb + from / kFp8Block + s0 / 2;
+    }
+    // 8-bit layers: a chunk of up to eight rows of h, quantised by the whole wave (a value once, not once for every lane that multiplies
+    // it: 48 of them) and left in the wave's own part of LDS as what the rounded values stand for.
+    static constexpr int kStaged = kParts * U * kStep;  // elements of a row and chunk
+    static_assert(!FP8 || (kStaged % 256 == 0 && kStaged <= kStagedRow), "four elements a lane at a time");
+    struct Staged {
+        floatx4 v[FP8 ? kStaged / 256 : 1];
+        uint32_t top[FP8 ? kStaged / 256 : 1];
+    };
+    __device__ __forceinline__ void stage_load(Staged &s, int s0, int pair) const {
 #pragma unroll
-            for (int u = 0; u < U / 2; ++u) b.top[u] = (s0 + 2 * u) * kStep < left ? peek(widest + u) : 0u;
+        for (int i = 0; i < kStaged / 256; ++i) {
+            const int x = i * 256 + lane * 4, part = x / (U * kStep), k = s0 * kStep + x - part * (U * kStep), at = part * length + k;
+            const bool in = k < length && at < (int)p.ldh;
+            const auto v = __builtin_amdgcn_raw_buffer_load_b128(h, (int)(in ? ((uint32_t)pair * (uint32_t)p.ldh + (uint32_t)at) * 4u : h_bytes), 0, kDeviceScope);
+            s.v[i] = __builtin_bit_cast(floatx4, v);
+            s.top[i] = 0u;
+            if (in && at < p.c.I) s.top[i] = peek(p.widest + (int64_t)pair * kb + at / kFp8Block);
         }
     }
+    __device__ __forceinline__ void stage_store(const Staged &s, bf16_t *row) const {
+        typedef __attribute__((ext_vector_type(2))) short shortx2;
+#pragma unroll
+        for (int i = 0; i < kStaged / 256; ++i) {
+            const float scale = fp8_scale_of(fp8_scale_byte(s.top[i]));
+            shortx2 r = {};
+            r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, s.v[i][0], s.v[i][1], scale, false);
+            r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, s.v[i][2], s.v[i][3], scale, true);
+            const int q = __builtin_bit_cast(int, r);
+            union {
+                bf16x2 p[2];
+                uint2_t d;
+            } o;
+            o.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q, scale, false);
+            o.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q, scale, true);
+            *(uint2_t *)(row + i * 256 + lane * 4) = o.d;
+        }
+    }
+
     // acc += the chunk times the lane's row (8-bit: total, block by block)
-    __device__ __forceinline__ void multiply(const Chunk<T, FP8> &c, const Rows &b, int s0, floatx4 &acc, floatx2 &total) const {
+    __device__ __forceinline__ void multiply(const Chunk<T, FP8, WHOLE> &c, const Rows &b, const bf16_t *staged, int s0, floatx4 &acc,
+                                             floatx2 &total) const {
         if constexpr (FP8) {
+            const bf16_t *const row = staged + n / kParts * kStagedRow + n % kParts * (U * kStep) + g * kRun;
 #pragma unroll
             for (int u = 0; u < U; u += 2) {
-                const float scale = fp8_scale_of(fp8_scale_byte(b.top[u / 2]));
                 floatx4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int o = 0; o < 2; ++o) {
@@ -602,7 +652,7 @@ struct Down {
                     } f = {weight(c, s0, u + o)};
 #pragma unroll
                     for (int z = 0; z < 2; ++z)
-                        sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp8_widen(f.t[z], 1.0f), fp8_rounded(b.v[u + o] + 8 * z, scale), sum, 0, 0, 0);
+                        sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp8_widen(f.t[z], 1.0f), *(const bf16x8 *)(row + (u + o) * kStep + 8 * z), sum, 0, 0, 0);
                 }
 #pragma unroll
                 for (int i = 0; i < 2; ++i) total[i] = __builtin_fmaf(c.scale[u / 2], n & 1 ? sum[2 * i + 1] : sum[2 * i], total[i]);
@@ -646,15 +696,33 @@ struct Down {
         return x;
     }
     // Place x with its weights in c; those of y, if there is one, are asked for behind the rows of x: loads come back in order.
-    __device__ __forceinline__ void one(const Chunk<T, FP8> &c, Place x, Chunk<T, FP8> &d, Place y, int tile, floatx4 &acc, floatx2 &total,
-                                        float (*sums)[kTokens][kColumns]) const {
+    __device__ __forceinline__ void one(const Chunk<T, FP8, WHOLE> &c, Place x, Chunk<T, FP8, WHOLE> &d, Place y, int tile, floatx4 &acc, floatx2 &total,
+                                        float (*sums)[kTokens][kColumns], bf16_t *staged) const {
         const int first = __builtin_amdgcn_readfirstlane(r.first[x.at]), rows = rows_of(x.at);
         const int mine = x.q + n / kParts, pair = first + (mine < rows ? mine : rows - 1);
         if (x.s0 == 0) acc = floatx4{0.0f, 0.0f, 0.0f, 0.0f}, total = floatx2{0.0f, 0.0f};
         Rows b;
-        load_rows(b, x.s0, pair);
-        if (y.at < r.experts) load(d, tile, y.at, y.s0);
-        multiply(c, b, x.s0, acc, total);
+        if constexpr (FP8) {
+            // (two rows in flight; hardly any expert has more)
+            Staged s[2];
+            const int count = rows - x.q < kColumns ? rows - x.q : kColumns;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                if (j < count) stage_load(s[j], x.s0, first + x.q + j);
+            if (y.at < r.experts) load(d, tile, y.at, y.s0);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                if (j < count) stage_store(s[j], staged + j * kStagedRow);
+            for (int j = 2; j < count; ++j) {
+                stage_load(s[0], x.s0, first + x.q + j);
+                stage_store(s[0], staged + j * kStagedRow);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        } else {
+            load_rows(b, x.s0, pair);
+            if (y.at < r.experts) load(d, tile, y.at, y.s0);
+        }
+        multiply(c, b, staged, x.s0, acc, total);
         if (x.s0 + U < steps) return;
         // lane (n, g): columns 2 g and 2 g + 1, part i % 2 in acc[i], for the token and the part of n
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -667,19 +735,19 @@ struct Down {
     }
 
     // `c`: the wave's first chunk of the item, loaded already where it has one.  What comes next is asked for before a chunk is multiplied.
-    __device__ __forceinline__ void item(Chunk<T, FP8> &c, int tile, float (*sums)[kTokens][kColumns]) const {
+    __device__ __forceinline__ void item(Chunk<T, FP8, WHOLE> &c, int tile, float (*sums)[kTokens][kColumns], bf16_t *staged) const {
         static_assert(kTokens * kColumns == 128, "two sums a lane");
         (&sums[wave][0][0])[lane] = 0.0f;  // (a wave's own: its LDS operations keep their order)
         (&sums[wave][0][0])[lane + 64] = 0.0f;
         floatx4 acc;
         floatx2 total;
-        Chunk<T, FP8> d;
+        Chunk<T, FP8, WHOLE> d;
         for (Place x = {wave, 0, 0}; x.at < r.experts;) {
             const Place y = after(x);
-            one(c, x, d, y, tile, acc, total, sums);
+            one(c, x, d, y, tile, acc, total, sums, staged);
             if (y.at >= r.experts) break;
             x = after(y);
-            one(d, y, c, x, tile, acc, total, sums);
+            one(d, y, c, x, tile, acc, total, sums, staged);
         }
         __syncthreads();
         const int t = threadIdx.x / kColumns, col = tile * kColumns + threadIdx.x % kColumns;
@@ -704,7 +772,10 @@ __global__ __launch_bounds__(kThreads, 2) void layer_experts_kernel(Layer p) {
     __shared__ Routing r;
     __shared__ union {
         Parts parts;
-        Sums sums[2];
+        struct {
+            Sums sums[2];
+            alignas(16) bf16_t staged[FP8 ? kWaves : 1][FP8 ? kColumns * kStagedRow : 8];
+        } back;
     } room;
     __shared__ int found;
     const int tid = threadIdx.x, G = (int)gridDim.x;
@@ -717,7 +788,7 @@ __global__ __launch_bounds__(kThreads, 2) void layer_experts_kernel(Layer p) {
     const int last = ceil_div(p.c.H, kColumns);
     int turn = 0;
     const Down<T, FP8, WHOLE> down(p, r);
-    Chunk<T, FP8> c;
+    Chunk<T, FP8, WHOLE> c;
     if ((int)blockIdx.x >= units) unit = -1;
     for (;;) {
         // (of thread 0: the unit that it claimed)
@@ -757,7 +828,7 @@ __global__ __launch_bounds__(kThreads, 2) void layer_experts_kernel(Layer p) {
     turn = 0;
     for (int i = blockIdx.x; i < last; i += G, ++turn) {
         if (turn != 0 && wave < r.experts) down.load(c, i, wave, 0);
-        down.item(c, i, room.sums[turn & 1]);
+        down.item(c, i, room.back.sums[turn & 1], room.back.staged[FP8 ? wave : 0]);
     }
 }
 
