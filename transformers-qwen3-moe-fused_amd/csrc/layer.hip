@@ -156,66 +156,95 @@ __device__ __forceinline__ int wave_max(int x) {
     return wave_last(x);
 }
 
-// One token by one wave; PER_LANE: experts lane, lane + 64, ...
-template <typename T, int PER_LANE>
-__device__ __forceinline__ void choose(const T *logits, int t, int E, int k, int renorm, Routing &r, int lane) {
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ float dpp_sum_step(float x) {
+    return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, ROW_MASK, 0xf, true));
+}
+__device__ __forceinline__ float wave_sum(float x) {
+    x = dpp_sum_step<0x111, 0xf>(x);
+    x = dpp_sum_step<0x112, 0xf>(x);
+    x = dpp_sum_step<0x114, 0xf>(x);
+    x = dpp_sum_step<0x118, 0xf>(x);
+    x = dpp_sum_step<0x142, 0xa>(x);
+    x = dpp_sum_step<0x143, 0xc>(x);
+    return __int_as_float(wave_last(__float_as_int(x)));
+}
+
+// TOKENS tokens t, t + 8, ... by one wave, side by side (each is a chain of dependent steps); PER_LANE: experts lane, lane + 64, ...
+// `ready` is called when the logits are on their way.
+template <typename T, int PER_LANE, int TOKENS, typename F>
+__device__ __forceinline__ void choose(const Layer &p, int t, Routing &r, int lane, F &&ready) {
     constexpr int kNone = -0x7fffffff - 1;
-    float v[PER_LANE];
-    int key[PER_LANE];  // the order of the values as whole numbers (-0 as 0)
-    int top = kNone;
-    bool nan = false;
-    T raw[PER_LANE];
+    const int E = p.c.E, k = p.c.k;
+    T raw[TOKENS][PER_LANE];
 #pragma unroll
-    for (int i = 0; i < PER_LANE; ++i) raw[i] = logits[(int64_t)t * E + (lane + 64 * i < E ? lane + 64 * i : E - 1)];  // (in flight together)
+    for (int o = 0; o < TOKENS; ++o) {
+        const int at = t + o * kWaves < (int)p.c.T ? t + o * kWaves : (int)p.c.T - 1;  // (a wave without a token looks at the last one)
 #pragma unroll
-    for (int i = 0; i < PER_LANE; ++i) {
-        const int e = lane + 64 * i;
-        v[i] = e < E ? to_f32(raw[i]) + 0.0f : -INFINITY;
-        nan |= v[i] != v[i];
-        const int bits = __float_as_int(v[i]);
-        key[i] = e < E ? bits ^ ((bits >> 31) & 0x7fffffff) : kNone;
-        top = top > key[i] ? top : key[i];
+        for (int i = 0; i < PER_LANE; ++i) raw[o][i] = ((const T *)p.logits)[(int64_t)at * E + (lane + 64 * i < E ? lane + 64 * i : E - 1)];
     }
-    top = wave_max(top);
-    const float largest = __int_as_float(top ^ ((top >> 31) & 0x7fffffff));
-    if (__any(nan) || __builtin_isinf(largest)) {
-        if (lane == 0) atomicOr(&r.lost, 1u << t);
-        for (int j = lane; j < k; j += 64) r.own_expert[t][j] = -1;
-        return;
-    }
-    float sum = 0.0f;
+    ready();
+    float share[TOKENS][PER_LANE], sum[TOKENS], chosen[TOKENS], mine[TOKENS];
+    int key[TOKENS][PER_LANE], top[TOKENS], mine_e[TOKENS];
+    bool lost[TOKENS];
 #pragma unroll
-    for (int i = 0; i < PER_LANE; ++i) sum += expf(v[i] - largest);  // (0 past the last expert)
+    for (int o = 0; o < TOKENS; ++o) {
+        top[o] = kNone;
+        bool nan = false;
 #pragma unroll
-    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
-    float mine = 0.0f, chosen = 0.0f;
-    int mine_e = 0;
-    for (int j = 0; j < k; ++j) {
-        int best = kNone, at = 0;
-#pragma unroll
-        for (int i = 0; i < PER_LANE; ++i)
-            if (key[i] > best) best = key[i], at = i;  // (ascending ids: the lower of equals)
-        const int m = j == 0 ? top : wave_max(best);
-        // of the lanes with that value the lowest expert id: the least i, then the least lane
-        const uint64_t owners = __ballot(best == m);
-        int e;
-        if (__popcll(owners) == 1) {
-            const int o = __ffsll((unsigned long long)owners) - 1;
-            e = __builtin_amdgcn_readlane(at, o) * 64 + o;
-        } else {
-            e = -wave_max(best == m ? -(at * 64 + lane) : kNone);
+        for (int i = 0; i < PER_LANE; ++i) {
+            const bool in = lane + 64 * i < E;
+            share[o][i] = in ? to_f32(raw[o][i]) + 0.0f : -INFINITY;
+            nan |= share[o][i] != share[o][i];
+            const int bits = __float_as_int(share[o][i]);
+            key[o][i] = in ? bits ^ ((bits >> 31) & 0x7fffffff) : kNone;  // the order of the values as whole numbers (-0 as 0)
+            top[o] = top[o] > key[o][i] ? top[o] : key[o][i];
         }
-        const float p = expf(__int_as_float(m ^ ((m >> 31) & 0x7fffffff)) - largest) / sum;
+        top[o] = wave_max(top[o]);
+        const float largest = __int_as_float(top[o] ^ ((top[o] >> 31) & 0x7fffffff));
+        lost[o] = __any(nan) || __builtin_isinf(largest);
+        sum[o] = chosen[o] = mine[o] = 0.0f, mine_e[o] = 0;
 #pragma unroll
-        for (int i = 0; i < PER_LANE; ++i)
-            if (e == lane + 64 * i) key[i] = kNone;
-        if (lane == j) mine = p, mine_e = e;
-        chosen += p;
+        for (int i = 0; i < PER_LANE; ++i) share[o][i] = expf(share[o][i] - largest), sum[o] += share[o][i];  // (0 past the last expert)
+        sum[o] = wave_sum(sum[o]);
     }
-    if (lane < k) {
-        r.own_expert[t][lane] = (int16_t)mine_e;
-        r.own_weight[t][lane] = renorm ? mine / chosen : mine;
-        atomicOr(&r.mask[mine_e], 1u << t);
+    for (int j = 0; j < k; ++j) {
+#pragma unroll
+        for (int o = 0; o < TOKENS; ++o) {
+            int best = kNone, at = 0;
+            float s = 0.0f;
+#pragma unroll
+            for (int i = 0; i < PER_LANE; ++i)
+                if (key[o][i] > best) best = key[o][i], at = i, s = share[o][i];  // (ascending ids: the lower of equals)
+            const int m = j == 0 ? top[o] : wave_max(best);
+            // of the lanes with that value the lowest expert id: the least i, then the least lane
+            const uint64_t owners = __ballot(best == m);
+            int e;
+            if (__popcll(owners) == 1) {
+                const int owner = __ffsll((unsigned long long)owners) - 1;
+                e = __builtin_amdgcn_readlane(at, owner) * 64 + owner;
+            } else {
+                e = -wave_max(best == m ? -(at * 64 + lane) : kNone);
+            }
+            const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(s), e & 63));
+#pragma unroll
+            for (int i = 0; i < PER_LANE; ++i)
+                if (e == lane + 64 * i) key[o][i] = kNone;
+            if (lane == j) mine[o] = w, mine_e[o] = e;
+            chosen[o] += w;
+        }
+    }
+#pragma unroll
+    for (int o = 0; o < TOKENS; ++o) {
+        const int at = t + o * kWaves;
+        if (at >= (int)p.c.T || lane >= k) continue;
+        r.own_expert[at][lane] = lost[o] ? -1 : (int16_t)mine_e[o];
+        if (lost[o]) {
+            if (lane == 0) atomicOr(&r.lost, 1u << at);
+            continue;
+        }
+        r.own_weight[at][lane] = mine[o] / (p.c.renorm ? chosen[o] : sum[o]);
+        atomicOr(&r.mask[mine_e[o]], 1u << at);
     }
 }
 
@@ -224,13 +253,18 @@ __device__ __forceinline__ void find_routing(const Layer &p, Routing &r) {
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int E = p.c.E, k = p.c.k, tokens = (int)p.c.T;
-    for (int e = tid; e < E; e += kThreads) r.mask[e] = 0u;
-    if (tid == 0) r.lost = 0u;
-    __syncthreads();
-    for (int t = wave; t < tokens; t += kWaves) {
-        const T *const logits = (const T *)p.logits;
-        if (E <= 128) choose<T, 2>(logits, t, E, k, p.c.renorm, r, lane);
-        else choose<T, 16>(logits, t, E, k, p.c.renorm, r, lane);
+    auto clear = [&] {
+        for (int e = tid; e < E; e += kThreads) r.mask[e] = 0u;
+        if (tid == 0) r.lost = 0u;
+        __syncthreads();
+    };
+    if (E > 128) {
+        choose<T, 16, 1>(p, wave, r, lane, clear);
+        if (tokens > kWaves) choose<T, 16, 1>(p, wave + kWaves, r, lane, [] {});
+    } else if (tokens > kWaves) {
+        choose<T, 2, 2>(p, wave, r, lane, clear);
+    } else {
+        choose<T, 2, 1>(p, wave, r, lane, clear);
     }
     __syncthreads();
     if (wave == 0) {
@@ -658,6 +692,7 @@ struct Down {
                 for (int i = 0; i < 2; ++i) total[i] = __builtin_fmaf(c.scale[u / 2], n & 1 ? sum[2 * i + 1] : sum[2 * i], total[i]);
             }
         } else {
+            floatx4 less = {0.0f, 0.0f, 0.0f, 0.0f};  // (a chain of its own)
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const Run run = weight(c, s0, u);
@@ -665,7 +700,7 @@ struct Down {
                     bf16x8 high, low;
                     __builtin_memcpy(&high, b.v[u], 16);
                     __builtin_memcpy(&low, b.v[u] + 4, 16);
-                    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, run), low, acc, 0, 0, 0);
+                    less = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, run), low, less, 0, 0, 0);
                     acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, run), high, acc, 0, 0, 0);
                 } else {
                     T narrow[kRun];
@@ -678,6 +713,7 @@ struct Down {
                     }
                 }
             }
+            acc += less;
         }
     }
 
@@ -834,7 +870,8 @@ __global__ __launch_bounds__(kThreads, 2) void layer_experts_kernel(Layer p) {
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
-int most_workgroups() { return device_info().cu_count; }
+// one a CU; and a thread of each for every other's word
+int most_workgroups() { return device_info().cu_count < kThreads ? device_info().cu_count : kThreads; }
 
 struct Room {
     size_t stream, rows, h, widest, flags;  // bytes
