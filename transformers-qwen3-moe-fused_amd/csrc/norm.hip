@@ -78,6 +78,7 @@ __global__ __launch_bounds__(THREADS) void norm_bwd_kernel(const T *__restrict__
                                                           const TW *__restrict__ weight, T *__restrict__ dx,
                                                           float *__restrict__ partial, int64_t R, int H, double eps) {
     constexpr int GROUPS = THREADS / LANES, WAVES = LANES / 64;
+    constexpr bool AHEAD = WHOLE && C == 1;  // the next row is asked for before this one's sums are there (16384 x 2048: 61 -> 50 us)
     __shared__ double squares[2][GROUPS * WAVES];
     __shared__ float alongs[2][GROUPS * WAVES];
     extern __shared__ float shared_dw[];  // (GROUPS - 1, LANES * C * 8) where the groups are many
@@ -91,19 +92,32 @@ __global__ __launch_bounds__(THREADS) void norm_bwd_kernel(const T *__restrict__
         for (int u = 0; u < 8; ++u) dw[c][u] = 0.0f;
     }
     int turn = 0;
+    Eight<T, WHOLE> sv[C], g[C], d[C], next_s[C], next_g[C], next_d[C];
+    const bool add = ds != nullptr && dx != nullptr;
+    auto fetch = [&](int64_t row0, Eight<T, WHOLE>(&a)[C], Eight<T, WHOLE>(&b)[C], Eight<T, WHOLE>(&e)[C]) {
+        const int64_t at = (row0 + group < R ? row0 + group : R - 1) * H;
+#pragma unroll
+        for (int c = 0; c < C; ++c) a[c].load(s + at, (c * LANES + i) * 8, H);
+#pragma unroll
+        for (int c = 0; c < C; ++c) b[c].load(dy + at, (c * LANES + i) * 8, H);
+        if (add) {
+#pragma unroll
+            for (int c = 0; c < C; ++c) e[c].load(ds + at, (c * LANES + i) * 8, H);
+        }
+    };
+    const int64_t first = (int64_t)blockIdx.x * GROUPS, by = (int64_t)gridDim.x * GROUPS;
+    if (AHEAD) fetch(first, next_s, next_g, next_d);
     // (every group of a workgroup takes as many turns: the rows' sums wait for one another where a row has several waves)
-    for (int64_t row0 = (int64_t)blockIdx.x * GROUPS; row0 < R; row0 += (int64_t)gridDim.x * GROUPS, turn ^= 1) {
+    for (int64_t row0 = first; row0 < R; row0 += by, turn ^= 1) {
         const int64_t row = row0 + group;
         const bool in = row < R;
         const int64_t at = (in ? row : R - 1) * H;
-        Eight<T, WHOLE> sv[C], g[C], d[C];
+        if (AHEAD) {
 #pragma unroll
-        for (int c = 0; c < C; ++c) sv[c].load(s + at, (c * LANES + i) * 8, H);
-#pragma unroll
-        for (int c = 0; c < C; ++c) g[c].load(dy + at, (c * LANES + i) * 8, H);
-        if (ds != nullptr && dx != nullptr) {
-#pragma unroll
-            for (int c = 0; c < C; ++c) d[c].load(ds + at, (c * LANES + i) * 8, H);
+            for (int c = 0; c < C; ++c) sv[c] = next_s[c], g[c] = next_g[c], d[c] = next_d[c];
+            if (row0 + by < R) fetch(row0 + by, next_s, next_g, next_d);
+        } else {
+            fetch(row0, sv, g, d);
         }
         double square = 0.0;  // (32 bits hold no square of a 32-bit or bf16 value past 2^64)
         float along = 0.0f;
@@ -135,7 +149,7 @@ __global__ __launch_bounds__(THREADS) void norm_bwd_kernel(const T *__restrict__
                 const float a = to_f32(sv[c].v[u]), b = to_f32(g[c].v[u]);
                 dw[c][u] = __builtin_fmaf(b, a * r, dw[c][u]);
                 float o = r * __builtin_fmaf(-a, back, b * to_f32(w[c].v[u]));
-                if (ds != nullptr && dx != nullptr) o += to_f32(d[c].v[u]);
+                if (add) o += to_f32(d[c].v[u]);
                 sv[c].v[u] = from_f32<T>(o);
             }
             if (dx != nullptr) sv[c].store(dx + at, (c * LANES + i) * 8, H);
@@ -167,21 +181,39 @@ __global__ __launch_bounds__(THREADS) void norm_bwd_kernel(const T *__restrict__
     }
 }
 
-// dw (H) = the sum of `parts` rows of partial; 16 columns a workgroup, 16 threads a column.
+// dw (H) = the sum of `parts` rows of partial; 16 columns a workgroup, four of them a thread, 64 threads a column (512 rows of 2048:
+// 10.8 us with a column and a load of four bytes a thread, 2.5 so).
 template <typename TW>
 __global__ __launch_bounds__(256) void norm_dw_kernel(const float *__restrict__ partial, TW *__restrict__ dw, int parts, int H) {
-    __shared__ float sums[16][17];
-    const int col = threadIdx.x & 15, part = threadIdx.x >> 4, k = blockIdx.x * 16 + col;
-    float sum = 0.0f;
-    if (k < H)
-        for (int p = part; p < parts; p += 16) sum += partial[(int64_t)p * H + k];
-    sums[part][col] = sum;
-    __syncthreads();
-    if (part != 0 || k >= H) return;
-    sum = 0.0f;
+    __shared__ float sums[64][17];
+    const int part = threadIdx.x >> 2, k = blockIdx.x * 16 + (threadIdx.x & 3) * 4;
+    floatx4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (k + 4 <= H) {
+#pragma unroll 8
+        for (int p = part; p < parts; p += 64) {
+            floatx4 v;
+            __builtin_memcpy(&v, partial + (int64_t)p * H + k, 16);
+            sum += v;
+        }
+    } else {
+        for (int p = part; p < parts; p += 64)
 #pragma unroll
-    for (int p = 0; p < 16; ++p) sum += sums[p][col];
-    dw[k] = from_f32<TW>(sum);
+            for (int u = 0; u < 4; ++u)
+                if (k + u < H) sum[u] += partial[(int64_t)p * H + k + u];
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) sums[part][(threadIdx.x & 3) * 4 + u] = sum[u];
+    __syncthreads();
+    const int col = threadIdx.x & 15, group = threadIdx.x >> 4;
+    float v = sums[group * 4][col] + sums[group * 4 + 1][col] + sums[group * 4 + 2][col] + sums[group * 4 + 3][col];
+    __syncthreads();
+    sums[group][col] = v;
+    __syncthreads();
+    if (threadIdx.x >= 16 || blockIdx.x * 16 + col >= H) return;
+    v = 0.0f;
+#pragma unroll
+    for (int p = 0; p < 16; ++p) v += sums[p][col];
+    dw[blockIdx.x * 16 + col] = from_f32<TW>(v);
 }
 
 static_assert(MFL_NORM_WIDTH == 1024 * 4 * 8, "1024 threads of four runs");
@@ -191,7 +223,8 @@ constexpr int kBwdThreads = 512;
 int lanes_of(int H) { return H <= 512 ? 64 : H <= 1024 ? 128 : H <= 2048 ? 256 : H <= 4096 ? 512 : 1024; }
 int bwd_grid(int64_t R, int H) {
     const int lanes = lanes_of(H), groups = lanes < kBwdThreads ? kBwdThreads / lanes : 1;
-    const int64_t want = (R + groups - 1) / groups, most = 2 * device_info().cu_count;
+    // (as many as are resident at once)
+    const int64_t want = (R + groups - 1) / groups, most = (lanes < 1024 ? 2 : 1) * device_info().cu_count;
     return (int)(want < most ? want : most);
 }
 
