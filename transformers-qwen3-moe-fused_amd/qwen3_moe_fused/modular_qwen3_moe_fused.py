@@ -79,6 +79,14 @@ class Qwen3MoeFusedRouter(nn.Linear):
                 out = router_linear(input, self.weight)
             return super().forward(input) if out is None else out
 
+    _own_forward = forward  # (as in MoeFusedLinear)
+
+
+def _stands_for_itself(module: nn.Module) -> bool:
+    """Whether a module's call is its class's forward and nothing else: no hooks, no replaced forward."""
+    return not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks
+                or "forward" in module.__dict__ or type(module).forward is not type(module)._own_forward)
+
 
 class Qwen3MoeFusedSparseMoeBlock(nn.Module):
     """``config`` needs: num_experts, num_experts_per_tok, norm_topk_prob, hidden_size,
@@ -105,6 +113,10 @@ class Qwen3MoeFusedSparseMoeBlock(nn.Module):
     # at 32768 routed rows).  Off by default: the kernel's epilogue then does the unit's arithmetic with the matrix
     # units idle, and a training step of the block takes 1.62-1.67 ms instead of 1.58-1.63 ms.
     fuse_backward = False
+    # set to True for calls of up to 16 tokens without gradients as the whole layer in two launches (fused_mlp.moe_fused_layer; bf16,
+    # fp16, fp32 and 8-bit expert matrices; one token of 128 experts in bf16 28 us a call against 59).  Off by default: the results are
+    # not those of the separate steps bit for bit, since less is rounded on the way.
+    fuse_layer = False
     # set to True to keep the expert ids of the last call in ``last_selected`` (tests read the block's own routing)
     keep_routing = False
 
@@ -131,7 +143,37 @@ class Qwen3MoeFusedSparseMoeBlock(nn.Module):
                                       self.num_selected)
         return None
 
-    def _fused_mlp(self, tokens, m_sizes, sort_idx, inv_sort_idx) -> Optional[torch.Tensor]:
+    def whole_layer(self, tokens: torch.Tensor, residual: Optional[torch.Tensor] = None, norm_weight: Optional[torch.Tensor] = None,
+                    eps: float = 1e-6) -> Optional[Tuple[torch.Tensor, torch.Tensor]]:
+        """(out, router logits) of ``moe_fused_layer`` on the block's weights, or None where ``fuse_layer`` is off or the call is not one
+        for it: more tokens, gradients, other kinds of weights, modules that somebody watches."""
+        from .fused_mlp import LAYER_TOKENS, moe_fused_layer, moe_fused_layer_fp8
+        from .quantize.layer_fp8 import MoeFusedLinearFp8
+
+        if not (self.fuse_layer and self.fuse_front) or self.keep_routing or not 0 < tokens.shape[0] <= LAYER_TOKENS:
+            return None
+        gate, projs = self.gate, (self.gate_proj, self.up_proj, self.down_proj)
+        kind = type(projs[0])
+        if (type(gate) is not Qwen3MoeFusedRouter or gate.bias is not None or kind not in (MoeFusedLinear, MoeFusedLinearFp8)
+                or any(type(m) is not kind for m in projs) or not all(map(_stands_for_itself, (gate, *projs)))):
+            return None
+        if torch.nn.modules.module._has_any_global_hook() or not _lib.plain_call() or torch.is_autocast_enabled("cuda"):
+            return None
+        same = [gate.weight] + ([p.weight for p in projs] if kind is MoeFusedLinear else [])
+        same += [t for t in (residual, norm_weight) if t is not None]
+        if not tokens.is_cuda or tokens.dtype not in (torch.bfloat16, torch.float16, torch.float32) or self.num_experts > 1024:
+            return None
+        if any(t.dtype != tokens.dtype or t.device != tokens.device or not t.is_contiguous() for t in same):
+            return None
+        if torch.is_grad_enabled() and any(t.requires_grad for t in (tokens, *same)):
+            return None
+        if kind is MoeFusedLinear:
+            return moe_fused_layer(tokens, gate.weight, *(m.weight for m in projs), self.num_selected, self.norm_topk_prob,
+                                   residual, norm_weight, eps)
+        pairs = [t for m in projs for t in (m.weight, m.weight_scale_inv)]
+        return moe_fused_layer_fp8(tokens, gate.weight, *pairs, self.num_selected, self.norm_topk_prob, residual, norm_weight, eps)
+
+    def _fused_mlp(self, tokens, m_sizes, sort_idx, inv_sort_idx, quantized=None) -> Optional[torch.Tensor]:
         """The three projections as one node of the graph when all are plain bf16 expert matrices and a gradient
         will be asked for: the backward then runs the gated unit's backward inside the down projection's input
         gradient.  Without gradients the front half and the down projection are the same two launches anyway."""
@@ -147,7 +189,7 @@ class Qwen3MoeFusedSparseMoeBlock(nn.Module):
                     or torch.nn.modules.module._has_any_global_hook()):
                 return None
             weights = [t for p in projs for t in (p.weight, p.weight_scale_inv)]
-            return moe_fused_mlp_fp8(tokens, *weights, m_sizes, sort_idx, inv_sort_idx, self.num_selected)
+            return moe_fused_mlp_fp8(tokens, *weights, m_sizes, sort_idx, inv_sort_idx, self.num_selected, quantized)
         if not self.fuse_backward or tokens.dtype != torch.bfloat16 or not torch.is_grad_enabled():
             return None
         if any(type(p) is not MoeFusedLinear or p.weight.dtype != torch.bfloat16 for p in projs):
@@ -211,9 +253,14 @@ class Qwen3MoeFusedSparseMoeBlock(nn.Module):
             self.last_selected = ws[:n * k * 8].view(torch.int64).view(n, k).clone()  # (not the whole workspace)
         return out
 
-    def forward(self, hidden_states: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    def forward(self, hidden_states: torch.Tensor, quantized: Optional[Tuple[torch.Tensor, torch.Tensor]] = None
+                ) -> Tuple[torch.Tensor, torch.Tensor]:
+        """``quantized``: what ``add_rms_norm_fp8`` made of the hidden states already, which 8-bit experts then do not make again."""
         batch, seq, hidden = hidden_states.shape
         tokens = hidden_states.reshape(batch * seq, hidden).contiguous()
+        whole = self.whole_layer(tokens) if self.fuse_layer else None
+        if whole is not None:
+            return whole[0].view(batch, seq, hidden), whole[1]
         if self.fuse_front and not self.fuse_backward:
             router_logits = self.gate(tokens)
             out = self._one_call(tokens, router_logits.contiguous())
@@ -225,7 +272,7 @@ class Qwen3MoeFusedSparseMoeBlock(nn.Module):
             routed = route_tokens(self, tokens)
         router_logits, routing_weights, m_sizes, sort_idx, inv_sort_idx = routed
 
-        y = self._fused_mlp(tokens, m_sizes, sort_idx, inv_sort_idx) if self.fuse_front else None
+        y = self._fused_mlp(tokens, m_sizes, sort_idx, inv_sort_idx, quantized) if self.fuse_front else None
         if y is None:
             h = self._fused_front(tokens, m_sizes, sort_idx, inv_sort_idx) if self.fuse_front else None
             if h is None:
@@ -242,8 +289,8 @@ def _hf_subclasses():
     built on demand so that importing this module does not import transformers."""
     import inspect
 
-    from transformers.models.qwen3_moe.modeling_qwen3_moe import (Qwen3MoeDecoderLayer, Qwen3MoeForCausalLM,
-                                                                  Qwen3MoeMLP, Qwen3MoeModel, Qwen3MoeSparseMoeBlock)
+    from transformers.models.qwen3_moe.modeling_qwen3_moe import (Qwen3MoeDecoderLayer, Qwen3MoeForCausalLM, Qwen3MoeMLP,
+                                                                  Qwen3MoeModel, Qwen3MoeRMSNorm, Qwen3MoeSparseMoeBlock)
 
     # The reference was written against a transformers revision whose sparse block returns
     # (hidden_states, router_logits) (modular_qwen3_moe_fused.py:1,118); later releases return the
@@ -251,18 +298,63 @@ def _hf_subclasses():
     block_cls = Qwen3MoeFusedSparseMoeBlock
     if inspect.signature(Qwen3MoeSparseMoeBlock.forward).return_annotation is torch.Tensor:
         class _TensorBlock(Qwen3MoeFusedSparseMoeBlock):
-            def forward(self, hidden_states: torch.Tensor) -> torch.Tensor:
-                return super().forward(hidden_states)[0]
+            def forward(self, hidden_states: torch.Tensor,
+                        quantized: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> torch.Tensor:
+                return super().forward(hidden_states, quantized)[0]
 
         block_cls = _TensorBlock
 
+    stock_forward = inspect.signature(Qwen3MoeDecoderLayer.forward)
+
     class Qwen3MoeFusedDecoderLayer(Qwen3MoeDecoderLayer):
+        # set to True for the addition behind the attention and the norm in front of the experts as one kernel (kernels/norm.py), both
+        # ways, with 8-bit experts also to the rows that they multiply; with the block's ``fuse_layer`` a call of up to 16 tokens without
+        # gradients is two launches from there to the layer's result.  Off by default: the stock norm rounds once more.
+        fuse_norm = False
+
         def __init__(self, config, layer_idx: int) -> None:
             super().__init__(config, layer_idx)
             sparse = (layer_idx not in config.mlp_only_layers and config.num_experts > 0
                       and (layer_idx + 1) % config.decoder_sparse_step == 0)
             self.mlp = (block_cls(config) if sparse
                         else Qwen3MoeMLP(config, intermediate_size=config.intermediate_size))
+
+        def forward(self, hidden_states: torch.Tensor, *args, **kwargs):
+            norm = self.post_attention_layernorm
+            # (of releases whose block returns its logits the layer's results are another matter: their forward stays theirs)
+            if (not self.fuse_norm or block_cls is Qwen3MoeFusedSparseMoeBlock or type(norm) is not Qwen3MoeRMSNorm
+                    or norm._forward_hooks or norm._forward_pre_hooks or norm._backward_hooks or norm._backward_pre_hooks
+                    or "forward" in norm.__dict__ or torch.nn.modules.module._has_any_global_hook() or not _lib.plain_call()):
+                return super().forward(hidden_states, *args, **kwargs)
+            given = stock_forward.bind(self, hidden_states, *args, **kwargs)
+            given.apply_defaults()
+            rest = {k: v for k, v in list(given.arguments.items())[2:] if k != "kwargs"}
+            rest.update(given.arguments.get("kwargs", {}))
+            attention = self.self_attn(hidden_states=self.input_layernorm(hidden_states), **rest)[0]
+            return self._feed_forward(attention, hidden_states, norm)
+
+        def _feed_forward(self, x: torch.Tensor, residual: torch.Tensor, norm: nn.Module) -> torch.Tensor:
+            from .kernels.norm import add_rms_norm, add_rms_norm_fp8
+            from .quantize.layer_fp8 import MoeFusedLinearFp8
+
+            weight, eps = norm.weight, norm.variance_epsilon
+            if (not x.is_cuda or x.dtype != residual.dtype or x.shape != residual.shape or x.device != residual.device
+                    or x.dtype not in (torch.bfloat16, torch.float16, torch.float32) or weight.dtype not in (x.dtype, torch.float32)
+                    or x.shape[-1] > 32768 or torch.is_autocast_enabled("cuda")):
+                s = residual + x
+                return s + self.mlp(norm(s))
+            x, residual = _lib.dense(x), _lib.dense(residual)
+            if isinstance(self.mlp, Qwen3MoeFusedSparseMoeBlock) and x.numel():
+                flat, flat_residual = x.view(-1, x.shape[-1]), residual.view(-1, x.shape[-1])
+                watched = self.mlp._forward_hooks or self.mlp._forward_pre_hooks or "forward" in self.mlp.__dict__
+                whole = None if watched else self.mlp.whole_layer(flat, flat_residual, weight, eps)
+                if whole is not None:
+                    return whole[0].view(x.shape)
+                if type(self.mlp.gate_proj) is MoeFusedLinearFp8:
+                    values, scales, s, y = add_rms_norm_fp8(flat, flat_residual, weight, eps, return_normed=True)
+                    return s.view(x.shape) + self.mlp(y.view(x.shape), quantized=(values, scales))
+            y, s = add_rms_norm(x, residual, weight, eps)
+            return s + self.mlp(y)
 
     # Releases that record outputs through forward hooks take the router logits from the stock router
     # class; the fused block's router is hooked the same way (output_router_logits, the auxiliary
