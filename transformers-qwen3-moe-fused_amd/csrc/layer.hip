@@ -309,17 +309,20 @@ struct alignas(16) Run {
     uint64_t v[2];
 };
 
-// 16 bytes of a row from element k on, zeros from element K on; WHOLE: K is a multiple of what they hold.  In two steps, so that
-// nothing is computed from what is still on its way: `fetch` loads (the row's last 16 bytes where its end cuts the run), `settle`, called
-// where the values are needed, moves them down.
-template <bool WHOLE, typename E>
+// How the sizes fit the loads.  kExact: every load of every wave lies in its row (64 KB of a row of gate and up, as many of down): nothing
+// is asked, 3 % of a call; kWhole: rows are whole loads long; kRagged: any.
+enum Fit { kRagged, kWhole, kExact };
+
+// 16 bytes of a row from element k on, zeros from element K on.  In two steps: `fetch` loads, always and without a branch, so that the
+// compiler can count what is on its way behind what it waits for; `settle`, called where the values are needed, puts zeros in the place of
+// what lies behind the row's end (ragged: fetch loads the row's last 16 bytes where the end cuts the run, and settle moves them down).
+template <int FIT, typename E>
 __device__ __forceinline__ Run fetch(const E *row, int k, int K) {
     constexpr int count = 16 / (int)sizeof(E);
     Run run;
-    if (WHOLE) {
-        if (k < K) __builtin_memcpy(&run, row + k, 16);
-        else run.v[0] = run.v[1] = 0u;
-    } else if (K >= count) {
+    if (FIT == kExact) {
+        __builtin_memcpy(&run, row + k, 16);
+    } else if (FIT == kWhole || K >= count) {
         __builtin_memcpy(&run, row + (k + count <= K ? k : K - count), 16);
     } else {
         run.v[0] = run.v[1] = 0u;
@@ -334,10 +337,16 @@ __device__ __forceinline__ Run fetch(const E *row, int k, int K) {
     }
     return run;
 }
-template <bool WHOLE, typename E>
+template <int FIT, typename E>
 __device__ __forceinline__ Run settle(Run run, int k, int K) {
     constexpr int count = 16 / (int)sizeof(E);
-    if (WHOLE || K < count) return run;
+    if (FIT == kExact) return run;
+    if (FIT == kWhole) {
+        run.v[0] = k < K ? run.v[0] : 0u;
+        run.v[1] = k < K ? run.v[1] : 0u;
+        return run;
+    }
+    if (K < count) return run;
     const int moved = k + count <= K ? 0 : (k + count - K) * 8 * (int)sizeof(E);
     const uint64_t lo = run.v[0], hi = run.v[1];
     run.v[0] = moved == 0 ? lo : moved < 64 ? lo >> moved | hi << (64 - moved) : moved < 128 ? hi >> (moved - 64) : 0u;
@@ -376,7 +385,7 @@ constexpr int kDeviceScope = 16;  // a buffer load's sc1 bit
 // registers where its share of the reduction is one chunk.  The next item's weights are asked for before the waves meet.
 typedef floatx4 Parts[2][2][kWaves][64];
 
-template <typename T, bool FP8, bool WHOLE>
+template <typename T, bool FP8, int FIT>
 struct GateUp {
     typedef Weights<T, FP8> W;
     typedef typename W::Element Element;
@@ -409,13 +418,13 @@ struct GateUp {
     }
 
     // the first element of the lane's run of a step; H behind the wave's share
-    __device__ __forceinline__ int element(int step) const { return step < end ? step * kStep + g * kRun : p.c.H; }
+    __device__ __forceinline__ int element(int step) const { return FIT == kExact || step < end ? step * kStep + g * kRun : p.c.H; }
     __device__ __forceinline__ void load_weights(Weight &to, int item, int s0) const {
         const int H = p.c.H, I = p.c.I, tile = item % tiles, col = tile * 8 + (n & 7);
         const int e = __builtin_amdgcn_readfirstlane(r.expert[item / tiles]);
         const Element *const w = (const Element *)(n < 8 ? p.c.w_gate : p.c.w_up) + ((int64_t)e * I + (col < I ? col : I - 1)) * H;
 #pragma unroll
-        for (int u = 0; u < U; ++u) to.a[u] = fetch<WHOLE>(w, element(s0 + u), H);
+        for (int u = 0; u < U; ++u) to.a[u] = fetch<FIT>(w, element(s0 + u), H);
         if (FP8) {
             const int64_t block = ((int64_t)e * fp8_blocks(I) + tile * 8 / kFp8Block) * fp8_blocks(H);
             // (of the results that the lane holds, not of the rows that it loads)
@@ -430,13 +439,13 @@ struct GateUp {
         for (int u = 0; u < U; ++u) {
             // (8-bit layers: rows of whole blocks, zeros behind column H)
             if constexpr (FP8) __builtin_memcpy(b[u], s0 + u < end ? x + (s0 + u) * kStep + g * kRun : x, sizeof(b[u]));
-            else b[u][0] = settle<WHOLE, X>(fetch<WHOLE>(x, element(s0 + u), p.c.H), element(s0 + u), p.c.H);
+            else b[u][0] = settle<FIT, X>(fetch<FIT>(x, element(s0 + u), p.c.H), element(s0 + u), p.c.H);
         }
     }
     __device__ __forceinline__ void multiply(const Weight &weight, int s0, floatx4 &acc) const {
         Run a[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) a[u] = settle<WHOLE, Element>(weight.a[u], element(s0 + u), p.c.H);
+        for (int u = 0; u < U; ++u) a[u] = settle<FIT, Element>(weight.a[u], element(s0 + u), p.c.H);
         if constexpr (FP8) {
 #pragma unroll
             for (int u = 0; u < U / 2; ++u) {
@@ -471,43 +480,60 @@ struct GateUp {
         }
     }
 
-    // Items from, from + by, ... below to; the waves meet once for kGroup of them.  `turn` counts a workgroup's meetings.
-    __device__ __forceinline__ void run(int from, int to, int by, Parts &parts, int &turn) {
+    // One meeting of the waves: items item, item + by, ... (kGroup of them, as far as they are below to) from w[d], w[d + 1], ..., which are
+    // loaded again, with the items D on: ALL, or as far as there are any.
+    template <bool ALL>
+    __device__ __forceinline__ void meet(int d, int item, int to, int by, Parts &parts, int turn) {
+        floatx4 acc[kGroup];
 #pragma unroll
-        for (int d = 0; d < D; ++d)
-            if (from + d * by < to) load_weights(w[d], from + d * by, begin);
-        for (int i = from; i < to; i += D * by) {
+        for (int o = 0; o < kGroup; ++o) acc[o] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int c = 0; c < chunks; ++c) {
+            if (c != 0) {
+#pragma unroll
+                for (int o = 0; o < kGroup; ++o)
+                    if (ALL || item + o * by < to) load_weights(w[d + o], item + o * by, begin + c * U);
+            }
+            if (chunks != 1) load_rows(begin + c * U);
+#pragma unroll
+            for (int o = 0; o < kGroup; ++o)
+                if (ALL || item + o * by < to) multiply(w[d + o], begin + c * U, acc[o]);
+        }
+        floatx4(*const part)[kWaves][64] = parts[turn & 1];
+#pragma unroll
+        for (int o = 0; o < kGroup; ++o) {
+            if (ALL || item + (D + o) * by < to) load_weights(w[d + o], item + (D + o) * by, begin);
+            if (ALL || item + o * by < to) part[o][wave][lane] = acc[o];
+        }
+        __syncthreads();
+        // as many waves finish an item each, others every time
+        const int mine = (wave - kGroup * turn) & (kWaves - 1);
+        if (mine >= kGroup || (!ALL && item + mine * by >= to)) return;
+#pragma unroll
+        for (int v = 0; v < kWaves; ++v) acc[0] = v == 0 ? part[mine][0][lane] : acc[0] + part[mine][v][lane];
+        finish(item + mine * by, acc[0]);
+    }
+    // Items from, from + by, ... below to; `turn` counts a workgroup's meetings.
+    __device__ __forceinline__ void run(int from, int to, int by, Parts &parts, int &turn) {
+        int i = from;
+        // (A loop in which nothing is loaded or not: else the compiler waits for all that might be the last.  Four items of 4 KB a wave
+        // need it, 13 tokens in 8 bits 84 -> 70 us; two of 8 KB fill the memory without, and lose what its registers cost.)
+        if (FP8 && i + (2 * D - 1) * by < to) {
+#pragma unroll
+            for (int d = 0; d < D; ++d) load_weights(w[d], i + d * by, begin);
+            for (; i + (2 * D - 1) * by < to; i += D * by) {
+#pragma unroll
+                for (int d = 0; d < D; d += kGroup, ++turn) meet<true>(d, i + d * by, to, by, parts, turn);
+            }
+        } else {
+#pragma unroll
+            for (int d = 0; d < D; ++d)
+                if (i + d * by < to) load_weights(w[d], i + d * by, begin);
+        }
+        for (; i < to; i += D * by) {
 #pragma unroll
             for (int d = 0; d < D; d += kGroup, ++turn) {
-                const int item = i + d * by;
-                if (item >= to) break;
-                floatx4 acc[kGroup];
-#pragma unroll
-                for (int o = 0; o < kGroup; ++o) acc[o] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-                for (int c = 0; c < chunks; ++c) {
-                    if (c != 0) {
-#pragma unroll
-                        for (int o = 0; o < kGroup; ++o)
-                            if (item + o * by < to) load_weights(w[d + o], item + o * by, begin + c * U);
-                    }
-                    if (chunks != 1) load_rows(begin + c * U);
-#pragma unroll
-                    for (int o = 0; o < kGroup; ++o)
-                        if (item + o * by < to) multiply(w[d + o], begin + c * U, acc[o]);
-                }
-                floatx4(*const part)[kWaves][64] = parts[turn & 1];
-#pragma unroll
-                for (int o = 0; o < kGroup; ++o) {
-                    if (item + (D + o) * by < to) load_weights(w[d + o], item + (D + o) * by, begin);
-                    if (item + o * by < to) part[o][wave][lane] = acc[o];
-                }
-                __syncthreads();
-                // as many waves finish an item each, others every time
-                const int mine = (wave - kGroup * turn) & (kWaves - 1);
-                if (mine >= kGroup || item + mine * by >= to) continue;
-#pragma unroll
-                for (int v = 0; v < kWaves; ++v) acc[0] = v == 0 ? part[mine][0][lane] : acc[0] + part[mine][v][lane];
-                finish(item + mine * by, acc[0]);
+                if (i + d * by >= to) break;
+                meet<false>(d, i + d * by, to, by, parts, turn);
             }
         }
     }
@@ -561,23 +587,23 @@ struct GateUp {
 // work is for nothing, but it has a thirtieth of its time to do.)
 constexpr int kParts = 2, kColumns = 16 / kParts;
 typedef float Sums[kWaves][kTokens][kColumns];
-constexpr int kStagedRow = kParts * 6 * 64 + 8;  // (8-bit layers) elements of a staged row: a chunk, and 16 bytes more for the banks
+constexpr int kStageBytes = 12544;  // of LDS for a wave's rows of h
 
 // A chunk of an expert's weights for an item: U steps of the lane's row and part.
 // (Six where more would not fit the registers: rows that have to be moved down, and fp16, which is widened: 61 -> 44 us at 5 tokens of
 // 1001 x 333.)
-template <typename T, bool FP8, bool WHOLE>
+template <typename T, bool FP8, int FIT>
 struct Chunk {
-    static constexpr int U = FP8 || !WHOLE || std::is_same<T, f16_t>::value ? 6 : 12;
+    static constexpr int U = FP8 || FIT == kRagged || std::is_same<T, f16_t>::value ? 6 : 12;
     Run a[U];
     float scale[U / 2];
 };
 
-template <typename T, bool FP8, bool WHOLE>
+template <typename T, bool FP8, int FIT>
 struct Down {
     typedef Weights<T, FP8> W;
     typedef typename W::Element Element;
-    static constexpr int kRun = W::kRun, kStep = W::kStep, U = Chunk<T, FP8, WHOLE>::U;
+    static constexpr int kRun = W::kRun, kStep = W::kStep, U = Chunk<T, FP8, FIT>::U;
     static constexpr int kUnit = FP8 ? kFp8Block : kRun;
     const Layer &p;
     const Routing &r;
@@ -593,14 +619,14 @@ struct Down {
           left(p.c.I - from < length ? (p.c.I - from < 0 ? 0 : p.c.I - from) : length), nb(fp8_blocks(p.c.H)), kb(fp8_blocks(p.c.I)),
           h_bytes((uint32_t)(p.c.T * p.c.k * p.ldh * 4)), h(__builtin_amdgcn_make_buffer_rsrc(p.h, 0, (int)h_bytes, 0x00020000)) {}
 
-    __device__ __forceinline__ void load(Chunk<T, FP8, WHOLE> &c, int tile, int at, int s0) const {
+    __device__ __forceinline__ void load(Chunk<T, FP8, FIT> &c, int tile, int at, int s0) const {
         const int row = tile * kColumns + n / kParts, H = p.c.H, e = __builtin_amdgcn_readfirstlane(r.expert[at]);
         const Element *const w = (const Element *)p.c.w_down + ((int64_t)e * H + (row < H ? row : H - 1)) * p.c.I;
         // (the lane's part ends where the next begins, or with the row: a run that the row's end cuts is the last one of all)
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int k = (s0 + u) * kStep + g * kRun;
-            c.a[u] = fetch<WHOLE>(w, s0 + u < steps && k < length ? from + k : p.c.I, p.c.I);
+            c.a[u] = fetch<FIT>(w, FIT == kExact || (s0 + u < steps && k < length) ? from + k : p.c.I, p.c.I);
         }
         if (FP8) {
             const float *const scale = p.c.s_down + ((int64_t)e * nb + tile * kColumns / kFp8Block) * kb;
@@ -609,72 +635,66 @@ struct Down {
         }
     }
 
-    __device__ __forceinline__ Run weight(const Chunk<T, FP8, WHOLE> &c, int s0, int u) const {
+    __device__ __forceinline__ Run weight(const Chunk<T, FP8, FIT> &c, int s0, int u) const {
         const int k = (s0 + u) * kStep + g * kRun;
-        return settle<WHOLE, Element>(c.a[u], s0 + u < steps && k < length ? from + k : p.c.I, p.c.I);
+        return settle<FIT, Element>(c.a[u], s0 + u < steps && k < length ? from + k : p.c.I, p.c.I);
     }
 
-    // The lane's row of h for a chunk.  (8-bit: not here, but in LDS, see stage.)
-    struct alignas(16) Rows {
-        float v[FP8 ? 1 : U][kRun];
+    // The rows of h for a chunk go through LDS, a part of it for every wave: loaded by the whole wave, each value once (in registers the
+    // lanes that multiply the same one would each load it, twice the bytes of the weights), and in 8-bit layers rounded on the way, to what
+    // the rounded values stand for.  The next chunk's first rows are on their way while this one is multiplied.
+    static constexpr int kSize = FP8 ? 2 : 4, kSlots = FP8 ? kColumns : 4;  // bytes of an element, rows
+    static constexpr int kPart = U * kStep, kStaged = kParts * kPart;         // elements of a part and of both
+    static constexpr int kPartBytes = kPart * kSize + 16, kRowBytes = kParts * kPartBytes;  // (16 bytes more: other banks for every part)
+    static constexpr int kTurns = (kStaged + 255) / 256, kAhead = 2;
+    static_assert(kSlots * kRowBytes <= kStageBytes, "room for a wave's rows");
+    struct Staged {
+        floatx4 v[kTurns];
+        uint32_t top[kTurns];
     };
-    __device__ __forceinline__ void load_rows(Rows &b, int s0, int pair) const {
-        // (rows of h are whole runs long, zeros behind column I; behind the last row the loads return zeros)
-        const uint32_t row = (uint32_t)pair * (uint32_t)p.ldh * 4u;
+    // (rows of h are whole runs long, zeros behind column I; behind the last row the loads return zeros)
+    __device__ __forceinline__ void stage_load(Staged &s, int s0, int pair) const {
 #pragma unroll
-        for (int u = 0; u < (FP8 ? 1 : U); ++u) {
-            const int k = (s0 + u) * kStep + g * kRun;
-            const uint32_t at = s0 + u < steps && k < left ? row + (uint32_t)(from + k) * 4u : h_bytes;
-#pragma unroll
-            for (int i = 0; i < kRun; i += 4) {
-                const auto v = __builtin_amdgcn_raw_buffer_load_b128(h, (int)at, i * 4, kDeviceScope);
-                __builtin_memcpy(b.v[u] + i, &v, 16);
+        for (int i = 0; i < kTurns; ++i) {
+            const int x = i * 256 + lane * 4, part = x / kPart, k = s0 * kStep + x - part * kPart, at = part * length + k;
+            const bool in = part < kParts && k < length && at < (int)p.ldh;
+            const auto v = __builtin_amdgcn_raw_buffer_load_b128(h, (int)(in ? ((uint32_t)pair * (uint32_t)p.ldh + (uint32_t)at) * 4u : h_bytes), 0, kDeviceScope);
+            s.v[i] = __builtin_bit_cast(floatx4, v);
+            if constexpr (FP8) {
+                s.top[i] = 0u;
+                if (in && at < p.c.I) s.top[i] = peek(p.widest + (int64_t)pair * kb + at / kFp8Block);
             }
         }
     }
-    // 8-bit layers: a chunk of up to eight rows of h, quantised by the whole wave (a value once, not once for every lane that multiplies
-    // it: 48 of them) and left in the wave's own part of LDS as what the rounded values stand for.
-    static constexpr int kStaged = kParts * U * kStep;  // elements of a row and chunk
-    static_assert(!FP8 || (kStaged % 256 == 0 && kStaged <= kStagedRow), "four elements a lane at a time");
-    struct Staged {
-        floatx4 v[FP8 ? kStaged / 256 : 1];
-        uint32_t top[FP8 ? kStaged / 256 : 1];
-    };
-    __device__ __forceinline__ void stage_load(Staged &s, int s0, int pair) const {
+    __device__ __forceinline__ void stage_store(const Staged &s, unsigned char *row) const {
 #pragma unroll
-        for (int i = 0; i < kStaged / 256; ++i) {
-            const int x = i * 256 + lane * 4, part = x / (U * kStep), k = s0 * kStep + x - part * (U * kStep), at = part * length + k;
-            const bool in = k < length && at < (int)p.ldh;
-            const auto v = __builtin_amdgcn_raw_buffer_load_b128(h, (int)(in ? ((uint32_t)pair * (uint32_t)p.ldh + (uint32_t)at) * 4u : h_bytes), 0, kDeviceScope);
-            s.v[i] = __builtin_bit_cast(floatx4, v);
-            s.top[i] = 0u;
-            if (in && at < p.c.I) s.top[i] = peek(p.widest + (int64_t)pair * kb + at / kFp8Block);
-        }
-    }
-    __device__ __forceinline__ void stage_store(const Staged &s, bf16_t *row) const {
-        typedef __attribute__((ext_vector_type(2))) short shortx2;
-#pragma unroll
-        for (int i = 0; i < kStaged / 256; ++i) {
-            const float scale = fp8_scale_of(fp8_scale_byte(s.top[i]));
-            shortx2 r = {};
-            r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, s.v[i][0], s.v[i][1], scale, false);
-            r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, s.v[i][2], s.v[i][3], scale, true);
-            const int q = __builtin_bit_cast(int, r);
-            union {
-                bf16x2 p[2];
-                uint2_t d;
-            } o;
-            o.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q, scale, false);
-            o.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q, scale, true);
-            *(uint2_t *)(row + i * 256 + lane * 4) = o.d;
+        for (int i = 0; i < kTurns; ++i) {
+            const int x = i * 256 + lane * 4, part = x / kPart;
+            unsigned char *const to = row + x * kSize + part * 16;
+            if (kStaged % 256 != 0 && part >= kParts) continue;
+            if constexpr (FP8) {
+                typedef __attribute__((ext_vector_type(2))) short shortx2;
+                const float scale = fp8_scale_of(fp8_scale_byte(s.top[i]));
+                shortx2 q = {};
+                q = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(q, s.v[i][0], s.v[i][1], scale, false);
+                q = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(q, s.v[i][2], s.v[i][3], scale, true);
+                union {
+                    bf16x2 p[2];
+                    uint2_t d;
+                } o;
+                o.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(__builtin_bit_cast(int, q), scale, false);
+                o.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(__builtin_bit_cast(int, q), scale, true);
+                *(uint2_t *)to = o.d;
+            } else {
+                *(floatx4 *)to = s.v[i];
+            }
         }
     }
 
     // acc += the chunk times the lane's row (8-bit: total, block by block)
-    __device__ __forceinline__ void multiply(const Chunk<T, FP8, WHOLE> &c, const Rows &b, const bf16_t *staged, int s0, floatx4 &acc,
-                                             floatx2 &total) const {
+    __device__ __forceinline__ void multiply(const Chunk<T, FP8, FIT> &c, const unsigned char *staged, int s0, floatx4 &acc, floatx2 &total) const {
+        const unsigned char *const row = staged + n / kParts % kSlots * kRowBytes + n % kParts * kPartBytes + g * kRun * kSize;
         if constexpr (FP8) {
-            const bf16_t *const row = staged + n / kParts * kStagedRow + n % kParts * (U * kStep) + g * kRun;
 #pragma unroll
             for (int u = 0; u < U; u += 2) {
                 floatx4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -686,7 +706,7 @@ struct Down {
                     } f = {weight(c, s0, u + o)};
 #pragma unroll
                     for (int z = 0; z < 2; ++z)
-                        sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp8_widen(f.t[z], 1.0f), *(const bf16x8 *)(row + (u + o) * kStep + 8 * z), sum, 0, 0, 0);
+                        sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp8_widen(f.t[z], 1.0f), *(const bf16x8 *)(row + (u + o) * kStep * kSize + 16 * z), sum, 0, 0, 0);
                 }
 #pragma unroll
                 for (int i = 0; i < 2; ++i) total[i] = __builtin_fmaf(c.scale[u / 2], n & 1 ? sum[2 * i + 1] : sum[2 * i], total[i]);
@@ -696,20 +716,18 @@ struct Down {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const Run run = weight(c, s0, u);
+                const unsigned char *const b = row + u * kStep * kSize;
                 if constexpr (kHalves<T, FP8>) {
-                    bf16x8 high, low;
-                    __builtin_memcpy(&high, b.v[u], 16);
-                    __builtin_memcpy(&low, b.v[u] + 4, 16);
-                    less = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, run), low, less, 0, 0, 0);
-                    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, run), high, acc, 0, 0, 0);
+                    less = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, run), *(const bf16x8 *)(b + 16), less, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, run), *(const bf16x8 *)b, acc, 0, 0, 0);
                 } else {
                     T narrow[kRun];
                     __builtin_memcpy(narrow, &run, 16);
 #pragma unroll
                     for (int z = 0; z < kRun; z += 4) {
-                        const float av[4] = {to_f32(narrow[z]), to_f32(narrow[z + 1]), to_f32(narrow[z + 2]), to_f32(narrow[z + 3])};
-                        const float bv[4] = {b.v[u][z], b.v[u][z + 1], b.v[u][z + 2], b.v[u][z + 3]};
-                        acc = mfma_f32(av, bv, acc);
+                        const floatx4 v = *(const floatx4 *)(b + 4 * z);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(to_f32(narrow[z + i]), v[i], acc, 0, 0, 0);
                     }
                 }
             }
@@ -717,7 +735,7 @@ struct Down {
         }
     }
 
-    // What a wave multiplies of an item, one after the other: experts, eight tokens at a time (hardly any expert has more: its weights
+    // What a wave multiplies of an item, one after the other: experts, kSlots tokens at a time (hardly any expert has more: its weights
     // are read again then, from the caches), chunks of the reduction.
     struct Place {
         int at, q, s0;
@@ -726,39 +744,37 @@ struct Down {
     __device__ __forceinline__ Place after(Place x) const {
         x.s0 += U;
         if (x.s0 < steps) return x;
-        x.s0 = 0, x.q += kColumns;
+        x.s0 = 0, x.q += kSlots;
         if (x.q < rows_of(x.at)) return x;
         x.q = 0, x.at += kWaves;
         return x;
     }
-    // Place x with its weights in c; those of y, if there is one, are asked for behind the rows of x: loads come back in order.
-    __device__ __forceinline__ void one(const Chunk<T, FP8, WHOLE> &c, Place x, Chunk<T, FP8, WHOLE> &d, Place y, int tile, floatx4 &acc, floatx2 &total,
-                                        float (*sums)[kTokens][kColumns], bf16_t *staged) const {
+    __device__ __forceinline__ void rows_ahead(Staged (&s)[kAhead], Place x) const {
+        const int first = __builtin_amdgcn_readfirstlane(r.first[x.at]), count = rows_of(x.at) - x.q;
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+            if (j < count) stage_load(s[j], x.s0, first + x.q + j);
+    }
+    // Place x with its weights in c and its first rows in s; those of y, if there is one, are asked for before it is multiplied, the rows
+    // first: loads come back in order.
+    __device__ __forceinline__ void one(const Chunk<T, FP8, FIT> &c, Place x, Chunk<T, FP8, FIT> &d, Place y, Staged (&s)[kAhead], int tile,
+                                        floatx4 &acc, floatx2 &total, float (*sums)[kTokens][kColumns], unsigned char *staged) const {
         const int first = __builtin_amdgcn_readfirstlane(r.first[x.at]), rows = rows_of(x.at);
-        const int mine = x.q + n / kParts, pair = first + (mine < rows ? mine : rows - 1);
+        const int slot = n / kParts, mine = x.q + slot, count = rows - x.q < kSlots ? rows - x.q : kSlots;
         if (x.s0 == 0) acc = floatx4{0.0f, 0.0f, 0.0f, 0.0f}, total = floatx2{0.0f, 0.0f};
-        Rows b;
-        if constexpr (FP8) {
-            // (two rows in flight; hardly any expert has more)
-            Staged s[2];
-            const int count = rows - x.q < kColumns ? rows - x.q : kColumns;
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-                if (j < count) stage_load(s[j], x.s0, first + x.q + j);
-            if (y.at < r.experts) load(d, tile, y.at, y.s0);
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-                if (j < count) stage_store(s[j], staged + j * kStagedRow);
-            for (int j = 2; j < count; ++j) {
-                stage_load(s[0], x.s0, first + x.q + j);
-                stage_store(s[0], staged + j * kStagedRow);
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        } else {
-            load_rows(b, x.s0, pair);
-            if (y.at < r.experts) load(d, tile, y.at, y.s0);
+        for (int j = 0; j < kAhead; ++j)
+            if (j < count) stage_store(s[j], staged + j * kRowBytes);
+        for (int j = kAhead; j < count; ++j) {
+            stage_load(s[0], x.s0, first + x.q + j);
+            stage_store(s[0], staged + j * kRowBytes);
         }
-        multiply(c, b, staged, x.s0, acc, total);
+        if (y.at < r.experts) {
+            rows_ahead(s, y);
+            load(d, tile, y.at, y.s0);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        multiply(c, staged, x.s0, acc, total);
         if (x.s0 + U < steps) return;
         // lane (n, g): columns 2 g and 2 g + 1, part i % 2 in acc[i], for the token and the part of n
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -766,24 +782,27 @@ struct Down {
         for (int i = 0; i < 2; ++i) {
             float v = FP8 ? total[i] : n & 1 ? acc[2 * i + 1] : acc[2 * i];
             v += __shfl_xor(v, 1);
-            if ((n & 1) == 0 && mine < rows) sums[wave][r.token[first + mine]][2 * g + i] += r.weight[first + mine] * v;
+            if ((n & 1) == 0 && slot < count) sums[wave][r.token[first + mine]][2 * g + i] += r.weight[first + mine] * v;
         }
     }
 
     // `c`: the wave's first chunk of the item, loaded already where it has one.  What comes next is asked for before a chunk is multiplied.
-    __device__ __forceinline__ void item(Chunk<T, FP8, WHOLE> &c, int tile, float (*sums)[kTokens][kColumns], bf16_t *staged) const {
+    __device__ __forceinline__ void item(Chunk<T, FP8, FIT> &c, int tile, float (*sums)[kTokens][kColumns], unsigned char *staged) const {
         static_assert(kTokens * kColumns == 128, "two sums a lane");
         (&sums[wave][0][0])[lane] = 0.0f;  // (a wave's own: its LDS operations keep their order)
         (&sums[wave][0][0])[lane + 64] = 0.0f;
         floatx4 acc;
         floatx2 total;
-        Chunk<T, FP8, WHOLE> d;
+        Chunk<T, FP8, FIT> d;
+        Staged s[kAhead];
+        if (wave < r.experts) rows_ahead(s, {wave, 0, 0});
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // (vmcnt(0): in the loop the rows are waited for with the weights behind them on their way)
         for (Place x = {wave, 0, 0}; x.at < r.experts;) {
             const Place y = after(x);
-            one(c, x, d, y, tile, acc, total, sums, staged);
+            one(c, x, d, y, s, tile, acc, total, sums, staged);
             if (y.at >= r.experts) break;
             x = after(y);
-            one(d, y, c, x, tile, acc, total, sums, staged);
+            one(d, y, c, x, s, tile, acc, total, sums, staged);
         }
         __syncthreads();
         const int t = threadIdx.x / kColumns, col = tile * kColumns + threadIdx.x % kColumns;
@@ -803,14 +822,14 @@ struct Down {
 // free, 1 claimed, 2 done.  A workgroup claims its own unit; before it waits for anything it looks whether there is one that nobody has
 // claimed (of a workgroup that has not started yet) and does it in the other's place.  Whoever claims a unit is running, and waits for
 // nothing before the unit is done: every wait ends, however many of the workgroups are there at once.
-template <typename T, bool FP8, bool WHOLE>
+template <typename T, bool FP8, int FIT>
 __global__ __launch_bounds__(kThreads, 2) void layer_experts_kernel(Layer p) {
     __shared__ Routing r;
     __shared__ union {
         Parts parts;
         struct {
             Sums sums[2];
-            alignas(16) bf16_t staged[FP8 ? kWaves : 1][FP8 ? kColumns * kStagedRow : 8];
+            alignas(16) unsigned char staged[kWaves][kStageBytes];
         } back;
     } room;
     __shared__ int found;
@@ -823,8 +842,8 @@ __global__ __launch_bounds__(kThreads, 2) void layer_experts_kernel(Layer p) {
     const int tiles = (int)(p.ldh / 8), items = r.experts * tiles, units = items < G ? items : G;
     const int last = ceil_div(p.c.H, kColumns);
     int turn = 0;
-    const Down<T, FP8, WHOLE> down(p, r);
-    Chunk<T, FP8, WHOLE> c;
+    const Down<T, FP8, FIT> down(p, r);
+    Chunk<T, FP8, FIT> c;
     if ((int)blockIdx.x >= units) unit = -1;
     for (;;) {
         // (of thread 0: the unit that it claimed)
@@ -832,7 +851,7 @@ __global__ __launch_bounds__(kThreads, 2) void layer_experts_kernel(Layer p) {
         __syncthreads();
         const int got = found;
         if (got >= 0) {
-            GateUp<T, FP8, WHOLE> front(p, r);
+            GateUp<T, FP8, FIT> front(p, r);
             front.run(got, items, G, room.parts, turn);
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // every wave's rows of h are there, before the word that says so
             __syncthreads();
@@ -864,7 +883,7 @@ __global__ __launch_bounds__(kThreads, 2) void layer_experts_kernel(Layer p) {
     turn = 0;
     for (int i = blockIdx.x; i < last; i += G, ++turn) {
         if (turn != 0 && wave < r.experts) down.load(c, i, wave, 0);
-        down.item(c, i, room.back.sums[turn & 1], room.back.staged[FP8 ? wave : 0]);
+        down.item(c, i, room.back.sums[turn & 1], room.back.staged[wave]);
     }
 }
 
@@ -889,7 +908,7 @@ struct Room {
     size_t all() const { return stream + rows + h + widest + flags; }
 };
 
-template <typename T, bool FP8, bool WHOLE>
+template <typename T, bool FP8, int FIT>
 int launch(const Layer &p, hipStream_t stream) {
     const int tokens = (int)p.c.T;
     // (few workgroups with two experts each are done before the same with eight would be: 64 x 2 at one token of 128 experts)
@@ -905,19 +924,23 @@ int launch(const Layer &p, hipStream_t stream) {
     const int hits = p.c.T * p.c.k < p.c.E ? (int)p.c.T * p.c.k : p.c.E;
     const int64_t front = hits * (p.ldh / 8), back = ceil_div(p.c.H, kColumns), want = front > back ? front : back;
     const unsigned most = (unsigned)most_workgroups();
-    layer_experts_kernel<T, FP8, WHOLE><<<want < most ? (unsigned)want : most, kThreads, 0, stream>>>(p);
+    layer_experts_kernel<T, FP8, FIT><<<want < most ? (unsigned)want : most, kThreads, 0, stream>>>(p);
     return launch_status();
+}
+
+template <typename T, bool FP8>
+int launch_fit(const Layer &p, hipStream_t stream) {
+    typedef GateUp<T, FP8, kExact> Front;
+    typedef Down<T, FP8, kExact> Back;
+    const int H = p.c.H, I = p.c.I;
+    if (H % (kWaves * Front::U * Front::kStep) == 0 && I % Back::kStaged == 0) return launch<T, FP8, kExact>(p, stream);
+    if (H % Front::kRun == 0 && I % Front::kRun == 0) return launch<T, FP8, kWhole>(p, stream);
+    return launch<T, FP8, kRagged>(p, stream);
 }
 
 template <typename T>
 int launch_type(const Layer &p, hipStream_t stream) {
-    constexpr int run = 16 / (int)sizeof(T);
-    if (p.c.s_gate != nullptr) {
-        if (p.c.H % 16 == 0 && p.c.I % 16 == 0) return launch<T, true, true>(p, stream);
-        return launch<T, true, false>(p, stream);
-    }
-    if (p.c.H % run == 0 && p.c.I % run == 0) return launch<T, false, true>(p, stream);
-    return launch<T, false, false>(p, stream);
+    return p.c.s_gate != nullptr ? launch_fit<T, true>(p, stream) : launch_fit<T, false>(p, stream);
 }
 
 }  // namespace
