@@ -36,6 +36,8 @@ struct Layer {
 // A workgroup has a token and EXPERTS experts.  It norms the token itself (the row is read once more per workgroup, from the
 // caches), so that nothing has to wait for another workgroup; the first one of a token writes its rows.  ONE: a row is one run of
 // eight elements a thread, and stays in registers.
+constexpr int kRouterExperts = 2;
+
 template <typename T, int EXPERTS, bool FP8, bool WHOLE, bool ONE>
 __global__ __launch_bounds__(256) void layer_router_kernel(Layer p) {
     __shared__ double squares[4];
@@ -354,11 +356,6 @@ __device__ __forceinline__ Run settle(Run run, int k, int K) {
     return run;
 }
 
-__device__ __forceinline__ floatx4 mfma_f32(const float (&a)[4], const float (&b)[4], floatx4 acc) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], acc, 0, 0, 0);
-    return acc;
-}
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 
 // bf16 layers keep a value h of the gated unit as two bf16 ones, h as rounded and what that leaves, as rounded: 2^-17 of it is lost at
@@ -911,16 +908,11 @@ struct Room {
 template <typename T, bool FP8, int FIT>
 int launch(const Layer &p, hipStream_t stream) {
     const int tokens = (int)p.c.T;
-    // (few workgroups with two experts each are done before the same with eight would be: 64 x 2 at one token of 128 experts)
-    const bool many = (int64_t)tokens * p.c.E >= 1024, whole8 = p.c.H % 8 == 0, one = p.c.H <= 2048;
-    const dim3 grid(ceil_div(p.c.E, many ? 8 : 2), tokens);
-#define MFL_LAYER_ROUTER(N)                                                                                       \
-    if (whole8 && one) layer_router_kernel<T, N, FP8, true, true><<<grid, 256, 0, stream>>>(p);                    \
-    else if (whole8) layer_router_kernel<T, N, FP8, true, false><<<grid, 256, 0, stream>>>(p);                     \
-    else layer_router_kernel<T, N, FP8, false, false><<<grid, 256, 0, stream>>>(p);
-    if (many) { MFL_LAYER_ROUTER(8) }
-    else { MFL_LAYER_ROUTER(2) }
-#undef MFL_LAYER_ROUTER
+    // (two experts a workgroup: with eight the call takes 2 us more at 13 to 16 tokens of 128 experts; with one the same at one token)
+    const dim3 grid(ceil_div(p.c.E, kRouterExperts), tokens);
+    if (p.c.H % 8 != 0) layer_router_kernel<T, kRouterExperts, FP8, false, false><<<grid, 256, 0, stream>>>(p);
+    else if (p.c.H <= 2048) layer_router_kernel<T, kRouterExperts, FP8, true, true><<<grid, 256, 0, stream>>>(p);
+    else layer_router_kernel<T, kRouterExperts, FP8, true, false><<<grid, 256, 0, stream>>>(p);
     const int hits = p.c.T * p.c.k < p.c.E ? (int)p.c.T * p.c.k : p.c.E;
     const int64_t front = hits * (p.ldh / 8), back = ceil_div(p.c.H, kColumns), want = front > back ? front : back;
     const unsigned most = (unsigned)most_workgroups();
