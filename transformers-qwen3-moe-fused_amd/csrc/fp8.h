@@ -197,25 +197,6 @@ __device__ __forceinline__ void fp8_store_wide(float (&v)[8], bf16_t *to) {
     *(bf16x8 *)to = fp8_widen(q, fp8_scale_of(byte));
 }
 
-// Eight values on the e4m3 grid of the power of two `scale`, as bf16; infinities as NaN.
-__device__ __forceinline__ bf16x8 fp8_rounded(const float *v, float scale) {
-    typedef __attribute__((ext_vector_type(2))) short shortx2;
-    shortx2 r[2] = {};
-    r[0] = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r[0], v[0], v[1], scale, false);
-    r[1] = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r[1], v[4], v[5], scale, false);
-    r[0] = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r[0], v[2], v[3], scale, true);
-    r[1] = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r[1], v[6], v[7], scale, true);
-    return fp8_widen(intx2{__builtin_bit_cast(int, r[0]), __builtin_bit_cast(int, r[1])}, scale);
-}
-
-// The largest of the four lanes lane % 16, + 16, + 32, + 48, in all of them.
-__device__ __forceinline__ uint32_t fp8_over_quarters(uint32_t a) {
-    const auto x = __builtin_amdgcn_permlane16_swap(a, a, false, false);
-    a = x[0] > x[1] ? x[0] : x[1];
-    const auto y = __builtin_amdgcn_permlane32_swap(a, a, false, false);
-    return y[0] > y[1] ? y[0] : y[1];
-}
-
 // The row counts of experts e, e + 64, ..., 0 past the last expert, their loads all in flight together.
 template <int N>
 __device__ __forceinline__ void fp8_load_counts(const void *m_sizes, int ms_i64, int e, int E, int64_t R, uint32_t (&count)[N]) {

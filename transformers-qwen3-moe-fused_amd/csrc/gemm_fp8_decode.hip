@@ -92,6 +92,14 @@ struct Piece {
     }
 };
 
+// The largest of the four lanes that hold a row's block, in all of them.
+__device__ __forceinline__ uint32_t over_block(uint32_t a) {
+    const auto x = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+    a = x[0] > x[1] ? x[0] : x[1];
+    const auto y = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+    return y[0] > y[1] ? y[0] : y[1];
+}
+
 // The row counts of up to 256 experts at once (their loads in flight together), then 64 at a time.  A launch has at most 2^16
 // tiles and so fewer than 2^20 rows: 64 counts of no more than that each sum to less than 2^31, and the two sums, which need not
 // wait for each other, are never taken past the first expert whose tiles pass `slot`.
@@ -212,8 +220,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void fp8_decode_kernel(Fp8Product p
                 }
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
-                uint32_t a = fp8_over_quarters(fx[u][1].widest(fx[u][0].widest(0u)));
-                if (__builtin_expect(__any(fp8_unusual(a)), 0)) a = fp8_over_quarters(fx[u][1].finite(fx[u][0].finite(0u)));
+                uint32_t a = over_block(fx[u][1].widest(fx[u][0].widest(0u)));
+                if (__builtin_expect(__any(fp8_unusual(a)), 0)) a = over_block(fx[u][1].finite(fx[u][0].finite(0u)));
                 byte[u] = fp8_scale_byte(a);
                 const float scale = fp8_scale_of(byte[u]);
                 int lo[4], hi[4];

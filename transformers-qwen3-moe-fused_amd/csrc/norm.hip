@@ -9,7 +9,9 @@ namespace mfl {
 namespace {
 
 // ---- forward --------------------------------------------------------------------------------------------------------------
-// A row belongs to LANES threads, which hold it in registers, 8 C elements each in C runs of 8: one pass over memory.
+// A row belongs to LANES threads, which hold it in registers, 8 C elements each in C runs of 8: one pass over memory, which is all
+// that bounds it where there are rows enough to fill the chip.  bf16 with a residual: 16384 x 2048 44.6 us, 6.0 TB/s of the 2 + 2
+// rows that it has to read and write, 4096 x 8192 44.3, 1024 x 32768 52.5; to 8-bit rows 16384 x 2048 50.
 template <typename T, typename TW, int LANES, int C, bool FP8, bool WHOLE>
 __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_fwd_kernel(const T *__restrict__ x, const T *__restrict__ residual,
                                                                            const TW *__restrict__ weight, T *__restrict__ y,
@@ -25,6 +27,7 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_fwd_kernel(con
     x += row * H;
     Eight<T, WHOLE> v[C];
     Eight<TW, WHOLE> w[C];
+    constexpr bool EARLY = C == 1;  // the weight is asked for before the sum's end where the registers hold it (1024 x 32768: 92 us, 52 late)
 #pragma unroll
     for (int c = 0; c < C; ++c) v[c].load(x, (c * LANES + i) * 8, H);
     if (residual != nullptr) {
@@ -40,8 +43,7 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_fwd_kernel(con
     double sum = 0.0;
 #pragma unroll
     for (int c = 0; c < C; ++c) sum = sum_of_squares(v[c], sum);
-#pragma unroll
-    for (int c = 0; c < C; ++c) w[c].load(weight, (c * LANES + i) * 8, H);
+    if (EARLY) w[0].load(weight, i * 8, H);
     sum = wave_sum(sum);
     if (LANES > 64) {
         if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = sum;
@@ -55,6 +57,7 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_fwd_kernel(con
 #pragma unroll
     for (int c = 0; c < C; ++c) {
         const int k = (c * LANES + i) * 8;
+        if (!EARLY) w[c].load(weight, k, H);
 #pragma unroll
         for (int u = 0; u < 8; ++u) v[c].v[u] = normed(v[c].v[u], r, w[c].v[u]);
         if (y != nullptr) v[c].store(y + row * H, k, H);
@@ -72,38 +75,37 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_fwd_kernel(con
 // With u = s r and g = dy w: dx = r (g - u mean(g u)) + ds, dw = sum over the rows of dy u.  s is read as the forward pass left
 // it and its r found again, which costs a sum beside the one that is needed anyway.  A group of LANES threads takes every
 // gridDim.x * GROUPS-th row and keeps its columns' share of dw in registers; the groups of a workgroup meet in LDS, the workgroups
-// in `partial` (workgroup, H), which a second kernel adds up in order.
+// in `partial` (workgroup, H), which a second kernel adds up in order.  Memory bounds it too: bf16 with ds, 16384 x 2048 49 us for
+// both kernels, 5.5 TB/s of three rows read and one written.
 template <typename T, typename TW, int LANES, int C, int THREADS, bool WHOLE>
 __global__ __launch_bounds__(THREADS) void norm_bwd_kernel(const T *__restrict__ dy, const T *__restrict__ ds, const T *__restrict__ s,
                                                           const TW *__restrict__ weight, T *__restrict__ dx,
                                                           float *__restrict__ partial, int64_t R, int H, double eps) {
     constexpr int GROUPS = THREADS / LANES, WAVES = LANES / 64;
-    constexpr bool AHEAD = WHOLE && C == 1;  // the next row is asked for before this one's sums are there (16384 x 2048: 61 -> 50 us)
+    constexpr bool ONE = C == 1;
+    // s and dy stay in registers between a row's two passes where they fit; else they are read again, from the caches (1024 x 32768
+    // in bf16: 251 us in registers that spill, 139 so; 2048 x 16384: 81 in registers, 90 so)
+    constexpr int HELD = C == 2 ? C : 1;
+    constexpr bool AHEAD = WHOLE && ONE;  // the next row is asked for before this one's sums are there (16384 x 2048: 61 -> 50 us)
     __shared__ double squares[2][GROUPS * WAVES];
     __shared__ float alongs[2][GROUPS * WAVES];
     extern __shared__ float shared_dw[];  // (GROUPS - 1, LANES * C * 8) where the groups are many
     const int i = threadIdx.x % LANES, group = threadIdx.x / LANES;
     float dw[C][8];
-    Eight<TW, WHOLE> w[C];
+    Eight<TW, WHOLE> w;
+    if (ONE) w.load(weight, i * 8, H);
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-        w[c].load(weight, (c * LANES + i) * 8, H);
+    for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int u = 0; u < 8; ++u) dw[c][u] = 0.0f;
-    }
     int turn = 0;
-    Eight<T, WHOLE> sv[C], g[C], d[C], next_s[C], next_g[C], next_d[C];
+    Eight<T, WHOLE> sv, g, d, next_s, next_g, next_d, held_s[HELD], held_g[HELD];
     const bool add = ds != nullptr && dx != nullptr;
-    auto fetch = [&](int64_t row0, Eight<T, WHOLE>(&a)[C], Eight<T, WHOLE>(&b)[C], Eight<T, WHOLE>(&e)[C]) {
+    auto fetch = [&](int64_t row0, Eight<T, WHOLE> &a, Eight<T, WHOLE> &b, Eight<T, WHOLE> &e) {
         const int64_t at = (row0 + group < R ? row0 + group : R - 1) * H;
-#pragma unroll
-        for (int c = 0; c < C; ++c) a[c].load(s + at, (c * LANES + i) * 8, H);
-#pragma unroll
-        for (int c = 0; c < C; ++c) b[c].load(dy + at, (c * LANES + i) * 8, H);
-        if (add) {
-#pragma unroll
-            for (int c = 0; c < C; ++c) e[c].load(ds + at, (c * LANES + i) * 8, H);
-        }
+        a.load(s + at, i * 8, H);
+        b.load(dy + at, i * 8, H);
+        if (add) e.load(ds + at, i * 8, H);
     };
     const int64_t first = (int64_t)blockIdx.x * GROUPS, by = (int64_t)gridDim.x * GROUPS;
     if (AHEAD) fetch(first, next_s, next_g, next_d);
@@ -113,22 +115,28 @@ __global__ __launch_bounds__(THREADS) void norm_bwd_kernel(const T *__restrict__
         const bool in = row < R;
         const int64_t at = (in ? row : R - 1) * H;
         if (AHEAD) {
-#pragma unroll
-            for (int c = 0; c < C; ++c) sv[c] = next_s[c], g[c] = next_g[c], d[c] = next_d[c];
+            sv = next_s, g = next_g, d = next_d;
             if (row0 + by < R) fetch(row0 + by, next_s, next_g, next_d);
-        } else {
+        } else if (ONE) {
             fetch(row0, sv, g, d);
         }
         double square = 0.0;  // (32 bits hold no square of a 32-bit or bf16 value past 2^64)
         float along = 0.0f;
-#pragma unroll
-        for (int c = 0; c < C; ++c)
+#pragma unroll HELD
+        for (int c = 0; c < C; ++c) {
+            if (!ONE) {
+                sv.load(s + at, (c * LANES + i) * 8, H);
+                g.load(dy + at, (c * LANES + i) * 8, H);
+                w.load(weight, (c * LANES + i) * 8, H);
+                if (HELD == C) held_s[c] = sv, held_g[c] = g;
+            }
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
-                const float a = to_f32(sv[c].v[u]);
+                const float a = to_f32(sv.v[u]);
                 square = __builtin_fma((double)a, (double)a, square);
-                along = __builtin_fmaf(to_f32(g[c].v[u]) * to_f32(w[c].v[u]), a, along);
+                along = __builtin_fmaf(to_f32(g.v[u]) * to_f32(w.v[u]), a, along);
             }
+        }
 #pragma unroll
         for (int step = 32; step; step >>= 1) along += __shfl_xor(along, step);
         square = wave_sum(square);
@@ -144,15 +152,25 @@ __global__ __launch_bounds__(THREADS) void norm_bwd_kernel(const T *__restrict__
         if (!in) continue;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
+            if (!ONE) {
+                if (HELD == C) {
+                    sv = held_s[c], g = held_g[c];
+                } else {
+                    sv.load(s + at, (c * LANES + i) * 8, H);
+                    g.load(dy + at, (c * LANES + i) * 8, H);
+                }
+                w.load(weight, (c * LANES + i) * 8, H);
+                if (add) d.load(ds + at, (c * LANES + i) * 8, H);
+            }
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
-                const float a = to_f32(sv[c].v[u]), b = to_f32(g[c].v[u]);
+                const float a = to_f32(sv.v[u]), b = to_f32(g.v[u]);
                 dw[c][u] = __builtin_fmaf(b, a * r, dw[c][u]);
-                float o = r * __builtin_fmaf(-a, back, b * to_f32(w[c].v[u]));
-                if (add) o += to_f32(d[c].v[u]);
-                sv[c].v[u] = from_f32<T>(o);
+                float o = r * __builtin_fmaf(-a, back, b * to_f32(w.v[u]));
+                if (add) o += to_f32(d.v[u]);
+                sv.v[u] = from_f32<T>(o);
             }
-            if (dx != nullptr) sv[c].store(dx + at, (c * LANES + i) * 8, H);
+            if (dx != nullptr) sv.store(dx + at, (c * LANES + i) * 8, H);
         }
     }
     if (partial == nullptr) return;
