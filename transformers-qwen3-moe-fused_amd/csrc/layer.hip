@@ -382,14 +382,17 @@ constexpr int kDeviceScope = 16;  // a buffer load's sc1 bit
 // registers where its share of the reduction is one chunk.  The next item's weights are asked for before the waves meet.
 typedef floatx4 Parts[2][2][kWaves][64];
 
-template <typename T, bool FP8, int FIT>
+// NARROW: rows of which a wave's share is half a chunk or less (1024 elements, 512 in 32 bits) are taken in chunks of half as many
+// steps, with twice as many items ahead: what is loaded behind a share is loaded for nothing, and where rows have to be moved down
+// its registers are short (5 tokens, 60 experts of 1001 x 333 in fp16 44 -> 34 us, of 1008 x 336 25.9 -> 24.3).
+template <typename T, bool FP8, int FIT, bool NARROW>
 struct GateUp {
     typedef Weights<T, FP8> W;
     typedef typename W::Element Element;
     typedef typename std::conditional<FP8, bf16_t, T>::type X;
     static constexpr int kRun = W::kRun, kStep = W::kStep, kPieces = kRun * (int)sizeof(X) / 16;
-    static constexpr int U = FP8 ? 4 : 8;      // steps of a chunk: their loads are in flight together
-    static constexpr int D = FP8 ? 4 : 2;      // items whose first chunks are
+    static constexpr int U = (FP8 ? 4 : 8) / (NARROW ? 2 : 1);  // steps of a chunk: their loads are in flight together
+    static constexpr int D = (FP8 ? 4 : 2) * (NARROW ? 2 : 1);  // items whose first chunks are
     static constexpr int kGroup = FP8 ? 2 : 1;
     static constexpr int kUnit = FP8 ? 2 : 1;  // (whole blocks of 128 a wave where weights have scales)
     const Layer &p;
@@ -819,7 +822,7 @@ struct Down {
 // free, 1 claimed, 2 done.  A workgroup claims its own unit; before it waits for anything it looks whether there is one that nobody has
 // claimed (of a workgroup that has not started yet) and does it in the other's place.  Whoever claims a unit is running, and waits for
 // nothing before the unit is done: every wait ends, however many of the workgroups are there at once.
-template <typename T, bool FP8, int FIT>
+template <typename T, bool FP8, int FIT, bool NARROW>
 __global__ __launch_bounds__(kThreads, 2) void layer_experts_kernel(Layer p) {
     __shared__ Routing r;
     __shared__ union {
@@ -848,7 +851,7 @@ __global__ __launch_bounds__(kThreads, 2) void layer_experts_kernel(Layer p) {
         __syncthreads();
         const int got = found;
         if (got >= 0) {
-            GateUp<T, FP8, FIT> front(p, r);
+            GateUp<T, FP8, FIT, NARROW> front(p, r);
             front.run(got, items, G, room.parts, turn);
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // every wave's rows of h are there, before the word that says so
             __syncthreads();
@@ -905,7 +908,7 @@ struct Room {
     size_t all() const { return stream + rows + h + widest + flags; }
 };
 
-template <typename T, bool FP8, int FIT>
+template <typename T, bool FP8, int FIT, bool NARROW>
 int launch(const Layer &p, hipStream_t stream) {
     const int tokens = (int)p.c.T;
     // (two experts a workgroup: with eight the call takes 2 us more at 13 to 16 tokens of 128 experts; with one the same at one token)
@@ -916,23 +919,29 @@ int launch(const Layer &p, hipStream_t stream) {
     const int hits = p.c.T * p.c.k < p.c.E ? (int)p.c.T * p.c.k : p.c.E;
     const int64_t front = hits * (p.ldh / 8), back = ceil_div(p.c.H, kColumns), want = front > back ? front : back;
     const unsigned most = (unsigned)most_workgroups();
-    layer_experts_kernel<T, FP8, FIT><<<want < most ? (unsigned)want : most, kThreads, 0, stream>>>(p);
+    layer_experts_kernel<T, FP8, FIT, NARROW><<<want < most ? (unsigned)want : most, kThreads, 0, stream>>>(p);
     return launch_status();
 }
 
-template <typename T, bool FP8>
+template <typename T, bool FP8, bool NARROW>
 int launch_fit(const Layer &p, hipStream_t stream) {
-    typedef GateUp<T, FP8, kExact> Front;
+    typedef GateUp<T, FP8, kExact, NARROW> Front;
     typedef Down<T, FP8, kExact> Back;
     const int H = p.c.H, I = p.c.I;
-    if (H % (kWaves * Front::U * Front::kStep) == 0 && I % Back::kStaged == 0) return launch<T, FP8, kExact>(p, stream);
-    if (H % Front::kRun == 0 && I % Front::kRun == 0) return launch<T, FP8, kWhole>(p, stream);
-    return launch<T, FP8, kRagged>(p, stream);
+    if (H % (kWaves * Front::U * Front::kStep) == 0 && I % Back::kStaged == 0) return launch<T, FP8, kExact, NARROW>(p, stream);
+    if (H % Front::kRun == 0 && I % Front::kRun == 0) return launch<T, FP8, kWhole, NARROW>(p, stream);
+    return launch<T, FP8, kRagged, NARROW>(p, stream);
+}
+
+template <typename T, bool FP8>
+int launch_width(const Layer &p, hipStream_t stream) {
+    typedef GateUp<T, FP8, kWhole, true> Narrow;
+    return p.c.H <= kWaves * Narrow::U * Narrow::kStep ? launch_fit<T, FP8, true>(p, stream) : launch_fit<T, FP8, false>(p, stream);
 }
 
 template <typename T>
 int launch_type(const Layer &p, hipStream_t stream) {
-    return p.c.s_gate != nullptr ? launch_fit<T, true>(p, stream) : launch_fit<T, false>(p, stream);
+    return p.c.s_gate != nullptr ? launch_width<T, true>(p, stream) : launch_width<T, false>(p, stream);
 }
 
 }  // namespace
