@@ -102,6 +102,27 @@ def test_layer_in_8_bits(size, dtype):
         case.check(*case.call())
 
 
+# rows that fill a wave's share, that do not, that take several chunks, either way
+WIDE = [
+    (5, 6, 2, 1024, 768),
+    (2, 4, 2, 1536, 96),
+    (3, 4, 2, 2050, 50),
+    (4, 3, 2, 2048, 1536),
+    (2, 3, 1, 4096, 768),
+    (1, 2, 2, 5003, 24),
+    (16, 2, 2, 6144, 40),
+    (9, 3, 2, 24, 5001),
+]
+
+
+@pytest.mark.parametrize("dtype", (BF16, F16, F32))
+@pytest.mark.parametrize("eight", (False, True))
+@pytest.mark.parametrize("size", WIDE, ids=str)
+def test_wide_rows(size, dtype, eight):
+    case = Case(*size, dtype, eight=eight, norm=True, residual=True, seed=sum(size))
+    case.check(*case.call())
+
+
 @pytest.mark.parametrize("eight", (False, True))
 def test_benchmark_sizes(eight):
     case = Case(3, 32, 8, 2048, 768, BF16, eight=eight, norm=True, residual=True)

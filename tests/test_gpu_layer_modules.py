@@ -96,6 +96,9 @@ def test_calls_that_stay_with_the_separate_steps(calls):
         block.up_proj = _block().up_proj
         block.fuse_layer = True
         assert block.whole_layer(x.view(4, 256)) is None
+        block = _block(experts=80, k=65)  # more experts a token than the call takes
+        block.fuse_layer = True
+        assert block.whole_layer(x.view(4, 256)) is None
 
 
 def _models(dtype=BF16, **changed):

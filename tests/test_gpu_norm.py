@@ -322,3 +322,42 @@ def test_more_elements_than_32_bits_count():
     want, _ = ref.norm_gradients(tail.flip(0), None, tail.double(), w, EPS)
     bound, _ = ref.norm_gradient_bounds(tail.flip(0), None, tail.double(), w, EPS, torch.bfloat16, torch.bfloat16)
     assert ((dx[-5:].cpu().double() - want).abs() <= bound).all()
+
+
+def test_weight_gradient_of_no_rows():
+    w, dw = torch.ones(72, device="cuda"), torch.full((72,), 5.0, device="cuda")
+    rows = torch.empty((1, 72), device="cuda")
+    rc = _lib.lib().mfl_add_rms_norm_bwd(rows.data_ptr(), None, rows.data_ptr(), w.data_ptr(), rows.data_ptr(), dw.data_ptr(), 0, 72, EPS,
+                                         _lib.dtype_code(w.dtype), _lib.dtype_code(w.dtype), None, 0, _lib.stream())
+    _lib.check(rc, "mfl_add_rms_norm_bwd")
+    assert not dw.any()
+
+
+@pytest.mark.parametrize("width", (2048, 16384, 32768, 20001))
+@pytest.mark.parametrize("onto", ("dy", "ds", "s"))
+def test_backward_onto_an_operand(width, onto):
+    dtype = torch.bfloat16
+    s, ds, w, g = _inputs(37, width, dtype, width)
+    dy = torch.randn((37, width), generator=g).to(dtype)
+    s, ds, w, dy = _cuda(s, ds, w, dy)
+    want_dx, want_dw = add_rms_norm_backward(dy, ds, s, w, EPS)
+    lib, dw = _lib.lib(), torch.empty_like(w)
+    size = lib.mfl_add_rms_norm_bwd_workspace(37, width)
+    ws = torch.empty(size, device="cuda", dtype=torch.uint8)
+    dx = {"dy": dy, "ds": ds, "s": s}[onto]
+    rc = lib.mfl_add_rms_norm_bwd(dy.data_ptr(), ds.data_ptr(), s.data_ptr(), w.data_ptr(), dx.data_ptr(), dw.data_ptr(), 37, width, EPS,
+                                  _lib.dtype_code(dtype), _lib.dtype_code(dtype), ws.data_ptr(), size, _lib.stream())
+    _lib.check(rc, "mfl_add_rms_norm_bwd")
+    assert torch.equal(dx, want_dx) and torch.equal(dw, want_dw)
+
+
+@pytest.mark.parametrize("width", (96, 2048, 16384, 32768))
+def test_forward_onto_its_operands(width):
+    dtype = torch.bfloat16
+    x, r, w, _ = _inputs(21, width, dtype, width)
+    x, r, w = _cuda(x, r, w)
+    want, want_s = add_rms_norm(x, r, w, EPS)
+    rc = _lib.lib().mfl_add_rms_norm(x.data_ptr(), r.data_ptr(), w.data_ptr(), x.data_ptr(), r.data_ptr(), 21, width, EPS,
+                                     _lib.dtype_code(dtype), _lib.dtype_code(dtype), _lib.stream())
+    _lib.check(rc, "mfl_add_rms_norm")
+    assert torch.equal(x, want) and torch.equal(r, want_s)

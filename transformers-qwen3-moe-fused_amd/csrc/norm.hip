@@ -273,8 +273,9 @@ int launch_bwd(const NormCall &n, const void *dy, const void *ds, void *dx, void
         constexpr int threads = L < kBwdThreads ? kBwdThreads : L;                                                             \
         constexpr int room = (threads / L - 1) * L * C * 8 * 4;  /* 14 KB at most */                                           \
         auto kernel = norm_bwd_kernel<T, TW, L, C, threads, WHOLE>;                                                            \
-        kernel<<<grid, threads, room, stream>>>((const T *)dy, (const T *)ds, (const T *)n.s, (const TW *)n.weight, (T *)dx,    \
-                                                dw != nullptr ? partial : nullptr, n.R, H, (double)n.eps);                             \
+        if (grid > 0)                                                                                                          \
+            kernel<<<grid, threads, room, stream>>>((const T *)dy, (const T *)ds, (const T *)n.s, (const TW *)n.weight, (T *)dx, \
+                                                    dw != nullptr ? partial : nullptr, n.R, H, (double)n.eps);                 \
     }
     if (H <= 512) MFL_NORM(64, 1)
     else if (H <= 1024) MFL_NORM(128, 1)

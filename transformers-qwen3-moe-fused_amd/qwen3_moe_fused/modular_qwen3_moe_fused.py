@@ -114,7 +114,7 @@ class Qwen3MoeFusedSparseMoeBlock(nn.Module):
     # units idle, and a training step of the block takes 1.62-1.67 ms instead of 1.58-1.63 ms.
     fuse_backward = False
     # set to True for calls of up to 16 tokens without gradients as the whole layer in two launches (fused_mlp.moe_fused_layer; bf16,
-    # fp16, fp32 and 8-bit expert matrices; one token of 128 experts in bf16 28 us a call against 59).  Off by default: the results are
+    # fp16, fp32 and 8-bit expert matrices; one token of 128 experts in bf16 26 us a call against 45, 16 tokens 135 against 146).  Off by default: the results are
     # not those of the separate steps bit for bit, since less is rounded on the way.
     fuse_layer = False
     # set to True to keep the expert ids of the last call in ``last_selected`` (tests read the block's own routing)
@@ -161,7 +161,9 @@ class Qwen3MoeFusedSparseMoeBlock(nn.Module):
             return None
         same = [gate.weight] + ([p.weight for p in projs] if kind is MoeFusedLinear else [])
         same += [t for t in (residual, norm_weight) if t is not None]
-        if not tokens.is_cuda or tokens.dtype not in (torch.bfloat16, torch.float16, torch.float32) or self.num_experts > 1024:
+        if not tokens.is_cuda or tokens.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+            return None
+        if self.num_experts > 1024 or self.num_selected > 64 or projs[0].out_features > 1 << 17:  # (the call's limits)
             return None
         if any(t.dtype != tokens.dtype or t.device != tokens.device or not t.is_contiguous() for t in same):
             return None
