@@ -1,5 +1,13 @@
 // The whole sparse expert layer for a few tokens: router, softmax and top-k, gated experts, weighted sum; with the residual's
 // addition and the norm in front and the stream's addition behind where asked for.
+//
+// Two launches: the logits (and the stream and the normed rows), then everything behind them, the routing found again by every
+// workgroup.  An expert's weights are read once, straight from memory into the matrix unit's operands, for all tokens that chose it.
+// With 128 experts of 2048 x 768, 8 a token, in bf16: 16 tokens 140 us, of which the router is 6: the weights of the 82 experts that
+// are hit on average (780 MB) at 5.8 TB/s, which is what the memory gives.  One token 25 us, where its 8 experts' 75 MB take 14: a chain of
+// round trips, the router 3.6, the routing 3.4, gate and up 9, the meeting of the workgroups 3.5, down 4.5 (8-bit weights, with addition and
+// norm: 25.5, and 13 tokens 65).  In three launches, with the gated unit and the down projection as kernels of their own, one token took 33 us
+// and 16 tokens 226.
 #include <type_traits>
 
 #include "fp8.h"

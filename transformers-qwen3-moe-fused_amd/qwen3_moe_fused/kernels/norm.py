@@ -13,7 +13,7 @@ from typing import Optional, Tuple
 import torch
 
 from .. import _lib
-from ..quantize.fp8 import BLOCK, FP8, blocks_of
+from ..quantize.fp8 import empty_fp8_rows
 
 
 def _check(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor) -> Tuple[int, int, int]:
@@ -44,17 +44,15 @@ def _forward(x, residual, weight, eps):
 def _forward_fp8(x, residual, weight, eps, return_normed):
     rows, width, dtype = _check(x, residual, weight)
     assert x.ndim == 2, "quantised rows are a matrix"
-    blocks = blocks_of(width)
     with _lib.on_device_of(x):
-        q = torch.empty((rows, blocks * BLOCK), device=x.device, dtype=torch.uint8)
-        scale = torch.empty((rows, (blocks + 3) // 4 * 4), device=x.device, dtype=torch.uint8)
+        q, scale = empty_fp8_rows(x)
         s = x if residual is None else torch.empty_like(x)
         y = torch.empty_like(x) if return_normed else None
         rc = _lib.lib().mfl_add_rms_norm_fp8(x.data_ptr(), _lib.ptr(residual), weight.data_ptr(), q.data_ptr(), scale.data_ptr(),
                                              _lib.ptr(y), s.data_ptr(), rows, width, eps, dtype, _lib.dtype_code(weight.dtype),
                                              _lib.stream())
     _lib.check(rc, "mfl_add_rms_norm_fp8")
-    return q.view(FP8)[:, :width], scale.view(torch.float8_e8m0fnu)[:, :blocks], s, y
+    return q, scale, s, y
 
 
 def add_rms_norm_backward(dy: Optional[torch.Tensor], ds: Optional[torch.Tensor], s: torch.Tensor, weight: torch.Tensor, eps: float,

@@ -47,20 +47,28 @@ def check_fp8_rows(values: torch.Tensor, scale: torch.Tensor, like: torch.Tensor
     assert (k == 1 or values.stride(1) == 1) and (blocks == 1 or scale.stride(1) == 1)
 
 
+def empty_fp8_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Room for ``x``'s quantised rows, laid out as ``quantize_fp8_rows`` says.  (Nothing is sliced that is whole: 2 us a tensor.)"""
+    rows, k = x.shape
+    blocks = blocks_of(k)
+    ld, ld_scale = blocks * BLOCK, (blocks + 3) // 4 * 4
+    values = torch.empty((rows, ld), device=x.device, dtype=FP8)
+    scale = torch.empty((rows, ld_scale), device=x.device, dtype=torch.float8_e8m0fnu)
+    return values if ld == k else values[:, :k], scale if ld_scale == blocks else scale[:, :blocks]
+
+
 def quantize_fp8_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """``x`` (rows, K) in bf16 / fp16 / fp32 -> (values (rows, K) float8_e4m3fn, scales (rows, ceil(K / 128))
     float8_e8m0fnu).  Rows of the values lie a multiple of 128 bytes apart (zeros behind column K), those of the scales a
     multiple of 4."""
     assert x.is_cuda and x.ndim == 2 and x.is_contiguous()
     rows, k = x.shape
-    blocks = blocks_of(k)
     dtype = _lib.dtype_code(x.dtype)
     with _lib.on_device_of(x):
-        q = torch.empty((rows, blocks * BLOCK), device=x.device, dtype=torch.uint8)
-        scale = torch.empty((rows, (blocks + 3) // 4 * 4), device=x.device, dtype=torch.uint8)
+        q, scale = empty_fp8_rows(x)
         rc = _lib.lib().mfl_fp8_quant_rows(x.data_ptr(), dtype, rows, k, q.data_ptr(), scale.data_ptr(), _lib.stream())
     _lib.check(rc, "mfl_fp8_quant_rows")
-    return q.view(FP8)[:, :k], scale.view(torch.float8_e8m0fnu)[:, :blocks]
+    return q, scale
 
 
 def dequantize_fp8_rows(values: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
