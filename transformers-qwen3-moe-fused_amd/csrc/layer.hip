@@ -320,7 +320,7 @@ struct alignas(16) Run {
 };
 
 // How the sizes fit the loads.  kExact: every load of every wave lies in its row (64 KB of a row of gate and up, as many of down): nothing
-// is asked, 3 % of a call; kWhole: rows are whole loads long; kRagged: any.
+// is asked (16 tokens of the sizes above 150 -> 142 us, one 27.8 -> 25.9); kWhole: rows are whole loads long; kRagged: any.
 enum Fit { kRagged, kWhole, kExact };
 
 // 16 bytes of a row from element k on, zeros from element K on.  In two steps: `fetch` loads, always and without a branch, so that the
