@@ -90,6 +90,17 @@ def test_magnitudes_whose_squares_32_bits_do_not_hold(dtype, std):
             assert ((a.cpu().double() - b).abs() <= c).all()
 
 
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float32))
+def test_gradients_whose_row_sums_32_bits_do_not_hold(dtype):
+    s, _, w, g = _inputs(4, 2048, dtype, residual=False, std=1e36)
+    dy = (torch.randn(s.shape, generator=g).abs() * s.sign() * 256.0).to(dtype)  # 2048 terms of one sign, 2e38 each
+    dx, dw = add_rms_norm_backward(dy.cuda(), None, s.cuda(), w.cuda(), EPS)
+    want = ref.norm_gradients(dy, None, s.double(), w, EPS)
+    bounds = ref.norm_gradient_bounds(dy, None, s.double(), w, EPS, dtype, dtype)
+    for a, b, c in zip((dx, dw), want, bounds):
+        assert ((a.cpu().double() - b).abs() <= c).all()
+
+
 def test_a_row_without_a_finite_length_leaves_the_others_alone():
     x, r, w, _ = _inputs(9, 700, torch.bfloat16)
     x[2, 5], x[4, 699], x[6] = float("nan"), float("inf"), 0.0

@@ -75,8 +75,8 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_fwd_kernel(con
 // With u = s r and g = dy w: dx = r (g - u mean(g u)) + ds, dw = sum over the rows of dy u.  s is read as the forward pass left
 // it and its r found again, which costs a sum beside the one that is needed anyway.  A group of LANES threads takes every
 // gridDim.x * GROUPS-th row and keeps its columns' share of dw in registers; the groups of a workgroup meet in LDS, the workgroups
-// in `partial` (workgroup, H), which a second kernel adds up in order.  Memory bounds it too: bf16 with ds, 16384 x 2048 49 us for
-// both kernels, 5.5 TB/s of three rows read and one written.
+// in `partial` (workgroup, H), which a second kernel adds up in order.  Memory bounds it too: bf16 with ds, 16384 x 2048 50 us for
+// both kernels, 5.4 TB/s of three rows read and one written (49 with the second sum in 32 bits, which rows near their type's end pass).
 template <typename T, typename TW, int LANES, int C, int THREADS, bool WHOLE>
 __global__ __launch_bounds__(THREADS) void norm_bwd_kernel(const T *__restrict__ dy, const T *__restrict__ ds, const T *__restrict__ s,
                                                           const TW *__restrict__ weight, T *__restrict__ dx,
@@ -84,11 +84,11 @@ __global__ __launch_bounds__(THREADS) void norm_bwd_kernel(const T *__restrict__
     constexpr int GROUPS = THREADS / LANES, WAVES = LANES / 64;
     constexpr bool ONE = C == 1;
     // s and dy stay in registers between a row's two passes where they fit; else they are read again, from the caches (1024 x 32768
-    // in bf16: 251 us in registers that spill, 139 so; 2048 x 16384: 81 in registers, 90 so)
+    // in bf16: 251 us in registers that spill, 155 so; 2048 x 16384: 81 in registers, 90 so)
     constexpr int HELD = C == 2 ? C : 1;
     constexpr bool AHEAD = WHOLE && ONE;  // the next row is asked for before this one's sums are there (16384 x 2048: 61 -> 50 us)
     __shared__ double squares[2][GROUPS * WAVES];
-    __shared__ float alongs[2][GROUPS * WAVES];
+    __shared__ double alongs[2][GROUPS * WAVES];
     extern __shared__ float shared_dw[];  // (GROUPS - 1, LANES * C * 8) where the groups are many
     const int i = threadIdx.x % LANES, group = threadIdx.x / LANES;
     float dw[C][8];
@@ -120,8 +120,7 @@ __global__ __launch_bounds__(THREADS) void norm_bwd_kernel(const T *__restrict__
         } else if (ONE) {
             fetch(row0, sv, g, d);
         }
-        double square = 0.0;  // (32 bits hold no square of a 32-bit or bf16 value past 2^64)
-        float along = 0.0f;
+        double square = 0.0, along = 0.0;  // (32 bits hold no square of a 32-bit or bf16 value past 2^64, nor a sum of many near 2^120)
 #pragma unroll HELD
         for (int c = 0; c < C; ++c) {
             if (!ONE) {
@@ -134,21 +133,19 @@ __global__ __launch_bounds__(THREADS) void norm_bwd_kernel(const T *__restrict__
             for (int u = 0; u < 8; ++u) {
                 const float a = to_f32(sv.v[u]);
                 square = __builtin_fma((double)a, (double)a, square);
-                along = __builtin_fmaf(to_f32(g.v[u]) * to_f32(w.v[u]), a, along);
+                along = __builtin_fma((double)(to_f32(g.v[u]) * to_f32(w.v[u])), (double)a, along);
             }
         }
-#pragma unroll
-        for (int step = 32; step; step >>= 1) along += __shfl_xor(along, step);
-        square = wave_sum(square);
+        square = wave_sum(square), along = wave_sum(along);
         if (WAVES > 1) {
             if ((threadIdx.x & 63) == 0) squares[turn][threadIdx.x >> 6] = square, alongs[turn][threadIdx.x >> 6] = along;
             __syncthreads();  // (two tables in turn: one barrier a row)
-            square = 0.0, along = 0.0f;
+            square = 0.0, along = 0.0;
 #pragma unroll
             for (int u = 0; u < WAVES; ++u) square += squares[turn][group * WAVES + u], along += alongs[turn][group * WAVES + u];
         }
         const double root = inverse_root(square / (double)H + eps);
-        const float r = (float)root, back = (float)((double)along / (double)H * root * root);  // dx = r (g - s back) + ds
+        const float r = (float)root, back = (float)(along / (double)H * root * root);  // dx = r (g - s back) + ds
         if (!in) continue;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
