@@ -7,6 +7,7 @@ import torch
 from qwen3_moe_fused import _lib
 from qwen3_moe_fused.fused_mlp import moe_fused_layer, moe_fused_layer_fp8
 from qwen3_moe_fused.kernels.norm import add_rms_norm, add_rms_norm_backward, add_rms_norm_fp8
+from qwen3_moe_fused.quantize.fp8 import check_fp8_rows
 
 BF16, F32, F16 = _lib.BF16, _lib.F32, _lib.F16
 NULL, SHAPE, DTYPE, ALIGN, WORKSPACE, LIMIT = -1, -2, -3, -4, -5, -7
@@ -211,3 +212,26 @@ def test_layer_operands(on_host, eight):
     with torch.no_grad(), pytest.raises(LibraryCalled):
         form(*good, 2, True)
 
+
+def _quantised(rows, k):
+    blocks = (k + 127) // 128
+    values = torch.zeros((rows, blocks * 128), dtype=torch.uint8).view(torch.float8_e4m3fn)[:, :k]
+    return values, torch.zeros((rows, (blocks + 3) // 4 * 4), dtype=torch.uint8).view(torch.float8_e8m0fnu)[:, :blocks]
+
+
+@pytest.mark.parametrize("rows", (0, 1, 2, 5))
+@pytest.mark.parametrize("k", (1, 96, 128, 200, 512))
+def test_quantised_rows_without_the_room_behind_them(rows, k):
+    like = torch.zeros((rows, k))
+    values, scales = _quantised(rows, k)
+    check_fp8_rows(values, scales, like)
+
+    def packed(t):
+        return t.view(torch.uint8).contiguous().clone(memory_format=torch.contiguous_format).view(t.dtype)
+
+    for whole, bad in ((k % 128 == 0, (packed(values), scales)), (k == 512, (values, packed(scales)))):
+        if rows == 0 or whole:
+            check_fp8_rows(*bad, like)
+        else:
+            with pytest.raises(AssertionError):
+                check_fp8_rows(*bad, like)

@@ -114,8 +114,8 @@ class Qwen3MoeFusedSparseMoeBlock(nn.Module):
     # units idle, and a training step of the block takes 1.62-1.67 ms instead of 1.58-1.63 ms.
     fuse_backward = False
     # set to True for calls of up to 16 tokens without gradients as the whole layer in two launches (fused_mlp.moe_fused_layer; bf16,
-    # fp16, fp32 and 8-bit expert matrices; one token of 128 experts in bf16 26 us a call against 45, 16 tokens 135 against 146).  Off by default: the results are
-    # not those of the separate steps bit for bit, since less is rounded on the way.
+    # fp16, fp32 and 8-bit expert matrices; 128 experts in bf16: one token 26 us a call against 45, 16 tokens 135 against 146).  Off
+    # by default: the results are not those of the separate steps bit for bit, since less is rounded on the way.
     fuse_layer = False
     # set to True to keep the expert ids of the last call in ``last_selected`` (tests read the block's own routing)
     keep_routing = False
