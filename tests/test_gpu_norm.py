@@ -372,3 +372,14 @@ def test_forward_onto_its_operands(width):
                                      _lib.dtype_code(dtype), _lib.dtype_code(dtype), _lib.stream())
     _lib.check(rc, "mfl_add_rms_norm")
     assert torch.equal(x, want) and torch.equal(r, want_s)
+
+
+@pytest.mark.parametrize("width", (1, 13, 200, 505, 1001))
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_single_row_is_written_out_from_where_it_stands(dtype, width):
+    x, _, w, _ = _inputs(1, width, dtype, width, residual=False)
+    values, scales, _ = add_rms_norm_fp8(x.cuda(), None, w.cuda())
+    want = dequantize_fp8_rows(values, scales, dtype)
+    tight = torch.zeros(7 + width, device="cuda", dtype=torch.uint8)
+    tight[7:] = values.view(torch.uint8)[0]
+    assert torch.equal(dequantize_fp8_rows(tight[7:].view(1, width).view(values.dtype), scales, dtype), want)

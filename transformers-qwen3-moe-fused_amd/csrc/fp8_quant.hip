@@ -91,7 +91,14 @@ __global__ __launch_bounds__(256) void dequant_rows_kernel(const uint8_t *__rest
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < runs; i += (int64_t)gridDim.x * 256) {
         const int64_t row = i / per_row;
         const int k = (int)(i - row * per_row) * 8;
-        const uint2_t v = *(const uint2_t *)(q + row * ld + k);
+        uint2_t v = {0u, 0u};
+        if (k + 8 <= K) {
+            __builtin_memcpy(&v, q + row * ld + k, sizeof(v));
+        } else {  // (a single row may end with its last column)
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                if (k + u < K) v[u / 4] |= (uint32_t)q[row * ld + k + u] << 8 * (u % 4);
+        }
         const float s = fp8_scale_of(scale[row * ld_scale + k / kFp8Block]);
         T o[8];
 #pragma unroll

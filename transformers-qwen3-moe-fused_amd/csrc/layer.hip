@@ -319,7 +319,7 @@ struct alignas(16) Run {
     uint64_t v[2];
 };
 
-// How the sizes fit the loads.  kExact: every load of every wave lies in its row (64 KB of a row of gate and up, as many of down): nothing
+// How the sizes fit the loads.  kExact: every load of every wave lies in its row (rows of whole chunks for all waves): nothing
 // is asked (16 tokens of the sizes above 150 -> 142 us, one 27.8 -> 25.9); kWhole: rows are whole loads long; kRagged: any.
 enum Fit { kRagged, kWhole, kExact };
 
