@@ -209,3 +209,22 @@ def test_hooks_keep_the_stock_forward(calls):
     with torch.no_grad():
         model(input_ids=ids)
     assert sorted(seen) == [1, 2]
+
+
+@pytest.mark.parametrize("tokens", (12, 90))
+def test_a_hook_in_front_of_8_bit_experts_decides_what_they_get(calls, tokens):
+    """The rows that the norm quantised are not those that the hook returns."""
+    model = _models(BF16, num_hidden_layers=1, mlp_only_layers=[]).eval()
+    block = model.layers[0].mlp
+    for name in ("gate_proj", "up_proj", "down_proj"):
+        setattr(block, name, MoeFusedLinearFp8.from_linear(getattr(block, name)))
+    ids = torch.randint(0, 300, (1, tokens), device="cuda")
+    _set(model)
+    seen = []
+    block.register_forward_pre_hook(lambda module, args: (seen.append(args[0]), args[0].roll(1, 1))[1])
+    block.register_forward_hook(lambda module, args, out: seen.append(out))
+    with torch.no_grad():
+        model(input_ids=ids)
+        assert "mfl_mlp_fwd_fp8_rows" not in calls
+        want = type(block).forward(block, seen[0].roll(1, 1))
+    assert torch.equal(seen[1], want)

@@ -235,3 +235,26 @@ def test_quantised_rows_without_the_room_behind_them(rows, k):
         else:
             with pytest.raises(AssertionError):
                 check_fp8_rows(*bad, like)
+
+
+@pytest.mark.parametrize("fuse", (False, True))
+def test_a_replaced_forward_of_the_block_gets_the_hidden_states_alone(monkeypatch, fuse):
+    pytest.importorskip("transformers")
+    from transformers import Qwen3MoeConfig
+
+    from qwen3_moe_fused.modular_qwen3_moe_fused import Qwen3MoeFusedModel, Qwen3MoeFusedSparseMoeBlock
+
+    config = Qwen3MoeConfig(vocab_size=20, hidden_size=16, intermediate_size=16, num_hidden_layers=1, num_attention_heads=2,
+                            num_key_value_heads=1, head_dim=8, moe_intermediate_size=8, num_experts=4, num_experts_per_tok=2)
+    model = Qwen3MoeFusedModel(config).eval()
+    model.layers[0].fuse_norm = model.layers[0].mlp.fuse_layer = fuse
+    seen = []
+
+    def replaced(self, hidden_states):
+        seen.append(hidden_states.shape)
+        return hidden_states, hidden_states.new_zeros(hidden_states.shape[1], 4)
+
+    monkeypatch.setattr(Qwen3MoeFusedSparseMoeBlock, "forward", replaced)
+    with torch.no_grad():
+        model(input_ids=torch.zeros((1, 3), dtype=torch.long))
+    assert seen == [(1, 3, 16)]

@@ -285,6 +285,8 @@ class Qwen3MoeFusedSparseMoeBlock(nn.Module):
         out = combine_rows(y, inv_sort_idx, routing_weights, sort_idx)
         return out.view(batch, seq, hidden), router_logits
 
+    _own_forward = forward
+
 
 def _hf_subclasses():
     """Model-level wiring (decoder layer / model / causal LM with the fused block swapped in),
@@ -302,7 +304,11 @@ def _hf_subclasses():
         class _TensorBlock(Qwen3MoeFusedSparseMoeBlock):
             def forward(self, hidden_states: torch.Tensor,
                         quantized: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> torch.Tensor:
-                return super().forward(hidden_states, quantized)[0]
+                # (a forward that somebody has put in the place of the block's takes the hidden states alone)
+                given = () if quantized is None else (quantized,)
+                return super().forward(hidden_states, *given)[0]
+
+            _own_forward = forward
 
         block_cls = _TensorBlock
 
@@ -348,11 +354,13 @@ def _hf_subclasses():
             x, residual = _lib.dense(x), _lib.dense(residual)
             if isinstance(self.mlp, Qwen3MoeFusedSparseMoeBlock) and x.numel():
                 flat, flat_residual = x.view(-1, x.shape[-1]), residual.view(-1, x.shape[-1])
-                watched = self.mlp._forward_hooks or self.mlp._forward_pre_hooks or "forward" in self.mlp.__dict__
-                whole = None if watched else self.mlp.whole_layer(flat, flat_residual, weight, eps)
+                # (who watches the block's call, or has replaced it, may change what it is given)
+                own = _stands_for_itself(self.mlp) and (Qwen3MoeFusedSparseMoeBlock.forward
+                                                        is Qwen3MoeFusedSparseMoeBlock._own_forward)
+                whole = self.mlp.whole_layer(flat, flat_residual, weight, eps) if own else None
                 if whole is not None:
                     return whole[0].view(x.shape)
-                if type(self.mlp.gate_proj) is MoeFusedLinearFp8:
+                if own and type(self.mlp.gate_proj) is MoeFusedLinearFp8:
                     values, scales, s, y = add_rms_norm_fp8(flat, flat_residual, weight, eps, return_normed=True)
                     return s.view(x.shape) + self.mlp(y.view(x.shape), quantized=(values, scales))
             y, s = add_rms_norm(x, residual, weight, eps)
