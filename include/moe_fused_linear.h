@@ -552,8 +552,9 @@ MFL_API int mfl_fp8_dequant_blocks(const void *q, const float *scale, int E, int
 
 /* s = x + residual, rounded to dtype; y = s / sqrt(mean(s^2) + eps) * weight along rows of H, rounded once behind sums and products
  * in 64 bits (to 32 bits and from there to dtype).  residual NULL: s is x, and the s given is not written.  weight (H) of dtype or
- * MFL_F32.  y may be x, s may be x or residual (no other overlap).  H is MFL_NORM_WIDTH at most (MFL_ERR_LIMIT).  The stock layers'
- * norm rounds once more between the two products. */
+ * MFL_F32.  y may be x, s may be x or residual (no other overlap).  H is MFL_NORM_WIDTH at most, and R 2^22 - 2^10 (64 threads a row
+ * up to H = 512, twice as many for every doubling up to 1024: more rows of narrower ones; MFL_ERR_LIMIT).  The stock layers' norm rounds
+ * once more between the two products. */
 #define MFL_NORM_WIDTH 32768
 MFL_API int mfl_add_rms_norm(const void *x, const void *residual, const void *weight, void *y, void *s, int64_t R, int H, float eps,
                      int dtype, int weight_dtype, void *stream);
