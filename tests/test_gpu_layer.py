@@ -220,6 +220,56 @@ def test_wide_values_of_the_gated_unit_in_fp16():
     case.check(out, logits)
 
 
+def _gated_units_of(case, wide):
+    """Token 0's gated unit is 2^128 (1 - 2^-12) in column 3 (past bf16's largest value, not past fp32's), or with ``wide`` times four of
+    that, of either sign in the experts' columns 3; token 1's values are small."""
+    case.x[:] = 0.0
+    case.x[0, :2] = 1.0
+    case.x[1] = torch.randn(case.x.shape[1], generator=torch.Generator().manual_seed(5)).to(case.dtype) * 2.0 ** -40
+    gate, up, down = case.weights
+    gate[:, 3], up[:, 3] = 0.0, 0.0
+    gate[:, 3, 0], up[:, 3, 0], up[:, 3, 1] = 2.0 ** 64, 2.0 ** 64, -(2.0 ** 52)
+    if wide:
+        up[:, 3] *= 4.0
+    up[1, 3] *= -1.0
+    down[:, :, 3] = torch.where(down[:, :, 3] < 0, -1.0, 1.0) * 2.0 ** -100
+
+
+@pytest.mark.parametrize("dtype", (BF16, F32))
+@pytest.mark.parametrize("k", (1, 2))
+def test_gated_unit_past_the_largest_bf16_value(dtype, k):
+    """In bf16 the unit is two bf16 values: the larger one stays finite where the unit is."""
+    case = Case(2, 2, k, 48, 40, dtype)
+    _gated_units_of(case, wide=False)
+    out, logits = case.call()
+    assert out.isfinite().all() and out[0].abs().min() > 0
+    case.check(out, logits)
+
+
+@pytest.mark.parametrize("dtype", (BF16, F32))
+def test_infinite_gated_unit(dtype):
+    """What the definition in 32 bits has: an infinity of the down projection's sign, and the other token as it is without it."""
+    case = Case(2, 2, 1, 48, 40, dtype)
+    _gated_units_of(case, wide=True)
+    out, logits = case.call()
+    ((expert, _),), _ = ref.choose(logits.cpu(), 1, True)
+    sign = case.weights[2][expert, :, 3].sign() * (-1 if expert else 1)
+    assert torch.equal(out[0].cpu(), sign * float("inf"))
+    case.x[0] = 0.0
+    assert torch.equal(case.call()[0][1], out[1]) and out[1].isfinite().all()
+
+
+def test_infinite_gated_unit_in_8_bits():
+    """An infinite element becomes NaN on its way to the grid, as in the expert MLP, and the other token is as it is without it."""
+    case = Case(2, 2, 2, 160, 200, BF16, eight=True)
+    case.scales[0], case.scales[1] = case.scales[0] * 2.0 ** 80, case.scales[1] * 2.0 ** 80
+    case.x[1] *= 2.0 ** -90
+    out, _ = case.call()
+    assert out[0].isnan().all() and out[1].isfinite().all()
+    case.x[0] = 0.0
+    assert torch.equal(case.call()[0][1], out[1])
+
+
 @pytest.mark.parametrize("eight", (False, True))
 def test_the_same_bits_every_time(eight):
     case = Case(16, 128, 8, 512, 256, BF16, eight=eight, norm=True, residual=True)

@@ -367,10 +367,12 @@ __device__ __forceinline__ Run settle(Run run, int k, int K) {
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 
 // bf16 layers keep a value h of the gated unit as two bf16 ones, h as rounded and what that leaves, as rounded: 2^-17 of it is lost at
-// most, where the output's own rounding is 2^-9.  fp16 weights are widened for h in 32 bits (it need not fit the type), and in 8-bit
+// most, where the output's own rounding is 2^-9.  The first is no further from zero than the type's largest value (past that h rounds
+// to an infinity, and what is left would be the other one): the second has what lies behind, an infinity or no number too.  fp16 weights are widened for h in 32 bits (it need not fit the type), and in 8-bit
 // layers h is quantised where it is read, by which time its blocks' largest magnitudes are known.
 template <typename T, bool FP8>
 constexpr bool kHalves = std::is_same<T, bf16_t>::value && !FP8;
+constexpr float kLargest = 3.3895313892515355e38f;  // of bf16: 2^128 (1 - 2^-8)
 
 // What workgroups hand to one another within a kernel goes past the L2s of the XCDs, both ways: stores and loads of the device's
 // scope.  (Ordinary ones with a fence before the word that says so write back and invalidate a whole L2 for every wave: 120 us.)
@@ -565,7 +567,7 @@ struct GateUp {
                 bf16x4 high, low;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    high[i] = (bf16_t)acc[i];
+                    high[i] = (bf16_t)__builtin_amdgcn_fmed3f(acc[i], -kLargest, kLargest);
                     low[i] = (bf16_t)(acc[i] - (float)high[i]);
                 }
                 publish((bf16_t *)to + 4 * g, __builtin_bit_cast(uint64_t, high));
