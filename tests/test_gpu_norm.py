@@ -5,7 +5,7 @@ import torch
 import layer_reference as ref
 from qwen3_moe_fused import _lib
 from qwen3_moe_fused.kernels.norm import add_rms_norm, add_rms_norm_backward, add_rms_norm_fp8
-from qwen3_moe_fused.quantize.fp8 import dequantize_fp8_rows, quantize_fp8_rows
+from qwen3_moe_fused.quantize.fp8 import dequantize_fp8_rows, empty_fp8_rows, quantize_fp8_rows
 
 pytestmark = pytest.mark.gpu
 DTYPES = (torch.bfloat16, torch.float16, torch.float32)
@@ -383,3 +383,50 @@ def test_a_single_row_is_written_out_from_where_it_stands(dtype, width):
     tight = torch.zeros(7 + width, device="cuda", dtype=torch.uint8)
     tight[7:] = values.view(torch.uint8)[0]
     assert torch.equal(dequantize_fp8_rows(tight[7:].view(1, width).view(values.dtype), scales, dtype), want)
+
+
+@pytest.mark.parametrize("dtype", (torch.float16, torch.float32))
+@pytest.mark.parametrize("width", (512, 1024, 4096, 8192, 300, 1001, 2050, 9001, 20001))
+@pytest.mark.parametrize("form", ("plain", "eight"))
+def test_forward_onto_its_operands_in_every_width(dtype, width, form):
+    x, r, w, _ = _inputs(23, width, dtype, width)
+    x, r, w = _cuda(x, r, w)
+    want, want_s = add_rms_norm(x, r, w, EPS)
+    code, lib = _lib.dtype_code(dtype), _lib.lib()
+    q, scale = quantize_fp8_rows(want)
+    got_q, got_scale = empty_fp8_rows(x)
+
+    def run(x, r, y, s):
+        if form == "plain":
+            rc = lib.mfl_add_rms_norm(x.data_ptr(), r.data_ptr(), w.data_ptr(), y.data_ptr(), s.data_ptr(), 23, width, EPS, code, code,
+                                      _lib.stream())
+        else:
+            rc = lib.mfl_add_rms_norm_fp8(x.data_ptr(), r.data_ptr(), w.data_ptr(), got_q.data_ptr(), got_scale.data_ptr(), y.data_ptr(),
+                                          s.data_ptr(), 23, width, EPS, code, code, _lib.stream())
+            assert torch.equal(got_q.view(torch.uint8), q.view(torch.uint8))
+            assert torch.equal(got_scale.view(torch.uint8), scale.view(torch.uint8))
+        _lib.check(rc, "norm")
+        assert torch.equal(y, want) and torch.equal(s, want_s)
+
+    a, b = x.clone(), r.clone()
+    run(a, b, a, b)  # y onto x, s onto the residual
+    a, b = x.clone(), r.clone()
+    run(a, b, torch.empty_like(x), a)  # s onto x
+
+
+@pytest.mark.parametrize("dtype", (torch.float16, torch.float32))
+@pytest.mark.parametrize("width", (512, 1024, 4096, 8192, 300, 1001, 2050, 9001, 20001, 32768))
+@pytest.mark.parametrize("onto", ("dy", "ds", "s"))
+def test_backward_onto_an_operand_in_every_width(dtype, width, onto):
+    s, ds, w, g = _inputs(1500 if width <= 4096 else 700, width, dtype, width)  # (several rows a group)
+    dy = torch.randn(s.shape, generator=g).to(dtype)
+    s, ds, w, dy = _cuda(s, ds, w, dy)
+    want, want_dw = add_rms_norm_backward(dy, ds, s, w, EPS)
+    ops = {"dy": dy, "ds": ds, "s": s}
+    lib, dw, code, rows = _lib.lib(), torch.empty_like(w), _lib.dtype_code(dtype), s.shape[0]
+    size = lib.mfl_add_rms_norm_bwd_workspace(rows, width)
+    ws = torch.empty(size, device="cuda", dtype=torch.uint8)
+    rc = lib.mfl_add_rms_norm_bwd(dy.data_ptr(), ds.data_ptr(), s.data_ptr(), w.data_ptr(), ops[onto].data_ptr(), dw.data_ptr(), rows, width,
+                                  EPS, code, code, ws.data_ptr(), size, _lib.stream())
+    _lib.check(rc, "norm backward")
+    assert torch.equal(ops[onto], want) and torch.equal(dw, want_dw)

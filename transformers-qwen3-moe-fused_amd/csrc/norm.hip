@@ -11,11 +11,11 @@ namespace {
 // ---- forward --------------------------------------------------------------------------------------------------------------
 // A row belongs to LANES threads, which hold it in registers, 8 C elements each in C runs of 8: one pass over memory, which is all
 // that bounds it where there are rows enough to fill the chip.  bf16 with a residual: 16384 x 2048 44.6 us, 6.0 TB/s of the 2 + 2
-// rows that it has to read and write, 4096 x 8192 44.3, 1024 x 32768 52.5; to 8-bit rows 16384 x 2048 50.
+// rows that it has to read and write, 4096 x 8192 44.3, 1024 x 32768 52.5; to 8-bit rows 16384 x 2048 50.  y may be x, and s x or
+// the residual: what a thread reads of a row it has read before it writes there.
 template <typename T, typename TW, int LANES, int C, bool FP8, bool WHOLE>
-__global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_fwd_kernel(const T *__restrict__ x, const T *__restrict__ residual,
-                                                                           const TW *__restrict__ weight, T *__restrict__ y,
-                                                                           T *__restrict__ s, uint8_t *__restrict__ q,
+__global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_fwd_kernel(const T *x, const T *residual, const TW *__restrict__ weight,
+                                                                           T *y, T *s, uint8_t *__restrict__ q,
                                                                            uint8_t *__restrict__ scale, int64_t R, int H,
                                                                            double eps) {
     constexpr int ROWS = LANES < 256 ? 256 / LANES : 1, WAVES = LANES / 64;
@@ -77,9 +77,9 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_fwd_kernel(con
 // gridDim.x * GROUPS-th row and keeps its columns' share of dw in registers; the groups of a workgroup meet in LDS, the workgroups
 // in `partial` (workgroup, H), which a second kernel adds up in order.  Memory bounds it too: bf16 with ds, 16384 x 2048 50 us for
 // both kernels, 5.4 TB/s of three rows read and one written (49 with the second sum in 32 bits, which rows near their type's end pass).
+// dx may be dy, ds or s, so whatever is to be on its way over a store is asked for in front of it.
 template <typename T, typename TW, int LANES, int C, int THREADS, bool WHOLE>
-__global__ __launch_bounds__(THREADS) void norm_bwd_kernel(const T *__restrict__ dy, const T *__restrict__ ds, const T *__restrict__ s,
-                                                          const TW *__restrict__ weight, T *__restrict__ dx,
+__global__ __launch_bounds__(THREADS) void norm_bwd_kernel(const T *dy, const T *ds, const T *s, const TW *__restrict__ weight, T *dx,
                                                           float *__restrict__ partial, int64_t R, int H, double eps) {
     constexpr int GROUPS = THREADS / LANES, WAVES = LANES / 64;
     constexpr bool ONE = C == 1;
