@@ -258,3 +258,56 @@ def test_a_replaced_forward_of_the_block_gets_the_hidden_states_alone(monkeypatc
     with torch.no_grad():
         model(input_ids=torch.zeros((1, 3), dtype=torch.long))
     assert seen == [(1, 3, 16)]
+
+
+def _small_model(**changed):
+    pytest.importorskip("transformers")
+    from transformers import Qwen3MoeConfig
+
+    from qwen3_moe_fused.modular_qwen3_moe_fused import Qwen3MoeFusedModel, Qwen3MoeFusedSparseMoeBlock
+
+    config = Qwen3MoeConfig(**{**dict(vocab_size=20, hidden_size=16, intermediate_size=16, num_hidden_layers=1, num_attention_heads=2,
+                                      num_key_value_heads=1, head_dim=8, moe_intermediate_size=8, num_experts=4,
+                                      num_experts_per_tok=2, mlp_only_layers=[0]), **changed})  # (a dense layer runs on the host)
+    model = Qwen3MoeFusedModel(config).eval()
+    if type(model.layers[0].mlp) is Qwen3MoeFusedSparseMoeBlock:
+        pytest.skip("this transformers release has blocks that return their logits")
+    return model
+
+
+@pytest.fixture
+def own_half(monkeypatch):
+    """A small model whose layers have the norm fused, and the calls of the half that goes past the norm's module."""
+    model, calls = _small_model(), []
+    cls = type(model.layers[0])
+    real = cls._feed_forward
+    monkeypatch.setattr(cls, "_feed_forward", lambda *args: (calls.append(1), real(*args))[1])
+    model.layers[0].fuse_norm = True
+    return model, calls
+
+
+def test_a_replaced_forward_of_the_norms_class_is_called(own_half, monkeypatch):
+    model, calls = own_half
+    ids = torch.zeros((1, 3), dtype=torch.long)
+    with torch.no_grad():
+        model(input_ids=ids)
+        assert calls == [1]
+        seen, norm = [], type(model.layers[0].post_attention_layernorm)
+        stock = norm.forward
+        monkeypatch.setattr(norm, "forward", lambda self, hidden_states: (seen.append(self), stock(self, hidden_states))[1])
+        model(input_ids=ids)
+    assert calls == [1] and model.layers[0].post_attention_layernorm in seen
+
+
+def test_a_forward_replaced_before_the_classes_are_built_is_known_too(monkeypatch):
+    pytest.importorskip("transformers")
+    import functools
+
+    from transformers.models.qwen3_moe.modeling_qwen3_moe import Qwen3MoeRMSNorm
+
+    from qwen3_moe_fused.modular_qwen3_moe_fused import _defined_forward
+
+    stock = Qwen3MoeRMSNorm.forward
+    assert _defined_forward(Qwen3MoeRMSNorm) is stock
+    monkeypatch.setattr(Qwen3MoeRMSNorm, "forward", functools.wraps(stock)(lambda self, hidden_states: stock(self, hidden_states)))
+    assert _defined_forward(Qwen3MoeRMSNorm) is None

@@ -9,6 +9,7 @@ load unchanged.
 from __future__ import annotations
 
 import math
+import sys
 from typing import Optional, Tuple
 
 import torch
@@ -86,6 +87,12 @@ def _stands_for_itself(module: nn.Module) -> bool:
     """Whether a module's call is its class's forward and nothing else: no hooks, no replaced forward."""
     return not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks
                 or "forward" in module.__dict__ or type(module).forward is not type(module)._own_forward)
+
+
+def _defined_forward(cls: type):
+    """A foreign class's forward, or None where somebody has put another in the place of the one in its module's source."""
+    forward = cls.forward
+    return forward if getattr(forward, "__globals__", None) is vars(sys.modules[cls.__module__]) else None
 
 
 class Qwen3MoeFusedSparseMoeBlock(nn.Module):
@@ -313,6 +320,7 @@ def _hf_subclasses():
         block_cls = _TensorBlock
 
     stock_forward = inspect.signature(Qwen3MoeDecoderLayer.forward)
+    stock_norm = _defined_forward(Qwen3MoeRMSNorm)
 
     class Qwen3MoeFusedDecoderLayer(Qwen3MoeDecoderLayer):
         # set to True for the addition behind the attention and the norm in front of the experts as one kernel (kernels/norm.py), both
@@ -332,7 +340,8 @@ def _hf_subclasses():
             # (of releases whose block returns its logits the layer's results are another matter: their forward stays theirs)
             if (not self.fuse_norm or block_cls is Qwen3MoeFusedSparseMoeBlock or type(norm) is not Qwen3MoeRMSNorm
                     or norm._forward_hooks or norm._forward_pre_hooks or norm._backward_hooks or norm._backward_pre_hooks
-                    or "forward" in norm.__dict__ or torch.nn.modules.module._has_any_global_hook() or not _lib.plain_call()):
+                    or "forward" in norm.__dict__ or Qwen3MoeRMSNorm.forward is not stock_norm
+                    or torch.nn.modules.module._has_any_global_hook() or not _lib.plain_call()):
                 return super().forward(hidden_states, *args, **kwargs)
             given = stock_forward.bind(self, hidden_states, *args, **kwargs)
             given.apply_defaults()
