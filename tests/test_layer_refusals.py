@@ -311,3 +311,13 @@ def test_a_forward_replaced_before_the_classes_are_built_is_known_too(monkeypatc
     assert _defined_forward(Qwen3MoeRMSNorm) is stock
     monkeypatch.setattr(Qwen3MoeRMSNorm, "forward", functools.wraps(stock)(lambda self, hidden_states: stock(self, hidden_states)))
     assert _defined_forward(Qwen3MoeRMSNorm) is None
+
+
+def test_a_replaced_forward_of_the_stock_layer_is_called(own_half, monkeypatch):
+    model, calls = own_half
+    stock_class = type(model.layers[0]).__mro__[1]
+    seen, stock = [], stock_class.forward
+    monkeypatch.setattr(stock_class, "forward", lambda self, *args, **kwargs: (seen.append(self), stock(self, *args, **kwargs))[1])
+    with torch.no_grad():
+        model(input_ids=torch.zeros((1, 3), dtype=torch.long))
+    assert seen == [model.layers[0]] and not calls

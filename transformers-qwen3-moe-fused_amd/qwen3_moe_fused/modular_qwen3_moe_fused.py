@@ -320,7 +320,7 @@ def _hf_subclasses():
         block_cls = _TensorBlock
 
     stock_forward = inspect.signature(Qwen3MoeDecoderLayer.forward)
-    stock_norm = _defined_forward(Qwen3MoeRMSNorm)
+    stock_layer, stock_norm = _defined_forward(Qwen3MoeDecoderLayer), _defined_forward(Qwen3MoeRMSNorm)
 
     class Qwen3MoeFusedDecoderLayer(Qwen3MoeDecoderLayer):
         # set to True for the addition behind the attention and the norm in front of the experts as one kernel (kernels/norm.py), both
@@ -341,6 +341,7 @@ def _hf_subclasses():
             if (not self.fuse_norm or block_cls is Qwen3MoeFusedSparseMoeBlock or type(norm) is not Qwen3MoeRMSNorm
                     or norm._forward_hooks or norm._forward_pre_hooks or norm._backward_hooks or norm._backward_pre_hooks
                     or "forward" in norm.__dict__ or Qwen3MoeRMSNorm.forward is not stock_norm
+                    or Qwen3MoeDecoderLayer.forward is not stock_layer
                     or torch.nn.modules.module._has_any_global_hook() or not _lib.plain_call()):
                 return super().forward(hidden_states, *args, **kwargs)
             given = stock_forward.bind(self, hidden_states, *args, **kwargs)
