@@ -6,7 +6,7 @@ import torch
 
 from qwen3_moe_fused import _lib
 from qwen3_moe_fused.fused_mlp import moe_fused_layer, moe_fused_layer_fp8
-from qwen3_moe_fused.kernels.norm import add_rms_norm, add_rms_norm_backward, add_rms_norm_fp8
+from qwen3_moe_fused.kernels.norm import add_rms_norm, add_rms_norm_backward, add_rms_norm_fp8, most_rows
 from qwen3_moe_fused.quantize.fp8 import check_fp8_rows
 
 BF16, F32, F16 = _lib.BF16, _lib.F32, _lib.F16
@@ -321,3 +321,25 @@ def test_a_replaced_forward_of_the_stock_layer_is_called(own_half, monkeypatch):
     with torch.no_grad():
         model(input_ids=torch.zeros((1, 3), dtype=torch.long))
     assert seen == [model.layers[0]] and not calls
+
+
+@pytest.mark.parametrize("width", (1, 512, 513, 1024, 1025, 2048, 2049, 4096, 4097, 8192, 8193, 32768))
+def test_rows_of_a_call(p, width):
+    """The bound that the header names, from either side (nothing is launched: without rows to read the call ends with NULL)."""
+    lib, most = _lib.lib(), most_rows(width)
+    assert most == 2 ** 32 // max(64, min(1024, 1 << ((width + 7) // 8 - 1).bit_length())) - 1024
+    assert width <= 4096 or most == 2 ** 22 - 2 ** 10
+    for rows, code in ((most, NULL), (most + 1, LIMIT)):
+        assert lib.mfl_add_rms_norm(None, None, p, p, p, rows, width, 1e-6, BF16, BF16, None) == code
+        assert lib.mfl_add_rms_norm_fp8(None, None, p, p, p, None, p, rows, width, 1e-6, BF16, BF16, None) == code
+    assert lib.mfl_add_rms_norm_bwd(None, None, p, p, p, None, most + 1, width, 1e-6, BF16, BF16, p, 4096, None) == NULL
+
+
+def test_more_rows_than_a_call_takes_stay_with_the_separate_steps(on_host, monkeypatch):
+    layer = _small_model().layers[0].to("meta", torch.bfloat16)
+    monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda t: True))
+    with torch.no_grad():
+        few, many = (torch.empty((1, rows, 16), device="meta", dtype=torch.bfloat16) for rows in (most_rows(16), most_rows(16) + 1))
+        with pytest.raises(LibraryCalled):
+            layer._feed_forward(few, few, layer.post_attention_layernorm)
+        assert layer._feed_forward(many, many, layer.post_attention_layernorm).shape == many.shape

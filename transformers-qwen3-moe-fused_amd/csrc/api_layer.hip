@@ -8,9 +8,9 @@ using namespace mfl;
 
 namespace {
 
-int check_norm(const NormCall &n) {
+int check_norm(const NormCall &n, bool forward) {
     if (n.R < 0 || n.H <= 0) return MFL_ERR_SHAPE;
-    if (n.H > MFL_NORM_WIDTH) return MFL_ERR_LIMIT;
+    if (n.H > MFL_NORM_WIDTH || (forward && n.R > add_rms_norm_rows(n.H))) return MFL_ERR_LIMIT;
     if (!(n.eps >= 0.0f) || isinf(n.eps)) return MFL_ERR_SHAPE;
     if (!dtype_ok(n.dtype) || (n.weight_dtype != n.dtype && n.weight_dtype != MFL_F32)) return MFL_ERR_DTYPE;
     if (n.R == 0) return MFL_OK;
@@ -35,7 +35,7 @@ extern "C" {
 int mfl_add_rms_norm(const void *x, const void *residual, const void *weight, void *y, void *s, int64_t R, int H, float eps, int dtype,
                      int weight_dtype, void *stream) {
     const NormCall n = {x, residual, weight, y, s, nullptr, nullptr, R, H, eps, dtype, weight_dtype};
-    const int rc = check_norm(n);
+    const int rc = check_norm(n, true);
     if (rc) return rc;
     if (R == 0) return MFL_OK;
     if (!y) return MFL_ERR_NULL;
@@ -45,7 +45,7 @@ int mfl_add_rms_norm(const void *x, const void *residual, const void *weight, vo
 int mfl_add_rms_norm_fp8(const void *x, const void *residual, const void *weight, void *q, uint8_t *scale, void *y, void *s, int64_t R,
                          int H, float eps, int dtype, int weight_dtype, void *stream) {
     const NormCall n = {x, residual, weight, y, s, (uint8_t *)q, scale, R, H, eps, dtype, weight_dtype};
-    const int rc = check_norm(n);
+    const int rc = check_norm(n, true);
     if (rc) return rc;
     if (R == 0) return MFL_OK;
     if (!q || !scale) return MFL_ERR_NULL;
@@ -60,7 +60,7 @@ size_t mfl_add_rms_norm_bwd_workspace(int64_t R, int H) {
 int mfl_add_rms_norm_bwd(const void *dy, const void *ds, const void *s, const void *weight, void *dx, void *dw, int64_t R, int H,
                          float eps, int dtype, int weight_dtype, void *workspace, size_t ws_bytes, void *stream) {
     const NormCall n = {s, nullptr, weight, nullptr, (void *)s, nullptr, nullptr, R, H, eps, dtype, weight_dtype};
-    int rc = check_norm(n);
+    int rc = check_norm(n, false);
     if (rc) return rc;
     if (!dx && !dw) return MFL_OK;
     const size_t size = dtype_size(dtype);

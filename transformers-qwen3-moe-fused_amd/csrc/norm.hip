@@ -299,10 +299,10 @@ int bwd(const NormCall &n, const void *dy, const void *ds, void *dx, void *dw, f
 
 }  // namespace
 
+// (a launch's threads are counted in 32 bits: below 2^32 with the last workgroup's, too)
+int64_t add_rms_norm_rows(int H) { return (1ll << 32) / lanes_of(H) - 1024; }
+
 int add_rms_norm(const NormCall &n, hipStream_t stream) {
-    // (a launch's threads are counted in 32 bits)
-    const int64_t lanes = lanes_of(n.H);
-    if (n.R > 0xffffffffll / lanes - 1024) return MFL_ERR_LIMIT;
     int rc = MFL_OK;
     MFL_DISPATCH_FLOAT(n.dtype, T, {
         if (n.weight_dtype == n.dtype) rc = fwd<T, T>(n, stream);

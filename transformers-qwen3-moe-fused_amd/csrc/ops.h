@@ -34,7 +34,7 @@ int nf4_quant(const void *w, int w_dtype, int64_t n, int blocksize, const float 
               hipStream_t stream);
 
 // s = x + residual (x itself, not written, where residual is null), y = s / sqrt(mean(s^2) + eps) * weight; y, and its 8-bit blocks
-// q with their scale bytes, where given.  H up to MFL_NORM_WIDTH.
+// q with their scale bytes, where given.  H up to MFL_NORM_WIDTH, R up to add_rms_norm_rows(H) (forward).
 struct NormCall {
     const void *x, *residual, *weight;
     void *y, *s;
@@ -44,6 +44,7 @@ struct NormCall {
     float eps;
     int dtype, weight_dtype;
 };
+int64_t add_rms_norm_rows(int H);
 int add_rms_norm(const NormCall &n, hipStream_t stream);
 size_t add_rms_norm_bwd_workspace(int64_t R, int H);
 // n.s: the stream that the forward pass left (read); dx, dw where wanted, ds may be null.

@@ -16,6 +16,18 @@ from .. import _lib
 from ..quantize.fp8 import empty_fp8_rows
 
 
+WIDTH = 32768  # MFL_NORM_WIDTH
+
+
+def most_rows(width: int) -> int:
+    """The rows that one call takes at a width up to ``WIDTH``: a launch's threads are counted in 32 bits, and a row has 64 of them up to
+    512 columns, twice as many for every doubling up to 1024."""
+    lanes = 64
+    while lanes < 1024 and lanes * 8 < width:
+        lanes *= 2
+    return (1 << 32) // lanes - 1024
+
+
 def _check(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor) -> Tuple[int, int, int]:
     """Returns (rows, width, the type's code)."""
     assert x.is_cuda and x.ndim >= 1 and x.is_contiguous(), "the norm runs on the GPU, on dense rows"

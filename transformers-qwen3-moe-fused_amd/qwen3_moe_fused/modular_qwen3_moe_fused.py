@@ -352,13 +352,14 @@ def _hf_subclasses():
             return self._feed_forward(attention, hidden_states, norm)
 
         def _feed_forward(self, x: torch.Tensor, residual: torch.Tensor, norm: nn.Module) -> torch.Tensor:
-            from .kernels.norm import add_rms_norm, add_rms_norm_fp8
+            from .kernels.norm import WIDTH, add_rms_norm, add_rms_norm_fp8, most_rows
             from .quantize.layer_fp8 import MoeFusedLinearFp8
 
             weight, eps = norm.weight, norm.variance_epsilon
             if (not x.is_cuda or x.dtype != residual.dtype or x.shape != residual.shape or x.device != residual.device
                     or x.dtype not in (torch.bfloat16, torch.float16, torch.float32) or weight.dtype not in (x.dtype, torch.float32)
-                    or x.shape[-1] > 32768 or torch.is_autocast_enabled("cuda")):
+                    or x.shape[-1] > WIDTH or x.numel() > most_rows(x.shape[-1]) * x.shape[-1]
+                    or torch.is_autocast_enabled("cuda")):
                 s = residual + x
                 return s + self.mlp(norm(s))
             x, residual = _lib.dense(x), _lib.dense(residual)
