@@ -343,3 +343,28 @@ def test_more_rows_than_a_call_takes_stay_with_the_separate_steps(on_host, monke
         with pytest.raises(LibraryCalled):
             layer._feed_forward(few, few, layer.post_attention_layernorm)
         assert layer._feed_forward(many, many, layer.post_attention_layernorm).shape == many.shape
+
+
+@pytest.mark.parametrize("rows", (1, 3))
+@pytest.mark.parametrize("k", (1, 96, 128, 200, 512))
+def test_quantised_rows_whose_storage_ends_with_the_last_column(rows, k):
+    """A copy of a single row keeps its stride without the room that this stands for."""
+    like = torch.zeros((rows, k))
+    values, scales = _quantised(rows, k)
+
+    def cut(t):
+        copy = t.view(torch.uint8)
+        copy = copy.clone() if rows == 1 else torch.empty_strided(copy.shape, copy.stride(), dtype=torch.uint8)
+        assert copy.stride() == t.stride()
+        return copy.view(t.dtype)
+
+    for whole, bad in ((k % 128 == 0, (cut(values), scales)), (k == 512, (values, cut(scales)))):
+        if whole:
+            check_fp8_rows(*bad, like)
+        else:
+            with pytest.raises(AssertionError):
+                check_fp8_rows(*bad, like)
+    # a row of a table has the next one's room in front of it, the last one its own
+    table, table_scales = _quantised(4, k)
+    for at in range(0, 5 - rows):
+        check_fp8_rows(table[at:at + rows], table_scales[at:at + rows], like)

@@ -41,9 +41,12 @@ def check_fp8_rows(values: torch.Tensor, scale: torch.Tensor, like: torch.Tensor
     assert scale.shape == (rows, blocks)
     device = like.get_device()
     assert values.get_device() == device and scale.get_device() == device
-    # (a single row's stride says whether there is room behind its last column; where it is whole blocks none is needed)
+    # (the last row has room behind its last column too: of a single row the stride does not say so, a copy keeps it and ends with the
+    # column; where rows are whole blocks none is needed)
     for t, width, ld in ((values, k, blocks * BLOCK), (scale, blocks, (blocks + 3) // 4 * 4)):
-        assert t.stride(0) == ld or rows == 0 or (rows == 1 and width == ld), "values and scales as quantize_fp8_rows lays them out"
+        assert rows == 0 or (rows == 1 and width == ld) or (
+            t.stride(0) == ld and t.untyped_storage().nbytes() >= t.storage_offset() + rows * ld), \
+            "values and scales as quantize_fp8_rows lays them out"
     assert (k == 1 or values.stride(1) == 1) and (blocks == 1 or scale.stride(1) == 1)
 
 
