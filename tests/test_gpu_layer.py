@@ -129,6 +129,32 @@ def test_benchmark_sizes(eight):
     case.check(*case.call())
 
 
+# 8-bit layers whose workgroups take many items of gate and up: the loop in which nothing is asked.  Rows of either chunk length that fit
+# its loads, that are whole loads, that are neither, and of two chunks.
+MANY = [
+    # tokens, experts, k, hidden, inter
+    (13, 40, 8, 2048, 768),
+    (16, 72, 8, 1536, 400),
+    (13, 64, 8, 1100, 500),
+    (16, 36, 8, 4096, 768),
+    (16, 80, 8, 1024, 768),
+    (16, 128, 8, 256, 768),
+    (16, 128, 8, 250, 700),
+]
+
+
+@pytest.mark.parametrize("size", MANY, ids=str)
+def test_many_items_a_workgroup_in_8_bits(size):
+    tokens, experts, k, hidden, inter = size
+    case = Case(*size, BF16, eight=True, norm=tokens == 13, residual=tokens == 13, seed=sum(size))
+    out, logits = case.call()
+    hit = len({e for picked in ref.choose(logits.cpu(), k, True) for e, _ in picked})
+    items, ahead = hit * 2 * ((inter + 15) // 16), 8 if hidden <= 1024 else 4
+    # (from the first item of a workgroup the loop takes another turn while 2 ahead - 1 more are there; two turns at least)
+    assert items > (3 * ahead - 1) * torch.cuda.get_device_properties(0).multi_processor_count
+    case.check(out, logits)
+
+
 @pytest.mark.parametrize("dtype", (BF16, F16))
 @pytest.mark.parametrize("eight", (False, True))
 def test_all_tokens_choose_the_same_experts(dtype, eight):

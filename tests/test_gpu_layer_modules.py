@@ -228,3 +228,66 @@ def test_a_hook_in_front_of_8_bit_experts_decides_what_they_get(calls, tokens):
         assert "mfl_mlp_fwd_fp8_rows" not in calls
         want = type(block).forward(block, seen[0].roll(1, 1))
     assert torch.equal(seen[1], want)
+
+
+def test_cached_decoding_calls_the_layer_and_agrees_with_the_stock_steps(calls):
+    pytest.importorskip("transformers")
+    from transformers import DynamicCache
+
+    model = _models(F32).eval()
+    ids = torch.randint(0, 300, (1, 9), device="cuda")
+    with torch.no_grad():
+        want = model(input_ids=ids).last_hidden_state
+        assert "mfl_moe_layer_fwd" not in calls and "mfl_add_rms_norm" not in calls
+        _set(model, layer=True)
+        cache, parts = DynamicCache(config=model.config), []
+        for step, (lo, hi) in enumerate(((0, 6), (6, 7), (7, 8), (8, 9)), 1):
+            parts.append(model(input_ids=ids[:, lo:hi], past_key_values=cache, use_cache=True).last_hidden_state)
+            assert calls["mfl_moe_layer_fwd"] == 2 * step  # (layers 0 and 2; layer 1 is dense)
+            assert calls["mfl_add_rms_norm"] == step
+    torch.testing.assert_close(torch.cat(parts, 1), want, rtol=1e-4, atol=1e-4)
+
+
+@pytest.mark.parametrize("eight", (False, True))
+@pytest.mark.parametrize("watch", ("autocast", "mode"))
+def test_autocast_and_watched_calls_keep_the_separate_steps(calls, watch, eight):
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Watching(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    model = _models(BF16).eval()
+    if eight:
+        for decoder in model.layers:
+            if isinstance(decoder.mlp, Qwen3MoeFusedSparseMoeBlock):
+                for name in ("gate_proj", "up_proj", "down_proj"):
+                    setattr(decoder.mlp, name, MoeFusedLinearFp8.from_linear(getattr(decoder.mlp, name)))
+    ids = torch.randint(0, 300, (1, 7), device="cuda")
+    results = []
+    with torch.no_grad():
+        for norm in (False, True):
+            _set(model, norm, layer=norm)
+            with torch.autocast("cuda", BF16) if watch == "autocast" else Watching():
+                results.append(model(input_ids=ids).last_hidden_state)
+    assert not {"mfl_moe_layer_fwd", "mfl_add_rms_norm", "mfl_add_rms_norm_fp8"} & set(calls)
+    assert torch.equal(*results)
+
+
+def test_checkpointed_layers_have_the_same_gradients(calls):
+    model = _models(F32).train()
+    _set(model)
+    ids = torch.randint(0, 300, (2, 24), device="cuda")
+    grads = []
+    for on in (False, True):
+        if on:
+            model.gradient_checkpointing_enable({"use_reentrant": False})
+        calls.clear()
+        model.zero_grad()
+        y = model(input_ids=ids).last_hidden_state
+        (y * y.detach().roll(1, -1)).mean().backward()
+        assert calls["mfl_add_rms_norm"] == (6 if on else 3) and calls["mfl_add_rms_norm_bwd"] == 3
+        grads.append({n: p.grad.clone() for n, p in model.named_parameters() if p.grad is not None})
+    assert grads[0].keys() == grads[1].keys()
+    for n, g in grads[0].items():
+        torch.testing.assert_close(grads[1][n], g, rtol=1e-5, atol=1e-5 * g.abs().max().item(), msg=n)

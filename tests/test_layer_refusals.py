@@ -368,3 +368,25 @@ def test_quantised_rows_whose_storage_ends_with_the_last_column(rows, k):
     table, table_scales = _quantised(4, k)
     for at in range(0, 5 - rows):
         check_fp8_rows(table[at:at + rows], table_scales[at:at + rows], like)
+
+
+@pytest.mark.parametrize("how", ("compiled", "mode", "traced"))
+def test_a_layer_that_is_watched_keeps_the_separate_steps(own_half, how):
+    from torch.utils.flop_counter import FlopCounterMode
+
+    model, calls = own_half
+    layer, x = model.layers[0].requires_grad_(False), torch.randn((1, 3, 16), generator=torch.Generator().manual_seed(0))
+    given = {"position_embeddings": model.rotary_emb(x, torch.arange(3)[None])}
+    with torch.no_grad():
+        want = layer(x, **given)
+        assert calls == [1]
+        if how == "compiled":
+            got = torch.compile(layer, backend="eager", fullgraph=True)(x, **given)
+        elif how == "mode":
+            with FlopCounterMode(display=False):
+                got = layer(x, **given)
+        else:
+            seen = []
+            torch.jit.trace(lambda t: seen.append(layer(t, **given)) or seen[-1], (x,), check_trace=False)
+            got = seen[0]
+    assert calls == [1] and torch.equal(got, want)
