@@ -560,7 +560,8 @@ MFL_API int mfl_add_rms_norm(const void *x, const void *residual, const void *we
                      int dtype, int weight_dtype, void *stream);
 /* Its gradients from dy and, where not NULL, ds (what arrives for s): dx (R,H), which is the residual's gradient too, and dw (H) in
  * weight_dtype, where not NULL.  s (R,H) as the forward call left it.  workspace: mfl_add_rms_norm_bwd_workspace(R, H) bytes where dw
- * is asked for, 16-byte aligned.  Same bits from run to run.  dx may be dy, ds or s. */
+ * is asked for, 16-byte aligned.  Same bits from run to run.  dx may be dy, ds or s.  A row's two sums are in 64 bits, its 1 / length,
+ * dy weight and the sums over the rows in 32 (eps 0 and rows that are shorter than 2^-128 on average: not held). */
 MFL_API size_t mfl_add_rms_norm_bwd_workspace(int64_t R, int H);
 MFL_API int mfl_add_rms_norm_bwd(const void *dy, const void *ds, const void *s, const void *weight, void *dx, void *dw, int64_t R,
                          int H, float eps, int dtype, int weight_dtype, void *workspace, size_t ws_bytes, void *stream);
@@ -572,7 +573,7 @@ MFL_API int mfl_add_rms_norm_fp8(const void *x, const void *residual, const void
 /* The whole sparse expert layer for up to MFL_LAYER_TOKENS tokens: logits = rows router^T (sums in 64 bits, rounded
  * once to dtype), softmax, the k largest (of the rounded logits; equal ones: lower expert id), their weights brought to a sum of one
  * where renorm; out = sum over the chosen experts of weight * down(silu(gate row) * (up row)), in fp32 without a rounding in between
- * (bf16: the gated unit's result as the sum of two bf16 values), rounded once.
+ * (bf16: the gated unit's result as the sum of two bf16 values, infinities as in 32 bits), rounded once.
  * norm_weight NULL: rows = x, residual has to be NULL.  Else rows = y of mfl_add_rms_norm(x, residual, norm_weight) and its s is added
  * to out.
  * s_gate, s_up, s_down given: expert weights are e4m3 bytes with these block scales, and the rows and the gated unit's result are

@@ -84,7 +84,7 @@ __global__ __launch_bounds__(THREADS) void norm_bwd_kernel(const T *dy, const T 
     constexpr int GROUPS = THREADS / LANES, WAVES = LANES / 64;
     constexpr bool ONE = C == 1;
     // s and dy stay in registers between a row's two passes where they fit; else they are read again, from the caches (1024 x 32768
-    // in bf16: 251 us in registers that spill, 155 so; 2048 x 16384: 81 in registers, 90 so)
+    // in bf16: 251 us in registers, 153 so, where dw and the rest still spill 47; 2048 x 16384: 81 in registers, 90 so)
     constexpr int HELD = C == 2 ? C : 1;
     constexpr bool AHEAD = WHOLE && ONE;  // the next row is asked for before this one's sums are there (16384 x 2048: 61 -> 50 us)
     __shared__ double squares[2][GROUPS * WAVES];

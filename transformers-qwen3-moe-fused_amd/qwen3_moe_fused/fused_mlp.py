@@ -223,7 +223,8 @@ def moe_fused_mlp_fp8(tokens: torch.Tensor, w_gate: torch.Tensor, gate_scale: to
                       quantized: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> torch.Tensor:
     """``moe_fused_mlp`` on weights in 8-bit floating point with their block scales (frozen), in bf16, fp16 or fp32: between
     the gated unit and the down projection there are only quantised rows, made from the unit's fp32 values.  Differentiable
-    in ``tokens``.  ``quantized``: what ``add_rms_norm_fp8`` (or ``quantize_fp8_rows``) made of ``tokens`` already."""
+    in ``tokens``.  ``quantized``: what ``add_rms_norm_fp8`` (or ``quantize_fp8_rows``) made of ``tokens`` already (the decode kernels, up to
+    8 rows an expert on average in 16-bit types, quantise ``tokens`` on the way all the same)."""
     assert not (w_gate.requires_grad or gate_scale.requires_grad or w_up.requires_grad or up_scale.requires_grad
                 or w_down.requires_grad or down_scale.requires_grad), "8-bit expert weights are frozen"
     _check_routing(tokens, sort_idx, inv_sort_idx, num_selected)

@@ -70,7 +70,8 @@ def _forward_fp8(x, residual, weight, eps, return_normed):
 def add_rms_norm_backward(dy: Optional[torch.Tensor], ds: Optional[torch.Tensor], s: torch.Tensor, weight: torch.Tensor, eps: float,
                           need_dx: bool = True, need_dw: bool = True) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
     """(dx, dw) from the gradients of the normed rows and of the stream ``s``, which is what the forward pass returned; ``dx`` is
-    the residual's gradient too.  Sums over the rows in 32 bits, in the same order every time."""
+    the residual's gradient too.  A row's own sums are in 64 bits, 1 / length, ``dy * weight`` and the sums over the rows in 32, these in the same
+    order every time."""
     rows, width, dtype = _check(s, ds, weight)
     if dy is None:  # (nobody used the normed rows)
         return ds if need_dx else None, torch.zeros_like(weight) if need_dw else None
@@ -129,7 +130,8 @@ def _watched(x, residual, weight) -> bool:
 
 def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor,
                  eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
-    """(y, s) of rows along the last dimension, bf16, fp16 or fp32 and dense, up to 32768 wide; ``weight`` in their type or float32.
+    """(y, s) of rows along the last dimension, bf16, fp16 or fp32 and dense, up to 32768 wide and
+    ``most_rows`` long; ``weight`` in their type or float32.
     Without a ``residual`` (None) the stream ``s`` is ``x`` itself.  Differentiable once in ``x``, ``residual`` and ``weight``."""
     if not _watched(x, residual, weight):
         return _forward(x, residual, weight, eps)
