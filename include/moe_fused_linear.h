@@ -561,7 +561,7 @@ MFL_API int mfl_add_rms_norm(const void *x, const void *residual, const void *we
 /* Its gradients from dy and, where not NULL, ds (what arrives for s): dx (R,H), which is the residual's gradient too, and dw (H) in
  * weight_dtype, where not NULL.  s (R,H) as the forward call left it.  workspace: mfl_add_rms_norm_bwd_workspace(R, H) bytes where dw
  * is asked for, 16-byte aligned.  Same bits from run to run.  dx may be dy, ds or s.  A row's two sums are in 64 bits, its 1 / length,
- * dy weight and the sums over the rows in 32 (eps 0 and rows that are shorter than 2^-128 on average: not held). */
+ * dy weight and the sums over the rows in 32. */
 MFL_API size_t mfl_add_rms_norm_bwd_workspace(int64_t R, int H);
 MFL_API int mfl_add_rms_norm_bwd(const void *dy, const void *ds, const void *s, const void *weight, void *dx, void *dw, int64_t R,
                          int H, float eps, int dtype, int weight_dtype, void *workspace, size_t ws_bytes, void *stream);

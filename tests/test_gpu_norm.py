@@ -430,3 +430,21 @@ def test_backward_onto_an_operand_in_every_width(dtype, width, onto):
                                   EPS, code, code, ws.data_ptr(), size, _lib.stream())
     _lib.check(rc, "norm backward")
     assert torch.equal(ops[onto], want) and torch.equal(dw, want_dw)
+
+
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float32))
+@pytest.mark.parametrize("width", (40, 300, 2048, 12000, 20001))
+def test_rows_whose_inverse_length_32_bits_do_not_hold(dtype, width):
+    """Rows below 2^-128 without eps, one of ordinary values among them: both sides of the pass are the definition's."""
+    g = torch.Generator().manual_seed(width)
+    s = (torch.randn((5, width), generator=g) * 2.0 ** -131).to(dtype)
+    s[3] = torch.randn(width, generator=g).to(dtype)
+    w = (1.0 + 0.1 * torch.randn(width, generator=g)).to(dtype)
+    dy = (torch.randn(s.shape, generator=g) * 2.0 ** -12).to(dtype)
+    y, same = add_rms_norm(s.cuda(), None, w.cuda(), 0.0)
+    _check(y, same, s, None, w, dtype, 0.0)
+    dx, dw = add_rms_norm_backward(dy.cuda(), None, s.cuda(), w.cuda(), 0.0)
+    want = ref.norm_gradients(dy, None, s.double(), w, 0.0)
+    bounds = ref.norm_gradient_bounds(dy, None, s.double(), w, 0.0, dtype, dtype)
+    for a, b, c in zip((dx, dw), want, bounds):
+        assert ((a.cpu().double() - b).abs() <= c).all()

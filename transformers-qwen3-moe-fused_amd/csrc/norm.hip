@@ -78,7 +78,9 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void norm_fwd_kernel(con
 // in `partial` (workgroup, H), which a second kernel adds up in order.  Memory bounds it too: bf16 with ds, 16384 x 2048 50 us for
 // both kernels, 5.4 TB/s of three rows read and one written (49 with the second sum in 32 bits, which rows near their type's end pass).
 // dx may be dy, ds or s, so whatever is to be on its way over a store is asked for in front of it.
-template <typename T, typename TW, int LANES, int C, int THREADS, bool WHOLE>
+// BARE: without eps a row around 2^-127 has an r that 32 bits do not hold: such rows are taken as 2^64 s.  (A kernel of its own: two products
+// more an element for every row take 16384 x 2048 from 50 to 59 us, a second copy of the loop behind a question to 56.)
+template <typename T, typename TW, int LANES, int C, int THREADS, bool WHOLE, bool BARE>
 __global__ __launch_bounds__(THREADS) void norm_bwd_kernel(const T *dy, const T *ds, const T *s, const TW *__restrict__ weight, T *dx,
                                                           float *__restrict__ partial, int64_t R, int H, double eps) {
     constexpr int GROUPS = THREADS / LANES, WAVES = LANES / 64;
@@ -144,7 +146,9 @@ __global__ __launch_bounds__(THREADS) void norm_bwd_kernel(const T *dy, const T 
 #pragma unroll
             for (int u = 0; u < WAVES; ++u) square += squares[turn][group * WAVES + u], along += alongs[turn][group * WAVES + u];
         }
-        const double root = inverse_root(square / (double)H + eps);
+        double root = inverse_root(square / (double)H + eps);
+        float up = 1.0f;
+        if (BARE && root > 0x1p127) up = 0x1p64f, root *= 0x1p-64, along *= 0x1p64;
         const float r = (float)root, back = (float)(along / (double)H * root * root);  // dx = r (g - s back) + ds
         if (!in) continue;
 #pragma unroll
@@ -161,9 +165,12 @@ __global__ __launch_bounds__(THREADS) void norm_bwd_kernel(const T *dy, const T 
             }
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
-                const float a = to_f32(sv.v[u]), b = to_f32(g.v[u]);
+                float a = to_f32(sv.v[u]);
+                if (BARE) a *= up;
+                const float b = to_f32(g.v[u]);
                 dw[c][u] = __builtin_fmaf(b, a * r, dw[c][u]);
                 float o = r * __builtin_fmaf(-a, back, b * to_f32(w.v[u]));
+                if (BARE) o *= up;
                 if (add) o += to_f32(d.v[u]);
                 sv.v[u] = from_f32<T>(o);
             }
@@ -269,7 +276,8 @@ int launch_bwd(const NormCall &n, const void *dy, const void *ds, void *dx, void
     {                                                                                                                          \
         constexpr int threads = L < kBwdThreads ? kBwdThreads : L;                                                             \
         constexpr int room = (threads / L - 1) * L * C * 8 * 4;  /* 14 KB at most */                                           \
-        auto kernel = norm_bwd_kernel<T, TW, L, C, threads, WHOLE>;                                                            \
+        auto kernel = n.eps == 0.0f ? norm_bwd_kernel<T, TW, L, C, threads, WHOLE, true>                                       \
+                                    : norm_bwd_kernel<T, TW, L, C, threads, WHOLE, false>;                                     \
         if (grid > 0)                                                                                                          \
             kernel<<<grid, threads, room, stream>>>((const T *)dy, (const T *)ds, (const T *)n.s, (const TW *)n.weight, (T *)dx, \
                                                     dw != nullptr ? partial : nullptr, n.R, H, (double)n.eps);                 \
