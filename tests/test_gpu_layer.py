@@ -285,6 +285,18 @@ def test_infinite_gated_unit(dtype):
     assert torch.equal(case.call()[0][1], out[1]) and out[1].isfinite().all()
 
 
+@pytest.mark.parametrize("dtype", (BF16, F16, F32))
+def test_an_expert_that_is_no_number_reaches_its_tokens_alone(dtype):
+    case = Case(6, 8, 2, 80, 56, dtype)
+    want, logits = case.call()
+    picked = [{e for e, _ in p} for p in ref.choose(logits.cpu(), 2, True)]
+    bad = next(e for e in range(8) if 0 < sum(e in p for p in picked) < 6)
+    case.weights[0][bad, 17, 3] = float("nan")
+    out, _ = case.call()
+    for t in range(6):
+        assert out[t].isnan().all() if bad in picked[t] else torch.equal(out[t], want[t])
+
+
 def test_infinite_gated_unit_in_8_bits():
     """An infinite element becomes NaN on its way to the grid, as in the expert MLP, and the other token is as it is without it."""
     case = Case(2, 2, 2, 160, 200, BF16, eight=True)
