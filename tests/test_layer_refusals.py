@@ -311,6 +311,10 @@ def test_a_forward_replaced_before_the_classes_are_built_is_known_too(monkeypatc
     assert _defined_forward(Qwen3MoeRMSNorm) is stock
     monkeypatch.setattr(Qwen3MoeRMSNorm, "forward", functools.wraps(stock)(lambda self, hidden_states: stock(self, hidden_states)))
     assert _defined_forward(Qwen3MoeRMSNorm) is None
+    decorated = {"__name__": "transformers.utils.deprecation"}
+    exec("def wrapper(self, hidden_states):\n    return None", decorated)
+    monkeypatch.setattr(Qwen3MoeRMSNorm, "forward", decorated["wrapper"])
+    assert _defined_forward(Qwen3MoeRMSNorm) is decorated["wrapper"]
 
 
 def test_a_replaced_forward_of_the_stock_layer_is_called(own_half, monkeypatch):

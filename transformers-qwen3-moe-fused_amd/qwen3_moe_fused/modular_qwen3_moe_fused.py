@@ -9,7 +9,6 @@ load unchanged.
 from __future__ import annotations
 
 import math
-import sys
 from typing import Optional, Tuple
 
 import torch
@@ -90,9 +89,11 @@ def _stands_for_itself(module: nn.Module) -> bool:
 
 
 def _defined_forward(cls: type):
-    """A foreign class's forward, or None where somebody has put another in the place of the one in its module's source."""
+    """A foreign class's forward, or None where somebody outside its package has put another in its place.  (The package's own decorators
+    are part of it.)"""
     forward = cls.forward
-    return forward if getattr(forward, "__globals__", None) is vars(sys.modules[cls.__module__]) else None
+    at = getattr(forward, "__globals__", {}).get("__name__", "")
+    return forward if at.split(".")[0] == cls.__module__.split(".")[0] else None
 
 
 class Qwen3MoeFusedSparseMoeBlock(nn.Module):
